@@ -49,6 +49,7 @@ typedef enum {
     KVHIP_KIND_SIMPLE = 0,    /* KVCacheSimple    KVCache.swift:391-538  */
     KVHIP_KIND_ROTATING = 1,  /* RotatingKVCache  KVCache.swift:541-900  */
     KVHIP_KIND_QUANTIZED = 2, /* QuantizedKVCache KVCache.swift:923-1210 */
+    KVHIP_KIND_BLOCK_SCALED = 3, /* no counterpart: 8-bit float codes, one scale to a block of 64 tokens and kv head (below) */
 } kvhip_kind;
 
 typedef enum {
@@ -139,8 +140,8 @@ void kvhip_set_kernel_policy(int32_t policy);
  * 0 generic, 1 matrix-core decode (quantized), 2 matrix-core decode (full precision),
  * 3 matrix-core chunked-prefill tile, 4 the same tile over scratch pages a quantized cache was dequantized into
  * first, 5 the vector-ALU kernel (float32 caches, 16-bit head sizes above 256), 6 the same over scratch pages a
- * quantized cache of such head sizes, or one with float32 scales, was dequantized into first; -1 before the first
- * call.  For tests and reports. */
+ * quantized cache of such head sizes, or one with float32 scales, was dequantized into first, 7 block-scaled, 8 the same
+ * over chosen blocks; -1 before the first call.  For tests and reports. */
 int32_t kvhip_last_attend_kernel(void);
 /* Which kernel the last append launch of this thread used: 0 rows (a workgroup to a row, or to a tile's few quantized rows),
  * 1 64-token tiles; -1 before the first.  Rows that the attention kernel writes itself do not count.  For tests. */
@@ -304,6 +305,44 @@ kvhip_status kvhip_cache_update_attend(kvhip_cache *cache, const void *queries, 
                                        const void *values, int32_t B, int32_t Hq, int32_t Hkv,
                                        int32_t L, int32_t Dk, int32_t Dv, int32_t dtype, float scale,
                                        const kvhip_mask *mask, void *out, void *stream);
+
+/* ---- block-scaled caches --------------------------------------------------- */
+/*
+ * KVHIP_KIND_BLOCK_SCALED has no counterpart in the reference.  It is a KVCacheSimple to its caller -- update, fetch, attend,
+ * update_attend (with rotary positions too), trim, copy, state ([keys, values], dense, as read back) -- that holds its rows in
+ * 8 bits.  Rows are cut into blocks of 64 by position.  A block of one kv head that has all its rows is held as e4m3 codes
+ * and one scale each for keys and values, a power of two:
+ *     a = max |x| over the block's finite elements;  e = the least integer with a 2^-e <= 448 (0 if a = 0; at least -100)
+ *     code = e4m3(x 2^-e), to nearest even;  the value read back is code 2^e
+ * and the rows behind the last such block are held as they came.  Values read back are exact in the cache's dtype, and
+ * written again they come out the same; infinities are held as NaN; values of a float16 cache beyond 61440 are held as that.
+ * float16 and bfloat16, head sizes up to 256 (stored zero-padded to 64, 96, 128 or 256; 192 with 128); else
+ * KVHIP_ERR_UNSUPPORTED.  kvhip_cache_trim and _set_offset take rows off what the cache presents at once; offsets are never
+ * set forward.  Query rows that see no key are zeros.  kvhip_last_attend_kernel: 7, over chosen blocks 8.
+ *
+ * Attention over chosen blocks.  Query row l of L sits at position p = presented length - L + l.  A query row's bound on a
+ * block is sum_d max(q_d hi_d, q_d lo_d), hi and lo the block's largest and smallest key element of each channel, with
+ * hi and lo taken as rint(code / 4) 2^(e + 2) and q as rint(q 2^-f) 2^f, f the least integer with max |q| 2^-f <= 127 over
+ * the row (elements that are not finite: 0), so that it is exact; a token's bound is the largest of its query rows'
+ * over one kv head.  The token sees blocks left_pad[b] / 64 to p / 64 (none if p < left_pad[b]).  The first `first` of these
+ * and the last `recent` are chosen, and as many more as make `count`, by their bounds, the lower block among equals.
+ * blocks: device [B, Hkv, L, count] int32, ascending, -1 behind the last; left_pad: device [B] or NULL.
+ * first >= 0, recent >= 1, first + recent <= count; up to 36 000 blocks (2.3 million rows) a cache.
+ */
+kvhip_status kvhip_cache_select_blocks(kvhip_cache *cache, const void *queries, int32_t B, int32_t Hq, int32_t L, int32_t D,
+                                       int32_t count, int32_t first, int32_t recent, const int32_t *left_pad, int32_t *blocks,
+                                       void *stream);
+/* Attention of each token over the keys of its listed blocks at positions left_pad[b] to p.  The list need not come from
+ * kvhip_cache_select_blocks; an entry that the token does not see, or that is not above the entry before it, is passed over. */
+kvhip_status kvhip_cache_attend_blocks(kvhip_cache *cache, const void *queries, int32_t B, int32_t Hq, int32_t L, int32_t D,
+                                       float scale, const int32_t *blocks, int32_t count, const int32_t *left_pad, void *out,
+                                       void *stream);
+/* kvhip_cache_update, kvhip_cache_select_blocks and kvhip_cache_attend_blocks in one call; a single new token that finishes no
+ * block is written by the attention kernel. */
+kvhip_status kvhip_cache_update_attend_blocks(kvhip_cache *cache, const void *queries, const void *keys, const void *values,
+                                              int32_t B, int32_t Hq, int32_t Hkv, int32_t L, int32_t Dk, int32_t Dv,
+                                              int32_t dtype, float scale, int32_t count, int32_t first, int32_t recent,
+                                              const int32_t *left_pad, int32_t *blocks, void *out, void *stream);
 
 /* `makeMask(n:windowSize:returnArray:)`; window_size <= 0 stands for nil. */
 kvhip_status kvhip_cache_mask_plan(const kvhip_cache *cache, int32_t n, int32_t window_size,

@@ -11,6 +11,7 @@
 #include <utility>
 #include <vector>
 
+#include "kvhip_block.hpp"
 #include "kvhip_internal.hpp"
 
 using namespace kvhip;
@@ -98,8 +99,8 @@ struct kvhip_cache {
     // zero value columns give output columns nobody reads), arrays are widened on the way in and narrowed on the
     // way out, and everything between works on the stored sizes.
     int Dk_user = 0, Dv_user = 0;
-    // widened keys, values, queries; outputs before narrowing; the rotated queries of a step
-    static constexpr int PAD_BUFS = 5;
+    // widened keys, values, queries; outputs before narrowing; the rotated queries of a step; rotated keys (block-scaled)
+    static constexpr int PAD_BUFS = 6;
     void *pad_buf[PAD_BUFS] = {};
     size_t pad_bytes[PAD_BUFS] = {};
     std::vector<Slab> slabs;   // the allocations behind the pages, in page order
@@ -118,6 +119,11 @@ struct kvhip_cache {
     void *stage_tmp_k = nullptr, *stage_tmp_v = nullptr;  // dense copy of the rows a commit keeps
     size_t stage_tmp_rows = 0;
     RopeDev *rope = nullptr;  // set for the duration of one update_rope call
+    // block-scaled only: blocks held as codes, and two tails (kvhip_block.hpp), one of them in use
+    int64_t coded = 0;
+    char *tail = nullptr;
+    size_t tail_bytes = 0;
+    int tail_now = 0;
     // scratch for attention
     float *ws = nullptr;
     size_t ws_bytes = 0;
@@ -332,6 +338,8 @@ kvhip_status set_geometry(kvhip_cache *c, int B, int Hkv, int Dk, int Dv, int dt
     if (dtype != KVHIP_F16 && dtype != KVHIP_BF16 && dtype != KVHIP_F32)
         return fail(KVHIP_ERR_INVALID_ARG, "cache dtype must be float16, bfloat16 or float32");
     if ((int64_t)B * Hkv > 65535) return fail(KVHIP_ERR_UNSUPPORTED, "B * Hkv above 65535");
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED && (dtype == KVHIP_F32 || Dk > BLOCK_MAX_HEAD || Dv > BLOCK_MAX_HEAD))
+        return fail(KVHIP_ERR_UNSUPPORTED, "block-scaled caches are float16 or bfloat16, of head sizes up to 256");
     if (c->has_geom) {
         const Store &s = c->st;
         if (s.BH != B * Hkv || c->B != B || c->Dk_user != Dk || c->Dv_user != Dv || s.dtype != dtype)
@@ -346,13 +354,21 @@ kvhip_status set_geometry(kvhip_cache *c, int B, int Hkv, int Dk, int Dv, int dt
     c->Hkv = Hkv;
     c->Dk_user = Dk;
     c->Dv_user = Dv;
-    stored_head_sizes(c->kind, c->gs, dtype, Dk, Dv, Dk, Dv);  // from here on: the stored sizes
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) stored_head_sizes(KVHIP_KIND_QUANTIZED, 1, dtype, Dk, Dv, Dk, Dv);  // (64, 96, 128, 256; 192 with 128)
+    else stored_head_sizes(c->kind, c->gs, dtype, Dk, Dv, Dk, Dv);  // from here on: the stored sizes
     s.BH = B * Hkv;
     s.Dk = Dk;
     s.Dv = Dv;
     s.dtype = dtype;
     s.es = elem_size(dtype);
-    if (c->kind == KVHIP_KIND_QUANTIZED) {
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) {
+        s.bits = 8;
+        s.k_row = (uint32_t)Dk;
+        s.k_cell = s.k_row * PAGE;
+        s.v_cell = (uint32_t)Dv * PAGE;
+        s.ksb_cell = BLOCK_PER_PAGE * 2 * sizeof(float);
+        s.vsb_cell = (uint32_t)(BLOCK_PER_PAGE * 2 * Dk);
+    } else if (c->kind == KVHIP_KIND_QUANTIZED) {
         if (!affine_bits_ok(c->bits))
             return fail(KVHIP_ERR_UNSUPPORTED, "affine KV quantization is implemented for 2, 3, 4, 5, 6 and 8 bits");
         if (Dk % c->gs || Dv % c->gs) return fail(KVHIP_ERR_INVALID_ARG, "head dim not divisible by the group size");
@@ -706,6 +722,60 @@ kvhip_status update_simple(kvhip_cache *c, const void *k, const void *v, int L, 
     return KVHIP_OK;
 }
 
+// ---- block-scaled caches (kvhip_block.hpp) -----------------------------------------
+kvhip_status ensure_tail(kvhip_cache *c) {
+    if (c->tail) return KVHIP_OK;
+    void *p = nullptr;
+    const size_t need = 2 * (size_t)c->st.BH * BLOCK_ROWS * (c->st.Dk + c->st.Dv) * c->st.es;  // (no row is read that was not written)
+    KV_HIP(pool_alloc(&p, need, &c->tail_bytes));
+    c->tail = static_cast<char *>(p);
+    return KVHIP_OK;
+}
+void tail_at(const kvhip_cache *c, int which, char *&k, char *&v) {
+    const size_t pair = (size_t)BLOCK_ROWS * c->st.es;
+    k = c->tail + (size_t)which * c->st.BH * pair * (c->st.Dk + c->st.Dv);
+    v = k + (size_t)c->st.BH * pair * c->st.Dk;
+}
+BlockStore block_store(const kvhip_cache *c) {
+    BlockStore s;
+    s.st = c->st;
+    tail_at(c, c->tail_now, s.tail_k, s.tail_v);
+    s.coded = (int32_t)c->coded;
+    s.Dk_user = c->Dk_user;
+    s.Dv_user = c->Dv_user;
+    return s;
+}
+// `launch` false: the attention kernel writes the row of a single token that finishes no block (block_step_fuses).
+kvhip_status update_blocks(kvhip_cache *c, const void *k, const void *v, int L, hipStream_t stream, bool launch = true) {
+    const int64_t prev = c->offset, next = prev + L;
+    KV_TRY(ensure_slots(c, next, stream));
+    KV_TRY(ensure_tail(c));
+    if (launch) {
+        if (c->rope) {  // the keys turn in a launch of their own
+            RopeDev turn = *c->rope;
+            turn.qx = nullptr;
+            KV_TRY(ensure_pad_buf(c, 5, (size_t)c->st.BH * L * c->Dk_user * c->st.es));
+            KV_HIP(launch_rope_apply(turn, k, c->pad_buf[5], c->B, c->Hkv, L, c->Dk_user, c->st.dtype, stream));
+            k = c->pad_buf[5];
+        }
+        const int to = prev / BLOCK_ROWS == (next - 1) / BLOCK_ROWS ? c->tail_now : 1 - c->tail_now;
+        char *to_k, *to_v;
+        tail_at(c, to, to_k, to_v);
+        KV_HIP(launch_block_append(block_store(c), k, v, prev, L, to_k, to_v, stream));
+        c->tail_now = to;
+    }
+    c->coded = next / BLOCK_ROWS;
+    c->ref_len = next;
+    c->has_buffers = true;
+    c->offset = c->presented = next;
+    return KVHIP_OK;
+}
+// Whether a new token's row can be left to the attention kernel: it finishes no block, and its block's rows are in the tail.
+bool block_step_fuses(const kvhip_cache *c, int L) {
+    return L == 1 && c->has_geom && c->has_buffers && c->tail && !c->padded() && !c->rope && c->offset >= c->coded * BLOCK_ROWS &&
+           c->offset % BLOCK_ROWS != BLOCK_ROWS - 1;
+}
+
 // deferred_slot (single-token steps only): the row is not written here; its physical slot is handed back and
 // the caller sees to the write (the decode kernel takes it along).
 kvhip_status update_rotating(kvhip_cache *c, const void *k, const void *v, int L, hipStream_t stream,
@@ -819,6 +889,7 @@ kvhip_status stage_update(kvhip_cache *c, const void *k, const void *v, int L, h
 int64_t state_rows(const kvhip_cache *c) {
     // KVCache.swift:449-460, :752-763, :1113-1130: sliced to offset when offset < extent
     if (!c->has_buffers) return 0;
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) return c->offset;
     return c->offset < c->ref_len ? std::max<int64_t>(c->offset, 0) : c->ref_len;
 }
 
@@ -891,7 +962,7 @@ kvhip_status kvhip_profile_read(int32_t *out_launches, double *out_total_ms) {
 
 kvhip_status kvhip_cache_create(const kvhip_config *cfg, kvhip_cache **out) {
     if (!cfg || !out) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
-    if (cfg->kind < 0 || cfg->kind > 2) return fail(KVHIP_ERR_INVALID_ARG, "unknown cache kind");
+    if (cfg->kind < 0 || cfg->kind > KVHIP_KIND_BLOCK_SCALED) return fail(KVHIP_ERR_INVALID_ARG, "unknown cache kind");
     kvhip_cache *c = new kvhip_cache();
     c->kind = cfg->kind;
     c->step = cfg->step > 0 ? cfg->step : 256;
@@ -908,6 +979,10 @@ kvhip_status kvhip_cache_create(const kvhip_config *cfg, kvhip_cache **out) {
         c->gs = cfg->group_size > 0 ? cfg->group_size : 64;
         c->bits = cfg->bits > 0 ? cfg->bits : 8;
     }
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) {
+        c->gs = BLOCK_ROWS;
+        c->bits = 8;
+    }
     *out = c;
     return KVHIP_OK;
 }
@@ -922,6 +997,7 @@ void kvhip_cache_free(kvhip_cache *c) {
     for (const Slab &sl : c->slabs) ptrs.push_back({sl.base, sl.bytes});
     if (c->st.pt) ptrs.push_back({const_cast<PageEntry *>(c->st.pt), (size_t)0});
     if (c->ws) ptrs.push_back({c->ws, c->ws_bytes});
+    if (c->tail) ptrs.push_back({c->tail, c->tail_bytes});
     for (int i = 0; i < kvhip_cache::PAD_BUFS; ++i)
         if (c->pad_buf[i]) ptrs.push_back({c->pad_buf[i], c->pad_bytes[i]});
     if (c->stage_tmp_k) ptrs.push_back({c->stage_tmp_k, (size_t)0});
@@ -963,6 +1039,12 @@ int32_t kvhip_cache_is_trimmable(const kvhip_cache *c, int64_t after) {
 
 int64_t kvhip_cache_trim(kvhip_cache *c, int64_t n) {
     if (!c) return 0;
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) {  // (what is left is what the cache presents; the next write sees to its last block)
+        const int64_t t = std::min(c->offset, std::max<int64_t>(n, 0));
+        c->offset -= t;
+        c->presented = c->offset;
+        return t;
+    }
     const int64_t t = std::min(c->offset, n);  // KVCache.swift:474-478, :826-831, :1171-1175
     c->offset -= t;
     if (c->kind == KVHIP_KIND_ROTATING) c->idx -= t;
@@ -971,6 +1053,10 @@ int64_t kvhip_cache_trim(kvhip_cache *c, int64_t n) {
 
 kvhip_status kvhip_cache_set_offset(kvhip_cache *c, int64_t offset) {
     if (!c) return fail(KVHIP_ERR_INVALID_ARG, "null cache");
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) {
+        if (offset < 0 || offset > c->offset) return fail(KVHIP_ERR_STATE, "the offset of a block-scaled cache can only be set back");
+        c->presented = offset;
+    }
     c->offset = offset;
     return KVHIP_OK;
 }
@@ -997,6 +1083,7 @@ kvhip_status kvhip_cache_reserve(kvhip_cache *c, int32_t B, int32_t Hkv, int32_t
     KV_TRY(set_geometry(c, B, Hkv, Dk, Dv, dtype));
     reap_retired();
     KV_TRY(ensure_slots(c, tokens, nullptr, true));
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) KV_TRY(ensure_tail(c));
     // the zero-fill of the new pages ran on the default stream: wait for it here, so that a
     // first update on any other (non-blocking) stream is ordered after it
     KV_HIP(hipStreamSynchronize(nullptr));
@@ -1020,6 +1107,7 @@ kvhip_status kvhip_cache_update(kvhip_cache *c, const void *keys, const void *va
         }
     }
     KV_TRY(set_geometry(c, B, Hkv, Dk, Dv, dtype));
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) return update_blocks(c, keys, values, L, S(c, stream));
     if (c->padded()) {  // rows of the stored head sizes, the added columns zero (a rotation reads its partners inside Dk)
         const size_t rows = (size_t)B * Hkv * L;
         KV_TRY(widen_rows(c, 0, keys, rows, Dk, c->st.Dk, S(c, stream), &keys));
@@ -1087,6 +1175,10 @@ kvhip_status kvhip_cache_fetch(const kvhip_cache *c, void *dk, void *dv, void *s
     if (c->staging && !c->stage_view.empty())
         return export_slots(c, c->stage_view.data(), (int64_t)c->stage_view.size(), dk, dv, S(c, stream));
     if (!c->has_buffers) return fail(KVHIP_ERR_STATE, "cache is empty");
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) {
+        KV_HIP(launch_block_fetch(block_store(c), c->presented, dk, dv, S(c, stream)));
+        return KVHIP_OK;
+    }
     if (c->kind == KVHIP_KIND_ROTATING)
         return export_slots(c, c->rows.data(), c->presented, dk, dv, S(c, stream));
     std::vector<int32_t> ident((size_t)c->presented);
@@ -1204,6 +1296,23 @@ bool attention_will_write_step(const kvhip_cache *c, int Hq) {
     return attention_writes_step(a);
 }
 
+// Attention over a block-scaled cache: under a.mask, or (`list`) over listed blocks.
+kvhip_status run_block_attend(kvhip_cache *c, const AttendArgs &a, const int32_t *list, int32_t count, const int32_t *left_pad, float *fixed,
+                              size_t fixed_bytes, hipStream_t s) {
+    BlockAttend x;
+    x.a = a;
+    x.b = block_store(c);
+    x.list = list;
+    x.count = count;
+    x.left_pad = left_pad;
+    const size_t need = plan_block_attend(x);
+    if (block_attend_rows(x) > 65535) return fail(KVHIP_ERR_UNSUPPORTED, "more query rows than one call takes");
+    KV_TRY(bind_workspace(c, x.a, need, fixed, fixed_bytes, s));
+    KV_HIP(launch_block_attend(x, s));
+    g_last_kernel = list ? 8 : 7;
+    return KVHIP_OK;
+}
+
 // new_k / new_v: the rows of a single-token step whose bookkeeping is done but whose write into physical
 // slot `new_slot` is still owed; the attention kernel takes them along when it can, else they are
 // appended by a launch of their own first.  `rope`: the queries and the new key row are still to be rotated (its H:
@@ -1279,7 +1388,15 @@ kvhip_status attend_impl(kvhip_cache *c, const void *q, int32_t B, int32_t Hq, i
     }
     hipStream_t s = S(c, stream);
     a.workspace_cap = fixed ? fixed_bytes : 0;
-    if (new_k) {
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) {
+        a.new_k = new_k;
+        a.new_v = new_v;
+        if (a.mask.mode == KVHIP_MASK_NONE) {  // (a window that every key is inside of)
+            a.mask.mode = KVHIP_MASK_WINDOW;
+            a.mask.offset = a.T;
+        }
+        KV_TRY(run_block_attend(c, a, nullptr, 0, nullptr, fixed, fixed_bytes, s));
+    } else if (new_k) {
         if (attention_writes_step(a)) {
             a.new_k = new_k;
             a.new_v = new_v;
@@ -1300,7 +1417,9 @@ kvhip_status attend_impl(kvhip_cache *c, const void *q, int32_t B, int32_t Hq, i
             else KV_HIP(launch_append_fp(c->st, new_k, new_v, 1, 0, new_slot, 1, s, rope));
         }
     }
-    if (g_policy != 1 && attend_decode_supported(a)) {
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) {
+        // (enqueued above)
+    } else if (g_policy != 1 && attend_decode_supported(a)) {
         KV_TRY(bind_workspace(c, a, attend_decode_workspace(a), fixed, fixed_bytes, s));
         KV_HIP(launch_attend_decode(a, s));
         g_last_kernel = a.st.bits ? 1 : 2;
@@ -1364,6 +1483,17 @@ kvhip_status kvhip_cache_update_attend(kvhip_cache *c, const void *q, const void
         }
         return st;
     }
+    // One new token into a block-scaled cache: the attention kernel writes it into the tail, unless it finishes a block.
+    if (c && k && v && q && out && c->kind == KVHIP_KIND_BLOCK_SCALED && block_step_fuses(c, L) && (!mask || mask->mode == KVHIP_MASK_NONE) &&
+        c->B == B && c->Hkv == Hkv && c->st.Dk == Dk && c->st.Dv == Dv && c->st.dtype == dtype) {
+        KV_TRY(update_blocks(c, k, v, 1, S(c, stream), false));
+        const kvhip_status st = attend_impl(c, q, B, Hq, L, Dk, scale, mask, out, stream, nullptr, 0, k, v, (int32_t)c->offset - 1);
+        if (st != KVHIP_OK) {  // nothing was written: take the row back
+            c->offset -= 1;
+            c->presented = c->offset;
+        }
+        return st;
+    }
     // One new token into a full-precision cache (KVCacheSimple, or the in-place step of a
     // RotatingKVCache): the attention kernel copies the row into its slot itself where it can.  The bookkeeping of `update`
     // runs here as usual; if the attention cannot be enqueued the row is written by the append kernel, so
@@ -1399,7 +1529,7 @@ kvhip_status kvhip_cache_update_attend_rope(kvhip_cache *c, const kvhip_rope *ro
     KV_TRY(rope_dev(rope, Dk, Hkv, dtype, pos0, batch_offsets, r));
     // One new token without a mask: the attention kernels rotate its rows themselves, as they write the new one
     // (kvhip_cache_update_attend), and the step is a launch less.
-    const bool token = L == 1 && !c->staging && (dtype != KVHIP_F32 || c->kind != KVHIP_KIND_QUANTIZED) && (!mask || mask->mode == KVHIP_MASK_NONE) &&
+    const bool token = L == 1 && !c->staging && c->kind != KVHIP_KIND_BLOCK_SCALED && (dtype != KVHIP_F32 || c->kind != KVHIP_KIND_QUANTIZED) && (!mask || mask->mode == KVHIP_MASK_NONE) &&
                        c->has_geom && c->has_buffers && !c->padded() && c->B == B && c->Hkv == Hkv && c->st.Dk == Dk && c->st.Dv == Dv &&
                        c->st.dtype == dtype && (size_t)B * Hkv + (size_t)B * Hq <= 65535;
     if (!q_rotated && !(token && attention_will_write_step(c, Hq))) {
@@ -1445,6 +1575,109 @@ kvhip_status kvhip_cache_update_attend_rope(kvhip_cache *c, const kvhip_rope *ro
         KV_HIP(launch_rope_apply(own, q, q_rotated, B, Hq, L, Dk, dtype, S(c, stream)));
     }
     return kvhip_cache_attend(c, q_rotated, B, Hq, L, Dk, scale, mask, out, stream);
+}
+
+namespace {
+// What a choice of blocks has to satisfy for queries [B, Hq, L, D] at the end of `T` rows.
+kvhip_status check_block_call(const kvhip_cache *c, int32_t B, int32_t Hq, int32_t L, int32_t D, int64_t T, int32_t count) {
+    if (c->kind != KVHIP_KIND_BLOCK_SCALED) return fail(KVHIP_ERR_INVALID_ARG, "blocks are chosen in a block-scaled cache");
+    if (!c->has_geom || T <= 0) return fail(KVHIP_ERR_STATE, "attention over an empty cache");
+    if (B != c->B || D != c->Dk_user) return fail(KVHIP_ERR_INVALID_ARG, "query shape does not match the cache");
+    if (Hq <= 0 || Hq % c->Hkv) return fail(KVHIP_ERR_INVALID_ARG, "query heads must be a multiple of KV heads");
+    if (L <= 0 || L > 65535 || L > T) return fail(KVHIP_ERR_INVALID_ARG, "query length out of range");
+    if (count <= 0) return fail(KVHIP_ERR_INVALID_ARG, "at least one block to a token");
+    return KVHIP_OK;
+}
+kvhip_status block_choice(const kvhip_cache *c, const void *q, int32_t B, int32_t Hq, int32_t L, int64_t T, int32_t count, int32_t first,
+                          int32_t recent, const int32_t *left_pad, int32_t *blocks, BlockSelect &x) {
+    if (first < 0 || recent < 1 || (int64_t)first + recent > count)
+        return fail(KVHIP_ERR_INVALID_ARG, "leading blocks (0 or more) and recent ones (1 or more) have to fit the count");
+    x.q = q;
+    x.B = B;
+    x.Hq = Hq;
+    x.Hkv = c->Hkv;
+    x.L = L;
+    x.T = (int32_t)T;
+    x.count = count;
+    x.first = first;
+    x.recent = recent;
+    x.left_pad = left_pad;
+    x.list = blocks;
+    x.b.st.BH = c->st.BH;
+    if (!block_select_supported(x)) return fail(KVHIP_ERR_UNSUPPORTED, "a cache of this length holds more blocks than one choice takes");
+    return KVHIP_OK;
+}
+kvhip_status attend_blocks_impl(kvhip_cache *c, const void *q, int32_t B, int32_t Hq, int32_t L, int32_t D, float scale, const int32_t *blocks,
+                                int32_t count, const int32_t *left_pad, void *out, const void *new_k, const void *new_v, hipStream_t s) {
+    AttendArgs a;
+    void *user_out = nullptr;
+    const size_t q_rows = (size_t)B * Hq * L;
+    if (c->padded()) {
+        KV_TRY(widen_rows(c, 2, q, q_rows, D, c->st.Dk, s, &q));
+        KV_TRY(ensure_pad_buf(c, 3, q_rows * c->st.Dv * c->st.es));
+        user_out = out;
+        out = c->pad_buf[3];
+    }
+    a.st = c->st;
+    a.q = q;
+    a.out = out;
+    a.B = B;
+    a.Hq = Hq;
+    a.Hkv = c->Hkv;
+    a.L = L;
+    a.T = a.slots = (int)c->presented;
+    a.scale = scale;
+    a.new_k = new_k;
+    a.new_v = new_v;
+    KV_TRY(run_block_attend(c, a, blocks, count, left_pad, nullptr, 0, s));
+    if (user_out) KV_HIP(launch_repitch_rows(user_out, (size_t)c->Dv_user * c->st.es, out, (size_t)c->st.Dv * c->st.es, q_rows, s));
+    return KVHIP_OK;
+}
+}  // namespace
+
+kvhip_status kvhip_cache_select_blocks(kvhip_cache *c, const void *q, int32_t B, int32_t Hq, int32_t L, int32_t D, int32_t count, int32_t first,
+                                       int32_t recent, const int32_t *left_pad, int32_t *blocks, void *stream) {
+    if (!c || !q || !blocks) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
+    KV_TRY(check_block_call(c, B, Hq, L, D, c->presented, count));
+    BlockSelect x;
+    KV_TRY(block_choice(c, q, B, Hq, L, c->presented, count, first, recent, left_pad, blocks, x));
+    x.b = block_store(c);
+    KV_HIP(launch_block_select(x, S(c, stream)));
+    return KVHIP_OK;
+}
+
+kvhip_status kvhip_cache_attend_blocks(kvhip_cache *c, const void *q, int32_t B, int32_t Hq, int32_t L, int32_t D, float scale,
+                                       const int32_t *blocks, int32_t count, const int32_t *left_pad, void *out, void *stream) {
+    if (!c || !q || !blocks || !out) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
+    KV_TRY(check_block_call(c, B, Hq, L, D, c->presented, count));
+    return attend_blocks_impl(c, q, B, Hq, L, D, scale, blocks, count, left_pad, out, nullptr, nullptr, S(c, stream));
+}
+
+kvhip_status kvhip_cache_update_attend_blocks(kvhip_cache *c, const void *q, const void *k, const void *v, int32_t B, int32_t Hq, int32_t Hkv,
+                                              int32_t L, int32_t Dk, int32_t Dv, int32_t dtype, float scale, int32_t count, int32_t first,
+                                              int32_t recent, const int32_t *left_pad, int32_t *blocks, void *out, void *stream) {
+    if (!c || !q || !k || !v || !blocks || !out) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
+    if (c->kind != KVHIP_KIND_BLOCK_SCALED) return fail(KVHIP_ERR_INVALID_ARG, "blocks are chosen in a block-scaled cache");
+    if (L <= 0) return fail(KVHIP_ERR_INVALID_ARG, "update needs at least one new row");
+    // (all that can be refused is, before anything is written)
+    KV_TRY(set_geometry(c, B, Hkv, Dk, Dv, dtype));
+    const int64_t T = c->offset + L;
+    KV_TRY(check_block_call(c, B, Hq, L, Dk, T, count));
+    BlockSelect x;
+    KV_TRY(block_choice(c, q, B, Hq, L, T, count, first, recent, left_pad, blocks, x));
+    hipStream_t s = S(c, stream);
+    const bool fuse = block_step_fuses(c, L);
+    KV_TRY(update_blocks(c, k, v, L, s, !fuse));
+    x.b = block_store(c);
+    hipError_t e = launch_block_select(x, s);
+    kvhip_status st = e == hipSuccess ? KVHIP_OK : fail(KVHIP_ERR_HIP, std::string("the choice of blocks: ") + hipGetErrorString(e));
+    if (st == KVHIP_OK)
+        st = attend_blocks_impl(c, q, B, Hq, L, Dk, scale, blocks, count, left_pad, out, fuse ? k : nullptr, fuse ? v : nullptr, s);
+    if (st != KVHIP_OK && fuse) {  // nothing was written: take the row back
+        c->offset -= 1;
+        c->presented = c->offset;
+    }
+    return st;
 }
 
 kvhip_status kvhip_cache_mask_plan(const kvhip_cache *c, int32_t n, int32_t window, int32_t return_array,
@@ -1567,6 +1800,10 @@ kvhip_status kvhip_cache_state_export(const kvhip_cache *c, int32_t i, void *dst
         KV_HIP(e);
         return KVHIP_OK;
     }
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) {
+        KV_HIP(launch_block_fetch(block_store(c), n, i == 0 ? dst : nullptr, i == 1 ? dst : nullptr, S(c, stream)));
+        return KVHIP_OK;
+    }
     std::vector<int32_t> ident;
     const int32_t *slots = c->rows.data();
     if (c->kind != KVHIP_KIND_ROTATING) {
@@ -1631,9 +1868,17 @@ kvhip_status kvhip_cache_state_import(kvhip_cache *c, int32_t count, const void 
         probe.bits = c->bits;
         KV_TRY(set_geometry(&probe, (int)B, (int)H, Dk, Dv, dtype));
     }
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED && n > INT32_MAX / 2) return fail(KVHIP_ERR_UNSUPPORTED, "cache longer than 2^30 rows");
     // a state setter replaces the buffers wholesale (the old pages go once the work enqueued
     // on this stream so far, which may still read them, has run)
     drop_pages(c, S(c, stream), false);
+    if (c->tail) {
+        retire({{c->tail, c->tail_bytes}}, S(c, stream));
+        c->tail = nullptr;
+        c->coded = 0;
+        c->offset = c->presented = 0;
+        c->has_buffers = false;
+    }
     c->st = Store();
     c->has_geom = false;
     c->rows.clear();
@@ -1642,6 +1887,10 @@ kvhip_status kvhip_cache_state_import(kvhip_cache *c, int32_t count, const void 
     KV_TRY(set_geometry(c, (int)B, (int)H, Dk, Dv, dtype));
     hipStream_t s = S(c, stream);
     KV_TRY(ensure_slots(c, std::max<int64_t>(n, 1), s, true));
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) {
+        c->has_buffers = true;
+        return n > 0 ? update_blocks(c, srcs[0], srcs[1], (int)n, s) : ensure_tail(c);
+    }
     const void *wide_srcs[6] = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
     std::vector<std::pair<void *, size_t>> tmp;
     if (c->padded() && n > 0) {
@@ -1690,7 +1939,7 @@ kvhip_status kvhip_cache_state_import(kvhip_cache *c, int32_t count, const void 
 
 int32_t kvhip_cache_meta_count(const kvhip_cache *c) {
     if (!c) return 0;
-    return c->kind == KVHIP_KIND_SIMPLE ? 1 : (c->kind == KVHIP_KIND_ROTATING ? 6 : 4);
+    return c->kind == KVHIP_KIND_SIMPLE || c->kind == KVHIP_KIND_BLOCK_SCALED ? 1 : (c->kind == KVHIP_KIND_ROTATING ? 6 : 4);
 }
 
 int32_t kvhip_cache_meta_get(const kvhip_cache *c, int32_t i, char *buf, int32_t len) {
@@ -1722,7 +1971,7 @@ kvhip_status kvhip_cache_meta_set(kvhip_cache *c, int32_t count, const char *con
     if (!c || !values) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
     if (c->staging)  // RotatingStagedKVCache.swift:105-111
         return fail(KVHIP_ERR_STATE, "RotatingStagedKVCache is round-scoped and cannot be restored from metaState");
-    if (c->kind == KVHIP_KIND_SIMPLE) {
+    if (c->kind == KVHIP_KIND_SIMPLE || c->kind == KVHIP_KIND_BLOCK_SCALED) {
         if (count != 1 || !values[0] || values[0][0])
             return fail(KVHIP_ERR_STATE, "This cache has no meta_state but a meta_state was set.");
         return KVHIP_OK;
@@ -1777,9 +2026,16 @@ kvhip_status kvhip_cache_copy(const kvhip_cache *c, void *stream, kvhip_cache **
         kvhip_status st = set_geometry(n, c->B, c->Hkv, c->Dk_user, c->Dv_user, c->st.dtype);
         if (st == KVHIP_OK) st = ensure_slots(n, std::max<int64_t>(rows, 1), s, true);
         if (st != KVHIP_OK) { kvhip_cache_free(n); return st; }
-        if (c->kind == KVHIP_KIND_QUANTIZED) {
+        if (c->kind == KVHIP_KIND_QUANTIZED || c->kind == KVHIP_KIND_BLOCK_SCALED) {
             const int64_t pages = (rows + PAGE - 1) / PAGE;
             KV_HIP_OR(launch_copy_pages(c->st, n->st, (int)pages, s), kvhip_cache_free(n));
+            if (c->kind == KVHIP_KIND_BLOCK_SCALED) {
+                st = ensure_tail(n);
+                if (st != KVHIP_OK) { kvhip_cache_free(n); return st; }
+                BlockStore from = block_store(c), to = block_store(n);
+                KV_HIP_OR(launch_copy_bytes(to.tail_k, from.tail_k, (size_t)c->st.BH * BLOCK_ROWS * (c->st.Dk + c->st.Dv) * c->st.es, s), kvhip_cache_free(n));
+                n->coded = std::min(c->coded, (rows + BLOCK_ROWS - 1) / BLOCK_ROWS);
+            }
         } else {
             std::vector<int32_t> ident;
             const int32_t *slots = c->rows.data();

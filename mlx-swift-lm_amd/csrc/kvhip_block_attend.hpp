@@ -1,0 +1,528 @@
+// Attention over the block-scaled cache (layout: kvhip_block.hpp), whole or over listed blocks.
+//
+// A wavefront takes every NW-th block of its workgroup's part and keeps the running maximum, the sum and the output of NM
+// tiles of 16 query rows in registers: one pass over the keys and values, nothing shared until the end.
+//   S^T = K Q^T   16x16x32 products, keys as the left operand: a lane is left with the scores of query row (lane & 15) at
+//                 tokens 16 t + 4 (lane >> 4) + i
+//   O^T = V^T P^T the same lane's weights, two tiles of tokens at a time, are the right operand as they stand -- the order of
+//                 the contraction is free, so the pages hold each lane's sixteen tokens of a channel side by side
+// Codes become operands by one conversion for two values, which takes the block's scale along.  Operands are loaded straight
+// from the pages, 1 KB to an instruction; the next block's are requested before the current one's are looked at.  The blocks'
+// addresses and scales are looked up 64 at a time, a lane to a block, instead of one dependent load after another.
+#pragma once
+#include "kvhip_block.hpp"
+#include "kvhip_mask.hpp"
+#include "kvhip_span_merge.hpp"
+
+namespace kvhip {
+
+// Tiles of 16 query rows that a wavefront takes (plan_block_attend chooses by the same rule).
+inline int block_row_tiles(const BlockAttend &x) {
+    const int rows = x.a.Hq / x.a.Hkv * x.a.L;
+    if (x.list || rows <= 16) return 1;
+    if (rows <= 32 || x.a.st.Dk > 192 || x.a.mask.mode == KVHIP_MASK_ARRAY) return 2;
+    return 4;
+}
+
+namespace {
+
+typedef float kv_f4 __attribute__((ext_vector_type(4)));
+typedef __bf16 kv_b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 kv_h8 __attribute__((ext_vector_type(8)));
+
+template <int DT> __device__ __forceinline__ kv_f4 block_mfma(const kv_u4 &x, const kv_u4 &y, const kv_f4 &c) {
+    if constexpr (DT == 1) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kv_b8, x), __builtin_bit_cast(kv_b8, y), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(kv_h8, x), __builtin_bit_cast(kv_h8, y), c, 0, 0, 0);
+}
+// eight codes as eight elements
+template <int DT> __device__ __forceinline__ kv_u4 block_operand(uint32_t lo, uint32_t hi, float scale) {
+    return kv_u4{block_values<DT, false>(lo, scale), block_values<DT, true>(lo, scale), block_values<DT, false>(hi, scale), block_values<DT, true>(hi, scale)};
+}
+// over the four lanes of a query row
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float row_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// What a wavefront requests of a block: keys as [token tile][chunk of 64 channels] of 16 bytes a lane (a last chunk of 32: 8),
+// values as [16 channels] of 16 bytes.
+template <int DK, int DV> struct BlockTile {
+    static constexpr int KC = DK / 64;
+    static constexpr bool HALF = DK % 64 != 0;
+    kv_u4 k[4][KC > 0 ? KC : 1];
+    kv_u2 kh[HALF ? 4 : 1];
+    kv_u4 v[DV / 16];
+    __device__ __forceinline__ void load_keys(gptr kp, int lane) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) k[t][c] = ld_global<kv_u4>(kp + t * 16 * DK + c * 1024 + lane * 16);
+            if constexpr (HALF) kh[t] = ld_global<kv_u2>(kp + t * 16 * DK + KC * 1024 + lane * 8);
+        }
+    }
+    __device__ __forceinline__ void load_values(gptr vp, int lane) {
+#pragma unroll
+        for (int i = 0; i < DV / 16; ++i) v[i] = ld_global<kv_u4>(vp + i * 1024 + lane * 16);
+    }
+};
+
+// MODE 1: index-only mask (no mask: one that every key passes); 2: array mask; 3: listed blocks
+template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
+    static constexpr int KS = DK / 32, VT = DV / 16;
+    static constexpr bool SAFE = MODE == 2;  // an added mask may hold the type's lowest value: no products in front of the difference
+    // float16 weights are taken times 2^14: those of keys far below the largest stay clear of the type's subnormals (the sums
+    // carry the factor too)
+    static constexpr float LIFT = DT == 0 ? 14.f : 0.f;
+
+    const BlockAttend &x;
+    const int lane, g, n;
+    const int b, h, bh;
+    kv_u4 q[NM][KS];
+    kv_f4 o[NM][VT];
+    float m[NM], l[NM];
+    KeyBounds see[NM];  // the keys of the lane's query row
+    int ql[NM], qh[NM]; // its position and head (MODE 2)
+
+    __device__ __forceinline__ BlockWalk(const BlockAttend &x_, int bh_)
+        : x(x_), lane(threadIdx.x & 63), g(lane >> 4), n(lane & 15), b(bh_ / x_.a.Hkv), h(bh_ % x_.a.Hkv), bh(bh_) {
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+#pragma unroll
+            for (int d = 0; d < VT; ++d) o[i][d] = kv_f4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+
+    // scores (already scaled) of one tile of query rows -> weights as operands; the outputs so far are brought to the new maximum
+    __device__ __forceinline__ void weigh(int i, kv_f4 (&s)[4], kv_u4 (&p)[2]) {
+        float mx = m[i];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) mx = fmaxf(mx, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
+        mx = row_max(mx);
+        const float ref = mx == -INFINITY ? 0.f : mx;  // (nothing seen yet: every difference is -infinity)
+        const float off = LIFT - ref * LOG2E;
+        float e[16], sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float y = SAFE ? __builtin_fmaf(s[t][k] - ref, LOG2E, LIFT) : __builtin_fmaf(s[t][k], LOG2E, off);
+                e[4 * t + k] = fast_exp2(y);
+                sum += e[4 * t + k];
+            }
+        if (__any(mx != m[i])) {
+            const float alpha = fast_exp2((m[i] - ref) * LOG2E);
+            l[i] *= alpha;
+#pragma unroll
+            for (int d = 0; d < VT; ++d) o[i][d] *= alpha;
+            m[i] = mx;
+        }
+        l[i] += sum;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                p[u][k] = DT == 1 ? pk_bf2(e[8 * u + 2 * k], e[8 * u + 2 * k + 1]) : pk_h2(e[8 * u + 2 * k], e[8 * u + 2 * k + 1]);
+    }
+
+    // which of the lane's sixteen tokens its query row sees, those it does not see set to -infinity; adds an array mask
+    __device__ __forceinline__ uint32_t mask(int i, int j0, kv_f4 (&s)[4]) {
+        uint32_t seen = 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int j = j0 + 16 * t + 4 * g + k;
+                bool keep;
+                if constexpr (MODE == 2) {
+                    float add = 0.f;
+                    keep = j < x.a.T && qh[i] >= 0 && mask_keep(x.a.mask, b, qh[i], ql[i], j, x.a.L, x.a.T, add);
+                    keep = keep && add != -INFINITY;
+                    s[t][k] += add;
+                } else {
+                    keep = see[i].keep(j);
+                }
+                if (!keep) s[t][k] = -INFINITY;
+                seen |= keep ? 1u << (4 * t + k) : 0u;
+            }
+        return seen;
+    }
+
+    // Values of a block with keys that some query row does not see: a weight of zero does not take a NaN away.  NaN become
+    // zeros, and channels that a seen token has NaN in are made NaN by a product of the two facts.  `bad`: 1 in the place of
+    // each NaN, 0 elsewhere.
+    __device__ __forceinline__ void poison(int i, int d, uint32_t seen, const kv_u4 (&bad)[2]) {
+        constexpr uint32_t ONE = DT == 1 ? 0x3f80u : 0x3c00u;
+        kv_f4 hit{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            kv_u4 w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                w[k] = ((seen >> (8 * u + 2 * k)) & 1u ? ONE : 0u) | ((seen >> (8 * u + 2 * k + 1)) & 1u ? ONE << 16 : 0u);
+            hit = block_mfma<DT>(bad[u], w, hit);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (hit[k] > 0.f) o[i][d][k] = __builtin_nanf("");
+    }
+
+    // a block of codes
+    __device__ __forceinline__ void block(BlockTile<DK, DV> &tile, float ks, float vs, int j0, bool masked) {
+        using Tile = BlockTile<DK, DV>;
+        kv_f4 s[NM][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int i = 0; i < NM; ++i) s[i][t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KS; ++c) {
+                kv_u4 w;
+                if (Tile::HALF && c == KS - 1) w = block_operand<DT>(tile.kh[t][0], tile.kh[t][1], ks);
+                else w = block_operand<DT>(tile.k[t][c >> 1][2 * (c & 1)], tile.k[t][c >> 1][2 * (c & 1) + 1], ks);
+#pragma unroll
+                for (int i = 0; i < NM; ++i) s[i][t] = block_mfma<DT>(w, q[i][c], s[i][t]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        kv_u4 p[NM][2];
+        uint32_t seen[NM];
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) s[i][t] *= x.a.scale;
+            seen[i] = 0xffffu;
+            if (masked) seen[i] = mask(i, j0, s[i]);
+            weigh(i, s[i], p[i]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (masked) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int d = 0; d < VT; ++d)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) any |= nan_codes(tile.v[d][k]);
+            if (__any(any != 0)) {
+#pragma unroll
+                for (int d = 0; d < VT; ++d) {
+                    kv_u4 bad[2];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t f = nan_codes(tile.v[d][k]) >> 7, one = f * 0x38u;  // 1.0
+                        tile.v[d][k] &= ~(f * 0xffu);
+                        bad[k >> 1][2 * (k & 1)] = block_values<DT, false>(one, 1.f);
+                        bad[k >> 1][2 * (k & 1) + 1] = block_values<DT, true>(one, 1.f);
+                    }
+#pragma unroll
+                    for (int i = 0; i < NM; ++i) poison(i, d, seen[i], bad);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < VT; ++d) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const kv_u4 a = block_operand<DT>(tile.v[d][2 * u], tile.v[d][2 * u + 1], vs);
+#pragma unroll
+                for (int i = 0; i < NM; ++i) o[i][d] = block_mfma<DT>(a, p[i][u], o[i][d]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // bit 7 of every byte of a word that is a NaN code
+    static __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+    // the rows of the unfinished block; with a.new_k its last row is still in the caller's arrays
+    __device__ __forceinline__ void tail(int j0) {
+        const AttendArgs &a = x.a;
+        const char *tk = x.b.tail_k + (size_t)bh * BLOCK_ROWS * DK * 2, *tv = x.b.tail_v + (size_t)bh * BLOCK_ROWS * DV * 2;
+        const int fresh = a.new_k ? a.T - 1 - j0 : -1;  // that row
+        const char *nk = static_cast<const char *>(a.new_k) + (size_t)bh * DK * 2;
+        const uint16_t *nv = static_cast<const uint16_t *>(a.new_v) + (size_t)bh * DV;
+        kv_f4 s[NM][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int r = 16 * t + n;
+            const char *row = r == fresh ? nk : tk + (size_t)r * DK * 2;
+#pragma unroll
+            for (int i = 0; i < NM; ++i) s[i][t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KS; ++c) {
+                // the channels that the query operands hold at this step (those of a block's chunks)
+                const int d = (c | 1) < KS ? (c >> 1) * 64 + g * 16 + (c & 1) * 8 : c * 32 + g * 8;
+                kv_u4 w = load_row16(row + 2 * d);
+                if (fresh >= 0) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[k] = no_infinities<DT>(w[k]);
+                }
+#pragma unroll
+                for (int i = 0; i < NM; ++i) s[i][t] = block_mfma<DT>(w, q[i][c], s[i][t]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        kv_u4 p[NM][2];
+        uint32_t seen[NM];
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) s[i][t] *= a.scale;
+            seen[i] = mask(i, j0, s[i]);
+            weigh(i, s[i], p[i]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        constexpr uint32_t INF = DT == 1 ? 0x7f80u : 0x7c00u, ONE = DT == 1 ? 0x3f80u : 0x3c00u;
+#pragma unroll
+        for (int d = 0; d < VT; ++d) {
+            const int col = 16 * d + n;
+            kv_u4 w[2], bad[2];
+            bool nan = false;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                w[u] = *reinterpret_cast<const kv_u4 *>(tv + ((size_t)(4 * u + g) * DV + col) * 16);
+                // (element 4 h + i is token 32 u + 16 h + 4 g + i)
+                if (fresh >= 0 && (fresh >> 5) == u && ((fresh >> 2) & 3) == g) {
+                    const int at = ((fresh >> 4) & 1) * 4 + (fresh & 3);
+                    const uint32_t e = no_infinities<DT>((uint32_t)nv[col]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if ((at >> 1) == k) w[u][k] = at & 1 ? (w[u][k] & 0xffffu) | (e << 16) : (w[u][k] & 0xffff0000u) | e;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    // (rows that were never written hold anything, infinities too)
+                    const bool lo = (w[u][k] & 0x7fffu) >= INF, hi = ((w[u][k] >> 16) & 0x7fffu) >= INF;
+                    bad[u][k] = (lo ? ONE : 0u) | (hi ? ONE << 16 : 0u);
+                    w[u][k] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+                    nan = nan || lo || hi;
+                }
+            }
+            if (__any(nan)) {
+#pragma unroll
+                for (int i = 0; i < NM; ++i) poison(i, d, seen[i], bad);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < NM; ++i) o[i][d] = block_mfma<DT>(w[u], p[i][u], o[i][d]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
+
+// grid (BH, tiles of query rows, parts), NW wavefronts.  MODE 3: (BH, tokens x tiles of heads, parts).
+template <int DK, int DV, int DT, int NM, int MODE, int NW>
+__global__ void __launch_bounds__(NW * 64, NM == 1 && DK <= 128 ? 2 : 1) block_attend_kernel(BlockAttend x) {
+    using Walk = BlockWalk<DK, DV, DT, NM, MODE, NW>;
+    using Tile = BlockTile<DK, DV>;
+    __shared__ WaveParts<DV, NW, 16> parts;
+    const AttendArgs &a = x.a;
+    const int bh = blockIdx.x, part = blockIdx.z;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int G = a.Hq / a.Hkv, R = MODE == 3 ? G : G * a.L;       // rows that the tiles of blockIdx.y cut
+    const int token = MODE == 3 ? blockIdx.y / x.tiles : 0;
+    const int row0 = (MODE == 3 ? blockIdx.y % x.tiles : blockIdx.y) * 16 * NM;
+    Walk w(x, bh);
+    // row i of a pair's query rows: head i / L, position i % L; a token's rows lie L apart
+    auto row_at = [&](int i) { return MODE == 3 ? i * a.L + token : i; };
+
+    // queries, and what their rows see
+    const SymMask sym = sym_mask_init(a.mask, w.b, a.L, a.T);
+    int in_lo = 0, in_hi = a.T - 1;  // keys that every row sees
+    int lo = 0, hi = a.T - 1;        // keys that some row sees
+    if constexpr (MODE == 1) {
+        const int last = min(row0 + 16 * NM, R) - 1;
+        const bool one_head = row0 / a.L == last / a.L;
+        const KeyBounds f = sym_mask_bounds(sym, one_head ? row0 % a.L : 0), e = sym_mask_bounds(sym, one_head ? last % a.L : a.L - 1);
+        in_lo = max(e.lo, 0);
+        in_hi = min(f.hi, a.T - 1);
+        lo = max(f.lo, 0);
+        hi = min(e.hi, a.T - 1);
+    }
+    if constexpr (MODE == 3) {
+        lo = in_lo = x.left_pad ? max(x.left_pad[w.b], 0) : 0;
+        hi = in_hi = a.T - a.L + token;
+    }
+    const char *qbase = static_cast<const char *>(a.q) + (size_t)bh * G * a.L * DK * 2;
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+        const int r = row0 + 16 * i + w.n;
+        const bool live = r < R;
+        const char *row = qbase + (size_t)row_at(live ? r : 0) * DK * 2;
+#pragma unroll
+        for (int c = 0; c < Walk::KS; ++c) {
+            const int d = (c | 1) < Walk::KS ? (c >> 1) * 64 + w.g * 16 + (c & 1) * 8 : c * 32 + w.g * 8;
+            w.q[i][c] = live ? load_row16(row + 2 * d) : kv_u4{0u, 0u, 0u, 0u};
+        }
+        w.ql[i] = live ? r % a.L : 0;
+        w.qh[i] = live ? w.h * G + r / a.L : -1;
+        w.see[i] = KeyBounds{lo, hi};
+        if constexpr (MODE == 1) {
+            const KeyBounds k = sym_mask_bounds(sym, w.ql[i]);
+            w.see[i] = KeyBounds{max(k.lo, 0), min(k.hi, a.T - 1)};
+        }
+    }
+
+    // the blocks of this part: positions [s0, s1) of the row's blocks, or of its list
+    const int first = MODE == 3 ? 0 : lo / BLOCK_ROWS;
+    const int total = MODE == 3 ? x.count : hi < lo ? 0 : hi / BLOCK_ROWS - first + 1;
+    const int each = (total + x.nsplit - 1) / x.nsplit;
+    const int s0 = min(part * each, total), s1 = min(s0 + each, total);
+    const int mine = s1 - s0 > wave ? (s1 - s0 - wave + NW - 1) / NW : 0;
+    const int32_t *list = MODE == 3 ? x.list + ((size_t)bh * a.L + token) * x.count : nullptr;
+    int tail_at = -1;
+
+    for (int at = 0; at < mine; at += 64) {
+        // a lane to a block: where it lies and its scales
+        const int turn = min(mine - at, 64);
+        const int i = s0 + wave + NW * (at + lane);
+        int blk = -1;
+        if (lane < turn) {
+            if constexpr (MODE == 3) {
+                blk = list[i];
+                const int before = i > 0 ? list[i - 1] : -1;
+                if (blk < lo / BLOCK_ROWS || blk > (hi < lo ? -1 : hi / BLOCK_ROWS) || (i > 0 && before >= blk)) blk = -1;
+            } else {
+                blk = first + i;
+            }
+        }
+        uint64_t kp = 0, vp = 0;
+        float ks = 1.f, vs = 1.f;
+        if (blk >= 0 && blk < x.b.coded) {
+            const PageEntry &e = a.st.pt[blk / BLOCK_PER_PAGE];
+            const int in_page = blk % BLOCK_PER_PAGE;
+            kp = reinterpret_cast<uint64_t>(e.k + (size_t)bh * a.st.k_cell + (size_t)in_page * BLOCK_ROWS * DK);
+            vp = reinterpret_cast<uint64_t>(e.v + (size_t)bh * a.st.v_cell + (size_t)in_page * BLOCK_ROWS * DV);
+            const kv_f2 sc = *reinterpret_cast<const kv_f2 *>(e.ksb + (size_t)bh * a.st.ksb_cell + in_page * 8);
+            ks = sc.x;
+            vs = sc.y;
+        }
+        const uint64_t open = __ballot(blk >= 0 && blk >= x.b.coded);
+        if (open) tail_at = __builtin_amdgcn_readlane(blk, __builtin_ctzll(open)) * BLOCK_ROWS;
+        uint64_t todo = __ballot(blk >= 0 && blk < x.b.coded);
+        auto at_lane = [](uint64_t v, int of) {  // (readlane returns a signed number)
+            const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, of), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), of);
+            return (gptr)(((uint64_t)hi << 32) | lo);
+        };
+        auto use = [&](Tile &t, int of) {
+            const float k = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), of));
+            const float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), of));
+            const int j0 = __builtin_amdgcn_readlane(blk, of) * BLOCK_ROWS;
+            w.block(t, k, v, j0, MODE == 2 || j0 < in_lo || j0 + BLOCK_ROWS - 1 > in_hi);
+        };
+        if (!todo) continue;
+        // One tile of rows: the next block's keys and values are requested ahead.  More: its keys, and the values of the current
+        // one, which have the score product and the weights in front of them.
+        Tile tile;
+        int cur = __builtin_ctzll(todo);
+        tile.load_keys(at_lane(kp, cur), lane);
+        if (NM == 1) tile.load_values(at_lane(vp, cur), lane);
+        while (true) {
+            todo &= todo - 1;
+            Tile next;
+            const int then = todo ? __builtin_ctzll(todo) : cur;
+            if (NM > 1) tile.load_values(at_lane(vp, cur), lane);
+            if (todo) {
+                next.load_keys(at_lane(kp, then), lane);
+                if (NM == 1) next.load_values(at_lane(vp, then), lane);
+            }
+            use(tile, cur);
+            if (!todo) break;
+            tile = next;
+            cur = then;
+        }
+    }
+    if (tail_at >= 0) w.tail(tail_at);
+
+    // a single token's row, still in the caller's arrays, into the tail (its reader above takes it from there as well)
+    if (a.new_k && blockIdx.y == 0 && part == 0 && wave == NW - 1) {
+        const int r = (a.T - 1) % BLOCK_ROWS;
+        const uint16_t *nk = static_cast<const uint16_t *>(a.new_k) + (size_t)bh * DK, *nv = static_cast<const uint16_t *>(a.new_v) + (size_t)bh * DV;
+        uint16_t *tk = reinterpret_cast<uint16_t *>(x.b.tail_k) + ((size_t)bh * BLOCK_ROWS + r) * DK;
+        uint16_t *tv = reinterpret_cast<uint16_t *>(x.b.tail_v) + (size_t)bh * BLOCK_ROWS * DV;
+        for (int d = lane; d < DK; d += 64) tk[d] = (uint16_t)no_infinities<DT>(nk[d]);
+        for (int d = lane; d < DV; d += 64) tv[tail_v_at(DV, r, d)] = (uint16_t)no_infinities<DT>(nv[d]);
+    }
+
+    // the wavefronts' parts joined, 16 rows at a time
+    const bool whole = x.nsplit == 1;
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+        const int rows = min(R - (row0 + 16 * i), 16);
+        if (rows <= 0) break;
+        if (i) __syncthreads();
+        const float l = row_sum(w.l[i]);
+        if (w.g == 0) parts.m[wave][w.n] = w.m[i];
+        __syncthreads();
+        const float weight = wave_weight(parts, w.n, w.m[i]);
+        if (w.g == 0) parts.l[wave][w.n] = l * weight;
+#pragma unroll
+        for (int d = 0; d < Walk::VT; ++d)
+            *reinterpret_cast<kv_f4 *>(&parts.rows[wave][w.n][16 * d + 4 * w.g]) = w.o[i][d] * weight;
+        __syncthreads();
+        constexpr int LPR = DV / 4, RPB = NW * 64 / LPR;
+        const int c = 4 * (threadIdx.x % LPR);
+        if (threadIdx.x >= RPB * LPR) continue;  // (96 columns: lanes left over)
+        for (int r = threadIdx.x / LPR; r < rows; r += RPB) {
+            float v[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < NW; ++k) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) v[d] += parts.rows[k][r][c + d];
+                sum += parts.l[k][r];
+            }
+            const int at = row_at(row0 + 16 * i + r);
+            const size_t all = (size_t)G * a.L;
+            if (whole) {
+                const float inv = 1.f / sum;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) v[d] = sum == 0.f ? 0.f : v[d] * inv;
+                store_columns<DT>(a.out, ((size_t)bh * all + at) * DV + c, v);
+            } else {
+                float *to = a.workspace + (((size_t)bh * x.nsplit + part) * all + at) * (DV + 2);
+                store_floats(to + c, v);
+                if (c == 0) {
+                    float mx = parts.m[0][r];
+#pragma unroll
+                    for (int k = 1; k < NW; ++k) mx = fmaxf(mx, parts.m[k][r]);
+                    *reinterpret_cast<kv_f2 *>(to + DV) = kv_f2{mx, sum};
+                }
+            }
+        }
+    }
+}
+
+template <int DK, int DV, int DT, int NM, int MODE> hipError_t block_attend_run(const BlockAttend &x, hipStream_t stream) {
+    constexpr int NW = 4;
+    hipLaunchKernelGGL((block_attend_kernel<DK, DV, DT, NM, MODE, NW>), dim3(x.a.st.BH, block_attend_rows(x), x.nsplit), dim3(NW * 64), 0, stream, x);
+    return hipGetLastError();
+}
+template <int DK, int DV, int DT> hipError_t block_attend_shape(const BlockAttend &x, hipStream_t stream) {
+    if (x.list) return block_attend_run<DK, DV, DT, 1, 3>(x, stream);
+    const int nm = block_row_tiles(x);
+    if (x.a.mask.mode == KVHIP_MASK_ARRAY)
+        return nm == 1 ? block_attend_run<DK, DV, DT, 1, 2>(x, stream) : block_attend_run<DK, DV, DT, 2, 2>(x, stream);
+    if (nm == 1) return block_attend_run<DK, DV, DT, 1, 1>(x, stream);
+    if constexpr (DK <= 192) {
+        if (nm == 4) return block_attend_run<DK, DV, DT, 4, 1>(x, stream);
+    }
+    return block_attend_run<DK, DV, DT, 2, 1>(x, stream);
+}
+template <int DT> hipError_t block_attend_dtype(const BlockAttend &x, hipStream_t stream) {
+    const int dk = x.a.st.Dk, dv = x.a.st.Dv;
+    if (dk == 64 && dv == 64) return block_attend_shape<64, 64, DT>(x, stream);
+    if (dk == 96 && dv == 96) return block_attend_shape<96, 96, DT>(x, stream);
+    if (dk == 128 && dv == 128) return block_attend_shape<128, 128, DT>(x, stream);
+    if (dk == 192 && dv == 128) return block_attend_shape<192, 128, DT>(x, stream);
+    if (dk == 256 && dv == 256) return block_attend_shape<256, 256, DT>(x, stream);
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+}  // namespace kvhip

@@ -1,7 +1,8 @@
 """kvhip: MI355X (gfx950) KV-cache hot path behind the reference's KVCache surface."""
 from ._lib import KVHipError, LIB_PATH, SIGNATURES, load  # noqa: F401
-from .attention import attention_with_cache_update, quantized_scaled_dot_product_attention  # noqa: F401
-from .cache import (KVCacheSimple, MaskMode, QuantizedKVCache, RotatingKVCache, affine_dequantize,  # noqa: F401
+from .attention import (attention_with_cache_update, quantized_scaled_dot_product_attention,  # noqa: F401
+                        sparse_attention_with_cache_update)
+from .cache import (BlockScaledKVCache, KVCacheSimple, MaskMode, QuantizedKVCache, RotatingKVCache, affine_dequantize,  # noqa: F401
                     affine_quantize, can_trim_prompt_cache, create_attention_mask,
                     KVCacheConfigurationError, make_attention_kv_cache, make_prompt_cache,
                     make_sliding_window_kv_cache,

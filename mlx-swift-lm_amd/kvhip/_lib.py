@@ -12,7 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libkvhip.so")
 
 OK, ERR_UNSUPPORTED = 0, -3
-KIND_SIMPLE, KIND_ROTATING, KIND_QUANTIZED = 0, 1, 2
+KIND_SIMPLE, KIND_ROTATING, KIND_QUANTIZED, KIND_BLOCK_SCALED = 0, 1, 2, 3
 F16, BF16, F32, U32, BOOL = 0, 1, 2, 3, 4
 MASK_NONE, MASK_CAUSAL, MASK_ARRAY, MASK_WINDOW = 0, 1, 2, 3
 
@@ -84,6 +84,10 @@ SIGNATURES = {
     "kvhip_cache_attend_static": (_I32, [_P, _P, _I32, _I32, _I32, _I32, _F, C.POINTER(Mask), _P, _P]),
     "kvhip_cache_update_attend": (_I32, [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F,
                                          C.POINTER(Mask), _P, _P]),
+    "kvhip_cache_select_blocks": (_I32, [_P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P, _P]),
+    "kvhip_cache_attend_blocks": (_I32, [_P, _P, _I32, _I32, _I32, _I32, _F, _P, _I32, _P, _P, _P]),
+    "kvhip_cache_update_attend_blocks": (_I32, [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F, _I32, _I32, _I32,
+                                                _P, _P, _P, _P]),
     "kvhip_cache_mask_plan": (_I32, [_P, _I32, _I32, _I32, C.POINTER(MaskPlan)]),
     "kvhip_mask_materialize": (_I32, [C.POINTER(MaskPlan), _P, _P]),
     "kvhip_cache_state_count": (_I32, [_P]),

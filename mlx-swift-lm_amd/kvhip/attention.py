@@ -1,7 +1,7 @@
 """`attentionWithCacheUpdate` (AttentionUtils.swift:37-95) over libkvhip caches."""
 from __future__ import annotations
 
-from .cache import MaskMode, QuantizedKVCache
+from .cache import BlockScaledKVCache, MaskMode, QuantizedKVCache
 
 
 def attention_with_cache_update(queries, keys, values, cache, scale, mask=None):
@@ -20,3 +20,9 @@ def quantized_scaled_dot_product_attention(queries, cache: QuantizedKVCache, sca
     """`quantizedScaledDotProductAttention` (KVCache.swift:2351-2447) over the rows
     `cache` already holds (the quantized tuples stay in device pages)."""
     return cache.attend(queries, scale, mask or MaskMode.none())
+
+
+def sparse_attention_with_cache_update(queries, keys, values, cache: BlockScaledKVCache, scale, count, first=1, recent=1, left_pad=None):
+    """Update `cache` and attend over `count` blocks of 64 positions that each token chooses: [B,Hq,L,Dv].  Runs as one C-ABI
+    call, kvhip_cache_update_attend_blocks; no counterpart in the reference."""
+    return cache.update_attend_blocks(queries, keys, values, scale, count, first, recent, left_pad)[0]

@@ -479,6 +479,85 @@ class QuantizedKVCache(_Cache):
         return s
 
 
+class BlockScaledKVCache(KVCacheSimple):
+    """A `KVCacheSimple` to its caller that holds its rows in 8 bits: blocks of 64 positions of one kv head as e4m3 codes with
+    a power of two as their scale, the rows behind the last whole block as they came.  No counterpart in the reference.
+    float16 and bfloat16, head sizes up to 256.  `update` and `fetch` hand out the rows as they are held; `state` likewise."""
+    kind = L.KIND_BLOCK_SCALED
+    block_rows = 64
+
+    def __init__(self, handle=None):
+        _Cache.__init__(self, handle=handle)
+
+    def to_quantized(self, group_size=64, bits=4):
+        raise TypeError("`to_quantized` belongs to `KVCacheSimple`: a BlockScaledKVCache is quantized")
+
+    def _block_arguments(self, queries, blocks, left_pad):
+        """The arrays of a call over blocks, looked over."""
+        q, dev = queries.contiguous(), torch._C._cuda_getDevice()
+        self._check_query_dtype(q)
+        if q.dim() != 4:
+            raise ValueError(f"queries are [B, Hq, L, D], not {tuple(q.shape)}")
+        if left_pad is not None:
+            left_pad = left_pad.to(device="cuda", dtype=torch.int32).contiguous()
+            if tuple(left_pad.shape) != (q.shape[0],):
+                raise ValueError(f"left_pad is one number to each of {q.shape[0]} sequences, not {tuple(left_pad.shape)}")
+        for t in (q, blocks, left_pad):
+            if t is not None and (not t.is_cuda or t.device.index != dev):
+                raise ValueError(f"an array lies on {t.device}, the current device is cuda:{dev}")
+        return q, left_pad
+
+    def _new_blocks(self, q, kv_heads, count):
+        return torch.empty((q.shape[0], kv_heads, q.shape[2], max(int(count), 0)), dtype=torch.int32, device=q.device)
+
+    def select_blocks(self, queries, count, first=1, recent=1, left_pad=None):
+        """`count` blocks of 64 cached positions for each token of `queries` [B,Hq,L,D], which are the last L positions, and each
+        kv head: int32 [B,Hkv,L,count], ascending, -1 behind the last.  The `first` leading and `recent` last blocks that the
+        token sees are always chosen, the others by a bound on the scores of their keys.  `left_pad` [B]: positions
+        that hold no tokens in front of each sequence."""
+        q, pad = self._block_arguments(queries, None, left_pad)
+        B, Hq, Lq, D = q.shape
+        out = self._new_blocks(q, self._shape[1] if self._shape else 1, count)
+        L.check(self._lib.kvhip_cache_select_blocks(self._h, _ptr(q), B, Hq, Lq, D, int(count), int(first), int(recent),
+                                                    _ptr(pad) if pad is not None else None, _ptr(out), _stream()))
+        return out
+
+    def attend_blocks(self, queries, blocks, scale, left_pad=None):
+        """Attention of each token over the blocks listed for it (`select_blocks`), at positions up to its own and from
+        `left_pad` on: [B,Hq,L,Dv]."""
+        if blocks.dtype != torch.int32 or blocks.dim() != 4:
+            raise ValueError(f"blocks are int32 [B, Hkv, L, count], not {blocks.dtype} {tuple(blocks.shape)}")
+        blocks = blocks.contiguous()
+        q, pad = self._block_arguments(queries, blocks, left_pad)
+        B, Hq, Lq, D = q.shape
+        if self._shape is None:
+            raise ValueError("the cache holds nothing yet")
+        if tuple(blocks.shape[:3]) != (B, self._shape[1], Lq):
+            raise ValueError(f"blocks {tuple(blocks.shape)} do not go with queries {tuple(q.shape)}")
+        out = torch.empty((B, Hq, Lq, self._shape[3]), dtype=q.dtype, device=q.device)
+        L.check(self._lib.kvhip_cache_attend_blocks(self._h, _ptr(q), B, Hq, Lq, D, float(scale), _ptr(blocks), blocks.shape[3],
+                                                    _ptr(pad) if pad is not None else None, _ptr(out), _stream()))
+        return out
+
+    def update_attend_blocks(self, queries, keys, values, scale, count, first=1, recent=1, left_pad=None):
+        """`update`, `select_blocks` and `attend_blocks` in one call: (outputs, blocks)."""
+        k, v = keys.contiguous(), values.contiguous()
+        self._check_query_dtype(queries, k)
+        q, pad = self._block_arguments(queries, k, left_pad)
+        if not v.is_cuda or v.device != k.device or v.dtype != k.dtype:
+            raise ValueError("keys and values do not go together")
+        B, Hq, Lq, D = q.shape
+        if k.shape != (B, k.shape[1], Lq, D) or tuple(v.shape[:3]) != tuple(k.shape[:3]):
+            raise ValueError(f"queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not go together")
+        out = torch.empty((B, Hq, Lq, v.shape[3]), dtype=q.dtype, device=q.device)
+        blocks = self._new_blocks(q, k.shape[1], count)
+        L.check(self._lib.kvhip_cache_update_attend_blocks(
+            self._h, _ptr(q), _ptr(k), _ptr(v), B, Hq, k.shape[1], Lq, D, v.shape[3], _DT[k.dtype], float(scale), int(count), int(first),
+            int(recent), _ptr(pad) if pad is not None else None, _ptr(blocks), _ptr(out), _stream()))
+        self._note_shape(k, v)
+        return out, blocks
+
+
 def resolved_kv_quantization_group_size(requested, key_head_dim, value_head_dim):
     """`resolvedKVQuantizationGroupSize` (KVCache.swift:902-920)."""
     g = L.load().kvhip_resolved_group_size(requested, key_head_dim, value_head_dim)

@@ -1,0 +1,524 @@
+"""The block-scaled cache, attention over it and over chosen blocks, against oracle/block_scaled.py in float64."""
+import numpy as np
+import pytest
+import torch
+
+import kvhip
+from kvhip import _lib as L
+from oracle import block_scaled as O
+from util import NAME, np32, randn
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+INF, NAN = float("inf"), float("nan")
+# (key size, value size): those that the kernels are built for, and others that are stored padded
+SIZES = [(64, 64), (96, 96), (128, 128), (256, 256), (192, 128), (80, 80), (50, 36), (112, 72)]
+
+
+def pair(dtype, rng, B=2, H=2, sizes=(128, 128)):
+    return lambda n: tuple(randn(rng, (B, H, n, d), dtype, 2.0) for d in sizes)
+
+
+def fill(cache, oracle, make, lengths):
+    for n in lengths:
+        (k, kd), (v, vd) = make(n)
+        cache.update(kd, vd, fetch=False)
+        oracle.update(k, v)
+
+
+def check_rows(cache, oracle):
+    assert cache.offset == cache.presented_length == oracle.offset
+    for got, want in zip(cache.fetch(), (oracle.keys, oracle.values)):
+        assert np.array_equal(np32(got).astype(np.float64), want, equal_nan=True)
+
+
+# ---- write and read back ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("sizes", SIZES)
+@pytest.mark.parametrize("lengths", [[1], [63, 1], [64], [65], [5, 190, 64, 1], [130, 126]])
+def test_rows_are_read_back_by_the_definition(dtype, sizes, lengths):
+    rng = np.random.default_rng(sum(lengths) + sizes[0])
+    cache, oracle = kvhip.BlockScaledKVCache(), O.BlockScaledCache(NAME[dtype])
+    fill(cache, oracle, pair(dtype, rng, sizes=sizes), lengths)
+    check_rows(cache, oracle)
+
+
+def test_rows_do_not_depend_on_how_many_came_together():
+    make = pair(BF16, np.random.default_rng(3))
+    (_, k), (_, v) = make(300)
+    one, many = kvhip.BlockScaledKVCache(), kvhip.BlockScaledKVCache()
+    one.update(k, v, fetch=False)
+    at = 0
+    for n in [1, 2, 60, 1, 1, 100, 64, 7, 63, 1]:
+        many.update(k[:, :, at:at + n], v[:, :, at:at + n], fetch=False)
+        at += n
+    assert at == 300
+    for a, b in zip(one.fetch(), many.fetch()):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_edges_of_the_codes(dtype):
+    """Zeros, the steps at 448 and at powers of two, ties, the type's largest and smallest values, infinities and NaN."""
+    x = np.zeros((1, 1, 8 * 64, 64), np.float32)
+    blocks = x[0, 0].reshape(8, 64, 64)
+    top = float(torch.finfo(dtype).max)
+    blocks[1, :, :8] = [448, 1, -1, 0.0625, 2.0 ** -9, 2.0 ** -10, 3 * 2.0 ** -10, -448]
+    blocks[2, 3, :6] = [225, 232, 17, 19, 21, -17]                  # ties of four bits, both ways
+    blocks[3, 5, :4] = [top, -top, 1.0, top / 2]
+    blocks[4, :, :3] = float(torch.finfo(dtype).tiny) * 2.0 ** (-8 if dtype == F16 else -5)
+    blocks[4, 0, :1] = float(torch.finfo(dtype).tiny)
+    blocks[5, 7, :5] = [INF, -INF, NAN, 3.0, -5.0]
+    blocks[6] = NAN
+    blocks[7, 0, 0], blocks[7, 1, 1] = 1.75, 1.7578125              # the scale's step
+    k = torch.from_numpy(x).to(dtype)
+    cache, oracle = kvhip.BlockScaledKVCache(), O.BlockScaledCache(NAME[dtype])
+    cache.update(k.cuda(), k.flip(3).contiguous().cuda(), fetch=False)
+    oracle.update(k.double().numpy(), k.flip(3).double().numpy())
+    check_rows(cache, oracle)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("sizes", [(64, 64), (192, 128), (50, 36)])
+@pytest.mark.parametrize("lengths,cut", [([200], 3), ([200], 72), ([200], 8), ([200], 136), ([128], 1), ([128], 128), ([70, 70], 100)])
+def test_trimmed_rows_are_written_again(dtype, sizes, lengths, cut):
+    rng = np.random.default_rng(cut)
+    make = pair(dtype, rng, sizes=sizes)
+    cache, oracle = kvhip.BlockScaledKVCache(), O.BlockScaledCache(NAME[dtype])
+    fill(cache, oracle, make, lengths)
+    assert cache.trim(cut) == cut
+    oracle.trim(cut)
+    if oracle.offset:
+        check_rows(cache, oracle)
+    for n in (1, 2, 61, 70):
+        fill(cache, oracle, make, [n])
+        check_rows(cache, oracle)
+
+
+def test_values_read_back_are_stored_the_same():
+    """Also those of a block whose scale shrinks because its largest value rounded down to 224 scales."""
+    for dtype in (F16, BF16):
+        gen = torch.Generator(device="cuda").manual_seed(7)
+        k = (torch.randn(2, 2, 640, 64, generator=gen, device="cuda") * 10).to(dtype)
+        k[0, 0, :64] = k[0, 0, :64].clamp(-1, 1)
+        k[0, 0, 5, 5] = 228.0 / 128
+        cache = kvhip.BlockScaledKVCache()
+        a, b = cache.update(k, -k)
+        again = kvhip.BlockScaledKVCache()
+        c, d = again.update(a, b)
+        assert torch.equal(a, c) and torch.equal(b, d)
+
+
+def test_state_copy_and_trim():
+    make = pair(BF16, np.random.default_rng(11), sizes=(112, 72))
+    cache, oracle = kvhip.BlockScaledKVCache(), O.BlockScaledCache("bfloat16")
+    assert cache.state == [] and cache.meta_state == [""] and cache.is_trimmable
+    fill(cache, oracle, make, [150])
+    other = cache.copy()
+    restored = kvhip.BlockScaledKVCache()
+    restored.state, restored.meta_state = cache.state, [""]
+    for c in (other, restored):
+        check_rows(c, oracle)
+    cache.trim(100)
+    fill(cache, O.BlockScaledCache("bfloat16"), make, [3])
+    check_rows(other, oracle)  # (a copy of its own)
+    fill(other, oracle, make, [60])
+    check_rows(other, oracle)
+    assert other.trim(-5) == 0 and other.trim(1000) == 210 and other.offset == 0
+    with pytest.raises(kvhip.KVHipError):
+        other.offset = 10
+    fresh = O.BlockScaledCache("bfloat16")
+    fill(other, fresh, make, [66])
+    check_rows(other, fresh)
+
+
+def test_saved_as_full_precision(tmp_path):
+    """A prompt-cache file holds the rows as they are read back, under the class that the reference knows."""
+    make = pair(BF16, np.random.default_rng(5))
+    cache, oracle = kvhip.BlockScaledKVCache(), O.BlockScaledCache("bfloat16")
+    fill(cache, oracle, make, [100])
+    kvhip.save_prompt_cache(tmp_path / "c.safetensors", [cache], {"a": "b"})
+    (loaded,), meta = kvhip.load_prompt_cache(tmp_path / "c.safetensors")
+    assert type(loaded) is kvhip.KVCacheSimple and meta == {"a": "b"}
+    for a, b in zip(loaded.state, cache.state):
+        assert torch.equal(a, b)
+
+
+# ---- attention ------------------------------------------------------------------------------------------------------
+def exact_and_bound(q, oracle, scale, weight, add=None):
+    """Attention in float64 over the rows that the cache holds, and how far the kernel's result may lie from it.
+
+    weight [B, 1 or Hkv or Hq, L, T]: how often a key counts.  The kernel's errors, each by its own bound (u: half a step):
+      - a score's float32 sum of D products (exact each: 8 and 4 bits) and its scaling: (D + 2) 2^-24 sum |q k| scale, and the
+        exponent's argument and value: 2^-22 (|s - max| + 1); both relative to the weight, so e = their sum
+      - a weight rounded to the cache's type: u of that type, relative
+      - the sums over T keys and the joining of parts: (T + 64) 2^-24, relative to sum w |v|
+      - the output's rounding: u of the type.
+    So |error| <= u |o| + (u + 2 e + 2 (T + 64) 2^-24) sum w |v|  (e twice and the sums twice: numerator and denominator)."""
+    B, Hq, n, D = q.shape
+    k, v = oracle.keys, oracle.values
+    Hkv, T = k.shape[1], k.shape[2]
+    G = Hq // Hkv
+    q = q.astype(np.float64)
+    out, bound = np.zeros((B, Hq, n, v.shape[3])), np.zeros((B, Hq, n, v.shape[3]))
+    u = (2.0 ** -11 if oracle.dtype == "float16" else 2.0 ** -8)
+    for b in range(B):
+        for hq in range(Hq):
+            h = hq // G
+            w = weight[b, {1: 0, Hkv: h}.get(weight.shape[1], hq)]
+            s = q[b, hq] @ k[b, h].T * scale
+            size = np.abs(q[b, hq]) @ np.abs(k[b, h]).T * scale
+            if add is not None:
+                s = s + add[b, hq]
+                size = size + np.where(np.isfinite(add[b, hq]), np.abs(add[b, hq]), 0.0)
+            s = np.where(w > 0, s, -np.inf)
+            top = s.max(-1, keepdims=True)
+            top = np.where(np.isfinite(top), top, 0.0)
+            p = np.exp(s - top) * w
+            total = p.sum(-1, keepdims=True)
+            p = p / np.where(total > 0, total, 1.0)
+            far = np.where(p > 0, top - s, 0.0)
+            e = (D + 2) * 2.0 ** -24 * size + 2.0 ** -22 * (far + 1)
+            vv = np.nan_to_num(v[b, h]) if np.isnan(v[b, h]).any() else v[b, h]
+            out[b, hq] = p @ vv
+            bound[b, hq] = u * np.abs(out[b, hq]) + (u + 2 * (T + 64) * 2.0 ** -24) * (p @ np.abs(vv)) + 2 * (p * e) @ np.abs(vv) + 1e-30
+            bound[b, hq] += 2 * (p * e).sum(-1, keepdims=True) * (p @ np.abs(vv))
+    return out, bound
+
+
+def check(got, want, bound):
+    got = np32(got).astype(np.float64)
+    assert np.isfinite(got).all()
+    worst = (np.abs(got - want) / bound).max()
+    assert worst <= 1.0, f"{worst:.3g} times the bound"
+
+
+def causal(T, n, pads, window=0):
+    pos, col = np.arange(T - n, T)[:, None], np.arange(T)[None]
+    keep = np.stack([(col <= pos) & (col >= p) & (col > pos - window if window else True) for p in pads])
+    return keep[:, None].astype(np.float64)
+
+
+# (query heads, kv heads, key size, value size)
+LAYOUTS = [(8, 2, 128, 128), (6, 2, 64, 64), (4, 4, 96, 96), (14, 2, 256, 256), (4, 4, 192, 128), (4, 2, 50, 36)]
+
+
+def held(dtype, T, layout, seed=0, B=2, rows=None):
+    rng = np.random.default_rng(seed + T)
+    cache, oracle = kvhip.BlockScaledKVCache(), O.BlockScaledCache(NAME[dtype])
+    hq, h, dk, dv = layout
+    fill(cache, oracle, pair(dtype, rng, B, h, (dk, dv)), rows or [T])
+    return cache, oracle, lambda n: randn(rng, (B, hq, n, dk), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("T,n", [(1, 1), (2, 1), (63, 1), (64, 1), (65, 1), (700, 1), (3000, 1), (2, 2), (66, 3), (300, 5), (64, 20),
+                                 (200, 40), (1000, 67), (5000, 9)])
+def test_attention_with_causal_masks(dtype, layout, T, n):
+    cache, oracle, queries = held(dtype, T, layout)
+    q, qd = queries(n)
+    scale = layout[2] ** -0.5
+    got = cache.attend(qd, scale, kvhip.MaskMode.causal() if n > 1 else None)
+    assert kvhip.load().kvhip_last_attend_kernel() == 7
+    check(got, *exact_and_bound(q, oracle, scale, causal(T, n, [0, 0])))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("layout", LAYOUTS[:4])
+@pytest.mark.parametrize("T,n,pads,window", [(500, 1, (0, 499), 0), (500, 3, (130, 498), 0), (500, 3, (500, 7), 0), (700, 40, (0, 690), 0),
+                                             (700, 1, (0, 0), 100), (700, 40, (3, 200), 65), (300, 130, (64, 128), 0), (90, 90, (0, 90), 1)])
+def test_attention_of_padded_batches_and_windows(dtype, layout, T, n, pads, window):
+    cache, oracle, queries = held(dtype, T, layout, seed=1)
+    q, qd = queries(n)
+    scale = layout[2] ** -0.5
+    mask = kvhip.MaskMode.window_mask(T - n, window, left_pad=torch.tensor(pads, device="cuda"))
+    got = cache.attend(qd, scale, mask)
+    check(got, *exact_and_bound(q, oracle, scale, causal(T, n, pads, window)))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("layout", [LAYOUTS[0], LAYOUTS[3], LAYOUTS[5]])
+@pytest.mark.parametrize("T,n", [(70, 1), (300, 3), (513, 20)])
+@pytest.mark.parametrize("kind", ["bool", "f32", "own", "lowest", "empty"])
+def test_attention_with_array_masks(dtype, layout, T, n, kind):
+    cache, oracle, queries = held(dtype, T, layout, seed=2)
+    q, qd = queries(n)
+    B, hq = q.shape[:2]
+    scale = layout[2] ** -0.5
+    gen = torch.Generator(device="cuda").manual_seed(T + n)
+    keep = torch.rand(B, hq if kind == "bool" else 1, n, T, generator=gen, device="cuda") < 0.6
+    keep[..., 0] = True
+    add = None
+    if kind == "empty":
+        keep[0, :, 0] = False
+        keep[1, :, n - 1, 5:] = False
+    if kind in ("bool", "empty"):
+        mask = keep
+    else:
+        t = {"f32": torch.float32, "own": dtype, "lowest": dtype}[kind]
+        mask = torch.randn(B, 1, n, T, generator=gen, device="cuda").to(t)
+        if kind == "lowest":
+            mask = torch.where(keep, mask, torch.full_like(mask, torch.finfo(t).min))
+            mask[0, 0, 0] = torch.finfo(t).min  # (equal weights: the score is lost beside it)
+        else:
+            mask = torch.where(keep, mask, torch.full_like(mask, -INF))
+            mask[1, 0, n - 1, 3:] = -INF
+            keep[1, 0, n - 1, 3:] = False
+        add = np.broadcast_to(mask.double().cpu().numpy(), (B, hq, n, T))
+    weight = np.broadcast_to(keep.double().cpu().numpy(), (B, hq, n, T))
+    if kind == "lowest":
+        weight = np.ones((B, hq, n, T))
+    got = cache.attend(qd, scale, kvhip.MaskMode.from_array(mask))
+    if kind == "lowest":
+        # what float32 leaves of a score beside the lowest value
+        h = np.repeat(oracle.keys, hq // layout[1], axis=1)
+        s = (np.einsum("bhld,bhtd->bhlt", q.astype(np.float64), h) * scale).astype(np.float32) + add.astype(np.float32)
+        want, bound = exact_and_bound(q * 0, oracle, scale, weight, s.astype(np.float64))
+        e = (layout[2] + 6) * 2.0 ** -24 * np.einsum("bhld,bhtd->bhlt", np.abs(q.astype(np.float64)), np.abs(h)).max() * scale
+        ones = np.repeat(np.abs(oracle.values), hq // layout[1], axis=1).max(2, keepdims=True)
+        far = 2.0 ** -22 * (np.where(s > -1e30, np.abs(s), 0).max() + 1)
+        _, plain = exact_and_bound(q * 0, oracle, scale, weight, np.where(add > -1e4, s, -INF).astype(np.float64))
+        row = (add > -1e4).any(-1, keepdims=True)
+        check(got, want, np.where(row, plain, bound * 0 + 2.0 ** -7 * ones) + 4 * (e + far) * ones)
+        return
+    check(got, *exact_and_bound(q, oracle, scale, weight, add))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("T,n", [(75, 1), (140, 4), (400, 30), (256, 70)])
+def test_values_that_are_no_numbers_in_masked_places(dtype, T, n):
+    """NaN and infinities in paddings, in later tokens of the chunk and in rows trimmed away reach no row that does not see
+    them, and every row that does."""
+    layout = LAYOUTS[0]
+    rng = np.random.default_rng(T)
+    make = pair(dtype, rng, 2, 2, (128, 128))
+    cache, oracle = kvhip.BlockScaledKVCache(), O.BlockScaledCache(NAME[dtype])
+    (k, kd), (v, vd) = make(T + 9)
+    bad = {(0, 3): NAN, (0, 10): INF, (1, 2): -INF, (0, T - 1): NAN}
+    for (b, t), x in bad.items():
+        v[b, 0, t, 5], vd[b, 0, t, 5] = x, x
+    for x in (k, v, kd, vd):
+        x[:, :, T:] = NAN if x is k or x is v or x is kd else INF
+    k[0, 1, 3, 2], kd[0, 1, 3, 2] = NAN, NAN
+    cache.update(kd, vd, fetch=False)
+    oracle.update(k, v)
+    cache.trim(9)
+    oracle.trim(9)
+    q, qd = randn(rng, (2, 8, n, 128), dtype)
+    scale = 128 ** -0.5
+    pads = (11, 3)
+    got = cache.attend(qd, scale, kvhip.MaskMode.window_mask(T - n, 0, left_pad=torch.tensor(pads, device="cuda")))
+    oracle.keys = np.nan_to_num(oracle.keys)
+    want, bound = exact_and_bound(q, oracle, scale, causal(T, n, pads))
+    seen = torch.zeros_like(got, dtype=torch.bool)
+    seen[0, :4, n - 1, 5] = True  # (the last token of the first sequence, kv head 0, sees the NaN at T - 1)
+    assert torch.isnan(got[seen]).all()
+    check(got.masked_fill(seen, 0), np.where(seen.cpu().numpy(), 0, want), bound)
+    # without the paddings every row of kv head 0 sees them, and kv head 1 of the first sequence has a key that is none
+    got = cache.attend(qd, scale, kvhip.MaskMode.causal())
+    assert torch.isnan(got[0, :4, :, 5]).all() and torch.isnan(got[1, :4, :, 5]).all() and torch.isnan(got[0, 4:]).all()
+    assert torch.isfinite(got[1, 4:]).all() and torch.isfinite(got[:, :4, :n - 1, 6:]).all()
+
+
+@pytest.mark.parametrize("dtype,layout", [(F16, LAYOUTS[0]), (BF16, LAYOUTS[1]), (BF16, LAYOUTS[5])])
+def test_a_conversation(dtype, layout):
+    """A prompt, tokens one by one over block ends, a rejected draft, a chunk, as the functions of the framework run them:
+    each call against the oracle, and the same as update and attention apart."""
+    hq, h, dk, dv = layout
+    rng = np.random.default_rng(21)
+    make = pair(dtype, rng, 2, h, (dk, dv))
+    cache, apart, oracle = kvhip.BlockScaledKVCache(), kvhip.BlockScaledKVCache(), O.BlockScaledCache(NAME[dtype])
+    scale = dk ** -0.5
+    for n in [100] + [1] * 30 + [4, -3] + [1] * 3 + [90, -40] + [1] * 20:
+        if n < 0:
+            assert kvhip.trim_prompt_cache([cache, apart], -n) == -n
+            oracle.trim(-n)
+            continue
+        (k, kd), (v, vd) = make(n)
+        q, qd = randn(rng, (2, hq, n, dk), dtype)
+        got = kvhip.attention_with_cache_update(qd, kd, vd, cache, scale, kvhip.create_attention_mask(n, cache))
+        mask = kvhip.create_attention_mask(n, apart)
+        apart.update(kd, vd, fetch=False)
+        assert torch.equal(got, apart.attend(qd, scale, mask))
+        oracle.update(k, v)
+        check(got, *exact_and_bound(q, oracle, scale, causal(oracle.offset, n, [0, 0])))
+    check_rows(cache, oracle)
+
+
+def test_rotary_steps():
+    """Keys turned on their way in are what kvhip_rope_apply makes of them."""
+    rng = np.random.default_rng(4)
+    rope = kvhip.RoPE(128, base=10000.0)
+    a, b = kvhip.BlockScaledKVCache(), kvhip.BlockScaledKVCache()
+    make = pair(BF16, rng)
+    for n in (70, 1, 1, 60, 1):
+        (_, k), (_, v) = make(n)
+        _, q = randn(rng, (2, 8, n, 128), BF16)
+        mask = kvhip.create_attention_mask(n, a)
+        got = kvhip.attention_with_rope_and_cache_update(rope, q, k, v, a, 0.1, mask)
+        qr, kr = (kvhip.apply_rotary_position(rope, x, b) for x in (q, k))
+        assert torch.equal(got, b.update_attend(qr, kr, v, 0.1, mask))
+    for x, y in zip(a.fetch(), b.fetch()):
+        assert torch.equal(x, y)
+
+
+def test_static_scratch_and_streams():
+    cache, oracle, queries = held(BF16, 2500, LAYOUTS[0])
+    q, qd = queries(3)
+    want = cache.attend(qd, 0.1, kvhip.MaskMode.causal())
+    got = cache.attend(qd, 0.1, kvhip.MaskMode.causal(), static_scratch=True)
+    assert torch.equal(got, want)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = cache.attend(qd, 0.1, kvhip.MaskMode.causal())
+    side.synchronize()
+    assert torch.equal(got, want)
+    q, qd = queries(1100)  # partials that would not fit: fewer parts
+    check(cache.attend(qd, 0.1, kvhip.MaskMode.causal(), static_scratch=True), *exact_and_bound(q, oracle, 0.1, causal(2500, 1100, [0, 0])))
+
+
+# ---- choosing blocks ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("layout", LAYOUTS + [(5, 5, 64, 64), (40, 2, 128, 128), (3, 1, 96, 96)])
+@pytest.mark.parametrize("T,n,count,first,recent,pads", [(1, 1, 3, 1, 1, (0, 0)), (64, 1, 2, 0, 1, (0, 0)), (1000, 1, 5, 1, 2, (0, 300)),
+                                                        (1000, 3, 16, 0, 1, (999, 1000)), (1003, 7, 3, 1, 1, (64, 130)),
+                                                        (1920, 1, 20, 2, 3, (0, 63)), (650, 70, 4, 0, 2, (0, 640))])
+def test_blocks_are_chosen_by_the_definition(dtype, layout, T, n, count, first, recent, pads):
+    cache, oracle, queries = held(dtype, T, layout, seed=3)
+    q, qd = queries(n)
+    got = cache.select_blocks(qd, count, first, recent, torch.tensor(pads, device="cuda"))
+    assert np.array_equal(got.cpu().numpy(), O.select(q, oracle, count, first, recent, pads))
+
+
+def test_equal_bounds_take_the_lower_block():
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    one = torch.randn(1, 2, 64, 64, generator=gen, device="cuda").to(BF16)
+    k = one.repeat(1, 1, 40, 1)
+    k[:, :, 64 * 17:64 * 18] *= 2
+    cache = kvhip.BlockScaledKVCache()
+    cache.update(k, k, fetch=False)
+    q = torch.randn(1, 8, 1, 64, generator=gen, device="cuda").to(BF16)
+    got = cache.select_blocks(q, 7, 0, 1)
+    assert (got[0, :, 0].cpu() == torch.tensor([0, 1, 2, 3, 4, 17, 39])).all()
+    assert (cache.select_blocks(q * 0, 4, 0, 1)[0, :, 0].cpu() == torch.tensor([0, 1, 2, 39])).all()
+    assert (cache.select_blocks(q * NAN, 4, 0, 1)[0, :, 0].cpu() == torch.tensor([0, 1, 2, 39])).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("layout", LAYOUTS + [(40, 2, 128, 128)])
+@pytest.mark.parametrize("T,n,count,pads", [(1, 1, 1, (0, 0)), (900, 1, 6, (0, 200)), (900, 1, 40, (0, 899)), (901, 5, 7, (901, 70)), (640, 40, 3, (0, 0))])
+def test_attention_over_chosen_blocks(dtype, layout, T, n, count, pads):
+    hq, h, dk, dv = layout
+    rng = np.random.default_rng(T)
+    make = pair(dtype, rng, 2, h, (dk, dv))
+    cache, oracle = kvhip.BlockScaledKVCache(), O.BlockScaledCache(NAME[dtype])
+    if T > n:
+        fill(cache, oracle, make, [T - n])
+    (k, kd), (v, vd) = make(n)
+    q, qd = randn(rng, (2, hq, n, dk), dtype)
+    pad = torch.tensor(pads, device="cuda")
+    scale = dk ** -0.5
+    got, blocks = cache.update_attend_blocks(qd, kd, vd, scale, count, first=0, recent=1, left_pad=pad)
+    assert kvhip.load().kvhip_last_attend_kernel() == 8
+    oracle.update(k, v)
+    want = O.select(q, oracle, count, 0, 1, pads)
+    assert np.array_equal(blocks.cpu().numpy(), want)
+    check(got, *exact_and_bound(q, oracle, scale, O.listed_keep(want, T, pads)))
+    assert torch.equal(cache.attend_blocks(qd, blocks, scale, pad), got)
+    assert torch.equal(cache.select_blocks(qd, count, 0, 1, pad), blocks)
+    check_rows(cache, oracle)
+
+
+def test_lists_of_any_content():
+    """Entries outside what the token sees, repeated and descending ones are passed over; nothing listed: zeros."""
+    cache, oracle, queries = held(BF16, 700, LAYOUTS[0])
+    q, qd = queries(4)
+    lists = [[-1, -1, -1, -1, -1], [10, 10, 10, 10, 10], [3, 2, 5, 1, 0], [-7, 4, 2 ** 31 - 1, 11, 12]]
+    blocks = torch.tensor(lists, dtype=torch.int32, device="cuda").expand(2, 2, 4, 5).contiguous()
+    blocks[1, 1, 0] = torch.tensor([0, 4, 6, 8, 10])
+    pads = (0, 75)
+    got = cache.attend_blocks(qd, blocks, 0.1, torch.tensor(pads, device="cuda"))
+    check(got, *exact_and_bound(q, oracle, 0.1, O.listed_keep(blocks.cpu().numpy(), 700, pads)))
+    assert (got[0, :, 0] == 0).all()
+
+
+def test_every_block_listed_is_the_whole_attention():
+    cache, oracle, queries = held(F16, 1000, LAYOUTS[0])
+    q, qd = queries(9)
+    out = kvhip.sparse_attention_with_cache_update
+    blocks = cache.select_blocks(qd, 16)
+    check(cache.attend_blocks(qd, blocks, 0.1), *exact_and_bound(q, oracle, 0.1, causal(1000, 9, [0, 0])))
+    (k, kd), (v, vd) = pair(F16, np.random.default_rng(0))(1)
+    oracle.update(k, v)
+    check(out(qd[:, :, :1].contiguous(), kd, vd, cache, 0.1, 16), *exact_and_bound(q[:, :, :1], oracle, 0.1, causal(1001, 1, [0, 0])))
+
+
+def test_captured_steps_replay():
+    """A captured step (the choice, both attentions) replayed with eager work in between."""
+    cache, oracle, queries = held(BF16, 5000, LAYOUTS[0])
+    _, q = queries(1)
+    out = torch.empty(2, 8, 1, 128, dtype=BF16, device="cuda")
+    cache.attend(q, 0.1, out=out)
+    chosen = cache.attend_blocks(q, cache.select_blocks(q, 9), 0.1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        blocks = cache.select_blocks(q, 9)
+        sparse = cache.attend_blocks(q, blocks, 0.1)
+        cache.attend(q, 0.1, out=out)
+    for i in range(4):
+        fresh = torch.randn(2, 8, 1, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(i)).to(BF16)
+        q.copy_(fresh)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got, got_sparse = out.clone(), sparse.clone()
+        assert torch.equal(got, cache.attend(fresh, 0.1))
+        assert torch.equal(got_sparse, cache.attend_blocks(fresh, cache.select_blocks(fresh, 9), 0.1))
+    assert torch.isfinite(chosen).all()
+
+
+# ---- refusals -------------------------------------------------------------------------------------------------------
+def test_refusals():
+    cache, oracle, queries = held(BF16, 200, LAYOUTS[0])
+    _, q = queries(2)
+    blocks = cache.select_blocks(q, 3)
+
+    def refused(status, call, *args, **kw):
+        with pytest.raises(kvhip.KVHipError) as e:
+            call(*args, **kw)
+        assert e.value.status == status
+
+    k = torch.zeros(2, 2, 1, 128, dtype=BF16, device="cuda")
+    refused(-2, cache.select_blocks, q, 0)
+    refused(-2, cache.select_blocks, q, 3, first=3, recent=1)
+    refused(-2, cache.select_blocks, q, 3, first=-1)
+    refused(-2, cache.select_blocks, q, 3, recent=0)
+    refused(-2, cache.select_blocks, q[:, :7].contiguous(), 3)
+    refused(-2, cache.select_blocks, queries(201)[1], 3)
+    refused(-2, cache.attend_blocks, queries(201)[1], blocks[:, :, :1].expand(2, 2, 201, 3).contiguous(), 0.1)
+    refused(-3, kvhip.BlockScaledKVCache().update, k.float(), k.float())
+    refused(-3, kvhip.BlockScaledKVCache().update, k.repeat(1, 1, 1, 3), k)
+    refused(-4, kvhip.BlockScaledKVCache().select_blocks, q, 3)
+    refused(-2, cache.update_attend_blocks, q[:, :, :1].contiguous(), k, k, 0.1, 2, first=2)
+    refused(-2, cache.update, k[:1], k[:1])
+    assert cache.offset == 200
+    with pytest.raises(ValueError):
+        cache.attend_blocks(q, blocks.long(), 0.1)
+    with pytest.raises(ValueError):
+        cache.attend_blocks(q, blocks[:, :1], 0.1)
+    with pytest.raises(ValueError):
+        cache.select_blocks(q, 3, left_pad=torch.zeros(3, device="cuda"))
+    with pytest.raises(ValueError):
+        cache.update_attend_blocks(q, k, k, 0.1, 3)
+    with pytest.raises(TypeError):
+        cache.select_blocks(q.half(), 3)
+    with pytest.raises(TypeError):
+        cache.to_quantized()
+    lib, simple = kvhip.load(), kvhip.KVCacheSimple()
+    simple.update(k, k, fetch=False)
+    assert lib.kvhip_cache_select_blocks(simple._h, q.data_ptr(), 2, 8, 1, 128, 3, 1, 1, None, blocks.data_ptr(), None) == L.OK - 2
+    check_rows(cache, oracle)
