@@ -78,7 +78,7 @@ size_t plan_block_attend(BlockAttend &x) {
     x.tiles = (G + 15) / 16;
     const int64_t base = a.st.BH * block_attend_rows(x);
     const int blocks = x.list ? x.count : (a.T + BLOCK_ROWS - 1) / BLOCK_ROWS;
-    const int64_t slots = nm == 1 ? 512 : 256;
+    const int64_t slots = a.st.Dk <= 128 ? 512 : 256;
     int64_t parts = std::max<int64_t>(1, slots / base);
     parts = std::min<int64_t>(parts, std::max(1, blocks / 8));
     parts = std::min<int64_t>(parts, MERGE_PARTS);

@@ -7,7 +7,7 @@
 //   O^T = V^T P^T the same lane's weights, two tiles of tokens at a time, are the right operand as they stand -- the order of
 //                 the contraction is free, so the pages hold each lane's sixteen tokens of a channel side by side
 // Codes become operands by one conversion for two values, which takes the block's scale along.  Operands are loaded straight
-// from the pages, 1 KB to an instruction; the next block's are requested before the current one's are looked at.  The blocks'
+// from the pages, 1 KB to an instruction, half a block ahead.  The blocks'
 // addresses and scales are looked up 64 at a time, a lane to a block, instead of one dependent load after another.
 #pragma once
 #include "kvhip_block.hpp"
@@ -20,8 +20,7 @@ namespace kvhip {
 inline int block_row_tiles(const BlockAttend &x) {
     const int rows = x.a.Hq / x.a.Hkv * x.a.L;
     if (x.list || rows <= 16) return 1;
-    if (rows <= 32 || x.a.st.Dk > 192 || x.a.mask.mode == KVHIP_MASK_ARRAY) return 2;
-    return 4;
+    return 2;
 }
 
 namespace {
@@ -84,11 +83,12 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
     kv_u4 q[NM][KS];
     kv_f4 o[NM][VT];
     float m[NM], l[NM];
+    float unit;         // log2 e, times the scale (its sign is the queries') where scores have not met it
     KeyBounds see[NM];  // the keys of the lane's query row
     int ql[NM], qh[NM]; // its position and head (MODE 2)
 
     __device__ __forceinline__ BlockWalk(const BlockAttend &x_, int bh_)
-        : x(x_), lane(threadIdx.x & 63), g(lane >> 4), n(lane & 15), b(bh_ / x_.a.Hkv), h(bh_ % x_.a.Hkv), bh(bh_) {
+        : x(x_), lane(threadIdx.x & 63), g(lane >> 4), n(lane & 15), b(bh_ / x_.a.Hkv), h(bh_ % x_.a.Hkv), bh(bh_), unit(SAFE || x_.a.scale == 0.f ? LOG2E : fabsf(x_.a.scale) * LOG2E) {
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
             m[i] = -INFINITY;
@@ -98,25 +98,26 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
         }
     }
 
-    // scores (already scaled) of one tile of query rows -> weights as operands; the outputs so far are brought to the new maximum
+    // Scores of one tile of query rows -> weights as operands; the outputs so far are brought to the new maximum.  Scores and
+    // maxima are products that the call's scale has yet to meet (MODE 2: has met, an added mask's terms among them).
     __device__ __forceinline__ void weigh(int i, kv_f4 (&s)[4], kv_u4 (&p)[2]) {
         float mx = m[i];
 #pragma unroll
         for (int t = 0; t < 4; ++t) mx = fmaxf(mx, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
         mx = row_max(mx);
         const float ref = mx == -INFINITY ? 0.f : mx;  // (nothing seen yet: every difference is -infinity)
-        const float off = LIFT - ref * LOG2E;
+        const float off = LIFT - ref * unit;
         float e[16], sum = 0.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float y = SAFE ? __builtin_fmaf(s[t][k] - ref, LOG2E, LIFT) : __builtin_fmaf(s[t][k], LOG2E, off);
+                const float y = SAFE ? __builtin_fmaf(s[t][k] - ref, LOG2E, LIFT) : __builtin_fmaf(s[t][k], unit, off);
                 e[4 * t + k] = fast_exp2(y);
                 sum += e[4 * t + k];
             }
         if (__any(mx != m[i])) {
-            const float alpha = fast_exp2((m[i] - ref) * LOG2E);
+            const float alpha = fast_exp2((m[i] - ref) * unit);
             l[i] *= alpha;
 #pragma unroll
             for (int d = 0; d < VT; ++d) o[i][d] *= alpha;
@@ -172,8 +173,8 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
             if (hit[k] > 0.f) o[i][d][k] = __builtin_nanf("");
     }
 
-    // a block of codes
-    __device__ __forceinline__ void block(BlockTile<DK, DV> &tile, float ks, float vs, int j0, bool masked) {
+    // a block of codes; `ahead` requests the next one's keys, into the registers of this one's
+    template <class AHEAD> __device__ __forceinline__ void block(BlockTile<DK, DV> &tile, float ks, float vs, int j0, bool masked, AHEAD ahead) {
         using Tile = BlockTile<DK, DV>;
         kv_f4 s[NM][4];
 #pragma unroll
@@ -190,12 +191,16 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        ahead();
+        __builtin_amdgcn_sched_barrier(0);
         kv_u4 p[NM][2];
         uint32_t seen[NM];
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
+            if constexpr (SAFE) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) s[i][t] *= x.a.scale;
+                for (int t = 0; t < 4; ++t) s[i][t] *= x.a.scale;
+            }
             seen[i] = 0xffffu;
             if (masked) seen[i] = mask(i, j0, s[i]);
             weigh(i, s[i], p[i]);
@@ -270,8 +275,10 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
         uint32_t seen[NM];
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
+            if constexpr (SAFE) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) s[i][t] *= a.scale;
+                for (int t = 0; t < 4; ++t) s[i][t] *= a.scale;
+            }
             seen[i] = mask(i, j0, s[i]);
             weigh(i, s[i], p[i]);
             __builtin_amdgcn_sched_barrier(0);
@@ -317,7 +324,7 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
 
 // grid (BH, tiles of query rows, parts), NW wavefronts.  MODE 3: (BH, tokens x tiles of heads, parts).
 template <int DK, int DV, int DT, int NM, int MODE, int NW>
-__global__ void __launch_bounds__(NW * 64, NM == 1 && DK <= 128 ? 2 : 1) block_attend_kernel(BlockAttend x) {
+__global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kernel(BlockAttend x) {
     using Walk = BlockWalk<DK, DV, DT, NM, MODE, NW>;
     using Tile = BlockTile<DK, DV>;
     __shared__ WaveParts<DV, NW, 16> parts;
@@ -357,7 +364,8 @@ __global__ void __launch_bounds__(NW * 64, NM == 1 && DK <= 128 ? 2 : 1) block_a
 #pragma unroll
         for (int c = 0; c < Walk::KS; ++c) {
             const int d = (c | 1) < Walk::KS ? (c >> 1) * 64 + w.g * 16 + (c & 1) * 8 : c * 32 + w.g * 8;
-            w.q[i][c] = live ? load_row16(row + 2 * d) : kv_u4{0u, 0u, 0u, 0u};
+            w.q[i][c] = live && a.scale != 0.f ? load_row16(row + 2 * d) : kv_u4{0u, 0u, 0u, 0u};
+            if (!Walk::SAFE && a.scale < 0.f) w.q[i][c] ^= 0x80008000u;
         }
         w.ql[i] = live ? r % a.L : 0;
         w.qh[i] = live ? w.h * G + r / a.L : -1;
@@ -409,31 +417,23 @@ __global__ void __launch_bounds__(NW * 64, NM == 1 && DK <= 128 ? 2 : 1) block_a
             const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, of), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), of);
             return (gptr)(((uint64_t)hi << 32) | lo);
         };
-        auto use = [&](Tile &t, int of) {
-            const float k = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), of));
-            const float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), of));
-            const int j0 = __builtin_amdgcn_readlane(blk, of) * BLOCK_ROWS;
-            w.block(t, k, v, j0, MODE == 2 || j0 < in_lo || j0 + BLOCK_ROWS - 1 > in_hi);
-        };
         if (!todo) continue;
-        // One tile of rows: the next block's keys and values are requested ahead.  More: its keys, and the values of the current
-        // one, which have the score product and the weights in front of them.
+        // One buffer, its halves skewed: a block's values are requested in front of its score product, the next block's keys
+        // behind it.
         Tile tile;
         int cur = __builtin_ctzll(todo);
         tile.load_keys(at_lane(kp, cur), lane);
-        if (NM == 1) tile.load_values(at_lane(vp, cur), lane);
         while (true) {
             todo &= todo - 1;
-            Tile next;
-            const int then = todo ? __builtin_ctzll(todo) : cur;
-            if (NM > 1) tile.load_values(at_lane(vp, cur), lane);
-            if (todo) {
-                next.load_keys(at_lane(kp, then), lane);
-                if (NM == 1) next.load_values(at_lane(vp, then), lane);
-            }
-            use(tile, cur);
+            const int then = todo ? __builtin_ctzll(todo) : cur;  // (the last block's keys again: no branch around the requests)
+            tile.load_values(at_lane(vp, cur), lane);
+            __builtin_amdgcn_sched_barrier(0);
+            const float k = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), cur));
+            const float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), cur));
+            const int j0 = __builtin_amdgcn_readlane(blk, cur) * BLOCK_ROWS;
+            w.block(tile, k, v, j0, MODE == 2 || j0 < in_lo || j0 + BLOCK_ROWS - 1 > in_hi,
+                    [&] { tile.load_keys(at_lane(kp, then), lane); });
             if (!todo) break;
-            tile = next;
             cur = then;
         }
     }
@@ -457,6 +457,7 @@ __global__ void __launch_bounds__(NW * 64, NM == 1 && DK <= 128 ? 2 : 1) block_a
         if (rows <= 0) break;
         if (i) __syncthreads();
         const float l = row_sum(w.l[i]);
+        if constexpr (!Walk::SAFE) w.m[i] = w.m[i] == -INFINITY ? -INFINITY : w.m[i] * fabsf(a.scale);  // (weights go by scores from here on)
         if (w.g == 0) parts.m[wave][w.n] = w.m[i];
         __syncthreads();
         const float weight = wave_weight(parts, w.n, w.m[i]);
@@ -508,9 +509,6 @@ template <int DK, int DV, int DT> hipError_t block_attend_shape(const BlockAtten
     if (x.a.mask.mode == KVHIP_MASK_ARRAY)
         return nm == 1 ? block_attend_run<DK, DV, DT, 1, 2>(x, stream) : block_attend_run<DK, DV, DT, 2, 2>(x, stream);
     if (nm == 1) return block_attend_run<DK, DV, DT, 1, 1>(x, stream);
-    if constexpr (DK <= 192) {
-        if (nm == 4) return block_attend_run<DK, DV, DT, 4, 1>(x, stream);
-    }
     return block_attend_run<DK, DV, DT, 2, 1>(x, stream);
 }
 template <int DT> hipError_t block_attend_dtype(const BlockAttend &x, hipStream_t stream) {
