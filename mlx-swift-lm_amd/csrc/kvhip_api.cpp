@@ -1603,7 +1603,7 @@ kvhip_status block_choice(const kvhip_cache *c, const void *q, int32_t B, int32_
     x.recent = recent;
     x.left_pad = left_pad;
     x.list = blocks;
-    x.b.st.BH = c->st.BH;
+    x.b.st = c->st;
     if (!block_select_supported(x)) return fail(KVHIP_ERR_UNSUPPORTED, "a cache of this length holds more blocks than one choice takes");
     return KVHIP_OK;
 }

@@ -6,6 +6,7 @@
 // its order (below 2^24 for 256 channels) and the choice the same on any machine.  As products:
 // q+ hi + q- lo, with q+ = max(q, 0) and q- = min(q, 0), on the 16x16x64 int8 instruction.
 #include <algorithm>
+#include <type_traits>
 
 #include "kvhip_block.hpp"
 #include "kvhip_wave.hpp"
@@ -21,198 +22,347 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t u = __float_as_uint(x);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ int wave_scan_int(int v) {  // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(v, d);
-        if ((int)(threadIdx.x & 63) >= d) v += o;
-    }
+// inclusive prefix sums over the lanes
+__device__ __forceinline__ int wave_scan_int(int v) {
+#define KV_SCAN_STEP(CTRL, ROWS, ZERO) v += __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, ZERO)
+    KV_SCAN_STEP(0x111, 0xF, true);  // row_shr:1, 2, 4, 8
+    KV_SCAN_STEP(0x112, 0xF, true);
+    KV_SCAN_STEP(0x114, 0xF, true);
+    KV_SCAN_STEP(0x118, 0xF, true);
+    KV_SCAN_STEP(0x142, 0xA, false);  // row_bcast:15 into rows 1 and 3, row_bcast:31 into rows 2 and 3
+    KV_SCAN_STEP(0x143, 0xC, false);
+#undef KV_SCAN_STEP
     return v;
 }
+// over the lanes, in each of them
+__device__ __forceinline__ uint32_t wave_or(uint32_t v) {
+#define KV_OR_STEP(CTRL, ROWS) v |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false)
+    KV_OR_STEP(0xB1, 0xF);   // quad_perm [1,0,3,2], [2,3,0,1], row_half_mirror, row_mirror
+    KV_OR_STEP(0x4E, 0xF);
+    KV_OR_STEP(0x141, 0xF);
+    KV_OR_STEP(0x140, 0xF);
+    KV_OR_STEP(0x142, 0xA);  // row_bcast:15, row_bcast:31: all of them in lane 63
+    KV_OR_STEP(0x143, 0xC);
+#undef KV_OR_STEP
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 
-constexpr int SELECT_WAVES = 4;
-constexpr uint32_t ALWAYS = 0xffffffffu;  // the key of a block that is always chosen; 0: of one that the token does not see
+constexpr int SELECT_WAVES = 16;
+constexpr int SELECT_TILES = 4;  // at most so many tiles of 16 query rows to a workgroup
+constexpr int SELECT_HEAD = SELECT_WAVES * 256 * 4;  // bytes of the histograms
 
-// grid (BH, groups of `tokens` tokens), 256 threads.  LDS: keys [tokens][stride] of the blocks from `lead` on, and a
-// histogram of 256 bins for each wavefront.
+// Eight channels of a query row as floats; elements that are no numbers, and those past the end, are zeros.
+template <int DT> __device__ __forceinline__ void query_chunk(const char *row, int ud, int d, bool live, float *y) {
+    kv_u4 w{0u, 0u, 0u, 0u};
+    if (live && d + 8 <= ud) {
+        w = load_row16(row + 2 * d);
+    } else if (live) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (d + i < ud) w[i >> 1] |= (uint32_t) reinterpret_cast<const uint16_t *>(row)[d + i] << (16 * (i & 1));
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t h = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+        const float v = DT == 1 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
+        y[i] = fabsf(v) < INFINITY ? v : 0.f;
+    }
+}
+
+// A token's list: `count` of the blocks lead .. lead + seen - 1, the first `first` and the last `recent` of them and the
+// best of the others by their keys (row[i]: block lead + i), in ascending order.  TEAM: the whole workgroup's token (a step of one
+// token: what it lasts is a chain of passes over the keys, which 16 wavefronts make short); else the wavefront's.
+//
+// The smallest chosen key is found digit by digit, eight bits at a time from the first bit in which the keys differ (their
+// exponents mostly agree: from bit 31 on nearly all fall into one bin, and one address takes one addition a cycle), until
+// a bin is taken whole.  `area`: 256 bins and, behind them, a pair of counts for every 64 blocks (TEAM).
+template <bool TEAM>
+__device__ __forceinline__ void choose(const uint32_t *row, uint32_t *area, int lane, int lead, int seen, int count, int first, int recent, int32_t *out) {
+    constexpr int T = TEAM ? SELECT_WAVES * 64 : 64;
+    const int t = TEAM ? threadIdx.x : lane, wave = TEAM ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+    auto sync = [] {
+        if constexpr (TEAM) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    };
+    if (seen <= count) {
+        for (int i = t; i < count; i += T) out[i] = i < seen ? lead + i : -1;
+        return;
+    }
+    const int end = seen - recent;
+    int want = count - first - recent;  // of the blocks first .. end - 1
+    const bool ranked = want > 0;
+    uint32_t prefix = 0;                // a key is above the line if key >> shift > prefix, on it if they are equal
+    int shift = 0, ties = 0;            // the first `ties` blocks on the line are chosen
+    uint32_t *bins = area;
+    if (ranked) {
+        const uint32_t one = row[first];
+        uint32_t differ = 0;
+#pragma unroll 4
+        for (int i = first + t; i < end; i += T) differ |= row[i] ^ one;
+        differ = wave_or(differ);
+        if constexpr (TEAM) {
+            if (t == 0) area[256] = 0;
+            __syncthreads();
+            if (lane == 0 && differ) atomicOr(&area[256], differ);
+            __syncthreads();
+            differ = area[256];
+        }
+        int bits = differ ? 32 - __builtin_clz(differ) : 0;  // keys agree in the bits from here up
+        prefix = bits < 32 ? one >> bits : 0u;
+        shift = bits;
+        while (true) {
+            if (bits == 0) {
+                ties = want;
+                break;
+            }
+            const int step = bits < 8 ? bits : 8;
+            shift = bits - step;
+            for (int i = t; i < 256; i += T) bins[i] = 0;
+            sync();
+#pragma unroll 4
+            for (int i = first + t; i < end; i += T) {
+                const uint32_t k = row[i];
+                if (bits == 32 || (k >> bits) == prefix) atomicAdd(&bins[(k >> shift) & ((1u << step) - 1u)], 1u);
+            }
+            sync();
+            // the lane's bins, from the top: 255 - 4 lane to 252 - 4 lane (every wavefront for itself)
+            int c[4], mine = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                c[i] = (int)bins[255 - 4 * lane - i];
+                mine += c[i];
+            }
+            const int upto = wave_scan_int(mine);
+            int run = upto - mine, digit = 0, above = 0, here = 0;
+            const int at = __builtin_ctzll(__ballot(run < want && upto >= want));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (run < want && run + c[i] >= want) {
+                    digit = 255 - 4 * lane - i;
+                    above = run;
+                    here = c[i];
+                }
+                run += c[i];
+            }
+            digit = __builtin_amdgcn_readlane(digit, at);
+            want -= __builtin_amdgcn_readlane(above, at);
+            here = __builtin_amdgcn_readlane(here, at);
+            prefix = bits == 32 ? (uint32_t)digit : (prefix << step) | (uint32_t)digit;
+            bits = shift;
+            if (want == here) {
+                ties = here;
+                break;
+            }
+            if constexpr (TEAM) __syncthreads();  // (the bins are cleared again)
+        }
+    }
+    // blocks in 64s: those above the line, and the first `ties` on it
+    const int groups = (seen + 63) / 64;
+    const uint64_t below = (1ull << lane) - 1;
+    auto look = [&](int group, bool &above, bool &line) {
+        const int i = group * 64 + lane;
+        const bool in = ranked && i >= first && i < end;
+        const uint32_t k = in ? row[i] >> shift : 0u;
+        above = i < first || (i >= end && i < seen) || (in && k > prefix);
+        line = in && k == prefix;
+    };
+    auto write = [&](int group, bool above, uint64_t line, int left, int filled) {
+        const bool take = above || ((line >> lane) & 1 && __builtin_popcountll(line & below) < left);
+        const uint64_t taken = __ballot(take);
+        if (take) out[filled + __builtin_popcountll(taken & below)] = lead + group * 64 + lane;
+    };
+    if constexpr (TEAM) {
+        uint32_t *counts = area + 257;  // [groups][2]
+        for (int group = wave; group < groups; group += SELECT_WAVES) {
+            bool above, line;
+            look(group, above, line);
+            const int a = __builtin_popcountll(__ballot(above)), l = __builtin_popcountll(__ballot(line));
+            if (lane == 0) counts[2 * group] = a, counts[2 * group + 1] = l;
+        }
+        __syncthreads();
+        int a0 = 0, l0 = 0;  // what the groups before `g0` hold
+        for (int g0 = 0; g0 < groups; g0 += 64) {
+            const int mine_a = g0 + lane < groups ? (int)counts[2 * (g0 + lane)] : 0, mine_l = g0 + lane < groups ? (int)counts[2 * (g0 + lane) + 1] : 0;
+            const int upto_a = wave_scan_int(mine_a), upto_l = wave_scan_int(mine_l);
+            for (int k = wave; k < 64 && g0 + k < groups; k += SELECT_WAVES) {
+                const int a = a0 + __builtin_amdgcn_readlane(upto_a - mine_a, k), l = l0 + __builtin_amdgcn_readlane(upto_l - mine_l, k);
+                bool above, line;
+                look(g0 + k, above, line);
+                write(g0 + k, above, __ballot(line), max(ties - l, 0), a + min(l, ties));
+            }
+            a0 += __builtin_amdgcn_readlane(upto_a, 63);
+            l0 += __builtin_amdgcn_readlane(upto_l, 63);
+        }
+    } else {
+        int filled = 0, left = ties;
+        for (int group = 0; group < groups; ++group) {
+            bool above, line;
+            look(group, above, line);
+            const uint64_t on = __ballot(line);
+            write(group, above, on, left, filled);
+            filled += __builtin_popcountll(__ballot(above)) + min(left, (int)__builtin_popcountll(on));
+            left -= min(left, (int)__builtin_popcountll(on));
+        }
+    }
+}
+
+// grid (BH, groups of `tokens` tokens), 16 wavefronts.  LDS: a histogram for each wavefront, the query operands and exponents
+// of up to four tiles of 16 rows (token by token, a token's heads side by side), keys [tokens][stride] of the blocks from
+// `lead` on.
+//
+// What it reads is a 64th of the keys' codes; at few sequences it is a chain of latencies -- queries, page entries,
+// summaries, the choice -- so that a wavefront requests the summaries of several groups of 16 blocks before it looks at the first.
 template <int D, int DT>
 __global__ void __launch_bounds__(SELECT_WAVES * 64) block_select_kernel(BlockSelect x, int tokens, int stride) {
-    constexpr int KS = (D + 63) / 64;
+    constexpr int KS = (D + 63) / 64, AHEAD = D <= 128 ? 4 : 2;
     extern __shared__ uint32_t lds[];
-    uint32_t *hist = lds;                             // [waves][256]
-    uint32_t *keys = lds + SELECT_WAVES * 256;        // [tokens][stride]
+    __shared__ int exps[SELECT_TILES][16];
+    kv_i4 *ops = reinterpret_cast<kv_i4 *>(lds + SELECT_WAVES * 256);       // [tiles][positive / negative][KS][64]
     const Store &st = x.b.st;
     const int bh = blockIdx.x, b = bh / x.Hkv, G = x.Hq / x.Hkv;
     const int tok0 = blockIdx.y * tokens, toks = min(tokens, x.L - tok0);
+    const int rows = toks * G, tiles = min((rows + 15) / 16, SELECT_TILES);
+    uint32_t *keys = reinterpret_cast<uint32_t *>(ops + SELECT_TILES * 2 * KS * 64);  // [tokens][stride]
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
     const int pad = x.left_pad ? max(x.left_pad[b], 0) : 0;
     const int lead = pad / BLOCK_ROWS;
-    const int top = (x.T - x.L + tok0 + toks - 1) / BLOCK_ROWS;  // the last token's own block
+    const int top = (x.T - x.L + tok0 + toks - 1) / BLOCK_ROWS;  // the last token's own block, which is always chosen
+    const int coded = min(x.b.coded, top);
 
     for (int i = threadIdx.x; i < toks * stride; i += SELECT_WAVES * 64) keys[i] = 0;
-    __syncthreads();
 
-    // bounds: 16 query rows (token by token, a token's heads side by side) by 16 blocks at a time
+    // (a token of more than 64 heads: its rows in turns)
     const int ud = x.b.Dk_user;
-    for (int r0 = 0; r0 < toks * G; r0 += 16) {
-        const int r = r0 + n;
-        const bool live = r < toks * G;
-        const int tok = live ? r / G : 0, head = live ? r % G : 0;
-        const char *row = static_cast<const char *>(x.q) + (((size_t)bh * G + head) * x.L + tok0 + tok) * ud * 2;
-        kv_i4 pos[KS], neg[KS];
-        float v[KS][16], amax = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const int d = s * 64 + g * 16 + k;
-                float y = live && d < ud ? Elem<DT>::load(row, d) : 0.f;
-                if (!(fabsf(y) < INFINITY)) y = 0.f;  // (elements that are no numbers have no say)
-                v[s][k] = y;
-                amax = fmaxf(amax, fabsf(y));
-            }
-        amax = fmaxf(amax, __shfl_xor(amax, 16));
-        amax = fmaxf(amax, __shfl_xor(amax, 32));
-        // (frexp: also of the values below the smallest normal one)
-        int ex = 0;
-        const float mant = frexpf(amax, &ex);
-        const int f = amax > 0.f ? ex - 7 + (mant > 127.f / 128.f ? 1 : 0) : 0;
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                int p = 0, m = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int i = (int)rintf(ldexpf(v[s][4 * w + k], -f));
-                    p |= (max(i, 0) & 0xff) << (8 * k);
-                    m |= (min(i, 0) & 0xff) << (8 * k);
-                }
-                pos[s][w] = p;
-                neg[s][w] = m;
-            }
-        int fr[4], tr[4];  // the four rows whose bounds the lane will hold
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            fr[i] = __shfl(f, 4 * g + i);
-            tr[i] = r0 + 4 * g + i < toks * G ? (r0 + 4 * g + i) / G : -1;
-        }
-        const int coded = min(x.b.coded, top);  // (the last token's own block is always chosen)
-        for (int n0 = lead + 16 * wave; n0 < coded; n0 += 16 * SELECT_WAVES) {
-            const int blk = min(n0 + n, coded - 1);
-            const PageEntry &e = st.pt[blk / BLOCK_PER_PAGE];
-            const char *sum = e.vsb + (size_t)bh * st.vsb_cell + (size_t)(blk % BLOCK_PER_PAGE) * 2 * D;
-            const float scale = reinterpret_cast<const float *>(e.ksb + (size_t)bh * st.ksb_cell)[2 * (blk % BLOCK_PER_PAGE)];
-            kv_i4 acc{0, 0, 0, 0};
+    for (int row0 = 0; row0 < rows; row0 += 16 * SELECT_TILES) {
+        if (row0) __syncthreads();
+        if (wave < tiles) {
+            const int r = row0 + 16 * wave + n;
+            const bool live = r < rows;
+            const int tok = live ? r / G : 0, head = live ? r % G : 0;
+            const char *row = static_cast<const char *>(x.q) + (((size_t)bh * G + head) * x.L + tok0 + tok) * ud * 2;
+            float v[KS][16], amax = 0.f;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                const int d = s * 64 + g * 16;
-                kv_i4 hi{0, 0, 0, 0}, lo{0, 0, 0, 0};
-                if (d < D) {
-                    hi = *reinterpret_cast<const kv_i4 *>(sum + d);
-                    lo = *reinterpret_cast<const kv_i4 *>(sum + D + d);
-                }
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(pos[s], hi, acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(neg[s], lo, acc, 0, 0, 0);
+                query_chunk<DT>(row, ud, s * 64 + g * 16, live, v[s]);
+                query_chunk<DT>(row, ud, s * 64 + g * 16 + 8, live, v[s] + 8);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) amax = fmaxf(amax, fabsf(v[s][k]));
             }
-            if (n0 + n < coded) {
-                uint32_t key[4];
+            amax = fmaxf(amax, __shfl_xor(amax, 16));
+            amax = fmaxf(amax, __shfl_xor(amax, 32));
+            int ex = 0;
+            const float mant = frexpf(amax, &ex);  // (also of values below the smallest normal one)
+            const int f = amax > 0.f ? ex - 7 + (mant > 127.f / 128.f ? 1 : 0) : 0;
+            if (g == 0) exps[wave][n] = f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) key[i] = ordered(ldexpf((float)acc[i] * (4.f * scale), fr[i]));
-                // (rows of one token side by side: one entry for all four)
-                if (tr[0] >= 0 && tr[0] == tr[3]) {
-                    atomicMax(&keys[tr[0] * stride + blk - lead], max(max(key[0], key[1]), max(key[2], key[3])));
-                } else {
+            for (int s = 0; s < KS; ++s) {
+                kv_i4 pos, neg;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (tr[i] >= 0) atomicMax(&keys[tr[i] * stride + blk - lead], key[i]);
+                for (int w = 0; w < 4; ++w) {
+                    int p = 0, m = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int i = (int)rintf(ldexpf(v[s][4 * w + k], -f));
+                        p |= (max(i, 0) & 0xff) << (8 * k);
+                        m |= (min(i, 0) & 0xff) << (8 * k);
+                    }
+                    pos[w] = p;
+                    neg[w] = m;
+                }
+                ops[((wave * 2 + 0) * KS + s) * 64 + lane] = pos;
+                ops[((wave * 2 + 1) * KS + s) * 64 + lane] = neg;
+            }
+        }
+        __syncthreads();
+        const int groups = coded > lead ? (coded - lead + 15) / 16 : 0;
+        for (int first = wave; first < groups; first += SELECT_WAVES * AHEAD) {
+            gptr sum[AHEAD];
+            float scale[AHEAD];
+            kv_i4 hi[AHEAD][KS], lo[AHEAD][KS];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int blk = min(lead + (first + u * SELECT_WAVES) * 16 + n, coded - 1);
+                const gptr entry = as_global(st.pt + blk / BLOCK_PER_PAGE);
+                const gptr ksb = as_global(ld_global<const char *>(entry + offsetof(PageEntry, ksb)));
+                sum[u] = as_global(ld_global<const char *>(entry + offsetof(PageEntry, vsb))) + (size_t)bh * st.vsb_cell + (size_t)(blk % BLOCK_PER_PAGE) * 2 * D;
+                scale[u] = ld_global<float>(ksb + (size_t)bh * st.ksb_cell + 8 * (blk % BLOCK_PER_PAGE));
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const int d = s * 64 + g * 16;
+                    const bool in = D % 64 == 0 || d < D;
+                    hi[u][s] = in ? ld_global<kv_i4>(sum[u] + d) : kv_i4{0, 0, 0, 0};
+                    lo[u][s] = in ? ld_global<kv_i4>(sum[u] + D + d) : kv_i4{0, 0, 0, 0};
+                }
+            for (int tile = 0; tile < tiles; ++tile) {
+                int fr[4], tr[4];  // exponents and tokens of the four rows whose bounds the lane is left with
+                const int r = row0 + 16 * tile + 4 * g;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    fr[i] = exps[tile][4 * g + i];
+                    tr[i] = r + i < rows ? (r + i) / G : -1;
+                }
+                kv_i4 acc[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) acc[u] = kv_i4{0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const kv_i4 pos = ops[((tile * 2 + 0) * KS + s) * 64 + lane], neg = ops[((tile * 2 + 1) * KS + s) * 64 + lane];
+#pragma unroll
+                    for (int u = 0; u < AHEAD; ++u) {
+                        acc[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(pos, hi[u][s], acc[u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(neg, lo[u][s], acc[u], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const int at = (first + u * SELECT_WAVES) * 16 + n;  // block lead + at
+                    if (lead + at >= coded) continue;
+                    uint32_t key[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) key[i] = ordered(ldexpf((float)acc[u][i] * (4.f * scale[u]), fr[i]));
+                    if (tr[0] >= 0 && tr[0] == tr[3]) {  // one token's rows: one entry for all four
+                        atomicMax(&keys[tr[0] * stride + at], max(max(key[0], key[1]), max(key[2], key[3])));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (tr[i] >= 0) atomicMax(&keys[tr[i] * stride + at], key[i]);
+                    }
                 }
             }
         }
     }
     __syncthreads();
-
-    // the choice: a wavefront to a token
-    for (int tok = wave; tok < toks; tok += SELECT_WAVES) {
-        const int p = x.T - x.L + tok0 + tok, last = p / BLOCK_ROWS;
-        const int seen = p < pad ? 0 : last - lead + 1;  // candidates lead .. last
-        uint32_t *row = keys + (size_t)tok * stride;
-        int32_t *out = x.list + ((size_t)bh * x.L + tok0 + tok) * x.count;
-        if (seen <= x.count) {
-            for (int i = lane; i < x.count; i += 64) out[i] = i < seen ? lead + i : -1;
-            continue;
-        }
-        auto key_at = [&](int i) -> uint32_t {
-            if (i >= seen) return 0u;
-            if (i < x.first || lead + i > last - x.recent) return ALWAYS;
-            return min(max(row[i], 1u), ALWAYS - 1u);
-        };
-        // the count-th largest key, eight bits at a time
-        uint32_t prefix = 0, want = x.count;
-        uint32_t *bins = hist + wave * 256;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) bins[4 * lane + i] = 0;
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-            for (int i = lane; i < seen; i += 64) {
-                const uint32_t k = key_at(i);
-                if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&bins[(k >> shift) & 255u], 1u);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-            // lane's bins from the top: 255 - 4 lane down to 252 - 4 lane
-            uint32_t c[4];
-            int mine = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                c[i] = bins[255 - 4 * lane - i];
-                mine += (int)c[i];
-            }
-            const int upto = wave_scan_int(mine), before = upto - mine;
-            const uint64_t found = __ballot(before < (int)want && upto >= (int)want);
-            const int at = __builtin_ctzll(found);
-            int digit = 0, above = 0, run = before;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (run < (int)want && run + (int)c[i] >= (int)want) {
-                    digit = 255 - 4 * lane - i;
-                    above = run;
-                }
-                run += (int)c[i];
-            }
-            digit = __shfl(digit, at);
-            above = __shfl(above, at);
-            prefix = (prefix << 8) | (uint32_t)digit;
-            want -= (uint32_t)above;
-        }
-        // everything above it, and the first `want` blocks that equal it, in ascending order
-        int filled = 0;
-        uint32_t equal = want;
-        for (int i0 = 0; i0 < seen; i0 += 64) {
-            const uint32_t k = key_at(i0 + lane);
-            const uint64_t below = (1ull << lane) - 1;
-            const uint64_t eq = __ballot(k == prefix);
-            const bool take = k > prefix || (k == prefix && (uint32_t)__builtin_popcountll(eq & below) < equal);
-            const uint64_t taken = __ballot(take);
-            if (take) out[filled + __builtin_popcountll(taken & below)] = lead + i0 + lane;
-            filled += __builtin_popcountll(taken);
-            equal -= min(equal, (uint32_t)__builtin_popcountll(eq));
-        }
+    auto list_of = [&](int tok, auto team, uint32_t *area) {
+        const int p = x.T - x.L + tok0 + tok;
+        choose<decltype(team)::value>(keys + (size_t)tok * stride, area, lane, lead, p < pad ? 0 : p / BLOCK_ROWS - lead + 1, x.count, x.first, x.recent,
+                                      x.list + ((size_t)bh * x.L + tok0 + tok) * x.count);
+    };
+    if (toks == 1) {
+        list_of(0, std::true_type(), lds);
+    } else {
+        for (int tok = wave; tok < toks; tok += SELECT_WAVES) list_of(tok, std::false_type(), lds + wave * 256);
     }
 }
 
-constexpr int SELECT_LDS = 144 << 10;
-// tokens a workgroup takes and the keys it keeps for each
+// Tokens a workgroup takes and the keys it keeps for each: as many tokens as fill four tiles of rows, where they are
+// that many, and fit the memory.
+constexpr int SELECT_LDS = 156 << 10;
+size_t select_ops(const BlockSelect &x) { return (size_t)SELECT_TILES * 2 * ((x.b.st.Dk + 63) / 64) * 64 * 16; }
 void select_plan(const BlockSelect &x, int &tokens, int &stride) {
     const int G = x.Hq / x.Hkv;
     stride = (x.T + BLOCK_ROWS - 1) / BLOCK_ROWS;
-    tokens = std::max(1, 16 / G);
-    tokens = (int)std::min<int64_t>(tokens, (SELECT_LDS - SELECT_WAVES * 1024) / 4 / std::max(stride, 1));
+    tokens = std::min(std::max(1, 16 * SELECT_TILES / G), SELECT_WAVES);
+    tokens = (int)std::min<int64_t>(tokens, (int64_t)(SELECT_LDS - SELECT_HEAD - select_ops(x)) / 4 / std::max(stride, 1));
+    tokens = std::min(tokens, x.L);
 }
 template <int DT> hipError_t select_dtype(const BlockSelect &x, hipStream_t stream) {
     int tokens, stride;
     select_plan(x, tokens, stride);
     const dim3 grid(x.b.st.BH, (x.L + tokens - 1) / tokens), block(SELECT_WAVES * 64);
-    const size_t lds = SELECT_WAVES * 1024 + (size_t)tokens * stride * 4;
+    const size_t lds = SELECT_HEAD + select_ops(x) + (size_t)tokens * stride * 4;
 #define KV_SELECT(D)                                                                                                    \
     do {                                                                                                                \
         if (lds > 65536) {                                                                                              \
@@ -239,7 +389,7 @@ template <int DT> hipError_t select_dtype(const BlockSelect &x, hipStream_t stre
 bool block_select_supported(const BlockSelect &x) {
     int tokens, stride;
     select_plan(x, tokens, stride);
-    return tokens >= 1;
+    return tokens >= 1;  // (the keys of one token fit)
 }
 hipError_t launch_block_select(const BlockSelect &x, hipStream_t stream) {
     return x.b.st.dtype == KVHIP_F16 ? select_dtype<0>(x, stream) : select_dtype<1>(x, stream);
