@@ -1641,6 +1641,8 @@ kvhip_status kvhip_cache_select_blocks(kvhip_cache *c, const void *q, int32_t B,
     KV_TRY(check_block_call(c, B, Hq, L, D, c->presented, count));
     BlockSelect x;
     KV_TRY(block_choice(c, q, B, Hq, L, c->presented, count, first, recent, left_pad, blocks, x));
+    KV_TRY(ensure_ws(c, block_select_workspace(x), S(stream)));
+    x.workspace = c->ws;
     x.b = block_store(c);
     KV_HIP(launch_block_select(x, S(c, stream)));
     return KVHIP_OK;
@@ -1665,6 +1667,8 @@ kvhip_status kvhip_cache_update_attend_blocks(kvhip_cache *c, const void *q, con
     KV_TRY(check_block_call(c, B, Hq, L, Dk, T, count));
     BlockSelect x;
     KV_TRY(block_choice(c, q, B, Hq, L, T, count, first, recent, left_pad, blocks, x));
+    KV_TRY(ensure_ws(c, block_select_workspace(x), S(stream)));
+    x.workspace = c->ws;
     hipStream_t s = S(c, stream);
     const bool fuse = block_step_fuses(c, L);
     KV_TRY(update_blocks(c, k, v, L, s, !fuse));

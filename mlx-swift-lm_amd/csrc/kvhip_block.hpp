@@ -72,8 +72,10 @@ struct BlockSelect {
     int32_t count = 0, first = 0, recent = 1;
     const int32_t *left_pad = nullptr;
     int32_t *list = nullptr;  // [BH, L, count]
+    void *workspace = nullptr;
 };
 bool block_select_supported(const BlockSelect &x);
+size_t block_select_workspace(const BlockSelect &x);
 hipError_t launch_block_select(const BlockSelect &x, hipStream_t stream);
 
 #if defined(__HIPCC__)

@@ -70,18 +70,18 @@ template <int DT> __device__ __forceinline__ void query_chunk(const char *row, i
 }
 
 // A token's list: `count` of the blocks lead .. lead + seen - 1, the first `first` and the last `recent` of them and the
-// best of the others by their keys (row[i]: block lead + i), in ascending order.  TEAM: the whole workgroup's token (a step of one
-// token: what it lasts is a chain of passes over the keys, which 16 wavefronts make short); else the wavefront's.
+// best of the others by their keys (row[i]: block lead + i), in ascending order.  TEAM wavefronts: the whole workgroup's token
+// (where there are few: what it lasts is a chain of passes over the keys, which more wavefronts make short); 1: the wavefront's own.
 //
 // The smallest chosen key is found digit by digit, eight bits at a time from the first bit in which the keys differ (their
 // exponents mostly agree: from bit 31 on nearly all fall into one bin, and one address takes one addition a cycle), until
-// a bin is taken whole.  `area`: 256 bins and, behind them, a pair of counts for every 64 blocks (TEAM).
-template <bool TEAM>
+// a bin is taken whole.  `area`: 256 bins and, behind them, a pair of counts for every 64 blocks (TEAM > 1).
+template <int TEAM>
 __device__ __forceinline__ void choose(const uint32_t *row, uint32_t *area, int lane, int lead, int seen, int count, int first, int recent, int32_t *out) {
-    constexpr int T = TEAM ? SELECT_WAVES * 64 : 64;
-    const int t = TEAM ? threadIdx.x : lane, wave = TEAM ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+    constexpr int T = TEAM * 64;
+    const int t = TEAM > 1 ? threadIdx.x : lane, wave = TEAM > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
     auto sync = [] {
-        if constexpr (TEAM) __syncthreads();
+        if constexpr (TEAM > 1) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     };
     if (seen <= count) {
@@ -100,7 +100,7 @@ __device__ __forceinline__ void choose(const uint32_t *row, uint32_t *area, int 
 #pragma unroll 4
         for (int i = first + t; i < end; i += T) differ |= row[i] ^ one;
         differ = wave_or(differ);
-        if constexpr (TEAM) {
+        if constexpr (TEAM > 1) {
             if (t == 0) area[256] = 0;
             __syncthreads();
             if (lane == 0 && differ) atomicOr(&area[256], differ);
@@ -153,7 +153,7 @@ __device__ __forceinline__ void choose(const uint32_t *row, uint32_t *area, int 
                 ties = here;
                 break;
             }
-            if constexpr (TEAM) __syncthreads();  // (the bins are cleared again)
+            if constexpr (TEAM > 1) __syncthreads();  // (the bins are cleared again)
         }
     }
     // blocks in 64s: those above the line, and the first `ties` on it
@@ -171,9 +171,9 @@ __device__ __forceinline__ void choose(const uint32_t *row, uint32_t *area, int 
         const uint64_t taken = __ballot(take);
         if (take) out[filled + __builtin_popcountll(taken & below)] = lead + group * 64 + lane;
     };
-    if constexpr (TEAM) {
+    if constexpr (TEAM > 1) {
         uint32_t *counts = area + 257;  // [groups][2]
-        for (int group = wave; group < groups; group += SELECT_WAVES) {
+        for (int group = wave; group < groups; group += TEAM) {
             bool above, line;
             look(group, above, line);
             const int a = __builtin_popcountll(__ballot(above)), l = __builtin_popcountll(__ballot(line));
@@ -184,7 +184,7 @@ __device__ __forceinline__ void choose(const uint32_t *row, uint32_t *area, int 
         for (int g0 = 0; g0 < groups; g0 += 64) {
             const int mine_a = g0 + lane < groups ? (int)counts[2 * (g0 + lane)] : 0, mine_l = g0 + lane < groups ? (int)counts[2 * (g0 + lane) + 1] : 0;
             const int upto_a = wave_scan_int(mine_a), upto_l = wave_scan_int(mine_l);
-            for (int k = wave; k < 64 && g0 + k < groups; k += SELECT_WAVES) {
+            for (int k = wave; k < 64 && g0 + k < groups; k += TEAM) {
                 const int a = a0 + __builtin_amdgcn_readlane(upto_a - mine_a, k), l = l0 + __builtin_amdgcn_readlane(upto_l - mine_l, k);
                 bool above, line;
                 look(g0 + k, above, line);
@@ -206,190 +206,290 @@ __device__ __forceinline__ void choose(const uint32_t *row, uint32_t *area, int 
     }
 }
 
-// grid (BH, groups of `tokens` tokens), 16 wavefronts.  LDS: a histogram for each wavefront, the query operands and exponents
-// of up to four tiles of 16 rows (token by token, a token's heads side by side), keys [tokens][stride] of the blocks from
-// `lead` on.
-//
-// What it reads is a 64th of the keys' codes; at few sequences it is a chain of latencies -- queries, page entries,
-// summaries, the choice -- so that a wavefront requests the summaries of several groups of 16 blocks before it looks at the first.
+// One tile of 16 query rows as operands -- the positive and the negative part, [KS][64] each -- and the rows' exponents, by
+// one wavefront.
+template <int D, int DT>
+__device__ __forceinline__ void query_operands(const char *row, bool live, int ud, int lane, kv_i4 *pos_out, kv_i4 *neg_out, int *exps) {
+    constexpr int KS = (D + 63) / 64;
+    const int g = lane >> 4;
+    float v[KS][16], amax = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        query_chunk<DT>(row, ud, s * 64 + g * 16, live, v[s]);
+        query_chunk<DT>(row, ud, s * 64 + g * 16 + 8, live, v[s] + 8);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) amax = fmaxf(amax, fabsf(v[s][k]));
+    }
+    amax = fmaxf(amax, __shfl_xor(amax, 16));
+    amax = fmaxf(amax, __shfl_xor(amax, 32));
+    int ex = 0;
+    const float mant = frexpf(amax, &ex);  // (also of values below the smallest normal one)
+    const int f = amax > 0.f ? ex - 7 + (mant > 127.f / 128.f ? 1 : 0) : 0;
+    if (g == 0) exps[lane] = f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        kv_i4 pos, neg;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            int p = 0, m = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = (int)rintf(ldexpf(v[s][4 * w + k], -f));
+                p |= (max(i, 0) & 0xff) << (8 * k);
+                m |= (min(i, 0) & 0xff) << (8 * k);
+            }
+            pos[w] = p;
+            neg[w] = m;
+        }
+        pos_out[s * 64 + lane] = pos;
+        neg_out[s * 64 + lane] = neg;
+    }
+}
+
+// The summaries of AHEAD groups of 16 blocks, STEP groups apart, as operands, and the blocks' key scales.
+template <int D, int AHEAD, int STEP> struct Summaries {
+    static constexpr int KS = (D + 63) / 64;
+    float scale[AHEAD];
+    kv_i4 hi[AHEAD][KS], lo[AHEAD][KS];
+    __device__ __forceinline__ void load(const Store &st, int bh, int blk0, int last, int lane) {
+        const int g = lane >> 4, n = lane & 15;
+        gptr sum[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int blk = min(blk0 + u * STEP * 16 + n, last);
+            const gptr entry = as_global(st.pt + blk / BLOCK_PER_PAGE);
+            const gptr ksb = as_global(ld_global<const char *>(entry + offsetof(PageEntry, ksb)));
+            sum[u] = as_global(ld_global<const char *>(entry + offsetof(PageEntry, vsb))) + (size_t)bh * st.vsb_cell + (size_t)(blk % BLOCK_PER_PAGE) * 2 * D;
+            scale[u] = ld_global<float>(ksb + (size_t)bh * st.ksb_cell + 8 * (blk % BLOCK_PER_PAGE));
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int d = s * 64 + g * 16;
+                const bool in = D % 64 == 0 || d < D;
+                hi[u][s] = in ? ld_global<kv_i4>(sum[u] + d) : kv_i4{0, 0, 0, 0};
+                lo[u][s] = in ? ld_global<kv_i4>(sum[u] + D + d) : kv_i4{0, 0, 0, 0};
+            }
+    }
+    // The bounds of one tile of rows on them, into keys[token][stride] at block0 + u STEP 16 + n (below `blocks`).
+    // tr0: the row that the lane's first of four bounds belongs to; `rows` in all, G to a token.
+    __device__ __forceinline__ void bounds(const kv_i4 *pos_in, const kv_i4 *neg_in, const int *exps, int tr0, int rows, int G, uint32_t *keys, int stride,
+                                           int block0, int blocks, int lane) const {
+        const int g = lane >> 4, n = lane & 15;
+        int fr[4], tr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            fr[i] = exps[4 * g + i];
+            tr[i] = tr0 + i < rows ? (tr0 + i) / G : -1;
+        }
+        kv_i4 acc[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) acc[u] = kv_i4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const kv_i4 pos = pos_in[s * 64 + lane], neg = neg_in[s * 64 + lane];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                acc[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(pos, hi[u][s], acc[u], 0, 0, 0);
+                acc[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(neg, lo[u][s], acc[u], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int at = block0 + u * STEP * 16 + n;
+            if (at >= blocks) continue;
+            uint32_t key[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) key[i] = ordered(ldexpf((float)acc[u][i] * (4.f * scale[u]), fr[i]));
+            if (tr[0] >= 0 && tr[0] == tr[3]) {  // one token's rows: one entry for all four
+                atomicMax(&keys[tr[0] * stride + at], max(max(key[0], key[1]), max(key[2], key[3])));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (tr[i] >= 0) atomicMax(&keys[tr[i] * stride + at], key[i]);
+            }
+        }
+    }
+};
+
+// What a workgroup of either kernel below works on.
+struct SelectView {
+    int bh, b, G, tok0, toks, rows, pad, lead, coded;
+    __device__ __forceinline__ SelectView(const BlockSelect &x, int bh_, int tok0_, int tokens) : bh(bh_), b(bh_ / x.Hkv), G(x.Hq / x.Hkv), tok0(tok0_) {
+        toks = min(tokens, x.L - tok0);
+        rows = toks * G;
+        pad = x.left_pad ? max(x.left_pad[b], 0) : 0;
+        lead = pad / BLOCK_ROWS;
+        coded = min(x.b.coded, (x.T - x.L + tok0 + toks - 1) / BLOCK_ROWS);  // (the last token's own block is always chosen)
+    }
+    // row r of the group: token by token, a token's heads side by side
+    __device__ __forceinline__ const char *row(const BlockSelect &x, int r) const {
+        const int tok = r / G, head = r % G;
+        return static_cast<const char *>(x.q) + (((size_t)bh * G + head) * x.L + tok0 + tok) * x.b.Dk_user * 2;
+    }
+    __device__ __forceinline__ int seen(const BlockSelect &x, int tok) const {
+        const int p = x.T - x.L + tok0 + tok;
+        return p < pad ? 0 : p / BLOCK_ROWS - lead + 1;
+    }
+};
+
+// Many tokens: grid (BH, groups of `tokens` tokens), 16 wavefronts.  LDS: a histogram for each wavefront, the query operands and
+// exponents of up to four tiles of 16 rows, keys [tokens][stride] of the blocks from `lead` on.  A wavefront requests the
+// summaries of several groups of 16 blocks before it looks at the first.
 template <int D, int DT>
 __global__ void __launch_bounds__(SELECT_WAVES * 64) block_select_kernel(BlockSelect x, int tokens, int stride) {
     constexpr int KS = (D + 63) / 64, AHEAD = D <= 128 ? 4 : 2;
     extern __shared__ uint32_t lds[];
     __shared__ int exps[SELECT_TILES][16];
-    kv_i4 *ops = reinterpret_cast<kv_i4 *>(lds + SELECT_WAVES * 256);       // [tiles][positive / negative][KS][64]
-    const Store &st = x.b.st;
-    const int bh = blockIdx.x, b = bh / x.Hkv, G = x.Hq / x.Hkv;
-    const int tok0 = blockIdx.y * tokens, toks = min(tokens, x.L - tok0);
-    const int rows = toks * G, tiles = min((rows + 15) / 16, SELECT_TILES);
+    kv_i4 *ops = reinterpret_cast<kv_i4 *>(lds + SELECT_WAVES * 256);                 // [tiles][positive / negative][KS][64]
     uint32_t *keys = reinterpret_cast<uint32_t *>(ops + SELECT_TILES * 2 * KS * 64);  // [tokens][stride]
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
-    const int pad = x.left_pad ? max(x.left_pad[b], 0) : 0;
-    const int lead = pad / BLOCK_ROWS;
-    const int top = (x.T - x.L + tok0 + toks - 1) / BLOCK_ROWS;  // the last token's own block, which is always chosen
-    const int coded = min(x.b.coded, top);
-
-    for (int i = threadIdx.x; i < toks * stride; i += SELECT_WAVES * 64) keys[i] = 0;
-
+    const SelectView v(x, blockIdx.x, blockIdx.y * tokens, tokens);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    for (int i = threadIdx.x; i < v.toks * stride; i += SELECT_WAVES * 64) keys[i] = 0;
+    const int groups = v.coded > v.lead ? (v.coded - v.lead + 15) / 16 : 0;
     // (a token of more than 64 heads: its rows in turns)
-    const int ud = x.b.Dk_user;
-    for (int row0 = 0; row0 < rows; row0 += 16 * SELECT_TILES) {
+    for (int row0 = 0; row0 < v.rows; row0 += 16 * SELECT_TILES) {
+        const int tiles = min((v.rows - row0 + 15) / 16, SELECT_TILES);
         if (row0) __syncthreads();
         if (wave < tiles) {
-            const int r = row0 + 16 * wave + n;
-            const bool live = r < rows;
-            const int tok = live ? r / G : 0, head = live ? r % G : 0;
-            const char *row = static_cast<const char *>(x.q) + (((size_t)bh * G + head) * x.L + tok0 + tok) * ud * 2;
-            float v[KS][16], amax = 0.f;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                query_chunk<DT>(row, ud, s * 64 + g * 16, live, v[s]);
-                query_chunk<DT>(row, ud, s * 64 + g * 16 + 8, live, v[s] + 8);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) amax = fmaxf(amax, fabsf(v[s][k]));
-            }
-            amax = fmaxf(amax, __shfl_xor(amax, 16));
-            amax = fmaxf(amax, __shfl_xor(amax, 32));
-            int ex = 0;
-            const float mant = frexpf(amax, &ex);  // (also of values below the smallest normal one)
-            const int f = amax > 0.f ? ex - 7 + (mant > 127.f / 128.f ? 1 : 0) : 0;
-            if (g == 0) exps[wave][n] = f;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                kv_i4 pos, neg;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    int p = 0, m = 0;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int i = (int)rintf(ldexpf(v[s][4 * w + k], -f));
-                        p |= (max(i, 0) & 0xff) << (8 * k);
-                        m |= (min(i, 0) & 0xff) << (8 * k);
-                    }
-                    pos[w] = p;
-                    neg[w] = m;
-                }
-                ops[((wave * 2 + 0) * KS + s) * 64 + lane] = pos;
-                ops[((wave * 2 + 1) * KS + s) * 64 + lane] = neg;
-            }
+            const int r = row0 + 16 * wave + (lane & 15);
+            query_operands<D, DT>(v.row(x, min(r, v.rows - 1)), r < v.rows, x.b.Dk_user, lane, ops + wave * 2 * KS * 64, ops + (wave * 2 + 1) * KS * 64, exps[wave]);
         }
         __syncthreads();
-        const int groups = coded > lead ? (coded - lead + 15) / 16 : 0;
         for (int first = wave; first < groups; first += SELECT_WAVES * AHEAD) {
-            gptr sum[AHEAD];
-            float scale[AHEAD];
-            kv_i4 hi[AHEAD][KS], lo[AHEAD][KS];
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const int blk = min(lead + (first + u * SELECT_WAVES) * 16 + n, coded - 1);
-                const gptr entry = as_global(st.pt + blk / BLOCK_PER_PAGE);
-                const gptr ksb = as_global(ld_global<const char *>(entry + offsetof(PageEntry, ksb)));
-                sum[u] = as_global(ld_global<const char *>(entry + offsetof(PageEntry, vsb))) + (size_t)bh * st.vsb_cell + (size_t)(blk % BLOCK_PER_PAGE) * 2 * D;
-                scale[u] = ld_global<float>(ksb + (size_t)bh * st.ksb_cell + 8 * (blk % BLOCK_PER_PAGE));
-            }
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const int d = s * 64 + g * 16;
-                    const bool in = D % 64 == 0 || d < D;
-                    hi[u][s] = in ? ld_global<kv_i4>(sum[u] + d) : kv_i4{0, 0, 0, 0};
-                    lo[u][s] = in ? ld_global<kv_i4>(sum[u] + D + d) : kv_i4{0, 0, 0, 0};
-                }
-            for (int tile = 0; tile < tiles; ++tile) {
-                int fr[4], tr[4];  // exponents and tokens of the four rows whose bounds the lane is left with
-                const int r = row0 + 16 * tile + 4 * g;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    fr[i] = exps[tile][4 * g + i];
-                    tr[i] = r + i < rows ? (r + i) / G : -1;
-                }
-                kv_i4 acc[AHEAD];
-#pragma unroll
-                for (int u = 0; u < AHEAD; ++u) acc[u] = kv_i4{0, 0, 0, 0};
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const kv_i4 pos = ops[((tile * 2 + 0) * KS + s) * 64 + lane], neg = ops[((tile * 2 + 1) * KS + s) * 64 + lane];
-#pragma unroll
-                    for (int u = 0; u < AHEAD; ++u) {
-                        acc[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(pos, hi[u][s], acc[u], 0, 0, 0);
-                        acc[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(neg, lo[u][s], acc[u], 0, 0, 0);
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < AHEAD; ++u) {
-                    const int at = (first + u * SELECT_WAVES) * 16 + n;  // block lead + at
-                    if (lead + at >= coded) continue;
-                    uint32_t key[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) key[i] = ordered(ldexpf((float)acc[u][i] * (4.f * scale[u]), fr[i]));
-                    if (tr[0] >= 0 && tr[0] == tr[3]) {  // one token's rows: one entry for all four
-                        atomicMax(&keys[tr[0] * stride + at], max(max(key[0], key[1]), max(key[2], key[3])));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (tr[i] >= 0) atomicMax(&keys[tr[i] * stride + at], key[i]);
-                    }
-                }
-            }
+            Summaries<D, AHEAD, SELECT_WAVES> sum;
+            sum.load(x.b.st, v.bh, v.lead + first * 16, v.coded - 1, lane);
+            for (int tile = 0; tile < tiles; ++tile)
+                sum.bounds(ops + tile * 2 * KS * 64, ops + (tile * 2 + 1) * KS * 64, exps[tile], row0 + 16 * tile + 4 * (lane >> 4), v.rows, v.G, keys, stride,
+                           first * 16, v.coded - v.lead, lane);
         }
     }
     __syncthreads();
-    auto list_of = [&](int tok, auto team, uint32_t *area) {
-        const int p = x.T - x.L + tok0 + tok;
-        choose<decltype(team)::value>(keys + (size_t)tok * stride, area, lane, lead, p < pad ? 0 : p / BLOCK_ROWS - lead + 1, x.count, x.first, x.recent,
-                                      x.list + ((size_t)bh * x.L + tok0 + tok) * x.count);
-    };
-    if (toks == 1) {
-        list_of(0, std::true_type(), lds);
-    } else {
-        for (int tok = wave; tok < toks; tok += SELECT_WAVES) list_of(tok, std::false_type(), lds + wave * 256);
-    }
+    for (int tok = wave; tok < v.toks; tok += SELECT_WAVES)
+        choose<1>(keys + (size_t)tok * stride, lds + wave * 256, lane, v.lead, v.seen(x, tok), x.count, x.first, x.recent,
+                  x.list + ((size_t)v.bh * x.L + v.tok0 + tok) * x.count);
 }
 
-// Tokens a workgroup takes and the keys it keeps for each: as many tokens as fill four tiles of rows, where they are
-// that many, and fit the memory.
+// Few tokens: the bounds by as many workgroups as there are stretches of 256 (head sizes above 128: 128) blocks -- one
+// compute unit takes in a step's summaries at 13 bytes a cycle, 20 000 cycles for the 131 000 keys of one head -- and the
+// choice, a workgroup to a token, in a launch of its own.
+// grid (BH, groups of `tokens` tokens, stretches), 4 wavefronts.  out: keys [BH, L, stride].
+constexpr int BOUND_WAVES = 4, BOUND_TILES = 2;
+template <int D> constexpr int bound_ahead() { return D <= 128 ? 4 : 2; }
+template <int D, int DT>
+__global__ void __launch_bounds__(BOUND_WAVES * 64) block_bounds_kernel(BlockSelect x, int tokens, int stride, uint32_t *out) {
+    constexpr int KS = (D + 63) / 64, AHEAD = bound_ahead<D>(), SPAN = BOUND_WAVES * AHEAD * 16;
+    __shared__ kv_i4 ops[BOUND_TILES][2][KS * 64];
+    __shared__ int exps[BOUND_TILES][16];
+    __shared__ uint32_t keys[16 * BOUND_TILES * SPAN];
+    const SelectView v(x, blockIdx.x, blockIdx.y * tokens, tokens);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int from = v.lead + blockIdx.z * SPAN;  // blocks from .. from + SPAN - 1, those of them that are coded
+    if (from >= v.coded) return;
+    const int blocks = min(v.coded - from, SPAN);
+    Summaries<D, AHEAD, BOUND_WAVES> sum;
+    sum.load(x.b.st, v.bh, from + wave * 16, v.coded - 1, lane);  // (in flight while the queries are made ready)
+    for (int i = threadIdx.x; i < v.toks * SPAN; i += BOUND_WAVES * 64) keys[i] = 0;
+    for (int row0 = 0; row0 < v.rows; row0 += 16 * BOUND_TILES) {
+        const int tiles = min((v.rows - row0 + 15) / 16, BOUND_TILES);
+        if (row0) __syncthreads();
+        if (wave < tiles) {
+            const int r = row0 + 16 * wave + (lane & 15);
+            query_operands<D, DT>(v.row(x, min(r, v.rows - 1)), r < v.rows, x.b.Dk_user, lane, ops[wave][0], ops[wave][1], exps[wave]);
+        }
+        __syncthreads();
+        for (int tile = 0; tile < tiles; ++tile)
+            sum.bounds(ops[tile][0], ops[tile][1], exps[tile], row0 + 16 * tile + 4 * (lane >> 4), v.rows, v.G, keys, SPAN, wave * 16, blocks, lane);
+    }
+    __syncthreads();
+    for (int tok = 0; tok < v.toks; ++tok) {
+        uint32_t *to = out + ((size_t)v.bh * x.L + v.tok0 + tok) * stride + (from - v.lead);
+        for (int i = threadIdx.x; i < blocks; i += BOUND_WAVES * 64) to[i] = keys[tok * SPAN + i];
+    }
+}
+// grid (BH, tokens), 8 wavefronts
+constexpr int CHOOSE_WAVES = 8;
+__global__ void __launch_bounds__(CHOOSE_WAVES * 64) block_choose_kernel(BlockSelect x, int stride, const uint32_t *in) {
+    extern __shared__ uint32_t lds[];  // [257 + 2 x 64s of blocks], keys [stride]
+    const SelectView v(x, blockIdx.x, blockIdx.y, 1);
+    uint32_t *keys = lds + 260 + 2 * ((stride + 63) / 64);
+    const uint32_t *from = in + ((size_t)v.bh * x.L + v.tok0) * stride;
+    const int seen = v.seen(x, 0);
+    if (seen > x.count) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < seen - x.recent; i += CHOOSE_WAVES * 64) keys[i] = from[i];
+        __syncthreads();
+    }
+    choose<CHOOSE_WAVES>(keys, lds, threadIdx.x & 63, v.lead, seen, x.count, x.first, x.recent, x.list + ((size_t)v.bh * x.L + v.tok0) * x.count);
+}
+
+// How a call is cut: tokens a workgroup takes, the keys it keeps for each, and whether bounds and choice are apart.
 constexpr int SELECT_LDS = 156 << 10;
+constexpr size_t BOUND_KEYS = (size_t)64 << 20;  // bytes of keys between the two launches, at most
+struct SelectPlan {
+    int tokens, stride, stretches;  // stretches 0: one launch
+};
 size_t select_ops(const BlockSelect &x) { return (size_t)SELECT_TILES * 2 * ((x.b.st.Dk + 63) / 64) * 64 * 16; }
-void select_plan(const BlockSelect &x, int &tokens, int &stride) {
+SelectPlan select_plan(const BlockSelect &x) {
     const int G = x.Hq / x.Hkv;
-    stride = (x.T + BLOCK_ROWS - 1) / BLOCK_ROWS;
-    tokens = std::min(std::max(1, 16 * SELECT_TILES / G), SELECT_WAVES);
-    tokens = (int)std::min<int64_t>(tokens, (int64_t)(SELECT_LDS - SELECT_HEAD - select_ops(x)) / 4 / std::max(stride, 1));
-    tokens = std::min(tokens, x.L);
+    SelectPlan p;
+    p.stride = (x.T + BLOCK_ROWS - 1) / BLOCK_ROWS;
+    p.stretches = 0;
+    p.tokens = std::min(std::max(1, 16 * SELECT_TILES / G), SELECT_WAVES);
+    p.tokens = (int)std::min<int64_t>(p.tokens, (int64_t)(SELECT_LDS - SELECT_HEAD - select_ops(x)) / 4 / std::max(p.stride, 1));
+    p.tokens = std::min(p.tokens, x.L);
+    if (p.tokens < 1) return p;
+    const int64_t groups = (int64_t)x.b.st.BH * ((x.L + p.tokens - 1) / p.tokens);
+    const int span = BOUND_WAVES * 16 * (x.b.st.Dk <= 128 ? 4 : 2);
+    // (up to that many blocks one launch is the shorter)
+    if (groups < 128 && p.stride > 256 && (size_t)x.b.st.BH * x.L * p.stride * 4 <= BOUND_KEYS) {
+        p.tokens = std::min(p.tokens, std::max(1, 16 * BOUND_TILES / G));
+        p.stretches = (p.stride + span - 1) / span;
+    }
+    return p;
+}
+template <int D, int DT> hipError_t select_run(const BlockSelect &x, hipStream_t stream) {
+    const SelectPlan p = select_plan(x);
+    const unsigned groups = (x.L + p.tokens - 1) / p.tokens;
+    if (p.stretches) {
+        uint32_t *keys = static_cast<uint32_t *>(x.workspace);
+        hipLaunchKernelGGL((block_bounds_kernel<D, DT>), dim3(x.b.st.BH, groups, p.stretches), dim3(BOUND_WAVES * 64), 0, stream, x, p.tokens, p.stride, keys);
+        hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        const size_t lds = 4 * (size_t)(260 + 2 * ((p.stride + 63) / 64) + p.stride);
+        if (lds > 65536) {
+            e = hipFuncSetAttribute(reinterpret_cast<const void *>(block_choose_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, SELECT_LDS);
+            if (e != hipSuccess) return e;
+        }
+        hipLaunchKernelGGL(block_choose_kernel, dim3(x.b.st.BH, x.L), dim3(CHOOSE_WAVES * 64), lds, stream, x, p.stride, keys);
+        return hipGetLastError();
+    }
+    const size_t lds = SELECT_HEAD + select_ops(x) + (size_t)p.tokens * p.stride * 4;
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(block_select_kernel<D, DT>), hipFuncAttributeMaxDynamicSharedMemorySize, SELECT_LDS);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((block_select_kernel<D, DT>), dim3(x.b.st.BH, groups), dim3(SELECT_WAVES * 64), lds, stream, x, p.tokens, p.stride);
+    return hipGetLastError();
 }
 template <int DT> hipError_t select_dtype(const BlockSelect &x, hipStream_t stream) {
-    int tokens, stride;
-    select_plan(x, tokens, stride);
-    const dim3 grid(x.b.st.BH, (x.L + tokens - 1) / tokens), block(SELECT_WAVES * 64);
-    const size_t lds = SELECT_HEAD + select_ops(x) + (size_t)tokens * stride * 4;
-#define KV_SELECT(D)                                                                                                    \
-    do {                                                                                                                \
-        if (lds > 65536) {                                                                                              \
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(block_select_kernel<D, DT>),        \
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, SELECT_LDS);           \
-            if (e != hipSuccess) return e;                                                                              \
-        }                                                                                                               \
-        hipLaunchKernelGGL((block_select_kernel<D, DT>), grid, block, lds, stream, x, tokens, stride);                  \
-        return hipGetLastError();                                                                                       \
-    } while (0)
     switch (x.b.st.Dk) {
-        case 64: KV_SELECT(64);
-        case 96: KV_SELECT(96);
-        case 128: KV_SELECT(128);
-        case 192: KV_SELECT(192);
-        case 256: KV_SELECT(256);
+        case 64: return select_run<64, DT>(x, stream);
+        case 96: return select_run<96, DT>(x, stream);
+        case 128: return select_run<128, DT>(x, stream);
+        case 192: return select_run<192, DT>(x, stream);
+        case 256: return select_run<256, DT>(x, stream);
     }
-#undef KV_SELECT
     return hipErrorInvalidValue;
 }
 
 }  // namespace
 
-bool block_select_supported(const BlockSelect &x) {
-    int tokens, stride;
-    select_plan(x, tokens, stride);
-    return tokens >= 1;  // (the keys of one token fit)
+bool block_select_supported(const BlockSelect &x) { return select_plan(x).tokens >= 1; }  // (the keys of one token fit)
+size_t block_select_workspace(const BlockSelect &x) {
+    const SelectPlan p = select_plan(x);
+    return p.stretches ? (size_t)x.b.st.BH * x.L * p.stride * 4 : 0;
 }
 hipError_t launch_block_select(const BlockSelect &x, hipStream_t stream) {
     return x.b.st.dtype == KVHIP_F16 ? select_dtype<0>(x, stream) : select_dtype<1>(x, stream);
