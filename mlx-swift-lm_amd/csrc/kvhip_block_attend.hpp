@@ -37,14 +37,19 @@ template <int DT> __device__ __forceinline__ kv_f4 block_mfma(const kv_u4 &x, co
 template <int DT> __device__ __forceinline__ kv_u4 block_operand(uint32_t lo, uint32_t hi, float scale) {
     return kv_u4{block_values<DT, false>(lo, scale), block_values<DT, true>(lo, scale), block_values<DT, false>(hi, scale), block_values<DT, true>(hi, scale)};
 }
-// over the four lanes of a query row
+// Over the four lanes of a query row (16 apart), in each of them: halves and rows of 16 change places by one vector
+// instruction each, nothing goes through LDS.
+template <class OP> __device__ __forceinline__ float row_reduce(float v, OP op) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ __forceinline__ float row_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    return row_reduce(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float row_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    return row_reduce(v, [](float a, float b) { return a + b; });
 }
 
 // What a wavefront requests of a block: keys as [token tile][chunk of 64 channels] of 16 bytes a lane (a last chunk of 32: 8),
