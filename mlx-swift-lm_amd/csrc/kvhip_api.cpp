@@ -743,6 +743,19 @@ BlockStore block_store(const kvhip_cache *c) {
     s.coded = (int32_t)c->coded;
     s.Dk_user = c->Dk_user;
     s.Dv_user = c->Dv_user;
+    if (c->slabs.size() <= (size_t)BLOCK_SLABS) {  // (as ensure_slots lays a slab out)
+        const size_t BH = c->st.BH;
+        s.slabs.n = (int32_t)c->slabs.size();
+        for (size_t i = 0; i < c->slabs.size(); ++i) {
+            const Slab &sl = c->slabs[i];
+            const size_t k = align256(BH * c->st.k_cell * sl.pages), v = align256(BH * c->st.v_cell * sl.pages);
+            s.slabs.first[i] = (int32_t)sl.first_page;
+            s.slabs.k[i] = static_cast<char *>(sl.base);
+            s.slabs.v[i] = s.slabs.k[i] + k;
+            s.slabs.ksb[i] = s.slabs.v[i] + v;
+            s.slabs.vsb[i] = s.slabs.ksb[i] + align256(BH * c->st.ksb_cell * sl.pages);
+        }
+    }
     return s;
 }
 // `launch` false: the attention kernel writes the row of a single token that finishes no block (block_step_fuses).

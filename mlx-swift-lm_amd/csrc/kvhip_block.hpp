@@ -32,12 +32,23 @@ constexpr int BLOCK_PER_PAGE = PAGE / BLOCK_ROWS;
 constexpr int BLOCK_LEAST_EXP = -100;
 constexpr int BLOCK_MAX_HEAD = 256;
 
+// Where pages lie, in a kernel's arguments: pages [first[i], first[i + 1]) are regular from the addresses of slab i on (one
+// allocation each; a cache that grew has a few).  A page's entry in the page table is a load in front of everything else a short
+// kernel reads: 3000 of a small step's 19 000 cycles.  n = 0: more slabs than this holds, the page table answers.
+constexpr int BLOCK_SLABS = 4;
+struct BlockSlabs {
+    int32_t n = 0;
+    int32_t first[BLOCK_SLABS] = {};
+    char *k[BLOCK_SLABS] = {}, *v[BLOCK_SLABS] = {}, *ksb[BLOCK_SLABS] = {}, *vsb[BLOCK_SLABS] = {};
+};
+
 // A block-scaled cache as its kernels see it.  `coded`: blocks held as codes; rows from 64 coded on are in the tail.
 struct BlockStore {
     Store st;
     char *tail_k = nullptr, *tail_v = nullptr;
     int32_t coded = 0;
     int32_t Dk_user = 0, Dv_user = 0;  // head sizes of the caller's arrays (the stored ones are padded with zeros)
+    BlockSlabs slabs;
 };
 
 // Rows [pos0, pos0 + n) of the dense arrays [BH, n, D], written behind the pos0 rows that the cache holds.  Those that leave
@@ -56,10 +67,11 @@ struct BlockAttend {
     int32_t count = 0;
     const int32_t *left_pad = nullptr;
     // plan
-    int32_t nsplit = 1;   // parts of a row's blocks
-    int32_t tiles = 1;    // (listed blocks) 16-row tiles of a token's heads
+    int32_t nsplit = 1;  // parts of a row's blocks
+    int32_t tiles = 1;   // (listed blocks) 16-row tiles of a token's heads
+    int32_t waves = 4;   // wavefronts of a workgroup
 };
-// Chooses nsplit and tiles within a.workspace_cap; returns the bytes of scratch.
+// Chooses the plan within a.workspace_cap; returns the bytes of scratch.
 size_t plan_block_attend(BlockAttend &x);
 int64_t block_attend_rows(const BlockAttend &x);  // tiles of query rows of a pair (at most 65535)
 hipError_t launch_block_attend(const BlockAttend &x, hipStream_t stream);
@@ -79,6 +91,24 @@ size_t block_select_workspace(const BlockSelect &x);
 hipError_t launch_block_select(const BlockSelect &x, hipStream_t stream);
 
 #if defined(__HIPCC__)
+// The entry of a page (of any lane's own).
+__device__ __forceinline__ PageEntry block_page(const BlockStore &s, int page) {
+    if (s.slabs.n == 0) return s.st.pt[page];
+    PageEntry e{s.slabs.k[0], s.slabs.ksb[0], s.slabs.v[0], s.slabs.vsb[0]};
+    int first = 0;
+#pragma unroll
+    for (int i = 1; i < BLOCK_SLABS; ++i)
+        if (i < s.slabs.n && page >= s.slabs.first[i]) {
+            e = PageEntry{s.slabs.k[i], s.slabs.ksb[i], s.slabs.v[i], s.slabs.vsb[i]};
+            first = s.slabs.first[i];
+        }
+    const uint64_t at = (uint64_t)(uint32_t)(page - first) * (uint32_t)s.st.BH;
+    e.k += at * s.st.k_cell;
+    e.ksb += at * s.st.ksb_cell;
+    e.v += at * s.st.v_cell;
+    e.vsb += at * s.st.vsb_cell;
+    return e;
+}
 // byte of (row, channel) inside a block of keys / of values
 __device__ __forceinline__ uint32_t block_k_at(uint32_t D, uint32_t r, uint32_t d) {
     const uint32_t c = d >> 6, m = r & 15, base = (r >> 4) * 16 * D + c * 1024;

@@ -78,8 +78,11 @@ size_t plan_block_attend(BlockAttend &x) {
     x.tiles = (G + 15) / 16;
     const int64_t base = a.st.BH * block_attend_rows(x);
     const int blocks = x.list ? x.count : (a.T + BLOCK_ROWS - 1) / BLOCK_ROWS;
-    const int64_t slots = a.st.Dk <= 128 ? 512 : 256;
-    int64_t parts = std::max<int64_t>(1, slots / base);
+    // Wavefronts that fill the chip, two to a SIMD where the registers allow it; workgroups of eight where they serve one row
+    // tile and there is work for them: their parts meet in LDS, and half as many are left to merge.
+    const int64_t wanted = (a.st.Dk <= 128 ? 2048 : 1024) / std::max<int64_t>(base, 1);
+    x.waves = nm == 1 && a.st.Dk <= 128 && a.mask.mode != KVHIP_MASK_ARRAY && wanted >= 8 && blocks > 4 ? 8 : 4;
+    int64_t parts = std::max<int64_t>(1, wanted / x.waves);
     parts = std::min<int64_t>(parts, std::max(1, blocks / 8));
     parts = std::min<int64_t>(parts, MERGE_PARTS);
     const size_t one = (size_t)a.st.BH * G * a.L * (a.st.Dv + 2) * sizeof(float);

@@ -255,27 +255,44 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
         const int fresh = a.new_k ? a.T - 1 - j0 : -1;  // that row
         const char *nk = static_cast<const char *>(a.new_k) + (size_t)bh * DK * 2;
         const uint16_t *nv = static_cast<const uint16_t *>(a.new_v) + (size_t)bh * DV;
-        kv_f4 s[NM][4];
+        // (everything is requested at once: keys, then, behind the score product, values)
+        kv_u4 w[4 * KS > 2 * VT ? 4 * KS : 2 * VT];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             const int r = 16 * t + n;
-            const char *row = r == fresh ? nk : tk + (size_t)r * DK * 2;
-#pragma unroll
-            for (int i = 0; i < NM; ++i) s[i][t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+            const gptr row = as_global(r == fresh ? nk : tk + (size_t)r * DK * 2);
 #pragma unroll
             for (int c = 0; c < KS; ++c) {
                 // the channels that the query operands hold at this step (those of a block's chunks)
                 const int d = (c | 1) < KS ? (c >> 1) * 64 + g * 16 + (c & 1) * 8 : c * 32 + g * 8;
-                kv_u4 w = load_row16(row + 2 * d);
+                w[t * KS + c] = ld_global<kv_out8>(row + 2 * d);
+            }
+        }
+        kv_f4 s[NM][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int i = 0; i < NM; ++i) s[i][t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KS; ++c) {
+                kv_u4 y = w[t * KS + c];
                 if (fresh >= 0) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) w[k] = no_infinities<DT>(w[k]);
+                    for (int k = 0; k < 4; ++k) y[k] = no_infinities<DT>(y[k]);
                 }
 #pragma unroll
-                for (int i = 0; i < NM; ++i) s[i][t] = block_mfma<DT>(w, q[i][c], s[i][t]);
+                for (int i = 0; i < NM; ++i) s[i][t] = block_mfma<DT>(y, q[i][c], s[i][t]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int d = 0; d < VT; ++d)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) w[2 * d + u] = ld_global<kv_u4>(as_global(tv + ((size_t)(4 * u + g) * DV + 16 * d + n) * 16));
+        uint32_t e[VT];
+#pragma unroll
+        for (int d = 0; d < VT; ++d) e[d] = fresh >= 0 ? (uint32_t)ld_global<uint16_t>(as_global(nv + 16 * d + n)) : 0u;
+        __builtin_amdgcn_sched_barrier(0);
         kv_u4 p[NM][2];
         uint32_t seen[NM];
 #pragma unroll
@@ -288,41 +305,55 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
             weigh(i, s[i], p[i]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        constexpr uint32_t INF = DT == 1 ? 0x7f80u : 0x7c00u, ONE = DT == 1 ? 0x3f80u : 0x3c00u;
+        if (fresh >= 0) {  // (element 4 h + i is token 32 u + 16 h + 4 g + i)
+            const int at = ((fresh >> 4) & 1) * 4 + (fresh & 3);
+            const uint32_t mine = ((fresh >> 2) & 3) == g ? (at & 1 ? 0xffff0000u : 0xffffu) : 0u;
 #pragma unroll
-        for (int d = 0; d < VT; ++d) {
-            const int col = 16 * d + n;
-            kv_u4 w[2], bad[2];
-            bool nan = false;
+            for (int d = 0; d < VT; ++d) {
+                const uint32_t x = no_infinities<DT>(e[d] | (e[d] << 16));
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                w[u] = *reinterpret_cast<const kv_u4 *>(tv + ((size_t)(4 * u + g) * DV + col) * 16);
-                // (element 4 h + i is token 32 u + 16 h + 4 g + i)
-                if (fresh >= 0 && (fresh >> 5) == u && ((fresh >> 2) & 3) == g) {
-                    const int at = ((fresh >> 4) & 1) * 4 + (fresh & 3);
-                    const uint32_t e = no_infinities<DT>((uint32_t)nv[col]);
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if ((at >> 1) == k) w[u][k] = at & 1 ? (w[u][k] & 0xffffu) | (e << 16) : (w[u][k] & 0xffff0000u) | e;
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    // (rows that were never written hold anything, infinities too)
-                    const bool lo = (w[u][k] & 0x7fffu) >= INF, hi = ((w[u][k] >> 16) & 0x7fffu) >= INF;
-                    bad[u][k] = (lo ? ONE : 0u) | (hi ? ONE << 16 : 0u);
-                    w[u][k] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
-                    nan = nan || lo || hi;
-                }
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t here = (fresh >> 5) == u && (at >> 1) == k ? mine : 0u;
+                        w[2 * d + u][k] = (w[2 * d + u][k] & ~here) | (x & here);
+                    }
             }
-            if (__any(nan)) {
+        }
+        // NaN (and, in rows that were never written, anything)
+        constexpr uint32_t INF = DT == 1 ? 0x7f80u : 0x7c00u, ONE = DT == 1 ? 0x3f80u : 0x3c00u;
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 2 * VT; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t h = w[j][k] & 0x7fff7fffu;
+                top = max(top, max(h & 0xffffu, h >> 16));
+            }
+        if (__any(top >= INF)) {
+#pragma unroll
+            for (int d = 0; d < VT; ++d) {
+                kv_u4 bad[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t y = w[2 * d + u][k];
+                        const bool lo = (y & 0x7fffu) >= INF, hi = ((y >> 16) & 0x7fffu) >= INF;
+                        bad[u][k] = (lo ? ONE : 0u) | (hi ? ONE << 16 : 0u);
+                        w[2 * d + u][k] = y & ((lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u));
+                    }
 #pragma unroll
                 for (int i = 0; i < NM; ++i) poison(i, d, seen[i], bad);
+                __builtin_amdgcn_sched_barrier(0);
             }
+        }
+#pragma unroll
+        for (int d = 0; d < VT; ++d) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int i = 0; i < NM; ++i) o[i][d] = block_mfma<DT>(w[u], p[i][u], o[i][d]);
-            __builtin_amdgcn_sched_barrier(0);
+                for (int i = 0; i < NM; ++i) o[i][d] = block_mfma<DT>(w[2 * d + u], p[i][u], o[i][d]);
         }
     }
 };
@@ -349,7 +380,7 @@ __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kerne
     int lo = 0, hi = a.T - 1;        // keys that some row sees
     if constexpr (MODE == 1) {
         const int last = min(row0 + 16 * NM, R) - 1;
-        const bool one_head = row0 / a.L == last / a.L;
+        const bool one_head = a.L > 1 && row0 / a.L == last / a.L;
         const KeyBounds f = sym_mask_bounds(sym, one_head ? row0 % a.L : 0), e = sym_mask_bounds(sym, one_head ? last % a.L : a.L - 1);
         in_lo = max(e.lo, 0);
         in_hi = min(f.hi, a.T - 1);
@@ -372,8 +403,13 @@ __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kerne
             w.q[i][c] = live && a.scale != 0.f ? load_row16(row + 2 * d) : kv_u4{0u, 0u, 0u, 0u};
             if (!Walk::SAFE && a.scale < 0.f) w.q[i][c] ^= 0x80008000u;
         }
-        w.ql[i] = live ? r % a.L : 0;
-        w.qh[i] = live ? w.h * G + r / a.L : -1;
+        if (MODE == 3 || a.L == 1) {  // (no divisions in front of a step's first request)
+            w.ql[i] = 0;
+            w.qh[i] = live ? w.h * G + r : -1;
+        } else {
+            w.ql[i] = live ? r % a.L : 0;
+            w.qh[i] = live ? w.h * G + r / a.L : -1;
+        }
         w.see[i] = KeyBounds{lo, hi};
         if constexpr (MODE == 1) {
             const KeyBounds k = sym_mask_bounds(sym, w.ql[i]);
@@ -407,11 +443,11 @@ __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kerne
         uint64_t kp = 0, vp = 0;
         float ks = 1.f, vs = 1.f;
         if (blk >= 0 && blk < x.b.coded) {
-            const PageEntry &e = a.st.pt[blk / BLOCK_PER_PAGE];
+            const PageEntry e = block_page(x.b, blk / BLOCK_PER_PAGE);
             const int in_page = blk % BLOCK_PER_PAGE;
             kp = reinterpret_cast<uint64_t>(e.k + (size_t)bh * a.st.k_cell + (size_t)in_page * BLOCK_ROWS * DK);
             vp = reinterpret_cast<uint64_t>(e.v + (size_t)bh * a.st.v_cell + (size_t)in_page * BLOCK_ROWS * DV);
-            const kv_f2 sc = *reinterpret_cast<const kv_f2 *>(e.ksb + (size_t)bh * a.st.ksb_cell + in_page * 8);
+            const kv_f2 sc = ld_global<kv_f2>(as_global(e.ksb) + (size_t)bh * a.st.ksb_cell + in_page * 8);
             ks = sc.x;
             vs = sc.y;
         }
@@ -503,12 +539,14 @@ __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kerne
     }
 }
 
-template <int DK, int DV, int DT, int NM, int MODE> hipError_t block_attend_run(const BlockAttend &x, hipStream_t stream) {
-    constexpr int NW = 4;
+template <int DK, int DV, int DT, int NM, int MODE, int NW = 4> hipError_t block_attend_run(const BlockAttend &x, hipStream_t stream) {
     hipLaunchKernelGGL((block_attend_kernel<DK, DV, DT, NM, MODE, NW>), dim3(x.a.st.BH, block_attend_rows(x), x.nsplit), dim3(NW * 64), 0, stream, x);
     return hipGetLastError();
 }
 template <int DK, int DV, int DT> hipError_t block_attend_shape(const BlockAttend &x, hipStream_t stream) {
+    if constexpr (DK <= 128) {
+        if (x.waves == 8) return x.list ? block_attend_run<DK, DV, DT, 1, 3, 8>(x, stream) : block_attend_run<DK, DV, DT, 1, 1, 8>(x, stream);
+    }
     if (x.list) return block_attend_run<DK, DV, DT, 1, 3>(x, stream);
     const int nm = block_row_tiles(x);
     if (x.a.mask.mode == KVHIP_MASK_ARRAY)

@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(256) block_append_kernel(BlockStore s, const c
     a.blk = (int)(pos0 / BLOCK_ROWS) + blockIdx.x;
     a.bh = blockIdx.y;
     a.reopened = a.blk < s.coded && pos0 > a.lo();
-    const PageEntry &e = s.st.pt[a.blk / BLOCK_PER_PAGE];
+    const PageEntry e = block_page(s, a.blk / BLOCK_PER_PAGE);
     const int in_page = a.blk % BLOCK_PER_PAGE, bh = a.bh;
     float *scales = reinterpret_cast<float *>(e.ksb + (size_t)bh * s.st.ksb_cell) + 2 * in_page + (v ? 1 : 0);
     const float held = a.reopened ? *scales : 1.f;
@@ -360,7 +360,7 @@ __device__ __forceinline__ void fetch_block(const BlockStore &s, int64_t rows, c
     const int64_t lo = (int64_t)blk * BLOCK_ROWS;
     const int upto = (int)(rows - lo < BLOCK_ROWS ? rows - lo : BLOCK_ROWS);
     const bool coded = blk < s.coded;
-    const PageEntry &e = s.st.pt[blk / BLOCK_PER_PAGE];
+    const PageEntry e = block_page(s, blk / BLOCK_PER_PAGE);
     const int in_page = blk % BLOCK_PER_PAGE;
     const char *tail = (V ? s.tail_v : s.tail_k) + (size_t)bh * BLOCK_ROWS * D * 2;
     char *out = dst + ((size_t)bh * rows + lo) * ud * 2;

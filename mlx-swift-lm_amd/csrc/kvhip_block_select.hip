@@ -251,16 +251,16 @@ template <int D, int AHEAD, int STEP> struct Summaries {
     static constexpr int KS = (D + 63) / 64;
     float scale[AHEAD];
     kv_i4 hi[AHEAD][KS], lo[AHEAD][KS];
-    __device__ __forceinline__ void load(const Store &st, int bh, int blk0, int last, int lane) {
+    __device__ __forceinline__ void load(const BlockStore &b, int bh, int blk0, int last, int lane) {
+        const Store &st = b.st;
         const int g = lane >> 4, n = lane & 15;
         gptr sum[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int blk = min(blk0 + u * STEP * 16 + n, last);
-            const gptr entry = as_global(st.pt + blk / BLOCK_PER_PAGE);
-            const gptr ksb = as_global(ld_global<const char *>(entry + offsetof(PageEntry, ksb)));
-            sum[u] = as_global(ld_global<const char *>(entry + offsetof(PageEntry, vsb))) + (size_t)bh * st.vsb_cell + (size_t)(blk % BLOCK_PER_PAGE) * 2 * D;
-            scale[u] = ld_global<float>(ksb + (size_t)bh * st.ksb_cell + 8 * (blk % BLOCK_PER_PAGE));
+            const PageEntry e = block_page(b, blk / BLOCK_PER_PAGE);
+            sum[u] = as_global(e.vsb) + (size_t)bh * st.vsb_cell + (size_t)(blk % BLOCK_PER_PAGE) * 2 * D;
+            scale[u] = ld_global<float>(as_global(e.ksb) + (size_t)bh * st.ksb_cell + 8 * (blk % BLOCK_PER_PAGE));
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(SELECT_WAVES * 64) block_select_kernel(BlockSe
         __syncthreads();
         for (int first = wave; first < groups; first += SELECT_WAVES * AHEAD) {
             Summaries<D, AHEAD, SELECT_WAVES> sum;
-            sum.load(x.b.st, v.bh, v.lead + first * 16, v.coded - 1, lane);
+            sum.load(x.b, v.bh, v.lead + first * 16, v.coded - 1, lane);
             for (int tile = 0; tile < tiles; ++tile)
                 sum.bounds(ops + tile * 2 * KS * 64, ops + (tile * 2 + 1) * KS * 64, exps[tile], row0 + 16 * tile + 4 * (lane >> 4), v.rows, v.G, keys, stride,
                            first * 16, v.coded - v.lead, lane);
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(BOUND_WAVES * 64) block_bounds_kernel(BlockSel
     if (from >= v.coded) return;
     const int blocks = min(v.coded - from, SPAN);
     Summaries<D, AHEAD, BOUND_WAVES> sum;
-    sum.load(x.b.st, v.bh, from + wave * 16, v.coded - 1, lane);  // (in flight while the queries are made ready)
+    sum.load(x.b, v.bh, from + wave * 16, v.coded - 1, lane);  // (in flight while the queries are made ready)
     for (int i = threadIdx.x; i < v.toks * SPAN; i += BOUND_WAVES * 64) keys[i] = 0;
     for (int row0 = 0; row0 < v.rows; row0 += 16 * BOUND_TILES) {
         const int tiles = min((v.rows - row0 + 15) / 16, BOUND_TILES);
