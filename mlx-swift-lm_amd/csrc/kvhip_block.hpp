@@ -96,12 +96,14 @@ __device__ __forceinline__ PageEntry block_page(const BlockStore &s, int page) {
     if (s.slabs.n == 0) return s.st.pt[page];
     PageEntry e{s.slabs.k[0], s.slabs.ksb[0], s.slabs.v[0], s.slabs.vsb[0]};
     int first = 0;
+    if (s.slabs.n > 1) {
 #pragma unroll
-    for (int i = 1; i < BLOCK_SLABS; ++i)
-        if (i < s.slabs.n && page >= s.slabs.first[i]) {
-            e = PageEntry{s.slabs.k[i], s.slabs.ksb[i], s.slabs.v[i], s.slabs.vsb[i]};
-            first = s.slabs.first[i];
-        }
+        for (int i = 1; i < BLOCK_SLABS; ++i)
+            if (i < s.slabs.n && page >= s.slabs.first[i]) {
+                e = PageEntry{s.slabs.k[i], s.slabs.ksb[i], s.slabs.v[i], s.slabs.vsb[i]};
+                first = s.slabs.first[i];
+            }
+    }
     const uint64_t at = (uint64_t)(uint32_t)(page - first) * (uint32_t)s.st.BH;
     e.k += at * s.st.k_cell;
     e.ksb += at * s.st.ksb_cell;

@@ -16,6 +16,7 @@ namespace kvhip {
 namespace {
 
 typedef int kv_i4 __attribute__((ext_vector_type(4)));
+typedef unsigned short kv_us2 __attribute__((ext_vector_type(2)));
 
 // floats in an order that unsigned integers have too; 0 is below all of them
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -51,8 +52,8 @@ constexpr int SELECT_WAVES = 16;
 constexpr int SELECT_TILES = 4;  // at most so many tiles of 16 query rows to a workgroup
 constexpr int SELECT_HEAD = SELECT_WAVES * 256 * 4;  // bytes of the histograms
 
-// Eight channels of a query row as floats; elements that are no numbers, and those past the end, are zeros.
-template <int DT> __device__ __forceinline__ void query_chunk(const char *row, int ud, int d, bool live, float *y) {
+// Eight channels of a query row, two to a word (zeros past the end).
+__device__ __forceinline__ kv_u4 query_chunk(const char *row, int ud, int d, bool live) {
     kv_u4 w{0u, 0u, 0u, 0u};
     if (live && d + 8 <= ud) {
         w = load_row16(row + 2 * d);
@@ -61,12 +62,11 @@ template <int DT> __device__ __forceinline__ void query_chunk(const char *row, i
         for (int i = 0; i < 8; ++i)
             if (d + i < ud) w[i >> 1] |= (uint32_t) reinterpret_cast<const uint16_t *>(row)[d + i] << (16 * (i & 1));
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t h = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-        const float v = DT == 1 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
-        y[i] = fabsf(v) < INFINITY ? v : 0.f;
-    }
+    return w;
+}
+template <int DT> __device__ __forceinline__ float float_at(uint32_t w, int half) {
+    const uint32_t h = half ? w >> 16 : w & 0xffffu;
+    return DT == 1 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
 }
 
 // A token's list: `count` of the blocks lead .. lead + seen - 1, the first `first` and the last `recent` of them and the
@@ -75,7 +75,7 @@ template <int DT> __device__ __forceinline__ void query_chunk(const char *row, i
 //
 // The smallest chosen key is found digit by digit, eight bits at a time from the first bit in which the keys differ (their
 // exponents mostly agree: from bit 31 on nearly all fall into one bin, and one address takes one addition a cycle), until
-// a bin is taken whole.  `area`: 256 bins and, behind them, a pair of counts for every 64 blocks (TEAM > 1).
+// a bin is taken whole.  `area`: 256 bins and, behind them, the differing bits and a pair of counts for each wavefront (TEAM > 1).
 template <int TEAM>
 __device__ __forceinline__ void choose(const uint32_t *row, uint32_t *area, int lane, int lead, int seen, int count, int first, int recent, int32_t *out) {
     constexpr int T = TEAM * 64;
@@ -172,26 +172,32 @@ __device__ __forceinline__ void choose(const uint32_t *row, uint32_t *area, int 
         if (take) out[filled + __builtin_popcountll(taken & below)] = lead + group * 64 + lane;
     };
     if constexpr (TEAM > 1) {
-        uint32_t *counts = area + 257;  // [groups][2]
-        for (int group = wave; group < groups; group += TEAM) {
+        // a wavefront to a stretch of groups, behind what the wavefronts before it hold
+        uint32_t *counts = area + 257;  // [TEAM][2]
+        const int each = (groups + TEAM - 1) / TEAM, g0 = wave * each, g1 = min(g0 + each, groups);
+        int a = 0, l = 0;
+        for (int group = g0; group < g1; ++group) {
             bool above, line;
             look(group, above, line);
-            const int a = __builtin_popcountll(__ballot(above)), l = __builtin_popcountll(__ballot(line));
-            if (lane == 0) counts[2 * group] = a, counts[2 * group + 1] = l;
+            a += __builtin_popcountll(__ballot(above));
+            l += __builtin_popcountll(__ballot(line));
         }
+        if (lane == 0) counts[2 * wave] = a, counts[2 * wave + 1] = l;
         __syncthreads();
-        int a0 = 0, l0 = 0;  // what the groups before `g0` hold
-        for (int g0 = 0; g0 < groups; g0 += 64) {
-            const int mine_a = g0 + lane < groups ? (int)counts[2 * (g0 + lane)] : 0, mine_l = g0 + lane < groups ? (int)counts[2 * (g0 + lane) + 1] : 0;
-            const int upto_a = wave_scan_int(mine_a), upto_l = wave_scan_int(mine_l);
-            for (int k = wave; k < 64 && g0 + k < groups; k += TEAM) {
-                const int a = a0 + __builtin_amdgcn_readlane(upto_a - mine_a, k), l = l0 + __builtin_amdgcn_readlane(upto_l - mine_l, k);
-                bool above, line;
-                look(g0 + k, above, line);
-                write(g0 + k, above, __ballot(line), max(ties - l, 0), a + min(l, ties));
-            }
-            a0 += __builtin_amdgcn_readlane(upto_a, 63);
-            l0 += __builtin_amdgcn_readlane(upto_l, 63);
+        int filled = 0, lines = 0;
+        for (int w = 0; w < wave; ++w) {
+            filled += (int)counts[2 * w];
+            lines += (int)counts[2 * w + 1];
+        }
+        filled += min(lines, ties);
+        int left = max(ties - lines, 0);
+        for (int group = g0; group < g1; ++group) {
+            bool above, line;
+            look(group, above, line);
+            const uint64_t on = __ballot(line);
+            write(group, above, on, left, filled);
+            filled += __builtin_popcountll(__ballot(above)) + min(left, (int)__builtin_popcountll(on));
+            left -= min(left, (int)__builtin_popcountll(on));
         }
     } else {
         int filled = 0, left = ties;
@@ -206,40 +212,67 @@ __device__ __forceinline__ void choose(const uint32_t *row, uint32_t *area, int 
     }
 }
 
-// One tile of 16 query rows as operands -- the positive and the negative part, [KS][64] each -- and the rows' exponents, by
-// one wavefront.
+// What is kept of a tile of 16 query rows beside its operands: exponents, and the token (of the workgroup's) of each, or -1.
+struct RowsOf {
+    int exp[16], tok[16];
+};
+// One tile of 16 query rows as operands -- the positive and the negative part, [KS][64] each -- by one wavefront.  Everything
+// else in the workgroup waits for it: the largest magnitude as a packed integer maximum, a number that is none only looked for
+// where there is one, whole numbers by an addition that leaves them in the low bits (5700 -> 2000 cycles of a step).
 template <int D, int DT>
-__device__ __forceinline__ void query_operands(const char *row, bool live, int ud, int lane, kv_i4 *pos_out, kv_i4 *neg_out, int *exps) {
+__device__ __forceinline__ void query_operands(const char *row, int tok, int ud, int lane, kv_i4 *pos_out, kv_i4 *neg_out, RowsOf &of) {
     constexpr int KS = (D + 63) / 64;
+    constexpr uint32_t INF = DT == 1 ? 0x7f80u : 0x7c00u;
     const int g = lane >> 4;
-    float v[KS][16], amax = 0.f;
+    kv_u4 w[KS][2];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        query_chunk<DT>(row, ud, s * 64 + g * 16, live, v[s]);
-        query_chunk<DT>(row, ud, s * 64 + g * 16 + 8, live, v[s] + 8);
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) amax = fmaxf(amax, fabsf(v[s][k]));
+        for (int h = 0; h < 2; ++h) w[s][h] = query_chunk(row, ud, s * 64 + g * 16 + 8 * h, tok >= 0);
+    auto largest = [&] {
+        kv_us2 m{0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(kv_us2, w[s][i >> 2][i & 3] & 0x7fff7fffu));
+        return max((uint32_t)m[0], (uint32_t)m[1]);
+    };
+    uint32_t mag = largest();
+    if (mag >= INF) {  // elements that are no numbers have no say
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t x = w[s][i >> 2][i & 3];
+                w[s][i >> 2][i & 3] = ((x & 0x7fffu) >= INF ? 0u : x & 0xffffu) | (((x >> 16) & 0x7fffu) >= INF ? 0u : x & 0xffff0000u);
+            }
+        mag = largest();
     }
-    amax = fmaxf(amax, __shfl_xor(amax, 16));
-    amax = fmaxf(amax, __shfl_xor(amax, 32));
+    mag = max(mag, (uint32_t)__shfl_xor(mag, 16));
+    mag = max(mag, (uint32_t)__shfl_xor(mag, 32));
     int ex = 0;
-    const float mant = frexpf(amax, &ex);  // (also of values below the smallest normal one)
-    const int f = amax > 0.f ? ex - 7 + (mant > 127.f / 128.f ? 1 : 0) : 0;
-    if (g == 0) exps[lane] = f;
+    const float mant = frexpf(float_at<DT>(mag, 0), &ex);  // (also of values below the smallest normal one)
+    const int f = mag ? ex - 7 + (mant > 127.f / 128.f ? 1 : 0) : 0;
+    if (g == 0) {
+        of.exp[lane] = f;
+        of.tok[lane] = tok;
+    }
+    constexpr float WHOLE = 12582912.f;  // 1.5 2^23: a sum's low bits are the nearest whole number, to even
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         kv_i4 pos, neg;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            int p = 0, m = 0;
+        for (int k = 0; k < 4; ++k) {
+            uint32_t p[4], m[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int i = (int)rintf(ldexpf(v[s][4 * w + k], -f));
-                p |= (max(i, 0) & 0xff) << (8 * k);
-                m |= (min(i, 0) & 0xff) << (8 * k);
+            for (int i = 0; i < 4; ++i) {
+                const float x = ldexpf(float_at<DT>(w[s][k >> 1][2 * (k & 1) + (i >> 1)], i & 1), -f);
+                p[i] = __float_as_uint(fmaxf(x, 0.f) + WHOLE);
+                m[i] = __float_as_uint(fminf(x, 0.f) + WHOLE);
             }
-            pos[w] = p;
-            neg[w] = m;
+            // (the low bytes of four words)
+            pos[k] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(p[3], p[2], 0x0c0c0400u), __builtin_amdgcn_perm(p[1], p[0], 0x0c0c0400u), 0x05040100u);
+            neg[k] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(m[3], m[2], 0x0c0c0400u), __builtin_amdgcn_perm(m[1], m[0], 0x0c0c0400u), 0x05040100u);
         }
         pos_out[s * 64 + lane] = pos;
         neg_out[s * 64 + lane] = neg;
@@ -273,15 +306,14 @@ template <int D, int AHEAD, int STEP> struct Summaries {
             }
     }
     // The bounds of one tile of rows on them, into keys[token][stride] at block0 + u STEP 16 + n (below `blocks`).
-    // tr0: the row that the lane's first of four bounds belongs to; `rows` in all, G to a token.
-    __device__ __forceinline__ void bounds(const kv_i4 *pos_in, const kv_i4 *neg_in, const int *exps, int tr0, int rows, int G, uint32_t *keys, int stride,
-                                           int block0, int blocks, int lane) const {
+    __device__ __forceinline__ void bounds(const kv_i4 *pos_in, const kv_i4 *neg_in, const RowsOf &of, uint32_t *keys, int stride, int block0, int blocks,
+                                           int lane) const {
         const int g = lane >> 4, n = lane & 15;
         int fr[4], tr[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            fr[i] = exps[4 * g + i];
-            tr[i] = tr0 + i < rows ? (tr0 + i) / G : -1;
+            fr[i] = of.exp[4 * g + i];
+            tr[i] = of.tok[4 * g + i];
         }
         kv_i4 acc[AHEAD];
 #pragma unroll
@@ -323,9 +355,14 @@ struct SelectView {
         lead = pad / BLOCK_ROWS;
         coded = min(x.b.coded, (x.T - x.L + tok0 + toks - 1) / BLOCK_ROWS);  // (the last token's own block is always chosen)
     }
-    // row r of the group: token by token, a token's heads side by side
-    __device__ __forceinline__ const char *row(const BlockSelect &x, int r) const {
-        const int tok = r / G, head = r % G;
+    // row r of the group: token by token, a token's heads side by side; `tok`: its token, or -1 behind the last
+    __device__ __forceinline__ const char *row(const BlockSelect &x, int r, int &tok) const {
+        tok = toks == 1 ? 0 : r / G;
+        const int head = r - tok * G;
+        if (r >= rows) {
+            tok = -1;
+            return static_cast<const char *>(x.q);
+        }
         return static_cast<const char *>(x.q) + (((size_t)bh * G + head) * x.L + tok0 + tok) * x.b.Dk_user * 2;
     }
     __device__ __forceinline__ int seen(const BlockSelect &x, int tok) const {
@@ -341,7 +378,7 @@ template <int D, int DT>
 __global__ void __launch_bounds__(SELECT_WAVES * 64) block_select_kernel(BlockSelect x, int tokens, int stride) {
     constexpr int KS = (D + 63) / 64, AHEAD = D <= 128 ? 4 : 2;
     extern __shared__ uint32_t lds[];
-    __shared__ int exps[SELECT_TILES][16];
+    __shared__ RowsOf of[SELECT_TILES];
     kv_i4 *ops = reinterpret_cast<kv_i4 *>(lds + SELECT_WAVES * 256);                 // [tiles][positive / negative][KS][64]
     uint32_t *keys = reinterpret_cast<uint32_t *>(ops + SELECT_TILES * 2 * KS * 64);  // [tokens][stride]
     const SelectView v(x, blockIdx.x, blockIdx.y * tokens, tokens);
@@ -353,16 +390,16 @@ __global__ void __launch_bounds__(SELECT_WAVES * 64) block_select_kernel(BlockSe
         const int tiles = min((v.rows - row0 + 15) / 16, SELECT_TILES);
         if (row0) __syncthreads();
         if (wave < tiles) {
-            const int r = row0 + 16 * wave + (lane & 15);
-            query_operands<D, DT>(v.row(x, min(r, v.rows - 1)), r < v.rows, x.b.Dk_user, lane, ops + wave * 2 * KS * 64, ops + (wave * 2 + 1) * KS * 64, exps[wave]);
+            int tok;
+            const char *row = v.row(x, row0 + 16 * wave + (lane & 15), tok);
+            query_operands<D, DT>(row, tok, x.b.Dk_user, lane, ops + wave * 2 * KS * 64, ops + (wave * 2 + 1) * KS * 64, of[wave]);
         }
         __syncthreads();
         for (int first = wave; first < groups; first += SELECT_WAVES * AHEAD) {
             Summaries<D, AHEAD, SELECT_WAVES> sum;
             sum.load(x.b, v.bh, v.lead + first * 16, v.coded - 1, lane);
             for (int tile = 0; tile < tiles; ++tile)
-                sum.bounds(ops + tile * 2 * KS * 64, ops + (tile * 2 + 1) * KS * 64, exps[tile], row0 + 16 * tile + 4 * (lane >> 4), v.rows, v.G, keys, stride,
-                           first * 16, v.coded - v.lead, lane);
+                sum.bounds(ops + tile * 2 * KS * 64, ops + (tile * 2 + 1) * KS * 64, of[tile], keys, stride, first * 16, v.coded - v.lead, lane);
         }
     }
     __syncthreads();
@@ -381,7 +418,7 @@ template <int D, int DT>
 __global__ void __launch_bounds__(BOUND_WAVES * 64) block_bounds_kernel(BlockSelect x, int tokens, int stride, uint32_t *out) {
     constexpr int KS = (D + 63) / 64, AHEAD = bound_ahead<D>(), SPAN = BOUND_WAVES * AHEAD * 16;
     __shared__ kv_i4 ops[BOUND_TILES][2][KS * 64];
-    __shared__ int exps[BOUND_TILES][16];
+    __shared__ RowsOf of[BOUND_TILES];
     __shared__ uint32_t keys[16 * BOUND_TILES * SPAN];
     const SelectView v(x, blockIdx.x, blockIdx.y * tokens, tokens);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -395,12 +432,13 @@ __global__ void __launch_bounds__(BOUND_WAVES * 64) block_bounds_kernel(BlockSel
         const int tiles = min((v.rows - row0 + 15) / 16, BOUND_TILES);
         if (row0) __syncthreads();
         if (wave < tiles) {
-            const int r = row0 + 16 * wave + (lane & 15);
-            query_operands<D, DT>(v.row(x, min(r, v.rows - 1)), r < v.rows, x.b.Dk_user, lane, ops[wave][0], ops[wave][1], exps[wave]);
+            int tok;
+            const char *row = v.row(x, row0 + 16 * wave + (lane & 15), tok);
+            query_operands<D, DT>(row, tok, x.b.Dk_user, lane, ops[wave][0], ops[wave][1], of[wave]);
         }
         __syncthreads();
         for (int tile = 0; tile < tiles; ++tile)
-            sum.bounds(ops[tile][0], ops[tile][1], exps[tile], row0 + 16 * tile + 4 * (lane >> 4), v.rows, v.G, keys, SPAN, wave * 16, blocks, lane);
+            sum.bounds(ops[tile][0], ops[tile][1], of[tile], keys, SPAN, wave * 16, blocks, lane);
     }
     __syncthreads();
     for (int tok = 0; tok < v.toks; ++tok) {
@@ -408,12 +446,12 @@ __global__ void __launch_bounds__(BOUND_WAVES * 64) block_bounds_kernel(BlockSel
         for (int i = threadIdx.x; i < blocks; i += BOUND_WAVES * 64) to[i] = keys[tok * SPAN + i];
     }
 }
-// grid (BH, tokens), 8 wavefronts
-constexpr int CHOOSE_WAVES = 8;
+// grid (BH, tokens), 16 wavefronts
+constexpr int CHOOSE_WAVES = 16, CHOOSE_AREA = 260 + 2 * CHOOSE_WAVES;
 __global__ void __launch_bounds__(CHOOSE_WAVES * 64) block_choose_kernel(BlockSelect x, int stride, const uint32_t *in) {
-    extern __shared__ uint32_t lds[];  // [257 + 2 x 64s of blocks], keys [stride]
+    extern __shared__ uint32_t lds[];  // [CHOOSE_AREA], keys [stride]
     const SelectView v(x, blockIdx.x, blockIdx.y, 1);
-    uint32_t *keys = lds + 260 + 2 * ((stride + 63) / 64);
+    uint32_t *keys = lds + CHOOSE_AREA;
     const uint32_t *from = in + ((size_t)v.bh * x.L + v.tok0) * stride;
     const int seen = v.seen(x, 0);
     if (seen > x.count) {
@@ -457,7 +495,7 @@ template <int D, int DT> hipError_t select_run(const BlockSelect &x, hipStream_t
         hipLaunchKernelGGL((block_bounds_kernel<D, DT>), dim3(x.b.st.BH, groups, p.stretches), dim3(BOUND_WAVES * 64), 0, stream, x, p.tokens, p.stride, keys);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        const size_t lds = 4 * (size_t)(260 + 2 * ((p.stride + 63) / 64) + p.stride);
+        const size_t lds = 4 * (size_t)(CHOOSE_AREA + p.stride);
         if (lds > 65536) {
             e = hipFuncSetAttribute(reinterpret_cast<const void *>(block_choose_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, SELECT_LDS);
             if (e != hipSuccess) return e;

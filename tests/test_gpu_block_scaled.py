@@ -393,6 +393,27 @@ def test_blocks_are_chosen_by_the_definition(dtype, layout, T, n, count, first, 
     assert np.array_equal(got.cpu().numpy(), O.select(q, oracle, count, first, recent, pads))
 
 
+@pytest.mark.parametrize("layout", [(8, 2, 128, 128), (40, 1, 64, 64), (3, 1, 96, 96), (2, 1, 256, 256), (70, 1, 50, 36)])
+@pytest.mark.parametrize("n,count,first,recent,pads", [(1, 40, 1, 2, (0, 0)), (1, 3, 1, 2, (5000, 0)), (3, 17, 0, 1, (100, 17100)), (19, 300, 3, 4, (0, 64))])
+def test_blocks_of_long_caches(layout, n, count, first, recent, pads):
+    """More blocks than one workgroup takes in: bounds and choice in launches of their own."""
+    cache, oracle, queries = held(BF16, 17100, layout, seed=4)
+    q, qd = queries(n)
+    got = cache.select_blocks(qd, count, first, recent, torch.tensor(pads, device="cuda"))
+    assert np.array_equal(got.cpu().numpy(), O.select(q, oracle, count, first, recent, pads))
+
+
+def test_equal_bounds_of_long_caches():
+    one = torch.ones(1, 1, 64, 64, device="cuda").to(BF16)
+    k = one.repeat(1, 1, 400, 1)
+    k[:, :, 64 * 333:64 * 334] *= 2
+    cache = kvhip.BlockScaledKVCache()
+    cache.update(k, k, fetch=False)
+    got = cache.select_blocks(one[:, :, :1], 300, 0, 1)[0, 0, 0].cpu()
+    assert (got == torch.tensor(list(range(298)) + [333, 399])).all()
+    assert (cache.select_blocks(0 * one[:, :, :1], 300, 0, 1)[0, 0, 0].cpu() == torch.tensor(list(range(299)) + [399])).all()
+
+
 def test_equal_bounds_take_the_lower_block():
     gen = torch.Generator(device="cuda").manual_seed(1)
     one = torch.randn(1, 2, 64, 64, generator=gen, device="cuda").to(BF16)
