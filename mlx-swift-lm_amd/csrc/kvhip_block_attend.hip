@@ -69,7 +69,7 @@ template <int DT> hipError_t merge(const BlockAttend &x, hipStream_t stream) {
 }  // namespace
 
 int64_t block_attend_rows(const BlockAttend &x) {
-    const int64_t G = x.a.Hq / x.a.Hkv, cut = 16 * block_row_tiles(x);
+    const int64_t G = x.a.Hq / x.a.Hkv, cut = block_attend_tiled(x) ? block_tiled_rows(x.a.st.Dk) : 16 * block_row_tiles(x);
     return x.list ? x.a.L * ((G + 15) / 16) : (G * x.a.L + cut - 1) / cut;
 }
 size_t plan_block_attend(BlockAttend &x) {
@@ -82,7 +82,8 @@ size_t plan_block_attend(BlockAttend &x) {
     // tile and there is work for them: their parts meet in LDS, and half as many are left to merge.
     const int64_t wanted = (a.st.Dk <= 128 ? 2048 : 1024) / std::max<int64_t>(base, 1);
     x.waves = nm == 1 && a.st.Dk <= 128 && a.mask.mode != KVHIP_MASK_ARRAY && wanted >= 8 && blocks > 4 ? 8 : 4;
-    int64_t parts = std::max<int64_t>(1, wanted / x.waves);
+    if (block_attend_tiled(x)) x.waves = 8;  // (one workgroup to a compute unit)
+    int64_t parts = std::max<int64_t>(1, (block_attend_tiled(x) ? 2048 / std::max<int64_t>(base, 1) : wanted) / x.waves);
     parts = std::min<int64_t>(parts, std::max(1, blocks / 8));
     parts = std::min<int64_t>(parts, MERGE_PARTS);
     const size_t one = (size_t)a.st.BH * G * a.L * (a.st.Dv + 2) * sizeof(float);

@@ -12,9 +12,14 @@
 #pragma once
 #include "kvhip_block.hpp"
 #include "kvhip_mask.hpp"
+#include "kvhip_prefill_fp.hpp"
 #include "kvhip_span_merge.hpp"
 
 namespace kvhip {
+
+// Whether a call has rows enough for the kernel that shares blocks between wavefronts, and the rows its workgroup takes.
+inline bool block_attend_tiled(const BlockAttend &x) { return !x.list && x.a.mask.mode != KVHIP_MASK_ARRAY && x.a.Hq / x.a.Hkv * x.a.L > 32; }
+inline int block_tiled_rows(int Dk) { return Dk <= 128 || Dk > 192 ? 64 : 128; }
 
 // Tiles of 16 query rows that a wavefront takes (plan_block_attend chooses by the same rule).
 inline int block_row_tiles(const BlockAttend &x) {
@@ -245,6 +250,79 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
             __builtin_amdgcn_sched_barrier(0);
         }
     }
+    // The same from a block in LDS, keys and then values as they lie in the pages: operands are read as they are used.
+    __device__ __forceinline__ void block_shared(const char *lds, float ks, float vs, int j0, bool masked) {
+        constexpr bool HALF = DK % 64 != 0;
+        const char *keys = lds, *values = lds + BLOCK_ROWS * DK + lane * 16;
+        kv_f4 s[NM][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            kv_u4 raw[(KS + 1) / 2];
+#pragma unroll
+            for (int c = 0; c < KS / 2; ++c) raw[c] = *reinterpret_cast<const kv_u4 *>(keys + t * 16 * DK + c * 1024 + lane * 16);
+            if constexpr (HALF) {
+                const kv_u2 h = *reinterpret_cast<const kv_u2 *>(keys + t * 16 * DK + (KS / 2) * 1024 + lane * 8);
+                raw[KS / 2] = kv_u4{h[0], h[1], 0u, 0u};
+            }
+#pragma unroll
+            for (int i = 0; i < NM; ++i) s[i][t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KS; ++c) {
+                const kv_u4 w = block_operand<DT>(raw[c >> 1][2 * (c & 1)], raw[c >> 1][2 * (c & 1) + 1], ks);
+#pragma unroll
+                for (int i = 0; i < NM; ++i) s[i][t] = block_mfma<DT>(w, q[i][c], s[i][t]);
+            }
+        }
+        kv_u4 p[NM][2];
+        uint32_t seen[NM];
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+            seen[i] = 0xffffu;
+            if (masked) seen[i] = mask(i, j0, s[i]);
+            weigh(i, s[i], p[i]);
+        }
+        bool nan = false;
+        if (masked) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int d = 0; d < VT; ++d) {
+                const kv_u4 w = *reinterpret_cast<const kv_u4 *>(values + d * 1024);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) any |= nan_codes(w[k]);
+            }
+            nan = __any(any != 0);
+            if (nan) {
+#pragma unroll
+                for (int d = 0; d < VT; ++d) {
+                    const kv_u4 w = *reinterpret_cast<const kv_u4 *>(values + d * 1024);
+                    kv_u4 bad[2];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t one = (nan_codes(w[k]) >> 7) * 0x38u;  // 1.0
+                        bad[k >> 1][2 * (k & 1)] = block_values<DT, false>(one, 1.f);
+                        bad[k >> 1][2 * (k & 1) + 1] = block_values<DT, true>(one, 1.f);
+                    }
+#pragma unroll
+                    for (int i = 0; i < NM; ++i) poison(i, d, seen[i], bad);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < VT; ++d) {
+            kv_u4 w = *reinterpret_cast<const kv_u4 *>(values + d * 1024);
+            if (nan) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] &= ~((nan_codes(w[k]) >> 7) * 0xffu);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const kv_u4 a = block_operand<DT>(w[2 * u], w[2 * u + 1], vs);
+#pragma unroll
+                for (int i = 0; i < NM; ++i) o[i][d] = block_mfma<DT>(a, p[i][u], o[i][d]);
+            }
+        }
+    }
     // bit 7 of every byte of a word that is a NaN code
     static __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
@@ -358,6 +436,106 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
     }
 };
 
+// What the rows of a wavefront's tiles are, and what they see.
+struct RowsView {
+    int G, R, token, row0;  // heads a pair, rows that the tiles cut, (listed blocks) the token, the wavefront's first row
+    int in_lo, in_hi;       // keys that every row sees
+    int lo, hi;             // keys that some row sees
+    template <int MODE> __device__ __forceinline__ int at(const AttendArgs &a, int i) const { return MODE == 3 ? i * a.L + token : i; }
+};
+// rows row0 .. row0 + 16 NM - 1 of pair `w`: bounds (those of rows span0 .. span1 - 1, the workgroup's), queries
+template <class Walk, int DK, int NM, int MODE>
+__device__ __forceinline__ void take_rows(Walk &w, RowsView &v, const BlockAttend &x, int span0, int span1) {
+    const AttendArgs &a = x.a;
+    const SymMask sym = sym_mask_init(a.mask, w.b, a.L, a.T);
+    v.in_lo = v.lo = 0;
+    v.in_hi = v.hi = a.T - 1;
+    if constexpr (MODE == 1) {
+        const int last = min(span1, v.R) - 1;
+        const bool one_head = a.L > 1 && span0 / a.L == last / a.L;
+        const KeyBounds f = sym_mask_bounds(sym, one_head ? span0 % a.L : 0), e = sym_mask_bounds(sym, one_head ? last % a.L : a.L - 1);
+        v.in_lo = max(e.lo, 0);
+        v.in_hi = min(f.hi, a.T - 1);
+        v.lo = max(f.lo, 0);
+        v.hi = min(e.hi, a.T - 1);
+    }
+    if constexpr (MODE == 3) {
+        v.lo = v.in_lo = x.left_pad ? max(x.left_pad[w.b], 0) : 0;
+        v.hi = v.in_hi = a.T - a.L + v.token;
+    }
+    const char *qbase = static_cast<const char *>(a.q) + (size_t)w.bh * v.G * a.L * DK * 2;
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+        const int r = v.row0 + 16 * i + w.n;
+        const bool live = r < v.R;
+        const char *row = qbase + (size_t)v.template at<MODE>(a, live ? r : 0) * DK * 2;
+#pragma unroll
+        for (int c = 0; c < Walk::KS; ++c) {
+            const int d = (c | 1) < Walk::KS ? (c >> 1) * 64 + w.g * 16 + (c & 1) * 8 : c * 32 + w.g * 8;
+            w.q[i][c] = live && a.scale != 0.f ? load_row16(row + 2 * d) : kv_u4{0u, 0u, 0u, 0u};
+            if (!Walk::SAFE && a.scale < 0.f) w.q[i][c] ^= 0x80008000u;
+        }
+        if (MODE == 3 || a.L == 1) {  // (no divisions in front of a step's first request)
+            w.ql[i] = 0;
+            w.qh[i] = live ? w.h * v.G + r : -1;
+        } else {
+            w.ql[i] = live ? r % a.L : 0;
+            w.qh[i] = live ? w.h * v.G + r / a.L : -1;
+        }
+        w.see[i] = KeyBounds{v.lo, v.hi};
+        if constexpr (MODE == 1) {
+            const KeyBounds k = sym_mask_bounds(sym, w.ql[i]);
+            w.see[i] = KeyBounds{max(k.lo, 0), min(k.hi, a.T - 1)};
+        }
+    }
+}
+// Tile i of the wavefronts that share its rows (KW of them, this one is number k of it; `t` of KW * 64 threads) joined: output rows, or
+// a partial of part `part`.  Holds two barriers of the workgroup.
+template <class Walk, int DV, int DT, int MODE, int KW>
+__device__ __forceinline__ void leave_tile(Walk &w, const RowsView &v, const BlockAttend &x, WaveParts<DV, KW, 16> &parts, int i, int k, int t, int part) {
+    const AttendArgs &a = x.a;
+    const int rows = min(v.R - (v.row0 + 16 * i), 16);
+    const float l = row_sum(w.l[i]);
+    if constexpr (!Walk::SAFE) w.m[i] = w.m[i] == -INFINITY ? -INFINITY : w.m[i] * fabsf(a.scale);  // (weights go by scores from here on)
+    if (w.g == 0) parts.m[k][w.n] = w.m[i];
+    __syncthreads();
+    const float weight = wave_weight(parts, w.n, w.m[i]);
+    if (w.g == 0) parts.l[k][w.n] = l * weight;
+#pragma unroll
+    for (int d = 0; d < Walk::VT; ++d)
+        *reinterpret_cast<kv_f4 *>(&parts.rows[k][w.n][16 * d + 4 * w.g]) = w.o[i][d] * weight;
+    __syncthreads();
+    constexpr int LPR = DV / 4, RPB = KW * 64 / LPR;
+    const int c = 4 * (t % LPR);
+    if (t >= RPB * LPR) return;  // (96 columns: lanes left over)
+    for (int r = t / LPR; r < rows; r += RPB) {
+        float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) o[d] += parts.rows[j][r][c + d];
+            sum += parts.l[j][r];
+        }
+        const int at = v.template at<MODE>(a, v.row0 + 16 * i + r);
+        const size_t all = (size_t)v.G * a.L;
+        if (x.nsplit == 1) {
+            const float inv = 1.f / sum;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) o[d] = sum == 0.f ? 0.f : o[d] * inv;
+            store_columns<DT>(a.out, ((size_t)w.bh * all + at) * DV + c, o);
+        } else {
+            float *to = a.workspace + (((size_t)w.bh * x.nsplit + part) * all + at) * (DV + 2);
+            store_floats(to + c, o);
+            if (c == 0) {
+                float mx = parts.m[0][r];
+#pragma unroll
+                for (int j = 1; j < KW; ++j) mx = fmaxf(mx, parts.m[j][r]);
+                *reinterpret_cast<kv_f2 *>(to + DV) = kv_f2{mx, sum};
+            }
+        }
+    }
+}
+
 // grid (BH, tiles of query rows, parts), NW wavefronts.  MODE 3: (BH, tokens x tiles of heads, parts).
 template <int DK, int DV, int DT, int NM, int MODE, int NW>
 __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kernel(BlockAttend x) {
@@ -367,55 +545,14 @@ __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kerne
     const AttendArgs &a = x.a;
     const int bh = blockIdx.x, part = blockIdx.z;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int G = a.Hq / a.Hkv, R = MODE == 3 ? G : G * a.L;       // rows that the tiles of blockIdx.y cut
-    const int token = MODE == 3 ? blockIdx.y / x.tiles : 0;
-    const int row0 = (MODE == 3 ? blockIdx.y % x.tiles : blockIdx.y) * 16 * NM;
+    RowsView v;
+    v.G = a.Hq / a.Hkv;
+    v.R = MODE == 3 ? v.G : v.G * a.L;
+    v.token = MODE == 3 ? blockIdx.y / x.tiles : 0;
+    v.row0 = (MODE == 3 ? blockIdx.y % x.tiles : blockIdx.y) * 16 * NM;
     Walk w(x, bh);
-    // row i of a pair's query rows: head i / L, position i % L; a token's rows lie L apart
-    auto row_at = [&](int i) { return MODE == 3 ? i * a.L + token : i; };
-
-    // queries, and what their rows see
-    const SymMask sym = sym_mask_init(a.mask, w.b, a.L, a.T);
-    int in_lo = 0, in_hi = a.T - 1;  // keys that every row sees
-    int lo = 0, hi = a.T - 1;        // keys that some row sees
-    if constexpr (MODE == 1) {
-        const int last = min(row0 + 16 * NM, R) - 1;
-        const bool one_head = a.L > 1 && row0 / a.L == last / a.L;
-        const KeyBounds f = sym_mask_bounds(sym, one_head ? row0 % a.L : 0), e = sym_mask_bounds(sym, one_head ? last % a.L : a.L - 1);
-        in_lo = max(e.lo, 0);
-        in_hi = min(f.hi, a.T - 1);
-        lo = max(f.lo, 0);
-        hi = min(e.hi, a.T - 1);
-    }
-    if constexpr (MODE == 3) {
-        lo = in_lo = x.left_pad ? max(x.left_pad[w.b], 0) : 0;
-        hi = in_hi = a.T - a.L + token;
-    }
-    const char *qbase = static_cast<const char *>(a.q) + (size_t)bh * G * a.L * DK * 2;
-#pragma unroll
-    for (int i = 0; i < NM; ++i) {
-        const int r = row0 + 16 * i + w.n;
-        const bool live = r < R;
-        const char *row = qbase + (size_t)row_at(live ? r : 0) * DK * 2;
-#pragma unroll
-        for (int c = 0; c < Walk::KS; ++c) {
-            const int d = (c | 1) < Walk::KS ? (c >> 1) * 64 + w.g * 16 + (c & 1) * 8 : c * 32 + w.g * 8;
-            w.q[i][c] = live && a.scale != 0.f ? load_row16(row + 2 * d) : kv_u4{0u, 0u, 0u, 0u};
-            if (!Walk::SAFE && a.scale < 0.f) w.q[i][c] ^= 0x80008000u;
-        }
-        if (MODE == 3 || a.L == 1) {  // (no divisions in front of a step's first request)
-            w.ql[i] = 0;
-            w.qh[i] = live ? w.h * G + r : -1;
-        } else {
-            w.ql[i] = live ? r % a.L : 0;
-            w.qh[i] = live ? w.h * G + r / a.L : -1;
-        }
-        w.see[i] = KeyBounds{lo, hi};
-        if constexpr (MODE == 1) {
-            const KeyBounds k = sym_mask_bounds(sym, w.ql[i]);
-            w.see[i] = KeyBounds{max(k.lo, 0), min(k.hi, a.T - 1)};
-        }
-    }
+    take_rows<Walk, DK, NM, MODE>(w, v, x, v.row0, v.row0 + 16 * NM);
+    const int lo = v.lo, hi = v.hi, in_lo = v.in_lo, in_hi = v.in_hi, token = v.token;
 
     // the blocks of this part: positions [s0, s1) of the row's blocks, or of its list
     const int first = MODE == 3 ? 0 : lo / BLOCK_ROWS;
@@ -491,51 +628,115 @@ __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kerne
     }
 
     // the wavefronts' parts joined, 16 rows at a time
-    const bool whole = x.nsplit == 1;
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
-        const int rows = min(R - (row0 + 16 * i), 16);
-        if (rows <= 0) break;
         if (i) __syncthreads();
-        const float l = row_sum(w.l[i]);
-        if constexpr (!Walk::SAFE) w.m[i] = w.m[i] == -INFINITY ? -INFINITY : w.m[i] * fabsf(a.scale);  // (weights go by scores from here on)
-        if (w.g == 0) parts.m[wave][w.n] = w.m[i];
-        __syncthreads();
-        const float weight = wave_weight(parts, w.n, w.m[i]);
-        if (w.g == 0) parts.l[wave][w.n] = l * weight;
-#pragma unroll
-        for (int d = 0; d < Walk::VT; ++d)
-            *reinterpret_cast<kv_f4 *>(&parts.rows[wave][w.n][16 * d + 4 * w.g]) = w.o[i][d] * weight;
-        __syncthreads();
-        constexpr int LPR = DV / 4, RPB = NW * 64 / LPR;
-        const int c = 4 * (threadIdx.x % LPR);
-        if (threadIdx.x >= RPB * LPR) continue;  // (96 columns: lanes left over)
-        for (int r = threadIdx.x / LPR; r < rows; r += RPB) {
-            float v[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < NW; ++k) {
-#pragma unroll
-                for (int d = 0; d < 4; ++d) v[d] += parts.rows[k][r][c + d];
-                sum += parts.l[k][r];
-            }
-            const int at = row_at(row0 + 16 * i + r);
-            const size_t all = (size_t)G * a.L;
-            if (whole) {
-                const float inv = 1.f / sum;
-#pragma unroll
-                for (int d = 0; d < 4; ++d) v[d] = sum == 0.f ? 0.f : v[d] * inv;
-                store_columns<DT>(a.out, ((size_t)bh * all + at) * DV + c, v);
-            } else {
-                float *to = a.workspace + (((size_t)bh * x.nsplit + part) * all + at) * (DV + 2);
-                store_floats(to + c, v);
-                if (c == 0) {
-                    float mx = parts.m[0][r];
-#pragma unroll
-                    for (int k = 1; k < NW; ++k) mx = fmaxf(mx, parts.m[k][r]);
-                    *reinterpret_cast<kv_f2 *>(to + DV) = kv_f2{mx, sum};
-                }
-            }
+        leave_tile<Walk, DV, DT, MODE, NW>(w, v, x, parts, i, wave, threadIdx.x, part);
+    }
+}
+
+// Many query rows (prompt chunks): eight wavefronts, RW groups of 16 NM rows by KW of the blocks of a round.  The blocks of a
+// round lie in LDS, each read by the RW wavefronts that share it; the next round's are on their way, past the registers, while
+// this one's are looked at: whole lines from the pages, a round's work to cover them (requested half a block ahead by every
+// wavefront for itself, a third of the time went by waiting).  One barrier a round.
+// grid (BH, tiles of 16 NM RW rows, parts)
+template <int DK, int DV> struct TiledShape {
+    static constexpr int NM = DK <= 192 ? 2 : 1, RW = DK <= 128 ? 2 : 4, KW = 8 / RW, ROWS = 16 * NM * RW;
+};
+template <int DK, int DV, int DT>
+__global__ void __launch_bounds__(512, 2) block_attend_tiled_kernel(BlockAttend x) {
+    using Shape = TiledShape<DK, DV>;
+    constexpr int NM = Shape::NM, RW = Shape::RW, KW = Shape::KW, BYTES = BLOCK_ROWS * (DK + DV), CHUNKS = BYTES / 1024, MINE = CHUNKS / RW;
+    static_assert(CHUNKS % RW == 0, "whole requests a wavefront");
+    using Walk = BlockWalk<DK, DV, DT, NM, 1, 8>;
+    using Parts = WaveParts<DV, KW, 16>;
+    constexpr size_t RING = 2 * KW * BYTES, JOIN = RW * sizeof(Parts);
+    __shared__ __align__(16) char lds[RING > JOIN ? RING : JOIN];
+    const AttendArgs &a = x.a;
+    const int bh = blockIdx.x, part = blockIdx.z;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int rw = wave % RW, kw = wave / RW;
+    RowsView v;
+    v.G = a.Hq / a.Hkv;
+    v.R = v.G * a.L;
+    v.token = 0;
+    const int group0 = blockIdx.y * Shape::ROWS;
+    v.row0 = group0 + rw * 16 * NM;
+    Walk w(x, bh);
+    take_rows<Walk, DK, NM, 1>(w, v, x, group0, group0 + Shape::ROWS);
+
+    const int first = v.lo / BLOCK_ROWS, total = v.hi < v.lo ? 0 : v.hi / BLOCK_ROWS - first + 1;
+    const int each = (total + x.nsplit - 1) / x.nsplit, s0 = min(part * each, total), s1 = min(s0 + each, total);
+    const int rounds = (s1 - s0 + KW - 1) / KW;
+    // where the wavefront's blocks lie, a lane to a round, 64 rounds at a time
+    uint64_t kp = 0, vp = 0;
+    float ks = 1.f, vs = 1.f;
+    int known = -64, tail_at = -1;
+    auto block_of = [&](int round) {
+        const int i = s0 + round * KW + kw;
+        return i < s1 ? first + i : -1;
+    };
+    auto look_up = [&](int round) {
+        known = round;
+        const int blk = block_of(round + lane);
+        if (blk >= 0 && blk < x.b.coded) {
+            const PageEntry e = block_page(x.b, blk / BLOCK_PER_PAGE);
+            const int in_page = blk % BLOCK_PER_PAGE;
+            kp = reinterpret_cast<uint64_t>(e.k + (size_t)bh * a.st.k_cell + (size_t)in_page * BLOCK_ROWS * DK);
+            vp = reinterpret_cast<uint64_t>(e.v + (size_t)bh * a.st.v_cell + (size_t)in_page * BLOCK_ROWS * DV);
+            const kv_f2 sc = ld_global<kv_f2>(as_global(e.ksb) + (size_t)bh * a.st.ksb_cell + in_page * 8);
+            ks = sc.x;
+            vs = sc.y;
         }
+    };
+    auto at_lane = [](uint64_t p, int of) {  // (readlane returns a signed number)
+        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)p, of), hi = __builtin_amdgcn_readlane((uint32_t)(p >> 32), of);
+        return (gptr)(((uint64_t)hi << 32) | lo);
+    };
+    // the wavefront's share of its block of a round, 1 KB a request; what it needs of the block later
+    float k_scale = 1.f, v_scale = 1.f, k_next = 1.f, v_next = 1.f;
+    auto request = [&](int round) {
+        if (round >= known + 64) look_up(round);
+        const int blk = block_of(round);
+        if (blk < 0) return;
+        if (blk >= x.b.coded) {
+            tail_at = blk * BLOCK_ROWS;
+            return;
+        }
+        const int of = round - known;
+        const gptr k = at_lane(kp, of), val = at_lane(vp, of);
+        k_next = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), of));
+        v_next = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), of));
+        const char *to = lds + ((round & 1) * KW + kw) * BYTES;
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) {
+            const int c = rw * MINE + j;
+            const gptr from = c < DK / 16 ? k + c * 1024 : val + (c - DK / 16) * 1024;
+            prefill_fp::load_to_lds((const char *)from, lane * 16, to + c * 1024);  // (its invariant: the wait and the barrier below)
+        }
+    };
+    if (rounds > 0) request(0);
+    for (int round = 0; round < rounds; ++round) {
+        // the round's blocks are there (every wavefront has waited for its share), and the other half of the ring is free (every
+        // wavefront has read it)
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+        __syncthreads();
+        k_scale = k_next;
+        v_scale = v_next;
+        if (round + 1 < rounds) request(round + 1);
+        const int blk = block_of(round);
+        if (blk >= 0 && blk < x.b.coded) {
+            const int j0 = blk * BLOCK_ROWS;
+            w.block_shared(lds + ((round & 1) * KW + kw) * BYTES, k_scale, v_scale, j0, j0 < v.in_lo || j0 + BLOCK_ROWS - 1 > v.in_hi);
+        }
+    }
+    if (tail_at >= 0) w.tail(tail_at);
+    __syncthreads();  // (the ring's memory takes the parts)
+    Parts &parts = reinterpret_cast<Parts *>(lds)[rw];
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+        if (i) __syncthreads();
+        leave_tile<Walk, DV, DT, 1, KW>(w, v, x, parts, i, kw, kw * 64 + lane, part);
     }
 }
 
@@ -544,6 +745,10 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW = 4> hipError_t block
     return hipGetLastError();
 }
 template <int DK, int DV, int DT> hipError_t block_attend_shape(const BlockAttend &x, hipStream_t stream) {
+    if (block_attend_tiled(x)) {
+        hipLaunchKernelGGL((block_attend_tiled_kernel<DK, DV, DT>), dim3(x.a.st.BH, block_attend_rows(x), x.nsplit), dim3(512), 0, stream, x);
+        return hipGetLastError();
+    }
     if constexpr (DK <= 128) {
         if (x.waves == 8) return x.list ? block_attend_run<DK, DV, DT, 1, 3, 8>(x, stream) : block_attend_run<DK, DV, DT, 1, 1, 8>(x, stream);
     }
