@@ -80,7 +80,11 @@ template <int DK, int DV> struct BlockTile {
 };
 
 // MODE 1: index-only mask (no mask: one that every key passes); 2: array mask; 3: listed blocks
-template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
+// SUMS: the sums of the weights by a product with ones (prompt chunks: an addition to a weight is a fourteenth of their vector
+// instructions, and the matrix pipe has room); else by additions.
+template <int DK, int DV, int DT, int NM, int MODE, bool SUMS = false> struct BlockWalk {
+    static constexpr bool WHOLE_SUMS = SUMS;
+    static constexpr uint32_t ONES = DT == 1 ? 0x3f803f80u : 0x3c003c00u;
     static constexpr int KS = DK / 32, VT = DV / 16;
     static constexpr bool SAFE = MODE == 2;  // an added mask may hold the type's lowest value: no products in front of the difference
     // float16 weights are taken times 2^14: those of keys far below the largest stay clear of the type's subnormals (the sums
@@ -93,6 +97,7 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
     kv_u4 q[NM][KS];
     kv_f4 o[NM][VT];
     float m[NM], l[NM];
+    kv_f4 ls[SUMS ? NM : 1];  // (four times the same)
     float unit;         // log2 e, times the scale (its sign is the queries') where scores have not met it
     KeyBounds see[NM];  // the keys of the lane's query row
     int ql[NM], qh[NM]; // its position and head (MODE 2)
@@ -103,18 +108,27 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
         for (int i = 0; i < NM; ++i) {
             m[i] = -INFINITY;
             l[i] = 0.f;
+            if (SUMS || i == 0) ls[SUMS ? i : 0] = kv_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int d = 0; d < VT; ++d) o[i][d] = kv_f4{0.f, 0.f, 0.f, 0.f};
         }
     }
 
+    // (one instruction; through fmaxf every operand is quieted by another one)
+    static __device__ __forceinline__ float max3(float a, float b, float c) {
+        float r;
+        asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+        return r;
+    }
     // Scores of one tile of query rows -> weights as operands; the outputs so far are brought to the new maximum.  Scores and
     // maxima are products that the call's scale has yet to meet (MODE 2: has met, an added mask's terms among them).
     __device__ __forceinline__ void weigh(int i, kv_f4 (&s)[4], kv_u4 (&p)[2]) {
-        float mx = m[i];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) mx = fmaxf(mx, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
-        mx = row_max(mx);
+        float mx = max3(m[i], s[0][0], s[0][1]), my = max3(s[0][2], s[0][3], s[1][0]);
+        mx = max3(mx, s[1][1], s[1][2]);
+        my = max3(my, s[1][3], s[2][0]);
+        mx = max3(mx, s[2][1], s[2][2]);
+        my = max3(my, s[2][3], s[3][0]);
+        mx = row_max(max3(max3(mx, s[3][1], s[3][2]), my, s[3][3]));
         const float ref = mx == -INFINITY ? 0.f : mx;  // (nothing seen yet: every difference is -infinity)
         const float off = LIFT - ref * unit;
         float e[16], sum = 0.f;
@@ -124,21 +138,24 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW> struct BlockWalk {
             for (int k = 0; k < 4; ++k) {
                 const float y = SAFE ? __builtin_fmaf(s[t][k] - ref, LOG2E, LIFT) : __builtin_fmaf(s[t][k], unit, off);
                 e[4 * t + k] = fast_exp2(y);
-                sum += e[4 * t + k];
+                if constexpr (!SUMS) sum += e[4 * t + k];
             }
         if (__any(mx != m[i])) {
             const float alpha = fast_exp2((m[i] - ref) * unit);
-            l[i] *= alpha;
+            if constexpr (SUMS) ls[i] *= alpha;
+            else l[i] *= alpha;
 #pragma unroll
             for (int d = 0; d < VT; ++d) o[i][d] *= alpha;
             m[i] = mx;
         }
-        l[i] += sum;
+        if constexpr (!SUMS) l[i] += sum;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
                 p[u][k] = DT == 1 ? pk_bf2(e[8 * u + 2 * k], e[8 * u + 2 * k + 1]) : pk_h2(e[8 * u + 2 * k], e[8 * u + 2 * k + 1]);
+            if constexpr (SUMS) ls[i] = block_mfma<DT>(kv_u4{ONES, ONES, ONES, ONES}, p[u], ls[i]);
+        }
     }
 
     // which of the lane's sixteen tokens its query row sees, those it does not see set to -infinity; adds an array mask
@@ -495,7 +512,7 @@ template <class Walk, int DV, int DT, int MODE, int KW>
 __device__ __forceinline__ void leave_tile(Walk &w, const RowsView &v, const BlockAttend &x, WaveParts<DV, KW, 16> &parts, int i, int k, int t, int part) {
     const AttendArgs &a = x.a;
     const int rows = min(v.R - (v.row0 + 16 * i), 16);
-    const float l = row_sum(w.l[i]);
+    const float l = Walk::WHOLE_SUMS ? w.ls[Walk::WHOLE_SUMS ? i : 0][0] : row_sum(w.l[i]);
     if constexpr (!Walk::SAFE) w.m[i] = w.m[i] == -INFINITY ? -INFINITY : w.m[i] * fabsf(a.scale);  // (weights go by scores from here on)
     if (w.g == 0) parts.m[k][w.n] = w.m[i];
     __syncthreads();
@@ -539,7 +556,7 @@ __device__ __forceinline__ void leave_tile(Walk &w, const RowsView &v, const Blo
 // grid (BH, tiles of query rows, parts), NW wavefronts.  MODE 3: (BH, tokens x tiles of heads, parts).
 template <int DK, int DV, int DT, int NM, int MODE, int NW>
 __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kernel(BlockAttend x) {
-    using Walk = BlockWalk<DK, DV, DT, NM, MODE, NW>;
+    using Walk = BlockWalk<DK, DV, DT, NM, MODE>;
     using Tile = BlockTile<DK, DV>;
     __shared__ WaveParts<DV, NW, 16> parts;
     const AttendArgs &a = x.a;
@@ -648,7 +665,7 @@ __global__ void __launch_bounds__(512, 2) block_attend_tiled_kernel(BlockAttend 
     using Shape = TiledShape<DK, DV>;
     constexpr int NM = Shape::NM, RW = Shape::RW, KW = Shape::KW, BYTES = BLOCK_ROWS * (DK + DV), CHUNKS = BYTES / 1024, MINE = CHUNKS / RW;
     static_assert(CHUNKS % RW == 0, "whole requests a wavefront");
-    using Walk = BlockWalk<DK, DV, DT, NM, 1, 8>;
+    using Walk = BlockWalk<DK, DV, DT, NM, 1, true>;
     using Parts = WaveParts<DV, KW, 16>;
     constexpr size_t RING = 2 * KW * BYTES, JOIN = RW * sizeof(Parts);
     __shared__ __align__(16) char lds[RING > JOIN ? RING : JOIN];
