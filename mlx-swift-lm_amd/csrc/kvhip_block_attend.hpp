@@ -267,8 +267,10 @@ template <int DK, int DV, int DT, int NM, int MODE, bool SUMS = false> struct Bl
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    // The same from a block in LDS, keys and then values as they lie in the pages: operands are read as they are used.
-    __device__ __forceinline__ void block_shared(const char *lds, float ks, float vs, int j0, bool masked) {
+    // The same from a block in LDS, keys and then values as they lie in the pages: operands are read as they are used.  `ahead(t)`,
+    // four times between products, makes a quarter of the wavefront's requests for the next round: the compute unit takes in 64
+    // bytes a cycle, and a round's requests in one go held every wavefront up for a thousand cycles.
+    template <class AHEAD> __device__ __forceinline__ void block_shared(const char *lds, float ks, float vs, int j0, bool masked, AHEAD ahead) {
         constexpr bool HALF = DK % 64 != 0;
         const char *keys = lds, *values = lds + BLOCK_ROWS * DK + lane * 16;
         kv_f4 s[NM][4];
@@ -289,6 +291,7 @@ template <int DK, int DV, int DT, int NM, int MODE, bool SUMS = false> struct Bl
 #pragma unroll
                 for (int i = 0; i < NM; ++i) s[i][t] = block_mfma<DT>(w, q[i][c], s[i][t]);
             }
+            ahead(t);
         }
         kv_u4 p[NM][2];
         uint32_t seen[NM];
@@ -712,27 +715,33 @@ __global__ void __launch_bounds__(512, 2) block_attend_tiled_kernel(BlockAttend 
     };
     // the wavefront's share of its block of a round, 1 KB a request; what it needs of the block later
     float k_scale = 1.f, v_scale = 1.f, k_next = 1.f, v_next = 1.f;
-    auto request = [&](int round) {
+    gptr k_from = nullptr, v_from = nullptr;
+    char *to = lds;
+    auto locate = [&](int round) {  // the block of a round: whether there is one in codes, and where
         if (round >= known + 64) look_up(round);
         const int blk = block_of(round);
-        if (blk < 0) return;
+        if (blk < 0) return false;
         if (blk >= x.b.coded) {
             tail_at = blk * BLOCK_ROWS;
-            return;
+            return false;
         }
         const int of = round - known;
-        const gptr k = at_lane(kp, of), val = at_lane(vp, of);
+        k_from = at_lane(kp, of);
+        v_from = at_lane(vp, of);
         k_next = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), of));
         v_next = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), of));
-        const char *to = lds + ((round & 1) * KW + kw) * BYTES;
-#pragma unroll
-        for (int j = 0; j < MINE; ++j) {
-            const int c = rw * MINE + j;
-            const gptr from = c < DK / 16 ? k + c * 1024 : val + (c - DK / 16) * 1024;
-            prefill_fp::load_to_lds((const char *)from, lane * 16, to + c * 1024);  // (its invariant: the wait and the barrier below)
-        }
+        to = lds + ((round & 1) * KW + kw) * BYTES;
+        return true;
     };
-    if (rounds > 0) request(0);
+    auto request = [&](int j) {
+        const int c = rw * MINE + j;
+        const gptr from = c < DK / 16 ? k_from + c * 1024 : v_from + (c - DK / 16) * 1024;
+        prefill_fp::load_to_lds((const char *)from, lane * 16, to + c * 1024);  // (its invariant: the wait and the barrier below)
+    };
+    if (rounds > 0 && locate(0)) {
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) request(j);
+    }
     for (int round = 0; round < rounds; ++round) {
         // the round's blocks are there (every wavefront has waited for its share), and the other half of the ring is free (every
         // wavefront has read it)
@@ -740,11 +749,17 @@ __global__ void __launch_bounds__(512, 2) block_attend_tiled_kernel(BlockAttend 
         __syncthreads();
         k_scale = k_next;
         v_scale = v_next;
-        if (round + 1 < rounds) request(round + 1);
+        const bool more = round + 1 < rounds && locate(round + 1);
+        auto ahead = [&](int t) {
+            if (!more) return;
+#pragma unroll
+            for (int j = 0; j < MINE; ++j)
+                if (j * 4 / MINE == t) request(j);
+        };
         const int blk = block_of(round);
-        if (blk >= 0 && blk < x.b.coded) {
+        if (blk >= 0 && blk < x.b.coded) {  // (a wavefront with a block in the next round has one in this)
             const int j0 = blk * BLOCK_ROWS;
-            w.block_shared(lds + ((round & 1) * KW + kw) * BYTES, k_scale, v_scale, j0, j0 < v.in_lo || j0 + BLOCK_ROWS - 1 > v.in_hi);
+            w.block_shared(lds + ((round & 1) * KW + kw) * BYTES, k_scale, v_scale, j0, j0 < v.in_lo || j0 + BLOCK_ROWS - 1 > v.in_hi, ahead);
         }
     }
     if (tail_at >= 0) w.tail(tail_at);
