@@ -672,6 +672,7 @@ __global__ void __launch_bounds__(512, 2) block_attend_tiled_kernel(BlockAttend 
     using Parts = WaveParts<DV, KW, 16>;
     constexpr size_t RING = 2 * KW * BYTES, JOIN = RW * sizeof(Parts);
     __shared__ __align__(16) char lds[RING > JOIN ? RING : JOIN];
+    __shared__ int there[8];  // by wavefront: rounds that its share of the blocks has come for
     const AttendArgs &a = x.a;
     const int bh = blockIdx.x, part = blockIdx.z;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -682,6 +683,8 @@ __global__ void __launch_bounds__(512, 2) block_attend_tiled_kernel(BlockAttend 
     v.token = 0;
     const int group0 = blockIdx.y * Shape::ROWS;
     v.row0 = group0 + rw * 16 * NM;
+    if (threadIdx.x < 8) there[threadIdx.x] = 0;
+    __syncthreads();
     Walk w(x, bh);
     take_rows<Walk, DK, NM, 1>(w, v, x, group0, group0 + Shape::ROWS);
 
@@ -743,10 +746,15 @@ __global__ void __launch_bounds__(512, 2) block_attend_tiled_kernel(BlockAttend 
         for (int j = 0; j < MINE; ++j) request(j);
     }
     for (int round = 0; round < rounds; ++round) {
-        // the round's blocks are there (every wavefront has waited for its share), and the other half of the ring is free (every
-        // wavefront has read it)
+        // The round's block is there when each of the RW wavefronts that share it has waited for its share; a wavefront that says
+        // so has read the round's before, whose half of the ring the next requests fill.  Only those wait for one
+        // another, and they run the same rounds: the two groups on a SIMD drift apart, products of one over weights of the
+        // other.
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-        __syncthreads();
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        if (lane == 0) __hip_atomic_store(&there[wave], round + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        while (!__all(__hip_atomic_load(&there[kw * RW + (lane & (RW - 1))], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) > round)) {}
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
         k_scale = k_next;
         v_scale = v_next;
         const bool more = round + 1 < rounds && locate(round + 1);
