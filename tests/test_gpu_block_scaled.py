@@ -133,6 +133,45 @@ def test_state_copy_and_trim():
     check_rows(other, fresh)
 
 
+@pytest.mark.parametrize("step", [100, 257])
+def test_growth_over_many_allocations(step):
+    """Pages from a few allocations are found by the kernels' arguments, from more by the page table: the same rows either way."""
+    make = pair(BF16, np.random.default_rng(step), sizes=(64, 64))
+    cache, oracle = kvhip.BlockScaledKVCache(), O.BlockScaledCache("bfloat16")
+    rng = np.random.default_rng(0)
+    for i in range(4200 // step):
+        fill(cache, oracle, make, [step])
+        if i % 4 == 3:
+            check_rows(cache, oracle)
+            q, qd = randn(rng, (2, 4, 3, 64), BF16)
+            T = oracle.offset
+            check(cache.attend(qd, 0.1, kvhip.MaskMode.causal()), *exact_and_bound(q, oracle, 0.1, causal(T, 3, [0, 0])))
+            blocks = cache.select_blocks(qd, 5)
+            assert np.array_equal(blocks.cpu().numpy(), O.select(q, oracle, 5, 1, 1, [0, 0]))
+            check(cache.attend_blocks(qd, blocks, 0.1), *exact_and_bound(q, oracle, 0.1, O.listed_keep(blocks.cpu().numpy(), T, [0, 0])))
+    one = cache.copy()
+    check_rows(one, oracle)
+
+
+def test_emptied_caches():
+    make = pair(F16, np.random.default_rng(8))
+    cache = kvhip.BlockScaledKVCache()
+    fill(cache, O.BlockScaledCache("float16"), make, [70])
+    assert cache.trim(70) == 70
+    other, restored = cache.copy(), kvhip.BlockScaledKVCache()
+    assert all(a.shape[2] == 0 for a in cache.state) and all(a.shape[2] == 0 for a in cache.fetch())
+    restored.state = cache.state
+    for c in (cache, other, restored):
+        assert c.offset == 0
+        with pytest.raises(kvhip.KVHipError):
+            c.attend(torch.zeros(2, 4, 1, 128, dtype=F16, device="cuda"), 0.1)
+        with pytest.raises(kvhip.KVHipError):
+            c.select_blocks(torch.zeros(2, 4, 1, 128, dtype=F16, device="cuda"), 1)
+        fresh = O.BlockScaledCache("float16")
+        fill(c, fresh, make, [1, 64])
+        check_rows(c, fresh)
+
+
 def test_saved_as_full_precision(tmp_path):
     """A prompt-cache file holds the rows as they are read back, under the class that the reference knows."""
     make = pair(BF16, np.random.default_rng(5))
@@ -168,7 +207,7 @@ def exact_and_bound(q, oracle, scale, weight, add=None):
             h = hq // G
             w = weight[b, {1: 0, Hkv: h}.get(weight.shape[1], hq)]
             s = q[b, hq] @ k[b, h].T * scale
-            size = np.abs(q[b, hq]) @ np.abs(k[b, h]).T * scale
+            size = np.abs(q[b, hq]) @ np.abs(k[b, h]).T * abs(scale)
             if add is not None:
                 s = s + add[b, hq]
                 size = size + np.where(np.isfinite(add[b, hq]), np.abs(add[b, hq]), 0.0)
@@ -236,6 +275,76 @@ def test_attention_of_padded_batches_and_windows(dtype, layout, T, n, pads, wind
     mask = kvhip.MaskMode.window_mask(T - n, window, left_pad=torch.tensor(pads, device="cuda"))
     got = cache.attend(qd, scale, mask)
     check(got, *exact_and_bound(q, oracle, scale, causal(T, n, pads, window)))
+
+
+@pytest.mark.parametrize("layout", [LAYOUTS[0], LAYOUTS[3]])
+@pytest.mark.parametrize("n", [1, 3, 50])
+def test_attention_with_lengths(layout, n):
+    """Sequences that end before the cache does, one of them before its first key."""
+    cache, oracle, queries = held(BF16, 400, layout, seed=6, B=3)
+    rng = np.random.default_rng(n)
+    q, qd = randn(rng, (3, layout[0], n, layout[2]), BF16)
+    lengths = (400, 130, 0)
+    mask = kvhip.MaskMode.window_mask(400 - n, 0, lengths=torch.tensor(lengths, device="cuda"))
+    keep = causal(400, n, [0, 0, 0])
+    for b, m in enumerate(lengths):
+        keep[b, :, :, m:] = 0
+    got = cache.attend(qd, 0.1, mask)
+    check(got, *exact_and_bound(q, oracle, 0.1, keep))
+    assert (got[2] == 0).all()
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 3.0])
+@pytest.mark.parametrize("n", [1, 40])
+def test_scales_of_any_sign(scale, n):
+    cache, oracle, queries = held(BF16, 300, LAYOUTS[0], seed=7)
+    q, qd = queries(n)
+    check(cache.attend(qd, scale, kvhip.MaskMode.causal()), *exact_and_bound(q, oracle, scale, causal(300, n, [0, 0])))
+    blocks = cache.select_blocks(qd, 5)
+    want = O.listed_keep(blocks.cpu().numpy(), 300, [0, 0])
+    check(cache.attend_blocks(qd, blocks, scale), *exact_and_bound(q, oracle, scale, want))
+
+
+def test_arrays_that_start_anywhere():
+    """Keys, values, queries and outputs aligned as their elements are."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+
+    def at(shape, off):
+        n = int(np.prod(shape))
+        flat = torch.randn(n + off, generator=gen, device="cuda").to(BF16)
+        return flat[off:].view(shape)
+
+    k, v, q = at((2, 2, 130, 128), 1), at((2, 2, 130, 128), 3), at((2, 8, 40, 128), 5)
+    out = torch.zeros(2 * 8 * 40 * 128 + 1, dtype=BF16, device="cuda")[1:].view(2, 8, 40, 128)
+    a, b = kvhip.BlockScaledKVCache(), kvhip.BlockScaledKVCache()
+    a.update(k, v, fetch=False)
+    b.update(k.clone(), v.clone(), fetch=False)
+    for x, y in zip(a.fetch(), b.fetch()):
+        assert torch.equal(x, y)
+    a.attend(q, 0.1, kvhip.MaskMode.causal(), out=out)
+    assert torch.equal(out, b.attend(q.clone(), 0.1, kvhip.MaskMode.causal()))
+    chosen = a.select_blocks(q, 2)
+    assert torch.equal(chosen, b.select_blocks(q.clone(), 2))
+    one = at((2, 8, 1, 128), 7)
+    k1, v1 = at((2, 2, 1, 128), 1), at((2, 2, 1, 128), 1)
+    assert torch.equal(a.update_attend(one, k1, v1, 0.1), b.update_attend(one.clone(), k1.clone(), v1.clone(), 0.1))
+
+
+def test_speculative_rounds_write_through_and_trim():
+    """An append-only leaf of a round: drafts are written, the rejected ones trimmed, and accepted ones as if alone."""
+    make = pair(BF16, np.random.default_rng(12))
+    cache, oracle = kvhip.BlockScaledKVCache(), O.BlockScaledCache("bfloat16")
+    fill(cache, oracle, make, [61])
+    for accepted in (2, 0, 4, 1):
+        drafts = [make(1) for _ in range(4)]
+        for (k, kd), (v, vd) in drafts:
+            cache.update(kd, vd, fetch=False)
+            oracle.update(k, v)
+        assert cache.trim(4 - accepted) == 4 - accepted
+        if accepted < 4:
+            oracle.trim(4 - accepted)
+    check_rows(cache, oracle)
+    assert kvhip.can_trim_prompt_cache([cache]) and cache.is_trimmable_after(1000)
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
