@@ -79,7 +79,9 @@ size_t plan_block_attend(BlockAttend &x) {
     const int64_t base = a.st.BH * block_attend_rows(x);
     const int blocks = x.list ? x.count : (a.T + BLOCK_ROWS - 1) / BLOCK_ROWS;
     // Wavefronts that fill the chip, two to a SIMD where the registers allow it; workgroups of eight where they serve one row
-    // tile and there is work for them: their parts meet in LDS, and half as many are left to merge.
+    // tile and there is work for them: their parts meet in LDS, and half as many are left to merge, none at 256 pairs (four / eight
+    // wavefronts, us: 32 sequences at 32 768 keys 371 + a merge of 4.8 / 351; 8 of eight heads a pair 31.8 / 26.5; 16 of four
+    // tokens 76 / 65; 30 011 keys of one 19.6 / 14.2; 517 keys of 4 x 64 9.1 / 7.2; 64 listed blocks 13.1 / 10.5).
     const int64_t wanted = (a.st.Dk <= 128 ? 2048 : 1024) / std::max<int64_t>(base, 1);
     x.waves = nm == 1 && a.st.Dk <= 128 && a.mask.mode != KVHIP_MASK_ARRAY && wanted >= 8 && blocks > 4 ? 8 : 4;
     if (block_attend_tiled(x)) x.waves = 8;  // (one workgroup to a compute unit)

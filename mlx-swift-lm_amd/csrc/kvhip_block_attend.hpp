@@ -9,6 +9,11 @@
 // Codes become operands by one conversion for two values, which takes the block's scale along.  Operands are loaded straight
 // from the pages, 1 KB to an instruction, half a block ahead.  The blocks'
 // addresses and scales are looked up 64 at a time, a lane to a block, instead of one dependent load after another.
+//
+// Single tokens are bound by memory where the batch fills the chip (32 sequences at 32 768 keys, 8 x 128: 351 us, 6.1 TB/s;
+// 16 ragged ones of four tokens 65 us, 4.4 TB/s over the keys that they see) and by the chain of a launch where it does not
+// (517 keys of 4 x 64: 7.2 us; 30 011 of 8 x 128: 14.2 us, 4.3 TB/s, and 3.9 for the merge).  Chosen blocks of a prompt's
+// tokens come from the second-level caches, 16 KB to a token, block and pair (300 tokens x 32 blocks x 8 pairs: 78 us, 16 TB/s).
 #pragma once
 #include "kvhip_block.hpp"
 #include "kvhip_mask.hpp"
@@ -17,11 +22,19 @@
 
 namespace kvhip {
 
-// Whether a call has rows enough for the kernel that shares blocks between wavefronts, and the rows its workgroup takes.
-inline bool block_attend_tiled(const BlockAttend &x) { return !x.list && x.a.mask.mode != KVHIP_MASK_ARRAY && x.a.Hq / x.a.Hkv * x.a.L > 32; }
-inline int block_tiled_rows(int Dk) { return Dk <= 128 || Dk > 192 ? 64 : 128; }
+// Whether a call has rows enough for the kernel that shares blocks between wavefronts, and the rows its workgroup takes.  Against
+// two tiles of rows to a wavefront that loads for itself, bfloat16, us, shared / not: head size 128, 40 rows of a pair 35.6 / 39.9
+// (8 x 8 pairs, 8000 keys) and 54.0 / 73.6 (32 x 8 pairs, 4000), 64 rows 26.4 / 31.2, 256 rows 109 / 112, 2048 rows 109 / 107; 256, 40 rows
+// 23.3 / 33.4, 600 rows 49.8 / 73.3; keys of 192, 200 rows 41.1 / 47.1, 40 rows 24.4 / 21.5.  Head sizes below 128, whose blocks
+// need fewer registers, go the other way: 64, 160 rows 37.0 / 31.3, 2000 rows 234 / 210; 96, 200 rows 144 / 136.
+inline bool block_attend_tiled(const BlockAttend &x) {
+    return !x.list && x.a.mask.mode != KVHIP_MASK_ARRAY && x.a.st.Dk >= 128 && x.a.Hq / x.a.Hkv * x.a.L > 32;
+}
+inline int block_tiled_rows(int Dk) { return Dk == 192 ? 128 : 64; }
 
-// Tiles of 16 query rows that a wavefront takes (plan_block_attend chooses by the same rule).
+// Tiles of 16 query rows that a wavefront takes (plan_block_attend chooses by the same rule).  Two, where there are rows for them:
+// each conversion of a block's codes then serves both.  Four do not fit the registers of two wavefronts a SIMD (512 rows
+// over 8192 keys x 128, 32 heads: 227 us, and 104 with two).
 inline int block_row_tiles(const BlockAttend &x) {
     const int rows = x.a.Hq / x.a.Hkv * x.a.L;
     if (x.list || rows <= 16) return 1;
@@ -655,12 +668,15 @@ __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kerne
     }
 }
 
-// Many query rows (prompt chunks): eight wavefronts, RW groups of 16 NM rows by KW of the blocks of a round.  The blocks of a
+// Many query rows of head sizes from 128 on (prompt chunks): eight wavefronts, RW groups of 16 NM rows by KW of the blocks of a round.  The blocks of a
 // round lie in LDS, each read by the RW wavefronts that share it; the next round's are on their way, past the registers, while
-// this one's are looked at: whole lines from the pages, a round's work to cover them (requested half a block ahead by every
-// wavefront for itself, a third of the time went by waiting).  One barrier a round.
+// this one's are looked at.  Wavefronts wait only for those that they share a block with.
+// What bounds it: vector instructions and products share a SIMD's issue -- a block costs two tiles of rows 2700 cycles alone and
+// 3000 beside another wavefront, of 1360 for its 68 products and 2050 for 128 conversions, 32 exponentials and the rest -- at a clock
+// that falls to about 2 GHz under them: 512 rows over 8192 keys x 128 (2048 rows of 8 pairs) 102 us, 655 TFLOP/s.
 // grid (BH, tiles of 16 NM RW rows, parts)
 template <int DK, int DV> struct TiledShape {
+    // (registers: one tile of rows a wavefront at 256; LDS: two rounds of KW blocks)
     static constexpr int NM = DK <= 192 ? 2 : 1, RW = DK <= 128 ? 2 : 4, KW = 8 / RW, ROWS = 16 * NM * RW;
 };
 template <int DK, int DV, int DT>
@@ -785,9 +801,11 @@ template <int DK, int DV, int DT, int NM, int MODE, int NW = 4> hipError_t block
     return hipGetLastError();
 }
 template <int DK, int DV, int DT> hipError_t block_attend_shape(const BlockAttend &x, hipStream_t stream) {
-    if (block_attend_tiled(x)) {
-        hipLaunchKernelGGL((block_attend_tiled_kernel<DK, DV, DT>), dim3(x.a.st.BH, block_attend_rows(x), x.nsplit), dim3(512), 0, stream, x);
-        return hipGetLastError();
+    if constexpr (DK >= 128) {
+        if (block_attend_tiled(x)) {
+            hipLaunchKernelGGL((block_attend_tiled_kernel<DK, DV, DT>), dim3(x.a.st.BH, block_attend_rows(x), x.nsplit), dim3(512), 0, stream, x);
+            return hipGetLastError();
+        }
     }
     if constexpr (DK <= 128) {
         if (x.waves == 8) return x.list ? block_attend_run<DK, DV, DT, 1, 3, 8>(x, stream) : block_attend_run<DK, DV, DT, 1, 1, 8>(x, stream);

@@ -218,7 +218,7 @@ struct RowsOf {
 };
 // One tile of 16 query rows as operands -- the positive and the negative part, [KS][64] each -- by one wavefront.  Everything
 // else in the workgroup waits for it: the largest magnitude as a packed integer maximum, a number that is none only looked for
-// where there is one, whole numbers by an addition that leaves them in the low bits (5700 -> 2000 cycles of a step).
+// where there is one, whole numbers by an addition that leaves them in the low bits.
 template <int D, int DT>
 __device__ __forceinline__ void query_operands(const char *row, int tok, int ud, int lane, kv_i4 *pos_out, kv_i4 *neg_out, RowsOf &of) {
     constexpr int KS = (D + 63) / 64;
@@ -373,7 +373,8 @@ struct SelectView {
 
 // Many tokens: grid (BH, groups of `tokens` tokens), 16 wavefronts.  LDS: a histogram for each wavefront, the query operands and
 // exponents of up to four tiles of 16 rows, keys [tokens][stride] of the blocks from `lead` on.  A wavefront requests the
-// summaries of several groups of 16 blocks before it looks at the first.
+// summaries of several groups of 16 blocks before it looks at the first.  300 tokens of 32 heads over 30 000 keys, 8 pairs: 20.7 us,
+// a chain of its queries, its summaries (120 KB a workgroup) and the choice.
 template <int D, int DT>
 __global__ void __launch_bounds__(SELECT_WAVES * 64) block_select_kernel(BlockSelect x, int tokens, int stride) {
     constexpr int KS = (D + 63) / 64, AHEAD = D <= 128 ? 4 : 2;
@@ -408,15 +409,16 @@ __global__ void __launch_bounds__(SELECT_WAVES * 64) block_select_kernel(BlockSe
                   x.list + ((size_t)v.bh * x.L + v.tok0 + tok) * x.count);
 }
 
-// Few tokens: the bounds by as many workgroups as there are stretches of 256 (head sizes above 128: 128) blocks -- one
+// Few tokens: the bounds by as many workgroups as there are stretches of 128 (head sizes above 128: 64) blocks -- one
 // compute unit takes in a step's summaries at 13 bytes a cycle, 20 000 cycles for the 131 000 keys of one head -- and the
-// choice, a workgroup to a token, in a launch of its own.
+// choice, a workgroup to a token, in a launch of its own.  One token of eight sequences at 65 000 keys 6.5 + 5.5 us (in one launch
+// 19.9), of one at 131 000 5.2 + 7.5 (29.6; stretches of 256 blocks 6.6 + 7.4): chains of latencies, the 17 MB and 4 MB that they read are 3.4 and 0.9.
 // grid (BH, groups of `tokens` tokens, stretches), 4 wavefronts.  out: keys [BH, L, stride].
 constexpr int BOUND_WAVES = 4, BOUND_TILES = 2;
-template <int D> constexpr int bound_ahead() { return D <= 128 ? 4 : 2; }
+constexpr int bound_ahead(int D) { return D <= 128 ? 2 : 1; }
 template <int D, int DT>
 __global__ void __launch_bounds__(BOUND_WAVES * 64) block_bounds_kernel(BlockSelect x, int tokens, int stride, uint32_t *out) {
-    constexpr int KS = (D + 63) / 64, AHEAD = bound_ahead<D>(), SPAN = BOUND_WAVES * AHEAD * 16;
+    constexpr int KS = (D + 63) / 64, AHEAD = bound_ahead(D), SPAN = BOUND_WAVES * AHEAD * 16;
     __shared__ kv_i4 ops[BOUND_TILES][2][KS * 64];
     __shared__ RowsOf of[BOUND_TILES];
     __shared__ uint32_t keys[16 * BOUND_TILES * SPAN];
@@ -479,9 +481,9 @@ SelectPlan select_plan(const BlockSelect &x) {
     p.tokens = std::min(p.tokens, x.L);
     if (p.tokens < 1) return p;
     const int64_t groups = (int64_t)x.b.st.BH * ((x.L + p.tokens - 1) / p.tokens);
-    const int span = BOUND_WAVES * 16 * (x.b.st.Dk <= 128 ? 4 : 2);
-    // (up to that many blocks one launch is the shorter)
-    if (groups < 128 && p.stride > 256 && (size_t)x.b.st.BH * x.L * p.stride * 4 <= BOUND_KEYS) {
+    const int span = BOUND_WAVES * 16 * bound_ahead(x.b.st.Dk);
+    // (workgroups enough for half the chip, or one stretch of blocks: one launch)
+    if (groups < 128 && p.stride > 128 && (size_t)x.b.st.BH * x.L * p.stride * 4 <= BOUND_KEYS) {
         p.tokens = std::min(p.tokens, std::max(1, 16 * BOUND_TILES / G));
         p.stretches = (p.stride + span - 1) / span;
     }
