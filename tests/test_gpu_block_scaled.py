@@ -489,6 +489,60 @@ def test_static_scratch_and_streams():
     check(cache.attend(qd, 0.1, kvhip.MaskMode.causal(), static_scratch=True), *exact_and_bound(q, oracle, 0.1, causal(2500, 1100, [0, 0])))
 
 
+def close_to_float64(got, q, k, v, scale, keep):
+    """`got` [..., n, Dv] of one kv head against float64 over its rows as read back, within what the roundings allow: the output's
+    and the weights' half steps, relative to the output and to the weights' sum over |v|, and as much again for the sums."""
+    s = (q.double() @ k.double().T * scale).masked_fill(~keep, -INF)
+    p = torch.softmax(s, -1)
+    want, size = p @ v.double(), p @ v.double().abs()
+    u = torch.finfo(got.dtype).eps / 2
+    assert ((got.double() - want).abs() <= u * want.abs() + 2 * u * size).all()
+
+
+@pytest.mark.parametrize("B,H,G,D,T,n", [(32, 8, 1, 64, 38500, 1), (8, 8, 4, 128, 20100, 64), (16, 16, 8, 64, 17000, 4)])
+def test_walks_of_many_blocks(B, H, G, D, T, n):
+    """More than 64 blocks to a wavefront: their addresses are looked up in turns."""
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    cache = kvhip.BlockScaledKVCache()
+    cache.reserve(B, H, D, D, BF16, T)
+    for at in range(0, T, 4096):
+        m = min(4096, T - at)
+        k, v = (torch.randn(B, H, m, D, generator=gen, device="cuda").to(BF16) for _ in range(2))
+        cache.update(k, v, fetch=False)
+    q = torch.randn(B, H * G, n, D, generator=gen, device="cuda").to(BF16)
+    out = cache.attend(q, 0.2, kvhip.MaskMode.causal())
+    k, v = cache.fetch()
+    keep = torch.arange(T, device="cuda") <= torch.arange(T - n, T, device="cuda")[:, None]
+    for b, h in ((0, 0), (B - 1, H - 1), (B // 2, 3)):
+        close_to_float64(out[b, h * G:(h + 1) * G].flatten(0, 1), q[b, h * G:(h + 1) * G].flatten(0, 1), k[b, h], v[b, h], 0.2, keep.repeat(G, 1))
+
+
+def test_offsets_beyond_32_bits():
+    """Codes of keys past 4 GiB: rows at the far end, whole and listed, against a cache of nothing else."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    step, D = 1 << 20, 256
+    k, v = (torch.randn(1, 1, step, D, generator=gen, device="cuda").to(BF16) for _ in range(2))
+    cache, near = kvhip.BlockScaledKVCache(), kvhip.BlockScaledKVCache()
+    cache.reserve(1, 1, D, D, BF16, 17 * step)
+    for _ in range(16):
+        cache.update(k, v, fetch=False)
+    last = [x[:, :, :5000] * 0.5 for x in (k, v)]
+    cache.update(*last, fetch=False)
+    near.update(*last, fetch=False)
+    T = 16 * step + 5000
+    assert cache.offset == T and T * D > 1 << 32
+    q = torch.randn(1, 4, 20, D, generator=gen, device="cuda").to(BF16)
+    keep = torch.arange(5000, device="cuda") <= torch.arange(4980, 5000, device="cuda")[:, None]
+    nk, nv = (x[0, 0] for x in near.fetch())
+    far = torch.tensor([T - 5000], device="cuda")
+    out = cache.attend(q, 0.1, kvhip.MaskMode.window_mask(T - 20, 0, left_pad=far))
+    close_to_float64(out[0].flatten(0, 1), q[0].flatten(0, 1), nk, nv, 0.1, keep.repeat(4, 1))
+    blocks = torch.arange((T - 5000) // 64, (T + 63) // 64, dtype=torch.int32, device="cuda").expand(1, 1, 20, -1).contiguous()
+    out = cache.attend_blocks(q, blocks, 0.1, far)
+    close_to_float64(out[0].flatten(0, 1), q[0].flatten(0, 1), nk, nv, 0.1, keep.repeat(4, 1))
+    del cache
+
+
 # ---- choosing blocks ------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("layout", LAYOUTS + [(5, 5, 64, 64), (40, 2, 128, 128), (3, 1, 96, 96)])
@@ -510,6 +564,39 @@ def test_blocks_of_long_caches(layout, n, count, first, recent, pads):
     q, qd = queries(n)
     got = cache.select_blocks(qd, count, first, recent, torch.tensor(pads, device="cuda"))
     assert np.array_equal(got.cpu().numpy(), O.select(q, oracle, count, first, recent, pads))
+
+
+@pytest.mark.parametrize("H,G,T,n,count", [(1, 4, 1_200_000, 1, 50), (1, 4, 66_000, 2100, 33), (2, 16, 140_000, 3, 64)])
+def test_blocks_of_very_long_caches(H, G, T, n, count):
+    """Keys of the choice beyond 64 KiB of LDS, in either form of the launch."""
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    keys = torch.randn(1, H, T, 64, generator=gen, device="cuda").to(F16)
+    cache = kvhip.BlockScaledKVCache()
+    cache.update(keys, keys, fetch=False)
+    q = torch.randn(1, H * G, n, 64, generator=gen, device="cuda").to(F16)
+    got = cache.select_blocks(q, count, 1, 2)
+    whole = T // 64
+    x = keys[0, :, :whole * 64].double().unflatten(1, (whole, 64))
+    read = cache.fetch()[0][0, :, :whole * 64].double().unflatten(1, (whole, 64))
+    m, e = torch.frexp(x.abs().amax((2, 3)))
+    two_to = lambda n: ((n.long() + 1023) << 52).view(torch.float64)  # noqa: E731 (exactly)
+    unit = two_to(e - 9 + (m > 0.875).to(e.dtype) + 2)
+    units = torch.round(read / unit[..., None, None])
+    hi, lo = units.amax(2), units.amin(2)
+    rows = q[0].double().unflatten(0, (H, G))
+    m, f = torch.frexp(rows.abs().amax(-1))
+    grid = two_to(f - 7 + (m > 127 / 128).to(f.dtype))[..., None]
+    whole_q = torch.round(rows / grid)
+    at = torch.arange(T - n, T, device="cuda")[:, None] // 64
+    index = torch.arange((T + 63) // 64, device="cuda")
+    for h in range(H):
+        bound = ((whole_q[h].clamp(min=0) @ hi[h].T + whole_q[h].clamp(max=0) @ lo[h].T) * grid[h] * unit[h]).amax(0)
+        rank = torch.full((n, len(index)), -INF, dtype=torch.float64, device="cuda")
+        rank[:, :whole] = bound
+        rank = rank.masked_fill((index < 1) | (index > at - 2), INF).masked_fill(index > at, -INF)
+        want = torch.sort(rank, dim=-1, descending=True, stable=True).indices[:, :count].sort(-1).values
+        off = (got[0, h].long() != want).any(-1).nonzero()
+        assert len(off) == 0, f"{len(off)} tokens, the first {int(off[0])}: {got[0, h, off[0]].tolist()} for {want[off[0]].tolist()}"
 
 
 def test_equal_bounds_of_long_caches():
