@@ -534,9 +534,10 @@ __device__ __forceinline__ void leave_tile(Walk &w, const RowsView &v, const Blo
     __syncthreads();
     const float weight = wave_weight(parts, w.n, w.m[i]);
     if (w.g == 0) parts.l[k][w.n] = l * weight;
+    if (w.n < rows) {  // (a step has few rows of the sixteen)
 #pragma unroll
-    for (int d = 0; d < Walk::VT; ++d)
-        *reinterpret_cast<kv_f4 *>(&parts.rows[k][w.n][16 * d + 4 * w.g]) = w.o[i][d] * weight;
+        for (int d = 0; d < Walk::VT; ++d) *reinterpret_cast<kv_f4 *>(&parts.rows[k][w.n][16 * d + 4 * w.g]) = w.o[i][d] * weight;
+    }
     __syncthreads();
     constexpr int LPR = DV / 4, RPB = KW * 64 / LPR;
     const int c = 4 * (t % LPR);
