@@ -1310,8 +1310,10 @@ bool attention_will_write_step(const kvhip_cache *c, int Hq) {
 }
 
 // Attention over a block-scaled cache: under a.mask, or (`list`) over listed blocks.
+// `choice`: the lists are yet to be chosen; its bounds are formed here, and the choice is the attention's where that can, else
+// a launch of its own.
 kvhip_status run_block_attend(kvhip_cache *c, const AttendArgs &a, const int32_t *list, int32_t count, const int32_t *left_pad, float *fixed,
-                              size_t fixed_bytes, hipStream_t s) {
+                              size_t fixed_bytes, hipStream_t s, BlockSelect *choice = nullptr) {
     BlockAttend x;
     x.a = a;
     x.b = block_store(c);
@@ -1320,7 +1322,22 @@ kvhip_status run_block_attend(kvhip_cache *c, const AttendArgs &a, const int32_t
     x.left_pad = left_pad;
     const size_t need = plan_block_attend(x);
     if (block_attend_rows(x) > 65535) return fail(KVHIP_ERR_UNSUPPORTED, "more query rows than one call takes");
-    KV_TRY(bind_workspace(c, x.a, need, fixed, fixed_bytes, s));
+    // (the choice's keys lie behind the partials: the attention reads them while it writes those)
+    const size_t behind = choice ? align256(need) : need;
+    KV_TRY(bind_workspace(c, x.a, behind + (choice ? block_select_workspace(*choice) : 0), fixed, fixed_bytes, s));
+    if (choice) {
+        choice->workspace = reinterpret_cast<char *>(x.a.workspace) + behind;
+        const int stride = block_select_stride(*choice);
+        choice->bounds_only = block_attend_chooses(x, stride);
+        KV_HIP(launch_block_select(*choice, s));
+        if (choice->bounds_only) {
+            x.keys = static_cast<const uint32_t *>(choice->workspace);
+            x.key_stride = stride;
+            x.first = choice->first;
+            x.recent = choice->recent;
+            x.list_out = choice->list;
+        }
+    }
     KV_HIP(launch_block_attend(x, s));
     g_last_kernel = list ? 8 : 7;
     return KVHIP_OK;
@@ -1621,7 +1638,8 @@ kvhip_status block_choice(const kvhip_cache *c, const void *q, int32_t B, int32_
     return KVHIP_OK;
 }
 kvhip_status attend_blocks_impl(kvhip_cache *c, const void *q, int32_t B, int32_t Hq, int32_t L, int32_t D, float scale, const int32_t *blocks,
-                                int32_t count, const int32_t *left_pad, void *out, const void *new_k, const void *new_v, hipStream_t s) {
+                                int32_t count, const int32_t *left_pad, void *out, const void *new_k, const void *new_v, hipStream_t s,
+                                BlockSelect *choice = nullptr) {
     AttendArgs a;
     void *user_out = nullptr;
     const size_t q_rows = (size_t)B * Hq * L;
@@ -1642,7 +1660,7 @@ kvhip_status attend_blocks_impl(kvhip_cache *c, const void *q, int32_t B, int32_
     a.scale = scale;
     a.new_k = new_k;
     a.new_v = new_v;
-    KV_TRY(run_block_attend(c, a, blocks, count, left_pad, nullptr, 0, s));
+    KV_TRY(run_block_attend(c, a, blocks, count, left_pad, nullptr, 0, s, choice));
     if (user_out) KV_HIP(launch_repitch_rows(user_out, (size_t)c->Dv_user * c->st.es, out, (size_t)c->st.Dv * c->st.es, q_rows, s));
     return KVHIP_OK;
 }
@@ -1680,16 +1698,11 @@ kvhip_status kvhip_cache_update_attend_blocks(kvhip_cache *c, const void *q, con
     KV_TRY(check_block_call(c, B, Hq, L, Dk, T, count));
     BlockSelect x;
     KV_TRY(block_choice(c, q, B, Hq, L, T, count, first, recent, left_pad, blocks, x));
-    KV_TRY(ensure_ws(c, block_select_workspace(x), S(stream)));
-    x.workspace = c->ws;
     hipStream_t s = S(c, stream);
     const bool fuse = block_step_fuses(c, L);
     KV_TRY(update_blocks(c, k, v, L, s, !fuse));
     x.b = block_store(c);
-    hipError_t e = launch_block_select(x, s);
-    kvhip_status st = e == hipSuccess ? KVHIP_OK : fail(KVHIP_ERR_HIP, std::string("the choice of blocks: ") + hipGetErrorString(e));
-    if (st == KVHIP_OK)
-        st = attend_blocks_impl(c, q, B, Hq, L, Dk, scale, blocks, count, left_pad, out, fuse ? k : nullptr, fuse ? v : nullptr, s);
+    const kvhip_status st = attend_blocks_impl(c, q, B, Hq, L, Dk, scale, blocks, count, left_pad, out, fuse ? k : nullptr, fuse ? v : nullptr, s, &x);
     if (st != KVHIP_OK && fuse) {  // nothing was written: take the row back
         c->offset -= 1;
         c->presented = c->offset;

@@ -66,6 +66,10 @@ struct BlockAttend {
     const int32_t *list = nullptr;
     int32_t count = 0;
     const int32_t *left_pad = nullptr;
+    // with `keys` the lists are yet to be chosen, by every workgroup for itself (block_attend_chooses), and written to list_out
+    const uint32_t *keys = nullptr;
+    int32_t key_stride = 0, first = 0, recent = 1;
+    int32_t *list_out = nullptr;
     // plan
     int32_t nsplit = 1;  // parts of a row's blocks
     int32_t tiles = 1;   // (listed blocks) 16-row tiles of a token's heads
@@ -74,6 +78,8 @@ struct BlockAttend {
 // Chooses the plan within a.workspace_cap; returns the bytes of scratch.
 size_t plan_block_attend(BlockAttend &x);
 int64_t block_attend_rows(const BlockAttend &x);  // tiles of query rows of a pair (at most 65535)
+// Whether the attention of a planned call can choose its lists itself: they and the keys fit the memory of the parts.
+bool block_attend_chooses(const BlockAttend &x, int key_stride);
 hipError_t launch_block_attend(const BlockAttend &x, hipStream_t stream);
 
 struct BlockSelect {
@@ -85,8 +91,10 @@ struct BlockSelect {
     const int32_t *left_pad = nullptr;
     int32_t *list = nullptr;  // [BH, L, count]
     void *workspace = nullptr;
+    bool bounds_only = false;  // leave the choice to the attention (keys [BH, L, block_select_stride] in the workspace)
 };
 bool block_select_supported(const BlockSelect &x);
+int block_select_stride(const BlockSelect &x);  // blocks a row of keys, where bounds and choice are launches of their own; else 0
 size_t block_select_workspace(const BlockSelect &x);
 hipError_t launch_block_select(const BlockSelect &x, hipStream_t stream);
 

@@ -94,6 +94,11 @@ size_t plan_block_attend(BlockAttend &x) {
     return parts > 1 ? one * parts : 0;
 }
 
+bool block_attend_chooses(const BlockAttend &x, int key_stride) {
+    const size_t parts = sizeof(float) * x.waves * 16 * (x.a.st.Dv + 4);  // (WaveParts)
+    return key_stride > 0 && x.count <= CHOSEN_MAX && (size_t)key_stride * sizeof(uint32_t) <= parts;
+}
+
 hipError_t launch_block_attend(const BlockAttend &x, hipStream_t stream) {
     const bool f16 = x.a.st.dtype == KVHIP_F16;
     const hipError_t e = f16 ? launch_block_attend_f16(x, stream) : launch_block_attend_bf16(x, stream);

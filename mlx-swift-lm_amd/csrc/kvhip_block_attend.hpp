@@ -15,7 +15,7 @@
 // (517 keys of 4 x 64: 7.2 us; 30 011 of 8 x 128: 14.2 us, 4.3 TB/s, and 3.9 for the merge).  Chosen blocks of a prompt's
 // tokens come from the second-level caches, 16 KB to a token, block and pair (300 tokens x 32 blocks x 8 pairs: 78 us, 16 TB/s).
 #pragma once
-#include "kvhip_block.hpp"
+#include "kvhip_block_choose.hpp"
 #include "kvhip_mask.hpp"
 #include "kvhip_prefill_fp.hpp"
 #include "kvhip_span_merge.hpp"
@@ -46,6 +46,8 @@ namespace {
 typedef float kv_f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 kv_b8 __attribute__((ext_vector_type(8)));
 typedef _Float16 kv_h8 __attribute__((ext_vector_type(8)));
+
+constexpr int CHOSEN_MAX = 1024;  // listed blocks that a workgroup chooses itself
 
 template <int DT> __device__ __forceinline__ kv_f4 block_mfma(const kv_u4 &x, const kv_u4 &y, const kv_f4 &c) {
     if constexpr (DT == 1) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kv_b8, x), __builtin_bit_cast(kv_b8, y), c, 0, 0, 0);
@@ -595,6 +597,25 @@ __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kerne
     const int s0 = min(part * each, total), s1 = min(s0 + each, total);
     const int mine = s1 - s0 > wave ? (s1 - s0 - wave + NW - 1) / NW : 0;
     const int32_t *list = MODE == 3 ? x.list + ((size_t)bh * a.L + token) * x.count : nullptr;
+    if constexpr (MODE == 3) {
+        if (x.keys) {
+            // The choice by every workgroup of the token for itself, keys in the memory that the parts take later (one sequence of 131 000
+            // keys, 64 blocks: 15.4 us, 7.5 + 10.5 with the choice in a launch of its own; 8 ragged ones of 65 000, 32 blocks: 14.4, 6 + 12.3).
+            __shared__ int32_t chosen[CHOSEN_MAX];
+            __shared__ uint32_t area[choose_area(NW)];
+            uint32_t *keys = reinterpret_cast<uint32_t *>(&parts);
+            const uint32_t *from = x.keys + ((size_t)bh * a.L + token) * x.key_stride;
+            const int lead = lo / BLOCK_ROWS, seen = hi < lo ? 0 : hi / BLOCK_ROWS - lead + 1;
+            if (seen > x.count)
+                for (int i = threadIdx.x; i < seen - x.recent; i += NW * 64) keys[i] = from[i];
+            __syncthreads();
+            choose<NW>(keys, area, lane, lead, seen, x.count, x.first, x.recent, chosen);
+            __syncthreads();
+            list = chosen;
+            if (part == 0 && v.row0 == 0)
+                for (int i = threadIdx.x; i < x.count; i += NW * 64) x.list_out[((size_t)bh * a.L + token) * x.count + i] = chosen[i];
+        }
+    }
     int tail_at = -1;
 
     for (int at = 0; at < mine; at += 64) {

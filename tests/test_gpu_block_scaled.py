@@ -649,6 +649,38 @@ def test_attention_over_chosen_blocks(dtype, layout, T, n, count, pads):
     check_rows(cache, oracle)
 
 
+@pytest.mark.parametrize("layout", LAYOUTS + [(40, 2, 128, 128)])
+@pytest.mark.parametrize("T,n,count,first,recent,pads", [(9000, 1, 20, 1, 2, (0, 0)), (9001, 3, 7, 0, 1, (8999, 300)), (12000, 1, 64, 2, 3, (11999, 64)),
+                                                        (9000, 2, 200, 1, 1, (0, 0)), (30000, 1, 1100, 1, 1, (0, 9000))])
+def test_steps_that_choose_their_blocks(layout, T, n, count, first, recent, pads):
+    """One call on a long cache -- the attention makes the choice itself where that is the shorter -- against the choice and the
+    attention apart, and against float64."""
+    hq, h, dk, dv = layout
+    rng = np.random.default_rng(T)
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    k, v = (torch.randn(2, h, T - n, d, generator=gen, device="cuda").to(BF16) for d in (dk, dv))
+    cache = kvhip.BlockScaledKVCache()
+    cache.update(k, v, fetch=False)
+    apart = cache.copy()
+    q, k, v = (torch.randn(2, x, n, d, generator=gen, device="cuda").to(BF16) for x, d in ((hq, dk), (h, dk), (h, dv)))
+    pad = torch.tensor(pads, device="cuda")
+    scale = dk ** -0.5
+    got, blocks = cache.update_attend_blocks(q, k, v, scale, count, first, recent, pad)
+    apart.update(k, v, fetch=False)
+    assert torch.equal(blocks, apart.select_blocks(q, count, first, recent, pad))
+    assert torch.equal(got, apart.attend_blocks(q, blocks, scale, pad))
+    keys, values = cache.fetch()
+    weight = torch.from_numpy(O.listed_keep(blocks[:, :1].cpu().numpy(), T, pads)).cuda()
+    G = hq // h
+    for b in range(2):
+        for t in range(n):
+            keep = weight[b, 0, t] > 0
+            if keep.any():
+                close_to_float64(got[b, :G, t], q[b, :G, t], keys[b, 0], values[b, 0], scale, keep[None])
+            else:
+                assert (got[b, :G, t] == 0).all()
+
+
 def test_lists_of_any_content():
     """Entries outside what the token sees, repeated and descending ones are passed over; nothing listed: zeros."""
     cache, oracle, queries = held(BF16, 700, LAYOUTS[0])
