@@ -1615,7 +1615,8 @@ kvhip_status check_block_call(const kvhip_cache *c, int32_t B, int32_t Hq, int32
     if (B != c->B || D != c->Dk_user) return fail(KVHIP_ERR_INVALID_ARG, "query shape does not match the cache");
     if (Hq <= 0 || Hq % c->Hkv) return fail(KVHIP_ERR_INVALID_ARG, "query heads must be a multiple of KV heads");
     if (L <= 0 || L > 65535 || L > T) return fail(KVHIP_ERR_INVALID_ARG, "query length out of range");
-    if (count <= 0) return fail(KVHIP_ERR_INVALID_ARG, "at least one block to a token");
+    if (count <= 0 || count > (1 << 24)) return fail(KVHIP_ERR_INVALID_ARG, "a token's blocks number from one to 2^24");
+    if ((int64_t)L * ((Hq / c->Hkv + 15) / 16) > 65535) return fail(KVHIP_ERR_UNSUPPORTED, "more query rows than one call takes");
     return KVHIP_OK;
 }
 kvhip_status block_choice(const kvhip_cache *c, const void *q, int32_t B, int32_t Hq, int32_t L, int64_t T, int32_t count, int32_t first,

@@ -730,6 +730,44 @@ def test_captured_steps_replay():
     assert torch.isfinite(chosen).all()
 
 
+@pytest.mark.parametrize("held_rows", [9000, 9023])
+def test_captured_steps_that_write(held_rows):
+    """A captured step writes its row and attends, replay after replay: the last inputs' row is what the cache holds.  The second
+    length ends its block with the row (63 rows of it held before), which is a launch of its own."""
+    cache, oracle, queries = held(BF16, held_rows, LAYOUTS[0], seed=9)
+    other = cache.copy()
+    gen = torch.Generator(device="cuda").manual_seed(3)
+
+    def fresh():
+        return [torch.randn(2, h, 1, 128, generator=gen, device="cuda").to(BF16) for h in (8, 2, 2)]
+
+    q, k, v = fresh()
+    for sparse in (False, True):
+        def step(c):
+            if sparse:
+                return c.update_attend_blocks(q, k, v, 0.1, 20)
+            return c.update_attend(q, k, v, 0.1)
+
+        step(cache)  # (scratch is there from here on)
+        cache.trim(1)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step(cache)
+        for _ in range(3):
+            for dst, src in zip((q, k, v), fresh()):
+                dst.copy_(src)
+            graph.replay()
+            torch.cuda.synchronize()
+            want = step(other)
+            for a, b in zip(got if sparse else [got], want if sparse else [want]):
+                assert torch.equal(a, b)
+            for a, b in zip(cache.fetch(), other.fetch()):
+                assert torch.equal(a, b)
+            other.trim(1)
+        cache.trim(1)
+
+
 # ---- refusals -------------------------------------------------------------------------------------------------------
 def test_refusals():
     cache, oracle, queries = held(BF16, 200, LAYOUTS[0])
@@ -743,6 +781,7 @@ def test_refusals():
 
     k = torch.zeros(2, 2, 1, 128, dtype=BF16, device="cuda")
     refused(-2, cache.select_blocks, q, 0)
+    assert kvhip.load().kvhip_cache_attend_blocks(cache._h, q.data_ptr(), 2, 8, 2, 128, 0.1, blocks.data_ptr(), (1 << 24) + 1, None, q.data_ptr(), None) == -2
     refused(-2, cache.select_blocks, q, 3, first=3, recent=1)
     refused(-2, cache.select_blocks, q, 3, first=-1)
     refused(-2, cache.select_blocks, q, 3, recent=0)
