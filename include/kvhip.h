@@ -315,7 +315,7 @@ kvhip_status kvhip_cache_update_attend(kvhip_cache *cache, const void *queries, 
  *     a = max |x| over the block's finite elements;  e = the least integer with a 2^-e <= 448 (0 if a = 0; at least -100)
  *     code = e4m3(x 2^-e), to nearest even;  the value read back is code 2^e
  * and the rows behind the last such block are held as they came.  Values read back are exact in the cache's dtype, and
- * written again they come out the same; infinities are held as NaN; values of a float16 cache beyond 61440 are held as that.
+ * written again they come out the same; infinities are held as NaN; values beyond 61440 (bfloat16: beyond 1.875 2^127) are held as that.
  * float16 and bfloat16, head sizes up to 256 (stored zero-padded to 64, 96, 128 or 256; 192 with 128); else
  * KVHIP_ERR_UNSUPPORTED.  kvhip_cache_trim and _set_offset take rows off what the cache presents at once; offsets are never
  * set forward.  Query rows that see no key are zeros.  kvhip_last_attend_kernel: 7, over chosen blocks 8.

@@ -3,7 +3,7 @@
 // A query row's bound on a block is sum_d max(q_d hi_d, q_d lo_d), with hi and lo the block's largest and smallest key element
 // of each channel: no key of the block scores higher.  Both sides are whole numbers times powers of two -- hi and lo are int8
 // in units of 4 scales, q is rint(q 2^-f), f the least integer with max |q| 2^-f <= 127 -- so that the sum is exact whatever
-// its order (below 2^24 for 256 channels) and the choice the same on any machine.  As products:
+// its order (below 2^22 for 256 channels) and the choice the same on any machine.  As products:
 // q+ hi + q- lo, with q+ = max(q, 0) and q- = min(q, 0), on the 16x16x64 int8 instruction.
 #include <algorithm>
 #include <type_traits>
@@ -18,11 +18,16 @@ namespace {
 typedef int kv_i4 __attribute__((ext_vector_type(4)));
 typedef unsigned short kv_us2 __attribute__((ext_vector_type(2)));
 
-// floats in an order that unsigned integers have too; 0 is below all of them
-__device__ __forceinline__ uint32_t ordered(float x) {
-    const uint32_t u = __float_as_uint(x);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+// whole 2^exp in an order that unsigned integers have too; 0 is below all of them.  The exponents of a bfloat16 cache's blocks and
+// queries add up to -237 .. 244, more than a float has: ten bits for the exponent, and 21 of the fraction are all that a whole
+// number below 2^22 (256 channels of 127 times 112) has.
+__device__ __forceinline__ uint32_t ordered(int whole, int exp) {
+    const uint32_t u = __float_as_uint((float)abs(whole)) >> 2;
+    const uint32_t mag = whole ? u + ((uint32_t)(exp + 128) << 21) : 0;
+    return whole < 0 ? 0x7fffffffu - mag : 0x80000000u | mag;
 }
+// the exponent of a power of two, in units of 4 of it
+__device__ __forceinline__ int unit_exponent(float scale) { return (int)(__float_as_uint(scale) >> 23) - 127 + 2; }
 constexpr int SELECT_WAVES = 16;
 constexpr int SELECT_TILES = 4;  // at most so many tiles of 16 query rows to a workgroup
 constexpr int SELECT_HEAD = SELECT_WAVES * 256 * 4;  // bytes of the histograms
@@ -111,10 +116,10 @@ __device__ __forceinline__ void query_operands(const char *row, int tok, int ud,
     }
 }
 
-// The summaries of AHEAD groups of 16 blocks, STEP groups apart, as operands, and the blocks' key scales.
+// The summaries of AHEAD groups of 16 blocks, STEP groups apart, as operands, and the exponents of the blocks' units.
 template <int D, int AHEAD, int STEP> struct Summaries {
     static constexpr int KS = (D + 63) / 64;
-    float scale[AHEAD];
+    int unit[AHEAD];
     kv_i4 hi[AHEAD][KS], lo[AHEAD][KS];
     __device__ __forceinline__ void load(const BlockStore &b, int bh, int blk0, int last, int lane) {
         const Store &st = b.st;
@@ -125,7 +130,7 @@ template <int D, int AHEAD, int STEP> struct Summaries {
             const int blk = min(blk0 + u * STEP * 16 + n, last);
             const PageEntry e = block_page(b, blk / BLOCK_PER_PAGE);
             sum[u] = as_global(e.vsb) + (size_t)bh * st.vsb_cell + (size_t)(blk % BLOCK_PER_PAGE) * 2 * D;
-            scale[u] = ld_global<float>(as_global(e.ksb) + (size_t)bh * st.ksb_cell + 8 * (blk % BLOCK_PER_PAGE));
+            unit[u] = unit_exponent(ld_global<float>(as_global(e.ksb) + (size_t)bh * st.ksb_cell + 8 * (blk % BLOCK_PER_PAGE)));
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
@@ -165,7 +170,7 @@ template <int D, int AHEAD, int STEP> struct Summaries {
             if (at >= blocks) continue;
             uint32_t key[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) key[i] = ordered(ldexpf((float)acc[u][i] * (4.f * scale[u]), fr[i]));
+            for (int i = 0; i < 4; ++i) key[i] = ordered(acc[u][i], unit[u] + fr[i]);
             if (tr[0] >= 0 && tr[0] == tr[3]) {  // one token's rows: one entry for all four
                 atomicMax(&keys[tr[0] * stride + at], max(max(key[0], key[1]), max(key[2], key[3])));
             } else {

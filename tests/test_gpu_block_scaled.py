@@ -556,6 +556,26 @@ def test_blocks_are_chosen_by_the_definition(dtype, layout, T, n, count, first, 
     assert np.array_equal(got.cpu().numpy(), O.select(q, oracle, count, first, recent, pads))
 
 
+@pytest.mark.parametrize("T,n", [(1300, 1), (1300, 9), (12000, 1)])
+@pytest.mark.parametrize("keys_at,queries_at", [(126, 126), (-100, -100), (126, -120), (-60, 100), (40, 100)])
+def test_bounds_beyond_float32(T, n, keys_at, queries_at):
+    """Blocks of sizes from 2^(keys_at - 24) on against queries about 2^queries_at: bounds beyond what a float holds, either side."""
+    rng = np.random.default_rng(T + n)
+    size = 2.0 ** np.repeat(keys_at - rng.integers(0, 25, (2, 2, (T + 63) // 64, 1)), 64, 2)[:, :, :T]
+
+    def drawn(x):
+        t = torch.from_numpy(x).to(BF16)
+        return t.double().numpy(), t.cuda()
+
+    k, kd = drawn(rng.uniform(-1, 1, (2, 2, T, 128)) * size)
+    q, qd = drawn(rng.uniform(-1, 1, (2, 8, n, 128)) * 2.0 ** queries_at)
+    cache, oracle = kvhip.BlockScaledKVCache(), O.BlockScaledCache("bfloat16")
+    cache.update(kd, kd, fetch=False)
+    oracle.update(k, k)
+    got = cache.select_blocks(qd, 9, 0, 1)
+    assert np.array_equal(got.cpu().numpy(), O.select(q, oracle, 9, 0, 1, (0, 0)))
+
+
 @pytest.mark.parametrize("layout", [(8, 2, 128, 128), (40, 1, 64, 64), (3, 1, 96, 96), (2, 1, 256, 256), (70, 1, 50, 36)])
 @pytest.mark.parametrize("n,count,first,recent,pads", [(1, 40, 1, 2, (0, 0)), (1, 3, 1, 2, (5000, 0)), (3, 17, 0, 1, (100, 17100)), (19, 300, 3, 4, (0, 64))])
 def test_blocks_of_long_caches(layout, n, count, first, recent, pads):
