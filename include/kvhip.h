@@ -327,7 +327,8 @@ kvhip_status kvhip_cache_update_attend(kvhip_cache *cache, const void *queries, 
  * over one kv head.  The token sees blocks left_pad[b] / 64 to p / 64 (none if p < left_pad[b]).  The first `first` of these
  * and the last `recent` are chosen, and as many more as make `count`, by their bounds, the lower block among equals.
  * blocks: device [B, Hkv, L, count] int32, ascending, -1 behind the last; left_pad: device [B] or NULL.
- * first >= 0, recent >= 1, first + recent <= count; up to 27 000 blocks (1.7 million rows) a cache.
+ * first >= 0, recent >= 1, first + recent <= count <= 2^20; up to 27 000 blocks (1.7 million rows) a cache.  At most 65 535
+ * tiles of 16 query rows a kv head (L times Hq / Hkv / 16, rounded up) to a call.
  */
 kvhip_status kvhip_cache_select_blocks(kvhip_cache *cache, const void *queries, int32_t B, int32_t Hq, int32_t L, int32_t D,
                                        int32_t count, int32_t first, int32_t recent, const int32_t *left_pad, int32_t *blocks,

@@ -1615,7 +1615,7 @@ kvhip_status check_block_call(const kvhip_cache *c, int32_t B, int32_t Hq, int32
     if (B != c->B || D != c->Dk_user) return fail(KVHIP_ERR_INVALID_ARG, "query shape does not match the cache");
     if (Hq <= 0 || Hq % c->Hkv) return fail(KVHIP_ERR_INVALID_ARG, "query heads must be a multiple of KV heads");
     if (L <= 0 || L > 65535 || L > T) return fail(KVHIP_ERR_INVALID_ARG, "query length out of range");
-    if (count <= 0 || count > (1 << 24)) return fail(KVHIP_ERR_INVALID_ARG, "a token's blocks number from one to 2^24");
+    if (count <= 0 || count > (1 << 20)) return fail(KVHIP_ERR_INVALID_ARG, "a token's blocks number from one to 2^20");
     if ((int64_t)L * ((Hq / c->Hkv + 15) / 16) > 65535) return fail(KVHIP_ERR_UNSUPPORTED, "more query rows than one call takes");
     return KVHIP_OK;
 }
@@ -1694,11 +1694,16 @@ kvhip_status kvhip_cache_update_attend_blocks(kvhip_cache *c, const void *q, con
     if (c->kind != KVHIP_KIND_BLOCK_SCALED) return fail(KVHIP_ERR_INVALID_ARG, "blocks are chosen in a block-scaled cache");
     if (L <= 0) return fail(KVHIP_ERR_INVALID_ARG, "update needs at least one new row");
     // (all that can be refused is, before anything is written)
+    const bool fresh = !c->has_geom;
     KV_TRY(set_geometry(c, B, Hkv, Dk, Dv, dtype));
     const int64_t T = c->offset + L;
-    KV_TRY(check_block_call(c, B, Hq, L, Dk, T, count));
     BlockSelect x;
-    KV_TRY(block_choice(c, q, B, Hq, L, T, count, first, recent, left_pad, blocks, x));
+    kvhip_status ok = check_block_call(c, B, Hq, L, Dk, T, count);
+    if (ok == KVHIP_OK) ok = block_choice(c, q, B, Hq, L, T, count, first, recent, left_pad, blocks, x);
+    if (ok != KVHIP_OK) {  // (a refused first call leaves the cache open to other shapes)
+        if (fresh) c->has_geom = false;
+        return ok;
+    }
     hipStream_t s = S(c, stream);
     const bool fuse = block_step_fuses(c, L);
     KV_TRY(update_blocks(c, k, v, L, s, !fuse));

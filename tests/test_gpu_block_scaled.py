@@ -789,6 +789,18 @@ def test_captured_steps_that_write(held_rows):
 
 
 # ---- refusals -------------------------------------------------------------------------------------------------------
+def test_a_refused_first_call_leaves_the_cache_open():
+    cache = kvhip.BlockScaledKVCache()
+    q, k = (torch.randn(1, h, 1, 128, device="cuda").to(BF16) for h in (4, 2))
+    for bad in ({"count": 0}, {"count": 2, "first": 2}, {"count": 2, "first": -1}):
+        with pytest.raises(kvhip.KVHipError):
+            cache.update_attend_blocks(q, k, k, 0.1, **bad)
+    assert cache.offset == 0
+    q, k = (torch.randn(3, h, 2, 64, device="cuda").to(F16) for h in (6, 3))
+    cache.update_attend_blocks(q, k, k, 0.1, 2)
+    assert cache.offset == 2 and torch.equal(cache.fetch()[0], k)
+
+
 def test_refusals():
     cache, oracle, queries = held(BF16, 200, LAYOUTS[0])
     _, q = queries(2)
@@ -801,7 +813,7 @@ def test_refusals():
 
     k = torch.zeros(2, 2, 1, 128, dtype=BF16, device="cuda")
     refused(-2, cache.select_blocks, q, 0)
-    assert kvhip.load().kvhip_cache_attend_blocks(cache._h, q.data_ptr(), 2, 8, 2, 128, 0.1, blocks.data_ptr(), (1 << 24) + 1, None, q.data_ptr(), None) == -2
+    assert kvhip.load().kvhip_cache_attend_blocks(cache._h, q.data_ptr(), 2, 8, 2, 128, 0.1, blocks.data_ptr(), (1 << 20) + 1, None, q.data_ptr(), None) == -2
     refused(-2, cache.select_blocks, q, 3, first=3, recent=1)
     refused(-2, cache.select_blocks, q, 3, first=-1)
     refused(-2, cache.select_blocks, q, 3, recent=0)
