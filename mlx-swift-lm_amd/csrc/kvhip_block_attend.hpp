@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kerne
                 for (int i = threadIdx.x; i < x.count; i += NW * 64) x.list_out[((size_t)bh * a.L + token) * x.count + i] = chosen[i];
         }
     }
-    int tail_at = -1;
+    int tail_at = -1, tails = 0;  // (a list may hold it more than once)
 
     for (int at = 0; at < mine; at += 64) {
         // a lane to a block: where it lies and its scales
@@ -645,6 +645,7 @@ __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kerne
         }
         const uint64_t open = __ballot(blk >= 0 && blk >= x.b.coded);
         if (open) tail_at = __builtin_amdgcn_readlane(blk, __builtin_ctzll(open)) * BLOCK_ROWS;
+        if (MODE == 3) tails += __builtin_popcountll(open);
         uint64_t todo = __ballot(blk >= 0 && blk < x.b.coded);
         auto at_lane = [](uint64_t v, int of) {  // (readlane returns a signed number)
             const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, of), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), of);
@@ -670,7 +671,11 @@ __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kerne
             cur = then;
         }
     }
-    if (tail_at >= 0) w.tail(tail_at);
+    if constexpr (MODE == 3) {
+        for (; tails > 0; --tails) w.tail(tail_at);
+    } else {
+        if (tail_at >= 0) w.tail(tail_at);
+    }
 
     // a single token's row, still in the caller's arrays, into the tail (its reader above takes it from there as well)
     if (a.new_k && blockIdx.y == 0 && part == 0 && wave == NW - 1) {

@@ -701,6 +701,17 @@ def test_steps_that_choose_their_blocks(layout, T, n, count, first, recent, pads
                 assert (got[b, :G, t] == 0).all()
 
 
+@pytest.mark.parametrize("n", [1, 4])
+def test_blocks_listed_again_count_again(n):
+    """Behind a lower entry a block counts anew, the unfinished one too, whichever wavefront meets it."""
+    cache, oracle, queries = held(BF16, 700, LAYOUTS[0])
+    q, qd = queries(n)
+    for entries in ([10, 3, 10], [10, -1, 10, -1, 10, -1, 10, -1, 10, 3, 4, 10], [4, 10] * 150 + [-1, 2], [10, 0, 10, 0, 0, 10, 10, 5, 5]):
+        blocks = torch.tensor(entries, dtype=torch.int32, device="cuda").expand(2, 2, n, -1).contiguous()
+        got = cache.attend_blocks(qd, blocks, 0.1)
+        check(got, *exact_and_bound(q, oracle, 0.1, O.listed_keep(blocks.cpu().numpy(), 700, (0, 0))))
+
+
 def test_lists_of_any_content():
     """Entries outside what the token sees, repeated and descending ones are passed over; nothing listed: zeros."""
     cache, oracle, queries = held(BF16, 700, LAYOUTS[0])
