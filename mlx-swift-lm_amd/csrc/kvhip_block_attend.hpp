@@ -572,6 +572,19 @@ __device__ __forceinline__ void leave_tile(Walk &w, const RowsView &v, const Blo
     }
 }
 
+// A single token's row, still in the caller's arrays, into the tail, by one wavefront of each pair (the readers of the tail take it from
+// there as well).  Each kernel that a single token may come to calls it.
+template <int DK, int DV, int DT> __device__ __forceinline__ void write_step(const BlockAttend &x, int bh, int lane) {
+    const AttendArgs &a = x.a;
+    if (!a.new_k || blockIdx.y != 0 || blockIdx.z != 0) return;
+    const int r = (a.T - 1) % BLOCK_ROWS;
+    const uint16_t *nk = static_cast<const uint16_t *>(a.new_k) + (size_t)bh * DK, *nv = static_cast<const uint16_t *>(a.new_v) + (size_t)bh * DV;
+    uint16_t *tk = reinterpret_cast<uint16_t *>(x.b.tail_k) + ((size_t)bh * BLOCK_ROWS + r) * DK;
+    uint16_t *tv = reinterpret_cast<uint16_t *>(x.b.tail_v) + (size_t)bh * BLOCK_ROWS * DV;
+    for (int d = lane; d < DK; d += 64) tk[d] = (uint16_t)no_infinities<DT>(nk[d]);
+    for (int d = lane; d < DV; d += 64) tv[tail_v_at(DV, r, d)] = (uint16_t)no_infinities<DT>(nv[d]);
+}
+
 // grid (BH, tiles of query rows, parts), NW wavefronts.  MODE 3: (BH, tokens x tiles of heads, parts).
 template <int DK, int DV, int DT, int NM, int MODE, int NW>
 __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kernel(BlockAttend x) {
@@ -677,15 +690,7 @@ __global__ void __launch_bounds__(NW * 64, DK <= 128 ? 2 : 1) block_attend_kerne
         if (tail_at >= 0) w.tail(tail_at);
     }
 
-    // a single token's row, still in the caller's arrays, into the tail (its reader above takes it from there as well)
-    if (a.new_k && blockIdx.y == 0 && part == 0 && wave == NW - 1) {
-        const int r = (a.T - 1) % BLOCK_ROWS;
-        const uint16_t *nk = static_cast<const uint16_t *>(a.new_k) + (size_t)bh * DK, *nv = static_cast<const uint16_t *>(a.new_v) + (size_t)bh * DV;
-        uint16_t *tk = reinterpret_cast<uint16_t *>(x.b.tail_k) + ((size_t)bh * BLOCK_ROWS + r) * DK;
-        uint16_t *tv = reinterpret_cast<uint16_t *>(x.b.tail_v) + (size_t)bh * BLOCK_ROWS * DV;
-        for (int d = lane; d < DK; d += 64) tk[d] = (uint16_t)no_infinities<DT>(nk[d]);
-        for (int d = lane; d < DV; d += 64) tv[tail_v_at(DV, r, d)] = (uint16_t)no_infinities<DT>(nv[d]);
-    }
+    if (wave == NW - 1) write_step<DK, DV, DT>(x, bh, lane);
 
     // the wavefronts' parts joined, 16 rows at a time
 #pragma unroll
@@ -814,6 +819,7 @@ __global__ void __launch_bounds__(512, 2) block_attend_tiled_kernel(BlockAttend 
         }
     }
     if (tail_at >= 0) w.tail(tail_at);
+    if (wave == 7) write_step<DK, DV, DT>(x, bh, lane);  // (a token of more than 32 heads to a kv head)
     __syncthreads();  // (the ring's memory takes the parts)
     Parts &parts = reinterpret_cast<Parts *>(lds)[rw];
 #pragma unroll
