@@ -318,7 +318,10 @@ kvhip_status kvhip_cache_update_attend(kvhip_cache *cache, const void *queries, 
  * written again they come out the same; infinities are held as NaN; values beyond 61440 (bfloat16: beyond 1.875 2^127) are held as that.
  * float16 and bfloat16, head sizes up to 256 (stored zero-padded to 64, 96, 128 or 256; 192 with 128); else
  * KVHIP_ERR_UNSUPPORTED.  kvhip_cache_trim and _set_offset take rows off what the cache presents at once; offsets are never
- * set forward.  Query rows that see no key are zeros.  kvhip_last_attend_kernel: 7, over chosen blocks 8.
+ * set forward.  Rows taken off leave no trace in the block that this opens again -- its rows are as they came -- where that is
+ * the block that was unfinished, the one in front of it, or the one that was unfinished before the last update: a draft or a
+ * whole call can be taken back.  In any other block the rows that are left stay what its codes say, and are coded from those when
+ * it is finished again.  Query rows that see no key are zeros.  kvhip_last_attend_kernel: 7, over chosen blocks 8.
  *
  * Attention over chosen blocks.  Query row l of L sits at position p = presented length - L + l.  A query row's bound on a
  * block is sum_d max(q_d hi_d, q_d lo_d), hi and lo the block's largest and smallest key element of each channel, with

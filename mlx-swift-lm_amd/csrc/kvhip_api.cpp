@@ -119,11 +119,16 @@ struct kvhip_cache {
     void *stage_tmp_k = nullptr, *stage_tmp_v = nullptr;  // dense copy of the rows a commit keeps
     size_t stage_tmp_rows = 0;
     RopeDev *rope = nullptr;  // set for the duration of one update_rope call
-    // block-scaled only: blocks held as codes, and two tails (kvhip_block.hpp), one of them in use
+    // block-scaled only: blocks held as codes, and the blocks whose first `rows` rows are there as they came too, each in a place
+    // of its own (kvhip_block.hpp).  The unfinished block, number `coded`, is one of them.
+    struct KeptRows {
+        int64_t block = -1;
+        int rows = 0;
+    };
     int64_t coded = 0;
     char *tail = nullptr;
     size_t tail_bytes = 0;
-    int tail_now = 0;
+    KeptRows kept[BLOCK_KEPT];
     // scratch for attention
     float *ws = nullptr;
     size_t ws_bytes = 0;
@@ -726,7 +731,7 @@ kvhip_status update_simple(kvhip_cache *c, const void *k, const void *v, int L, 
 kvhip_status ensure_tail(kvhip_cache *c) {
     if (c->tail) return KVHIP_OK;
     void *p = nullptr;
-    const size_t need = 2 * (size_t)c->st.BH * BLOCK_ROWS * (c->st.Dk + c->st.Dv) * c->st.es;  // (no row is read that was not written)
+    const size_t need = BLOCK_KEPT * (size_t)c->st.BH * BLOCK_ROWS * (c->st.Dk + c->st.Dv) * c->st.es;  // (no row is read that was not written)
     KV_HIP(pool_alloc(&p, need, &c->tail_bytes));
     c->tail = static_cast<char *>(p);
     return KVHIP_OK;
@@ -736,10 +741,16 @@ void tail_at(const kvhip_cache *c, int which, char *&k, char *&v) {
     k = c->tail + (size_t)which * c->st.BH * pair * (c->st.Dk + c->st.Dv);
     v = k + (size_t)c->st.BH * pair * c->st.Dk;
 }
+// the place of a block's rows as they came, or -1
+int kept_at(const kvhip_cache::KeptRows *kept, int64_t block) {
+    for (int i = 0; i < BLOCK_KEPT; ++i)
+        if (kept[i].block == block) return i;
+    return -1;
+}
 BlockStore block_store(const kvhip_cache *c) {
     BlockStore s;
     s.st = c->st;
-    tail_at(c, c->tail_now, s.tail_k, s.tail_v);
+    tail_at(c, std::max(kept_at(c->kept, c->coded), 0), s.tail_k, s.tail_v);  // (none: no row is behind the coded blocks)
     s.coded = (int32_t)c->coded;
     s.Dk_user = c->Dk_user;
     s.Dv_user = c->Dv_user;
@@ -760,9 +771,32 @@ BlockStore block_store(const kvhip_cache *c) {
 }
 // `launch` false: the attention kernel writes the row of a single token that finishes no block (block_step_fuses).
 kvhip_status update_blocks(kvhip_cache *c, const void *k, const void *v, int L, hipStream_t stream, bool launch = true) {
-    const int64_t prev = c->offset, next = prev + L;
+    const int64_t prev = c->offset, next = prev + L, from = prev / BLOCK_ROWS, open = next / BLOCK_ROWS;
     KV_TRY(ensure_slots(c, next, stream));
     KV_TRY(ensure_tail(c));
+    // Kept from here on: the unfinished block, the one in front of it, and the one that was unfinished so far.  (Those behind the
+    // rows that are left are gone, and so is the block that is written again from its codes.)
+    kvhip_cache::KeptRows kept[BLOCK_KEPT];
+    for (int i = 0; i < BLOCK_KEPT; ++i) {
+        const kvhip_cache::KeptRows &x = c->kept[i];
+        const bool unfinished = x.block == from && c->coded == from && prev % BLOCK_ROWS != 0;
+        if (unfinished || (x.block < from && x.block == open - 1)) kept[i] = x;
+    }
+    auto place = [&](int64_t block) {  // (there is an empty one: each of three blocks has at most one)
+        const int at = kept_at(kept, block);
+        return at >= 0 ? at : kept_at(kept, -1);
+    };
+    BlockKept to;
+    if (open > from) {
+        const int at = place(open - 1);
+        kept[at] = {open - 1, BLOCK_ROWS};
+        tail_at(c, at, to.done_k, to.done_v);
+    }
+    if (next % BLOCK_ROWS != 0) {
+        const int at = place(open);
+        kept[at] = {open, (int)(next % BLOCK_ROWS)};
+        tail_at(c, at, to.open_k, to.open_v);
+    }
     if (launch) {
         if (c->rope) {  // the keys turn in a launch of their own
             RopeDev turn = *c->rope;
@@ -771,17 +805,22 @@ kvhip_status update_blocks(kvhip_cache *c, const void *k, const void *v, int L, 
             KV_HIP(launch_rope_apply(turn, k, c->pad_buf[5], c->B, c->Hkv, L, c->Dk_user, c->st.dtype, stream));
             k = c->pad_buf[5];
         }
-        const int to = prev / BLOCK_ROWS == (next - 1) / BLOCK_ROWS ? c->tail_now : 1 - c->tail_now;
-        char *to_k, *to_v;
-        tail_at(c, to, to_k, to_v);
-        KV_HIP(launch_block_append(block_store(c), k, v, prev, L, to_k, to_v, stream));
-        c->tail_now = to;
+        KV_HIP(launch_block_append(block_store(c), k, v, prev, L, to, stream));
     }
-    c->coded = next / BLOCK_ROWS;
+    std::copy(kept, kept + BLOCK_KEPT, c->kept);
+    c->coded = open;
     c->ref_len = next;
     c->has_buffers = true;
     c->offset = c->presented = next;
     return KVHIP_OK;
+}
+// What the cache presents ends at row `rows` <= offset from now on.  A block that this opens again is the unfinished one, its
+// rows as they came, if they are there; else its rows stay what its codes say.
+void cut_blocks(kvhip_cache *c, int64_t rows) {
+    const int64_t block = rows / BLOCK_ROWS;
+    const int left = (int)(rows % BLOCK_ROWS), at = kept_at(c->kept, block);
+    if (left == 0 || (at >= 0 && c->kept[at].rows >= left)) c->coded = std::min(c->coded, block);
+    c->offset = c->presented = rows;
 }
 // Whether a new token's row can be left to the attention kernel: it finishes no block, and its block's rows are in the tail.
 bool block_step_fuses(const kvhip_cache *c, int L) {
@@ -1052,10 +1091,9 @@ int32_t kvhip_cache_is_trimmable(const kvhip_cache *c, int64_t after) {
 
 int64_t kvhip_cache_trim(kvhip_cache *c, int64_t n) {
     if (!c) return 0;
-    if (c->kind == KVHIP_KIND_BLOCK_SCALED) {  // (what is left is what the cache presents; the next write sees to its last block)
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) {  // (what is left is what the cache presents)
         const int64_t t = std::min(c->offset, std::max<int64_t>(n, 0));
-        c->offset -= t;
-        c->presented = c->offset;
+        cut_blocks(c, c->offset - t);
         return t;
     }
     const int64_t t = std::min(c->offset, n);  // KVCache.swift:474-478, :826-831, :1171-1175
@@ -1068,7 +1106,8 @@ kvhip_status kvhip_cache_set_offset(kvhip_cache *c, int64_t offset) {
     if (!c) return fail(KVHIP_ERR_INVALID_ARG, "null cache");
     if (c->kind == KVHIP_KIND_BLOCK_SCALED) {
         if (offset < 0 || offset > c->offset) return fail(KVHIP_ERR_STATE, "the offset of a block-scaled cache can only be set back");
-        c->presented = offset;
+        cut_blocks(c, offset);
+        return KVHIP_OK;
     }
     c->offset = offset;
     return KVHIP_OK;
@@ -1518,10 +1557,7 @@ kvhip_status kvhip_cache_update_attend(kvhip_cache *c, const void *q, const void
         c->B == B && c->Hkv == Hkv && c->st.Dk == Dk && c->st.Dv == Dv && c->st.dtype == dtype) {
         KV_TRY(update_blocks(c, k, v, 1, S(c, stream), false));
         const kvhip_status st = attend_impl(c, q, B, Hq, L, Dk, scale, mask, out, stream, nullptr, 0, k, v, (int32_t)c->offset - 1);
-        if (st != KVHIP_OK) {  // nothing was written: take the row back
-            c->offset -= 1;
-            c->presented = c->offset;
-        }
+        if (st != KVHIP_OK) cut_blocks(c, c->offset - 1);  // nothing was written: take the row back
         return st;
     }
     // One new token into a full-precision cache (KVCacheSimple, or the in-place step of a
@@ -1709,10 +1745,7 @@ kvhip_status kvhip_cache_update_attend_blocks(kvhip_cache *c, const void *q, con
     KV_TRY(update_blocks(c, k, v, L, s, !fuse));
     x.b = block_store(c);
     const kvhip_status st = attend_blocks_impl(c, q, B, Hq, L, Dk, scale, blocks, count, left_pad, out, fuse ? k : nullptr, fuse ? v : nullptr, s, &x);
-    if (st != KVHIP_OK && fuse) {  // nothing was written: take the row back
-        c->offset -= 1;
-        c->presented = c->offset;
-    }
+    if (st != KVHIP_OK && fuse) cut_blocks(c, c->offset - 1);  // nothing was written: take the row back
     return st;
 }
 
@@ -1912,6 +1945,7 @@ kvhip_status kvhip_cache_state_import(kvhip_cache *c, int32_t count, const void 
         retire({{c->tail, c->tail_bytes}}, S(c, stream));
         c->tail = nullptr;
         c->coded = 0;
+        std::fill(c->kept, c->kept + BLOCK_KEPT, kvhip_cache::KeptRows());
         c->offset = c->presented = 0;
         c->has_buffers = false;
     }
@@ -2068,8 +2102,9 @@ kvhip_status kvhip_cache_copy(const kvhip_cache *c, void *stream, kvhip_cache **
             if (c->kind == KVHIP_KIND_BLOCK_SCALED) {
                 st = ensure_tail(n);
                 if (st != KVHIP_OK) { kvhip_cache_free(n); return st; }
-                BlockStore from = block_store(c), to = block_store(n);
-                KV_HIP_OR(launch_copy_bytes(to.tail_k, from.tail_k, (size_t)c->st.BH * BLOCK_ROWS * (c->st.Dk + c->st.Dv) * c->st.es, s), kvhip_cache_free(n));
+                const size_t bytes = BLOCK_KEPT * (size_t)c->st.BH * BLOCK_ROWS * (c->st.Dk + c->st.Dv) * c->st.es;
+                KV_HIP_OR(launch_copy_bytes(n->tail, c->tail, bytes, s), kvhip_cache_free(n));
+                std::copy(c->kept, c->kept + BLOCK_KEPT, n->kept);
                 n->coded = std::min(c->coded, (rows + BLOCK_ROWS - 1) / BLOCK_ROWS);
             }
         } else {

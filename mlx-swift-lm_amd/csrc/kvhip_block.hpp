@@ -11,7 +11,10 @@
 //
 // Blocks are cut by position.  One that has all its rows is held as codes in the pages; the rows behind the last of them, the
 // tail, are held as they came (infinities as NaN) until the block is whole, so that what a row is read back as does not
-// depend on how many rows came with it.
+// depend on how many rows came with it.  Nor on rows that were there for a while: the rows of the block in front of the tail, and
+// of the one that was unfinished before the last call, are kept as they came as well, each block's in a place of its own, and
+// a block that loses rows again is the unfinished one as it was.  (Its codes would not do: they have the scale of all the rows
+// that finished it.)
 //
 // A page (256 tokens, four blocks) holds for every (batch row, kv head) pair, plane by plane of its PageEntry:
 //   k    four blocks of 64 Dk codes in the order in which a wavefront of the attention kernel loads its operands:
@@ -31,6 +34,9 @@ constexpr int BLOCK_ROWS = 64;
 constexpr int BLOCK_PER_PAGE = PAGE / BLOCK_ROWS;
 constexpr int BLOCK_LEAST_EXP = -100;
 constexpr int BLOCK_MAX_HEAD = 256;
+// Blocks whose rows are kept as they came: the unfinished one, the one in front of it, the one that was unfinished before the last
+// call.  Three places, also because a call's workgroups run at once: one reads the last of these while two others write the first two.
+constexpr int BLOCK_KEPT = 3;
 
 // Where pages lie, in a kernel's arguments: pages [first[i], first[i + 1]) are regular from the addresses of slab i on (one
 // allocation each; a cache that grew has a few).  A page's entry in the page table is a load in front of everything else a short
@@ -51,10 +57,13 @@ struct BlockStore {
     BlockSlabs slabs;
 };
 
-// Rows [pos0, pos0 + n) of the dense arrays [BH, n, D], written behind the pos0 rows that the cache holds.  Those that leave
-// their block unfinished go to `to_k` / `to_v`: the tail itself where they start in the block that they end in, else another
-// one (the workgroup that finishes a block reads the tail while the last block's writes its own).
-hipError_t launch_block_append(const BlockStore &s, const void *keys, const void *values, int64_t pos0, int n, char *to_k, char *to_v,
+// Where a call leaves rows as they came: those of the last block that it finishes, and those behind it.  Either is the tail itself
+// (which holds the block's rows so far) where the rows start in that block, else another place.
+struct BlockKept {
+    char *done_k = nullptr, *done_v = nullptr, *open_k = nullptr, *open_v = nullptr;
+};
+// Rows [pos0, pos0 + n) of the dense arrays [BH, n, D], written behind the pos0 rows that the cache holds.
+hipError_t launch_block_append(const BlockStore &s, const void *keys, const void *values, int64_t pos0, int n, const BlockKept &to,
                                hipStream_t stream);
 // Rows [0, rows) into dense arrays [BH, rows, D]; either may be NULL.
 hipError_t launch_block_fetch(const BlockStore &s, int64_t rows, void *dst_k, void *dst_v, hipStream_t stream);

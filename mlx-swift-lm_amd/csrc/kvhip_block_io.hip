@@ -115,7 +115,6 @@ struct AppendArgs {
     const char *src;  // the plane's rows [BH, n, ud]
     int64_t pos0;
     int n, ud;
-    char *tail, *to;
     int blk, bh;
     bool reopened;    // the block is held as codes and has lost rows since
     __device__ __forceinline__ int64_t lo() const { return (int64_t)blk * BLOCK_ROWS; }
@@ -124,24 +123,46 @@ struct AppendArgs {
     __device__ __forceinline__ const char *rows() const { return src + (size_t)bh * n * ud * 2; }
 };
 
-// New rows of a block that stays unfinished, into the tail (behind those of a reopened one).
+// New rows of a block as they came, into its place (behind those of a reopened one).
 template <int DT, int D, bool V>
 __device__ __forceinline__ void append_tail(const AppendArgs &a, const char *codes, const char *tail, char *to, float scale) {
     const int start = a.reopened ? 0 : a.from(), upto = a.upto(), from = a.from();
     const Unit u;
-    for (int d0 = 8 * u.ch; d0 < D; d0 += 128)
+    const int r0 = 4 * u.rq;
+    const bool all = r0 >= start && r0 + 4 <= upto;
+    for (int d0 = 8 * u.ch; d0 < D; d0 += 128) {
+        kv_u4 w[4];
+#pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int r = 4 * u.rq + i;
+            const int r = r0 + i;
+            if (r >= start && r < upto)
+                w[i] = r < from ? held_chunk<DT, V>(codes, tail, true, scale, D, r, d0) : dense_chunk<DT>(a.rows(), (size_t)(a.lo() + r - a.pos0), a.ud, d0);
+        }
+        if constexpr (V) {
+            uint16_t *t = reinterpret_cast<uint16_t *>(to);
+            if (all) {  // four rows of a channel lie side by side
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t pick = k & 1 ? 0x07060302u : 0x05040100u;
+                    *reinterpret_cast<kv_w2 *>(t + tail_v_at(D, r0, d0 + k)) =
+                        kv_w2{__builtin_amdgcn_perm(w[1][k >> 1], w[0][k >> 1], pick), __builtin_amdgcn_perm(w[3][k >> 1], w[2][k >> 1], pick)};
+                }
+                continue;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = r0 + i;
             if (r < start || r >= upto) continue;
-            const kv_u4 w = r < from ? held_chunk<DT, V>(codes, tail, true, scale, D, r, d0) : dense_chunk<DT>(a.rows(), (size_t)(a.lo() + r - a.pos0), a.ud, d0);
             if constexpr (V) {
                 uint16_t *t = reinterpret_cast<uint16_t *>(to);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) t[tail_v_at(D, r, d0 + k)] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+                for (int k = 0; k < 8; ++k) t[tail_v_at(D, r, d0 + k)] = (uint16_t)(w[i][k >> 1] >> (16 * (k & 1)));
             } else {
-                *reinterpret_cast<kv_u4 *>(to + ((size_t)r * D + d0) * 2) = w;
+                *reinterpret_cast<kv_u4 *>(to + ((size_t)r * D + d0) * 2) = w[i];
             }
         }
+    }
 }
 
 // A block that is whole after this call: its rows (those held so far and the new ones) become codes.  A wavefront takes what
@@ -320,9 +341,12 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, char *codes, 
     }
 }
 
-// grid (blocks touched, BH, keys / values), 256 threads
+// grid (blocks touched, and one more if one of them becomes whole, BH, keys / values), 256 threads.  The last workgroup keeps the rows
+// of the last whole block as they came, from the caller's arrays; where some of them are there as codes only, the block's own
+// workgroup does, in front of the barrier behind which it writes the codes anew.  (All of it by the block's own workgroup: 512 rows of
+// 8 heads written and attended for 102 us, with one more 97.5; 4 x 8 heads x 8191 rows stored and read back 118 us and 83.5.)
 template <int DT, int DK, int DV>
-__global__ void __launch_bounds__(256) block_append_kernel(BlockStore s, const char *keys, const char *values, int64_t pos0, int n, char *to_k, char *to_v) {
+__global__ void __launch_bounds__(256) block_append_kernel(BlockStore s, const char *keys, const char *values, int64_t pos0, int n, BlockKept to) {
     __shared__ __align__(16) uint32_t raw[64 * (DK / 2 + 4)];
     __shared__ uint32_t ends[4 * DK], amax_s[4];
     const bool v = blockIdx.z != 0;
@@ -332,25 +356,28 @@ __global__ void __launch_bounds__(256) block_append_kernel(BlockStore s, const c
     a.pos0 = pos0;
     a.n = n;
     a.ud = v ? s.Dv_user : s.Dk_user;
+    const int done = (int)((pos0 + n) / BLOCK_ROWS) - 1;
     a.blk = (int)(pos0 / BLOCK_ROWS) + blockIdx.x;
+    const bool keeper = a.blk > (int)((pos0 + n - 1) / BLOCK_ROWS);
+    if (keeper) a.blk = done;
     a.bh = blockIdx.y;
     a.reopened = a.blk < s.coded && pos0 > a.lo();
     const PageEntry e = block_page(s, a.blk / BLOCK_PER_PAGE);
     const int in_page = a.blk % BLOCK_PER_PAGE, bh = a.bh;
     float *scales = reinterpret_cast<float *>(e.ksb + (size_t)bh * s.st.ksb_cell) + 2 * in_page + (v ? 1 : 0);
     const float held = a.reopened ? *scales : 1.f;
-    const bool whole = pos0 + n >= a.lo() + BLOCK_ROWS;
+    const bool whole = pos0 + n >= a.lo() + BLOCK_ROWS, keep = a.blk == done && keeper != a.reopened;
     if (v) {
         const size_t at = (size_t)bh * BLOCK_ROWS * DV * 2;
         char *codes = e.v + (size_t)bh * s.st.v_cell + (size_t)in_page * BLOCK_ROWS * DV;
-        if (whole) append_values<DT, DV>(a, codes, s.tail_v + at, scales, held, amax_s);
-        else append_tail<DT, DV, true>(a, codes, s.tail_v + at, to_v + at, held);
+        if (!whole || keep) append_tail<DT, DV, true>(a, codes, s.tail_v + at, (whole ? to.done_v : to.open_v) + at, held);
+        if (whole && !keeper) append_values<DT, DV>(a, codes, s.tail_v + at, scales, held, amax_s);
     } else {
         const size_t at = (size_t)bh * BLOCK_ROWS * DK * 2;
         char *codes = e.k + (size_t)bh * s.st.k_cell + (size_t)in_page * BLOCK_ROWS * DK;
         char *summary = e.vsb + (size_t)bh * s.st.vsb_cell + (size_t)in_page * 2 * DK;
-        if (whole) append_keys<DT, DK>(a, codes, s.tail_k + at, scales, summary, held, raw, ends, amax_s);
-        else append_tail<DT, DK, false>(a, codes, s.tail_k + at, to_k + at, held);
+        if (!whole || keep) append_tail<DT, DK, false>(a, codes, s.tail_k + at, (whole ? to.done_k : to.open_k) + at, held);
+        if (whole && !keeper) append_keys<DT, DK>(a, codes, s.tail_k + at, scales, summary, held, raw, ends, amax_s);
     }
 }
 
@@ -417,16 +444,16 @@ template <int DT> __global__ void __launch_bounds__(256) block_fetch_kernel(Bloc
 
 }  // namespace
 
-hipError_t launch_block_append(const BlockStore &s, const void *keys, const void *values, int64_t pos0, int n, char *to_k, char *to_v,
+hipError_t launch_block_append(const BlockStore &s, const void *keys, const void *values, int64_t pos0, int n, const BlockKept &to,
                                hipStream_t stream) {
     const int64_t first = pos0 / BLOCK_ROWS, last = (pos0 + n - 1) / BLOCK_ROWS;
-    const dim3 grid((unsigned)(last - first + 1), s.st.BH, 2), block(256);
+    const dim3 grid((unsigned)(last - first + 1) + ((pos0 + n) / BLOCK_ROWS > first ? 1 : 0), s.st.BH, 2), block(256);
     const char *k = static_cast<const char *>(keys), *v = static_cast<const char *>(values);
-#define KV_APPEND(DK, DV)                                                                                                                        \
-    if (s.st.Dk == DK && s.st.Dv == DV) {                                                                                                        \
-        if (s.st.dtype == KVHIP_F16) hipLaunchKernelGGL((block_append_kernel<0, DK, DV>), grid, block, 0, stream, s, k, v, pos0, n, to_k, to_v); \
-        else hipLaunchKernelGGL((block_append_kernel<1, DK, DV>), grid, block, 0, stream, s, k, v, pos0, n, to_k, to_v);                         \
-        return hipGetLastError();                                                                                                                \
+#define KV_APPEND(DK, DV)                                                                                                                \
+    if (s.st.Dk == DK && s.st.Dv == DV) {                                                                                                \
+        if (s.st.dtype == KVHIP_F16) hipLaunchKernelGGL((block_append_kernel<0, DK, DV>), grid, block, 0, stream, s, k, v, pos0, n, to); \
+        else hipLaunchKernelGGL((block_append_kernel<1, DK, DV>), grid, block, 0, stream, s, k, v, pos0, n, to);                         \
+        return hipGetLastError();                                                                                                        \
     }
     KV_APPEND(64, 64)
     KV_APPEND(96, 96)

@@ -35,29 +35,52 @@ def code_block(x, dtype):
 
 
 class BlockScaledCache:
-    """Rows as they are read back, block by block."""
+    """Rows as they are read back, block by block.  Of some blocks the rows are kept as they came: of the unfinished one, the one in
+    front of it and the one that was unfinished before the last update."""
 
     def __init__(self, dtype):
         self.dtype, self.keys, self.values, self.coded = dtype, None, None, 0
         self.codes = {}  # (b, h, block) -> (codes of the keys, exponent)
+        self.kept = {}   # block -> (its first rows' keys, values)
 
     @property
     def offset(self):
         return 0 if self.keys is None else self.keys.shape[2]
 
     def trim(self, n):
-        self.keys, self.values = self.keys[:, :, :self.offset - n], self.values[:, :, :self.values.shape[2] - n]
+        left = self.offset - n
+        block, rows = left // BLOCK, left % BLOCK
+        arrays = [x[:, :, :left] for x in (self.keys, self.values)]
+        if rows and block in self.kept and self.kept[block][0].shape[2] >= rows:
+            arrays = [np.concatenate([x[:, :, :left - rows], raw[:, :, :rows]], 2) for x, raw in zip(arrays, self.kept[block])]
+            self.coded = min(self.coded, block)
+        elif not rows:
+            self.coded = min(self.coded, block)
+        self.keys, self.values = arrays
 
     def update(self, keys, values):
         before = self.offset
-        whole_before = min(self.coded, before // BLOCK)
+        begun = before // BLOCK
+        unfinished = before % BLOCK > 0 and self.coded == begun
         new = [np.where(np.isinf(x), np.nan, np.asarray(x, dtype=np.float64)) for x in (keys, values)]
         rows = [n if h is None else np.concatenate([h, n], 2) for h, n in zip((self.keys, self.values), new)]
         self.coded = rows[0].shape[2] // BLOCK
+
+        def raw(block, end):
+            return [x[:, :, block * BLOCK:end].copy() for x in rows]
+
+        kept = {self.coded - 1: self.kept[self.coded - 1]} if self.coded == begun and self.coded - 1 in self.kept else {}
+        if unfinished:
+            kept[begun] = raw(begun, before)
+        if self.coded > begun:
+            kept[self.coded - 1] = raw(self.coded - 1, self.coded * BLOCK)
+        if rows[0].shape[2] % BLOCK:
+            kept[self.coded] = raw(self.coded, rows[0].shape[2])
+        self.kept = kept
         for which, x in enumerate(rows):
             for b in range(x.shape[0]):
                 for h in range(x.shape[1]):
-                    for c in range(whole_before, self.coded):
+                    for c in range(begun, self.coded):
                         codes, e = code_block(x[b, h, c * BLOCK:(c + 1) * BLOCK], self.dtype)
                         x[b, h, c * BLOCK:(c + 1) * BLOCK] = codes * 2.0 ** e
                         if which == 0:
