@@ -517,6 +517,8 @@ class BlockScaledKVCache(KVCacheSimple):
         that hold no tokens in front of each sequence."""
         q, pad = self._block_arguments(queries, None, left_pad)
         B, Hq, Lq, D = q.shape
+        if self._shape is None and self.offset:
+            raise ValueError("how many kv heads this cache has is not known here: it was made from a handle")
         out = self._new_blocks(q, self._shape[1] if self._shape else 1, count)
         L.check(self._lib.kvhip_cache_select_blocks(self._h, _ptr(q), B, Hq, Lq, D, int(count), int(first), int(recent),
                                                     _ptr(pad) if pad is not None else None, _ptr(out), _stream()))

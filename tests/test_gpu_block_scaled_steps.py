@@ -35,3 +35,18 @@ def test_steps_of_many_heads_to_a_kv_head(dtype, sizes, heads):
         oracle.update(k, v)
         check(got, *exact_and_bound(q, oracle, scale, causal(oracle.offset, 1, [0, 0])))
         check_rows(cache, oracle)
+
+
+def test_a_choice_for_a_cache_made_from_a_handle():
+    """Its kv heads are known to the library alone: no array of lists can be made for them here."""
+    (_, k), (_, v) = pair(BF16, np.random.default_rng(1), 2, 4)(200)
+    owner = kvhip.BlockScaledKVCache()
+    owner.update(k, v, fetch=False)
+    other = kvhip.BlockScaledKVCache(handle=owner._h)
+    try:
+        with pytest.raises(ValueError):
+            other.select_blocks(torch.zeros(2, 8, 1, 128, dtype=BF16, device="cuda"), 3)
+        with pytest.raises(ValueError):
+            other.attend_blocks(torch.zeros(2, 8, 1, 128, dtype=BF16, device="cuda"), torch.zeros(2, 4, 1, 3, dtype=torch.int32, device="cuda"), 0.1)
+    finally:
+        other._h = None
