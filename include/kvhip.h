@@ -230,7 +230,9 @@ kvhip_status kvhip_rope_apply(const kvhip_rope *rope, const void *x, void *out, 
 
 /* `kvhip_cache_update` with the keys rotated inside the append / quantize-on-append kernel
  * (no rotated copy of the keys is written).  Positions start at the cache's `ropeOffset`:
- * its offset before this write (plus the staged rows of an open round), or batch_offsets[b]. */
+ * its offset before this write (plus the staged rows of an open round), or batch_offsets[b].
+ * The keys of a block-scaled cache turn in a buffer of the cache's, which grows with hipMalloc (on a stream that is being
+ * captured the call then returns KVHIP_ERR_UNSUPPORTED and has done nothing: kvhip_rope_apply and kvhip_cache_update do the same). */
 kvhip_status kvhip_cache_update_rope(kvhip_cache *cache, const kvhip_rope *rope, const int32_t *batch_offsets,
                                      const void *keys, const void *values, int32_t B, int32_t Hkv,
                                      int32_t L, int32_t Dk, int32_t Dv, int32_t dtype, void *stream);
@@ -240,7 +242,8 @@ kvhip_status kvhip_cache_update_rope(kvhip_cache *cache, const kvhip_rope *rope,
  * turn in the append's launch where their rows are whole 16-byte chunks; a single token's turn inside the attention
  * kernel where that writes the row too (kvhip_cache_update_attend).  `q_rotated`: device scratch of the queries' size that may hold them in between (it may be `queries`), of no
  * defined content afterwards; NULL: a buffer the cache keeps for it where there is need of one, which grows with
- * hipMalloc (on a stream that is being captured the call then returns KVHIP_ERR_UNSUPPORTED and has done nothing). */
+ * hipMalloc (on a stream that is being captured the call then returns KVHIP_ERR_UNSUPPORTED and has done nothing).  The keys of a
+ * block-scaled cache turn there too, before the queries; if it is `queries`, in such a buffer. */
 kvhip_status kvhip_cache_update_attend_rope(kvhip_cache *cache, const kvhip_rope *rope, const int32_t *batch_offsets,
                                             const void *queries, const void *keys, const void *values, int32_t B,
                                             int32_t Hq, int32_t Hkv, int32_t L, int32_t Dk, int32_t Dv, int32_t dtype,

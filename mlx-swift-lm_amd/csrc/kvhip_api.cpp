@@ -119,6 +119,7 @@ struct kvhip_cache {
     void *stage_tmp_k = nullptr, *stage_tmp_v = nullptr;  // dense copy of the rows a commit keeps
     size_t stage_tmp_rows = 0;
     RopeDev *rope = nullptr;  // set for the duration of one update_rope call
+    void *rope_keys = nullptr;  // likewise (block-scaled): where the keys turn
     // block-scaled only: blocks held as codes, and the blocks whose first `rows` rows are there as they came too, each in a place
     // of its own (kvhip_block.hpp).  The unfinished block, number `coded`, is one of them.
     struct KeptRows {
@@ -801,9 +802,8 @@ kvhip_status update_blocks(kvhip_cache *c, const void *k, const void *v, int L, 
         if (c->rope) {  // the keys turn in a launch of their own
             RopeDev turn = *c->rope;
             turn.qx = nullptr;
-            KV_TRY(ensure_pad_buf(c, 5, (size_t)c->st.BH * L * c->Dk_user * c->st.es));
-            KV_HIP(launch_rope_apply(turn, k, c->pad_buf[5], c->B, c->Hkv, L, c->Dk_user, c->st.dtype, stream));
-            k = c->pad_buf[5];
+            KV_HIP(launch_rope_apply(turn, k, c->rope_keys, c->B, c->Hkv, L, c->Dk_user, c->st.dtype, stream));
+            k = c->rope_keys;
         }
         KV_HIP(launch_block_append(block_store(c), k, v, prev, L, to, stream));
     }
@@ -1190,6 +1190,16 @@ kvhip_status rope_dev(const kvhip_rope *rope, int D, int H, int dtype, int64_t p
     r.vec = D % v == 0 && (r.traditional ? r.dims : r.dims / 2) % v == 0;
     return KVHIP_OK;
 }
+// A buffer of the cache's for rotated rows.  Refused before anything is written where a stream that is being captured cannot have
+// the memory: its caller can bring some and ask again.
+kvhip_status rope_buffer(kvhip_cache *c, int which, size_t need, hipStream_t stream, const char *refusal, void **out) {
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (need > c->pad_bytes[which]) KV_HIP(hipStreamIsCapturing(stream, &capture));
+    if (capture != hipStreamCaptureStatusNone) return fail(KVHIP_ERR_UNSUPPORTED, refusal);
+    KV_TRY(ensure_pad_buf(c, which, need));
+    *out = c->pad_buf[which];
+    return KVHIP_OK;
+}
 }  // namespace
 
 kvhip_status kvhip_rope_apply(const kvhip_rope *rope, const void *x, void *out, int32_t B, int32_t H,
@@ -1214,6 +1224,9 @@ kvhip_status kvhip_cache_update_rope(kvhip_cache *c, const kvhip_rope *rope, con
     // counts its staged rows (RotatingStagedKVCache.swift:33-37)
     const int64_t pos0 = c->offset + (c->staging ? (int64_t)c->staged.size() : 0);
     KV_TRY(rope_dev(rope, Dk, Hkv, dtype, pos0, batch_offsets, r));
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED && B > 0 && Hkv > 0 && L > 0 && Dk > 0)  // (else refused by the update)
+        KV_TRY(rope_buffer(c, 5, (size_t)B * Hkv * L * Dk * elem_size(dtype), S(stream),
+                           "a captured rotary update needs room for its keys: the cache's own buffer cannot grow here", &c->rope_keys));
     c->rope = &r;
     const kvhip_status st = kvhip_cache_update(c, keys, values, B, Hkv, L, Dk, Dv, dtype, stream);
     c->rope = nullptr;
@@ -1599,14 +1612,16 @@ kvhip_status kvhip_cache_update_attend_rope(kvhip_cache *c, const kvhip_rope *ro
                        c->has_geom && c->has_buffers && !c->padded() && c->B == B && c->Hkv == Hkv && c->st.Dk == Dk && c->st.Dv == Dv &&
                        c->st.dtype == dtype && (size_t)B * Hkv + (size_t)B * Hq <= 65535;
     if (!q_rotated && !(token && attention_will_write_step(c, Hq))) {
-        // (before anything is written: a stream that is being captured cannot have the memory, and its caller asks again)
-        const size_t need = (size_t)B * Hq * L * Dk * elem_size(dtype);
-        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-        if (need > c->pad_bytes[4]) KV_HIP(hipStreamIsCapturing(S(stream), &capture));
-        if (capture != hipStreamCaptureStatusNone)
-            return fail(KVHIP_ERR_UNSUPPORTED, "a captured rotary step needs q_rotated: the cache's own buffer cannot grow here");
-        KV_TRY(ensure_pad_buf(c, 4, need));
-        q_rotated = c->pad_buf[4];
+        KV_TRY(rope_buffer(c, 4, (size_t)B * Hq * L * Dk * elem_size(dtype), S(stream),
+                           "a captured rotary step needs q_rotated: the cache's own buffer cannot grow here", &q_rotated));
+    }
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED) {
+        // The keys turn where the queries do when the append has read them; in a buffer of their own if that is the queries' own place.
+        if (Hq % Hkv) return fail(KVHIP_ERR_INVALID_ARG, "query heads must be a multiple of KV heads");
+        c->rope_keys = q_rotated;
+        if (q_rotated == q)
+            KV_TRY(rope_buffer(c, 5, (size_t)B * Hkv * L * Dk * elem_size(dtype), S(stream),
+                               "a captured rotary step needs a q_rotated apart from its queries: the cache's own buffer cannot grow here", &c->rope_keys));
     }
     if (token) {
         int32_t slot = -1;

@@ -492,6 +492,16 @@ class BlockScaledKVCache(KVCacheSimple):
     def to_quantized(self, group_size=64, bits=4):
         raise TypeError("`to_quantized` belongs to `KVCacheSimple`: a BlockScaledKVCache is quantized")
 
+    def update_rope(self, rope, keys, values, batch_offsets=None):
+        try:
+            return super().update_rope(rope, keys, values, batch_offsets)
+        except L.KVHipError as e:
+            if e.status != L.ERR_UNSUPPORTED or not torch.cuda.is_current_stream_capturing():
+                raise
+        from .rope import apply_rotary_position
+        # (the cache's own buffer cannot grow under capture)
+        self._update(apply_rotary_position(rope, keys, self if batch_offsets is None else batch_offsets), values)
+
     def _block_arguments(self, queries, blocks, left_pad):
         """The arrays of a call over blocks, looked over."""
         q, dev = queries.contiguous(), torch._C._cuda_getDevice()

@@ -1,9 +1,12 @@
 """Single tokens into a block-scaled cache that the attention kernel writes, whichever kernel takes the call."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
 
 import kvhip
+from kvhip import _lib as L
 from oracle import block_scaled as O
 from test_gpu_block_scaled import causal, check, check_rows, exact_and_bound, fill, pair
 from util import NAME, randn
@@ -50,3 +53,110 @@ def test_a_choice_for_a_cache_made_from_a_handle():
             other.attend_blocks(torch.zeros(2, 8, 1, 128, dtype=BF16, device="cuda"), torch.zeros(2, 4, 1, 3, dtype=torch.int32, device="cuda"), 0.1)
     finally:
         other._h = None
+
+
+# ---- rotary positions ---------------------------------------------------------------------------------------------
+def heads_of(gen, dtype, n, sizes, heads, B=2):
+    hq, h = heads
+    return [torch.randn(B, x, n, d, generator=gen, device="cuda").to(dtype) for x, d in ((hq, sizes[0]), (h, sizes[0]), (h, sizes[1]))]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("sizes,dims", [((64, 64), 64), ((96, 96), 64), ((192, 128), 64), ((256, 256), 128), ((50, 36), 20), ((112, 72), 112)])
+@pytest.mark.parametrize("traditional", [False, True])
+def test_rotary_calls_equal_rotated_arrays(dtype, sizes, dims, traditional):
+    gen = torch.Generator(device="cuda").manual_seed(dims)
+    rope = kvhip.RoPE(dims, traditional=traditional)
+    a, b, c = (kvhip.BlockScaledKVCache() for _ in range(3))
+    for n in (70, 1, 1, 60, 300, 1):
+        q, k, v = heads_of(gen, dtype, n, sizes, (4, 2))
+        mask = kvhip.create_attention_mask(n, a)
+        at = None if n != 60 else torch.tensor([3, 900], device="cuda")
+        got = kvhip.attention_with_rope_and_cache_update(rope, q, k, v, a, 0.1, mask, batch_offsets=at)
+        qr, kr = (kvhip.apply_rotary_position(rope, x, b if at is None else at) for x in (q, k))
+        assert torch.equal(got, b.update_attend(qr, kr, v, 0.1, mask))
+        c.update_rope(rope, k, v, at)
+        assert torch.equal(got, c.attend(qr, 0.1, mask))
+    for other in (b, c):
+        for x, y in zip(a.fetch(), other.fetch()):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("sizes,heads", [((128, 128), (8, 2)), ((64, 64), (3, 3)), ((50, 36), (4, 1))])
+@pytest.mark.parametrize("n", [1, 4, 70])
+@pytest.mark.parametrize("warm", [False, True])
+@pytest.mark.parametrize("form", ["one", "apart"])
+def test_captured_rotary_calls(sizes, heads, n, warm, form):
+    """Also the first rotary call of a cache: what turns finds room without an allocation of the cache's.  Replay after replay."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    rope = kvhip.RoPE(sizes[0])
+    cache, other = kvhip.BlockScaledKVCache(), kvhip.BlockScaledKVCache()
+    _, k, v = heads_of(gen, BF16, 300, sizes, heads)
+    q, k1, v1 = heads_of(gen, BF16, n, sizes, heads)
+    for c in (cache, other):
+        c.update(k, v, fetch=False)
+        c.update_attend(q, k1, v1, 0.1, kvhip.create_attention_mask(n, c))  # (pages and attention scratch are there)
+        c.trim(n)
+
+    def step(c):
+        mask = kvhip.create_attention_mask(n, c)
+        if form == "one":
+            return kvhip.attention_with_rope_and_cache_update(rope, q, k1, v1, c, 0.1, mask)
+        turned = kvhip.apply_rotary_position(rope, q, c)
+        c.update_rope(rope, k1, v1)
+        return c.attend(turned, 0.1, mask)
+
+    if warm:
+        step(cache)
+        cache.trim(n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(cache)
+    for _ in range(3):
+        for dst, src in zip((q, k1, v1), heads_of(gen, BF16, n, sizes, heads)):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, step(other))
+        for a, b in zip(cache.fetch(), other.fetch()):
+            assert torch.equal(a, b)
+        other.trim(n)
+
+
+def test_a_captured_rotary_call_without_room_does_nothing():
+    """Through the C entries: refused before anything is written or allocated, and the capture goes on."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    rope = kvhip.RoPE(128)
+    cache = kvhip.BlockScaledKVCache()
+    _, k, v = heads_of(gen, BF16, 100, (128, 128), (8, 2))
+    cache.update(k, v, fetch=False)
+    q, k, v = heads_of(gen, BF16, 1, (128, 128), (8, 2))
+    want = cache.attend(q, 0.1)
+    r, keep = rope.to_c()
+    lib, mask, out = kvhip.load(), kvhip.MaskMode.none().to_c(2, 8, 1)[0], torch.empty_like(q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s = torch.cuda.current_stream().cuda_stream
+        for room in (None, q.data_ptr()):
+            status = lib.kvhip_cache_update_attend_rope(cache._h, C.byref(r), None, q.data_ptr(), k.data_ptr(), v.data_ptr(), 2, 8, 2, 1, 128, 128, L.BF16,
+                                                        0.1, C.byref(mask), room, out.data_ptr(), s)
+            assert status == L.ERR_UNSUPPORTED
+        status = lib.kvhip_cache_update_rope(cache._h, C.byref(r), None, k.data_ptr(), v.data_ptr(), 2, 2, 1, 128, 128, L.BF16, s)
+        assert status == L.ERR_UNSUPPORTED and cache.offset == 100
+        cache.attend(q, 0.1, out=out)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    # with room, also the queries' own place, which is a buffer's business outside a capture
+    other = cache.copy()
+    turned = kvhip.apply_rotary_position(rope, q, cache)
+    own = q.clone()
+    assert lib.kvhip_cache_update_attend_rope(cache._h, C.byref(r), None, own.data_ptr(), k.data_ptr(), v.data_ptr(), 2, 8, 2, 1, 128, 128, L.BF16,
+                                              0.1, C.byref(mask), own.data_ptr(), out.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    other.update_rope(rope, k, v)
+    assert torch.equal(out, other.attend(turned, 0.1))
+    assert lib.kvhip_cache_update_attend_rope(cache._h, C.byref(r), None, q.data_ptr(), k.data_ptr(), v.data_ptr(), 2, 7, 2, 1, 128, 128, L.BF16,
+                                              0.1, C.byref(mask), None, out.data_ptr(), None) == -2
+    assert cache.offset == 101
