@@ -129,12 +129,7 @@ template <int DK, int DV, int DT, int NM, int MODE, bool SUMS = false> struct Bl
         }
     }
 
-    // (one instruction; through fmaxf every operand is quieted by another one)
-    static __device__ __forceinline__ float max3(float a, float b, float c) {
-        float r;
-        asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-        return r;
-    }
+    static __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
     // Scores of one tile of query rows -> weights as operands; the outputs so far are brought to the new maximum.  Scores and
     // maxima are products that the call's scale has yet to meet (MODE 2: has met, an added mask's terms among them).
     __device__ __forceinline__ void weigh(int i, kv_f4 (&s)[4], kv_u4 (&p)[2]) {
