@@ -23,12 +23,16 @@
 namespace kvhip {
 
 // Whether a call has rows enough for the kernel that shares blocks between wavefronts, and the rows its workgroup takes.  Against
-// two tiles of rows to a wavefront that loads for itself, bfloat16, us, shared / not: head size 128, 40 rows of a pair 35.6 / 39.9
-// (8 x 8 pairs, 8000 keys) and 54.0 / 73.6 (32 x 8 pairs, 4000), 64 rows 26.4 / 31.2, 256 rows 109 / 112, 2048 rows 109 / 107; 256, 40 rows
-// 23.3 / 33.4, 600 rows 49.8 / 73.3; keys of 192, 200 rows 41.1 / 47.1, 40 rows 24.4 / 21.5.  Head sizes below 128, whose blocks
-// need fewer registers, go the other way: 64, 160 rows 37.0 / 31.3, 2000 rows 234 / 210; 96, 200 rows 144 / 136.
+// two tiles of rows to a wavefront that loads for itself, us, shared / not: head size 128, 48 rows of a pair 36.3 / 40.3
+// (8 x 8 pairs, 8000 keys), 40 rows 54.0 / 73.6 (32 x 8 pairs, 4000), but 48 rows of 8 pairs over 8192 keys 17.3 / 16.4, 96 rows 20.0 / 21.3;
+// 2048 rows 92.2 / 92.3 and, of 8 x 8 pairs, 695 / 691; 256, 4 x 8 pairs, 4000 keys, 34 rows 30.6 / 48.0, 2048 rows 377 / 652.  Keys of 192, whose
+// workgroups take 128 rows, from more than those on: 40 rows 36.5 / 30.2 (4 x 16 pairs, 4000 keys) and 22.9 / 18.0 (8 pairs, 8000),
+// 96 rows 40.9 / 41.8 and 26.1 / 21.2, 128 rows 44.5 / 42.1 and 27.7 / 21.9, 160 rows 65.1 / 80.4 and 28.6 / 25.1, 400 rows 103 / 152 and
+// 41.7 / 45.9.  Head sizes below 128, whose blocks need fewer registers, go the other way: 64, 160 rows 37.0 / 31.3, 2000 rows
+// 234 / 210; 96, 200 rows 144 / 136.
 inline bool block_attend_tiled(const BlockAttend &x) {
-    return !x.list && x.a.mask.mode != KVHIP_MASK_ARRAY && x.a.st.Dk >= 128 && x.a.Hq / x.a.Hkv * x.a.L > 32;
+    const int64_t rows = (int64_t)x.a.Hq / x.a.Hkv * x.a.L;
+    return !x.list && x.a.mask.mode != KVHIP_MASK_ARRAY && x.a.st.Dk >= 128 && rows > (x.a.st.Dk == 192 ? 128 : 32);
 }
 inline int block_tiled_rows(int Dk) { return Dk == 192 ? 128 : 64; }
 

@@ -160,3 +160,16 @@ def test_a_captured_rotary_call_without_room_does_nothing():
     assert lib.kvhip_cache_update_attend_rope(cache._h, C.byref(r), None, q.data_ptr(), k.data_ptr(), v.data_ptr(), 2, 7, 2, 1, 128, 128, L.BF16,
                                               0.1, C.byref(mask), None, out.data_ptr(), None) == -2
     assert cache.offset == 101
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n", [64, 65, 128, 129, 161, 300])
+@pytest.mark.parametrize("heads,pads", [((4, 4), (0, 0)), ((2, 2), (70, 300)), ((2, 1), (0, 11))])
+def test_prompt_chunks_of_keys_of_192(dtype, n, heads, pads):
+    """Either kernel, and the rows at which one takes over from the other."""
+    rng = np.random.default_rng(n)
+    cache, oracle = kvhip.BlockScaledKVCache(), O.BlockScaledCache(NAME[dtype])
+    fill(cache, oracle, pair(dtype, rng, 2, heads[1], (192, 128)), [730])
+    q, qd = randn(rng, (2, heads[0], n, 192), dtype)
+    mask = kvhip.MaskMode.window_mask(730 - n, 0, left_pad=torch.tensor(pads, device="cuda"))
+    check(cache.attend(qd, 0.07, mask), *exact_and_bound(q, oracle, 0.07, causal(730, n, pads)))
