@@ -318,7 +318,9 @@ kvhip_status kvhip_cache_update_attend(kvhip_cache *cache, const void *queries, 
  *     a = max |x| over the block's finite elements;  e = the least integer with a 2^-e <= 448 (0 if a = 0; at least -100)
  *     code = e4m3(x 2^-e), to nearest even;  the value read back is code 2^e
  * and the rows behind the last such block are held as they came.  Values read back are exact in the cache's dtype, and
- * written again they come out the same; infinities are held as NaN; values beyond 61440 (bfloat16: beyond 1.875 2^127) are held as that.
+ * written again they come out the same -- though a block's scale comes out half as large where its largest element had been
+ * rounded down to 448 of that half, so that a cache filled from another's state may choose other blocks (below; a copy has the
+ * scales too).  Infinities are held as NaN; values beyond 61440 (bfloat16: beyond 1.875 2^127) are held as that.
  * float16 and bfloat16, head sizes up to 256 (stored zero-padded to 64, 96, 128 or 256; 192 with 128); else
  * KVHIP_ERR_UNSUPPORTED.  kvhip_cache_trim and _set_offset take rows off what the cache presents at once; offsets are never
  * set forward.  Rows taken off leave no trace in the block that this opens again -- its rows are as they came -- where that is
@@ -326,12 +328,14 @@ kvhip_status kvhip_cache_update_attend(kvhip_cache *cache, const void *queries, 
  * whole call can be taken back.  In any other block the rows that are left stay what its codes say, and are coded from those when
  * it is finished again.  Query rows that see no key are zeros.  kvhip_last_attend_kernel: 7, over chosen blocks 8.
  *
- * Attention over chosen blocks.  Query row l of L sits at position p = presented length - L + l.  A query row's bound on a
- * block is sum_d max(q_d hi_d, q_d lo_d), hi and lo the block's largest and smallest key element of each channel, with
- * hi and lo taken as rint(code / 4) 2^(e + 2) and q as rint(q 2^-f) 2^f, f the least integer with max |q| 2^-f <= 127 over
- * the row (elements that are not finite: 0), so that it is exact; a token's bound is the largest of its query rows'
- * over one kv head.  The token sees blocks left_pad[b] / 64 to p / 64 (none if p < left_pad[b]).  The first `first` of these
- * and the last `recent` are chosen, and as many more as make `count`, by their bounds, the lower block among equals.
+ * Attention over chosen blocks.  Query row l of L sits at position p = presented length - L + l.  What is called a query
+ * row's bound on a block here is sum_d max(q_d hi_d, q_d lo_d), hi and lo the block's largest and smallest key element of each
+ * channel, with hi and lo taken as rint(code / 4) 2^(e + 2) and q as rint(q 2^-f) 2^f, f the least integer with max |q| 2^-f <= 127
+ * over the row (elements that are not finite: 0).  These roundings make its arithmetic exact, and make it an estimate: without
+ * them no key of the block would score higher, with them one may.  Channels whose codes stay within 2 of zero (1/224 to 1/112
+ * of the block's largest element) have no part in it.  A token's bound is the largest of its query rows' over one kv head.  The
+ * token sees blocks left_pad[b] / 64 to p / 64 (none if p < left_pad[b]).  The first `first` of these and the last `recent` are
+ * chosen, and as many more as make `count`, by their bounds, the lower block among equals.
  * blocks: device [B, Hkv, L, count] int32, ascending, -1 behind the last; left_pad: device [B] or NULL.
  * first >= 0, recent >= 1, first + recent <= count <= 2^20; up to 27 000 blocks (1.7 million rows) a cache.  At most 65 535
  * tiles of 16 query rows a kv head (L times Hq / Hkv / 16, rounded up) to a call.

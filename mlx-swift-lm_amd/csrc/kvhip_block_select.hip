@@ -1,9 +1,10 @@
-// Blocks for each token from a bound on what they hold (summaries: kvhip_block.hpp).
+// Blocks for each token from an estimate of the best score in them (summaries: kvhip_block.hpp).
 //
 // A query row's bound on a block is sum_d max(q_d hi_d, q_d lo_d), with hi and lo the block's largest and smallest key element
-// of each channel: no key of the block scores higher.  Both sides are whole numbers times powers of two -- hi and lo are int8
-// in units of 4 scales, q is rint(q 2^-f), f the least integer with max |q| 2^-f <= 127 -- so that the sum is exact whatever
-// its order (below 2^22 for 256 channels) and the choice the same on any machine.  As products:
+// of each channel.  Both sides are rounded to whole numbers times powers of two -- hi and lo are int8 in units of 4 scales, q is
+// rint(q 2^-f), f the least integer with max |q| 2^-f <= 127 -- so that the sum is exact whatever its order (below 2^22 for 256
+// channels) and the choice the same on any machine.  Without the roundings no key of the block would score higher; as it is one may, by
+// up to half a unit of either side in every channel, and channels that stay within half a unit of zero have no part.  As products:
 // q+ hi + q- lo, with q+ = max(q, 0) and q- = min(q, 0), on the 16x16x64 int8 instruction.
 #include <algorithm>
 #include <type_traits>

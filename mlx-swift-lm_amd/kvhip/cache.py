@@ -523,7 +523,7 @@ class BlockScaledKVCache(KVCacheSimple):
     def select_blocks(self, queries, count, first=1, recent=1, left_pad=None):
         """`count` blocks of 64 cached positions for each token of `queries` [B,Hq,L,D], which are the last L positions, and each
         kv head: int32 [B,Hkv,L,count], ascending, -1 behind the last.  The `first` leading and `recent` last blocks that the
-        token sees are always chosen, the others by a bound on the scores of their keys.  `left_pad` [B]: positions
+        token sees are always chosen, the others by an estimate of their keys' best score.  `left_pad` [B]: positions
         that hold no tokens in front of each sequence."""
         q, pad = self._block_arguments(queries, None, left_pad)
         B, Hq, Lq, D = q.shape

@@ -187,3 +187,32 @@ def test_random_schedules(dtype, seed):
         check(cache.attend(qd, 0.1), *exact_and_bound(q, oracle, 0.1, causal(oracle.offset, 1, [0])))
         blocks = cache.select_blocks(qd, 3, 0, 1)
         assert np.array_equal(blocks.cpu().numpy(), O.select(q, oracle, 3, 0, 1, [0]))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_choices_of_copies_and_of_caches_filled_from_a_state(dtype):
+    """A copy chooses as its source does.  A cache filled from a state holds the same values and chooses by what it was filled with: blocks
+    whose largest element was rounded down have half the scale there."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    k = torch.randn(1, 2, 64 * 40, 64, generator=gen, device="cuda")
+    k[..., 7] *= 8
+    top = k.unflatten(2, (40, 64)).abs().amax((3, 4), keepdim=True)
+    k = (k.unflatten(2, (40, 64)) * (228.0 / 128 / top)).flatten(2, 3).to(dtype)  # (every block's largest: 228 of 2^-7)
+    cache, filled = kvhip.BlockScaledKVCache(), kvhip.BlockScaledKVCache()
+    cache.update(k, k, fetch=False)
+    copy = cache.copy()
+    filled.state = cache.state
+    first, again = O.BlockScaledCache(NAME[dtype]), O.BlockScaledCache(NAME[dtype])
+    first.update(*[k.double().cpu().numpy()] * 2)
+    again.update(first.keys, first.values)
+    scales = [[c.codes[0, 0, i][1] for i in range(40)] for c in (first, again)]
+    assert all(a == b + 1 for a, b in zip(*scales))
+    for c in (copy, filled):
+        for a, b in zip(c.fetch(), cache.fetch()):
+            assert torch.equal(a, b)
+    q = torch.randn(1, 4, 9, 64, generator=gen, device="cuda").to(dtype)
+    qn = q.double().cpu().numpy()
+    got = cache.select_blocks(q, 6, 0, 1)
+    assert torch.equal(got, copy.select_blocks(q, 6, 0, 1))
+    assert np.array_equal(got.cpu().numpy(), O.select(qn, first, 6, 0, 1, [0]))
+    assert np.array_equal(filled.select_blocks(q, 6, 0, 1).cpu().numpy(), O.select(qn, again, 6, 0, 1, [0]))
