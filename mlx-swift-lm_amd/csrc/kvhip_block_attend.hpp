@@ -786,7 +786,7 @@ __global__ void __launch_bounds__(512, 2) block_attend_tiled_kernel(BlockAttend 
     auto request = [&](int j) {
         const int c = rw * MINE + j;
         const gptr from = c < DK / 16 ? k_from + c * 1024 : v_from + (c - DK / 16) * 1024;
-        prefill_fp::load_to_lds((const char *)from, lane * 16, to + c * 1024);  // (its invariant: the wait and the barrier below)
+        prefill_fp::load_to_lds((const char *)from, lane * 16, to + c * 1024);  // (its invariant: the wait and the counters below)
     };
     if (rounds > 0 && locate(0)) {
 #pragma unroll
