@@ -345,6 +345,9 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, char *codes, 
 // of the last whole block as they came, from the caller's arrays; where some of them are there as codes only, the block's own
 // workgroup does, in front of the barrier behind which it writes the codes anew.  (All of it by the block's own workgroup: 512 rows of
 // 8 heads written and attended for 102 us, with one more 97.5; 4 x 8 heads x 8191 rows stored and read back 118 us and 83.5.)
+// Workgroups go to the eight dies in turn: where a pair has a multiple of eight of them, each pair begins with another block, since the
+// ones that write rows as they came, the slowest, would all be on one die (4 x 8 heads x 8127 rows: 56 us, and 45 so; other numbers
+// spread by themselves: 8191 rows, 129 workgroups a pair, 44.5, and 54.6 if shifted).
 template <int DT, int DK, int DV>
 __global__ void __launch_bounds__(256) block_append_kernel(BlockStore s, const char *keys, const char *values, int64_t pos0, int n, BlockKept to) {
     __shared__ __align__(16) uint32_t raw[64 * (DK / 2 + 4)];
@@ -357,7 +360,7 @@ __global__ void __launch_bounds__(256) block_append_kernel(BlockStore s, const c
     a.n = n;
     a.ud = v ? s.Dv_user : s.Dk_user;
     const int done = (int)((pos0 + n) / BLOCK_ROWS) - 1;
-    a.blk = (int)(pos0 / BLOCK_ROWS) + blockIdx.x;
+    a.blk = (int)(pos0 / BLOCK_ROWS) + (int)(gridDim.x % 8 == 0 ? (blockIdx.x + blockIdx.y) % gridDim.x : blockIdx.x);
     const bool keeper = a.blk > (int)((pos0 + n - 1) / BLOCK_ROWS);
     if (keeper) a.blk = done;
     a.bh = blockIdx.y;

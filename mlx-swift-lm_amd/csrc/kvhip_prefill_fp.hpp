@@ -25,8 +25,9 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 // the same requests (which variant of an iteration it runs may differ) -- or, in the block-scaled kernel, each of
 // the wavefronts that share a buffer says so in a counter of its own in LDS, released behind the wait, and those
 // that share it run the same rounds and go on when they have acquired all of their counters; a buffer is requested
-// into again only behind the barrier, or the counters, by which all its readers are done with it; (2) vector-memory operations of one wavefront complete in order on this hardware -- the compiler's own
-// waits for register loads rely on that when an uncounted LDS load sits between them.
+// into again only behind the barrier, or the counters, by which all its readers are done with it; (2)
+// vector-memory operations of one wavefront complete in order on this hardware -- the compiler's own waits for
+// register loads rely on that when an uncounted LDS load sits between them.
 // (address = wave-uniform 64-bit `base` in scalar registers + the lane's unsigned 32-bit byte offset)
 __device__ __forceinline__ void load_to_lds(const char *base, uint32_t lane_off, const void *lds_wave_base) {
     // (the low half of a flat address inside the LDS aperture is the LDS address itself)
