@@ -109,6 +109,10 @@ template <int DK, int DV, int DT, int NM, int MODE, bool SUMS = false> struct Bl
     // float16 weights are taken times 2^14: those of keys far below the largest stay clear of the type's subnormals (the sums
     // carry the factor too)
     static constexpr float LIFT = DT == 0 ? 14.f : 0.f;
+    // Maxima beyond this (in powers of two) are taken off before the product with `unit`, an instruction more for each score: the
+    // roundings of the maximum's product and of what is added to it are 2^-11 here, less than half a step of float16, and
+    // would lift weights past the type's largest value from 2^24 on.
+    static constexpr float FAR = 4096.f;
 
     const BlockAttend &x;
     const int lane, g, n;
@@ -144,16 +148,23 @@ template <int DK, int DV, int DT, int NM, int MODE, bool SUMS = false> struct Bl
         my = max3(my, s[2][3], s[3][0]);
         mx = row_max(max3(max3(mx, s[3][1], s[3][2]), my, s[3][3]));
         const float ref = mx == -INFINITY ? 0.f : mx;  // (nothing seen yet: every difference is -infinity)
-        const float off = LIFT - ref * unit;
+        const float far = ref * unit, off = LIFT - far;
         float e[16], sum = 0.f;
+        if (SAFE || __any(fabsf(far) > FAR)) {  // the difference first: it is exact where it counts, and no exponent is above LIFT
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float y = SAFE ? __builtin_fmaf(s[t][k] - ref, LOG2E, LIFT) : __builtin_fmaf(s[t][k], unit, off);
-                e[4 * t + k] = fast_exp2(y);
-                if constexpr (!SUMS) sum += e[4 * t + k];
-            }
+                for (int k = 0; k < 4; ++k) e[4 * t + k] = fast_exp2(__builtin_fmaf(s[t][k] - ref, unit, LIFT));
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e[4 * t + k] = fast_exp2(__builtin_fmaf(s[t][k], unit, off));
+        }
+        if constexpr (!SUMS) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) sum += e[k];
+        }
         if (__any(mx != m[i])) {
             const float alpha = fast_exp2((m[i] - ref) * unit);
             if constexpr (SUMS) ls[i] *= alpha;

@@ -173,3 +173,43 @@ def test_prompt_chunks_of_keys_of_192(dtype, n, heads, pads):
     q, qd = randn(rng, (2, heads[0], n, 192), dtype)
     mask = kvhip.MaskMode.window_mask(730 - n, 0, left_pad=torch.tensor(pads, device="cuda"))
     check(cache.attend(qd, 0.07, mask), *exact_and_bound(q, oracle, 0.07, causal(730, n, pads)))
+
+
+# ---- scores far from zero -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("sizes", [(64, 64), (128, 128), (256, 256)])
+@pytest.mark.parametrize("n", [1, 4, 100])
+@pytest.mark.parametrize("scale", [0.37, 1.7, 3.1, -5.3])
+def test_scores_beyond_24_bits(dtype, sizes, n, scale):
+    """Scores whose units are beyond float32's: the keys that score highest, all alike, share the weight, and no other has any.
+    A query is one channel of 2^12 to 2^15, a key the same channel of 2^11 or 2^12; scores are exact."""
+    rng = np.random.default_rng(n)
+    dk, dv = sizes
+    T = 300
+    size = np.where(rng.random((2, 2, T)) < 0.1, 4096.0, 2048.0)
+    size[:, :, 0] = 4096.0
+    if scale < 0:
+        size = 6144.0 - size
+    k = np.zeros((2, 2, T, dk), np.float32)
+    k[..., 3] = size
+    v, vd = randn(rng, (2, 2, T, dv), dtype)
+    q = np.zeros((2, 8, n, dk), np.float32)
+    q[..., 3] = 2.0 ** rng.integers(12, 16, (2, 8, n)) * rng.choice([1.0, 1.5, 1.75], (2, 8, n))
+    cache = kvhip.BlockScaledKVCache()
+    kd, qd = (torch.from_numpy(x).to(dtype).cuda() for x in (k, q))
+    cache.update(kd, vd, fetch=False)
+    held, value = (x.double().cpu().numpy() for x in cache.fetch())
+    assert np.array_equal(held, k)
+    keep = np.arange(T) <= np.arange(T - n, T)[:, None]
+    best = 4096.0 if scale > 0 else 2048.0
+    weight = (keep & (size == best)[:, :, None]).astype(np.float64)
+    weight /= weight.sum(-1, keepdims=True)
+    want = np.repeat(weight @ value, 4, 1)
+    # the weights' and the output's half steps, and the sums over at most 300 of them
+    u = torch.finfo(dtype).eps / 2
+    bound = u * np.abs(want) + (2 * u + 2 * T * 2.0 ** -24) * np.repeat(weight @ np.abs(value), 4, 1) + 1e-30
+    check(cache.attend(qd, scale, kvhip.MaskMode.causal()), want, bound)
+    blocks = torch.arange(5, dtype=torch.int32, device="cuda").expand(2, 2, n, 5).contiguous()
+    check(cache.attend_blocks(qd, blocks, scale), want, bound)
+    array = torch.from_numpy(keep).cuda().expand(2, 1, n, T)
+    check(cache.attend(qd, scale, kvhip.MaskMode.from_array(array)), want, bound)
