@@ -123,7 +123,7 @@ struct AppendArgs {
     __device__ __forceinline__ const char *rows() const { return src + (size_t)bh * n * ud * 2; }
 };
 
-// New rows of a block as they came, into its place (behind those of a reopened one).
+// New rows of a block that stays unfinished, into its place (behind those of a reopened one).
 template <int DT, int D, bool V>
 __device__ __forceinline__ void append_tail(const AppendArgs &a, const char *codes, const char *tail, char *to, float scale) {
     const int start = a.reopened ? 0 : a.from(), upto = a.upto(), from = a.from();
@@ -165,19 +165,19 @@ __device__ __forceinline__ void append_tail(const AppendArgs &a, const char *cod
     }
 }
 
-// A block that is whole after this call: its rows (those held so far and the new ones) become codes.  A wavefront takes what
+// A block that is whole after this call: its rows (those held so far and the new ones) become codes, and, of the call's last such
+// block, stay in `keep` as they came.  A wavefront takes what
 // it can write out in whole lines, straight from registers; the largest magnitude meets in LDS.  Elements stay as they came,
 // two to a word: magnitudes and channel extremes are packed integer maxima, the division by the scale and the rounding one
 // conversion for two.  Elements past the largest that can be coded (infinities and NaN among them) are seen to where a
-// thread has met one.  Bound by memory, 2 bytes read and 1 written an element: 8 x 8 heads x 2048 rows x 128 18.8 us, 5.3 TB/s
-// (with rows in float32 and codes brought into order in LDS 34.7); 4 x 8 heads x 8191 rows, whose rows come from HBM while
-// what the pass before wrote is still on its way there, 72 us, 2.8 TB/s (98.8).
+// thread has met one.  Bound by memory, 2 bytes read and 1 written an element: 8 x 8 heads x 2048 rows x 128 20 us, 5.0 TB/s;
+// 4 x 8 heads x 8191 rows 43 us, 4.7 TB/s, what a copy gives.
 //
 // Keys: a wavefront to 16 rows, a lane to one of them and 16 channels of every 64 (8 of a last 32).  Extremes of the channels
 // go through LDS, each wavefront's own rows first.
 template <int DT, int D>
-__device__ __forceinline__ void append_keys(const AppendArgs &a, char *codes, const char *tail, float *scale_out, char *summary, float held_scale,
-                                            uint32_t *raw, uint32_t *ends, uint32_t *amax_s) {
+__device__ __forceinline__ void append_keys(const AppendArgs &a, char *codes, const char *tail, char *keep, float *scale_out, char *summary,
+                                            float held_scale, uint32_t *raw, uint32_t *ends, uint32_t *amax_s) {
     constexpr int KC = D / 64, CH = KC * 8 + (D % 64 ? 4 : 0);  // words of two a lane
     constexpr int PITCH = D / 2 + 4;                           // words of a row in LDS
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15, r = 16 * wave + m;
@@ -192,6 +192,12 @@ __device__ __forceinline__ void append_keys(const AppendArgs &a, char *codes, co
         else x = raw_chunk(rows, (size_t)(a.lo() + r - a.pos0), a.ud, channel(c));
 #pragma unroll
         for (int k = 0; k < 4; ++k) w[4 * c + k] = x[k];
+    }
+    if (keep && (r >= from || a.reopened)) {  // (its first rows are there already)
+#pragma unroll
+        for (int c = 0; c < CH / 4; ++c)
+            *reinterpret_cast<kv_u4 *>(keep + ((size_t)r * D + channel(c)) * 2) = kv_u4{no_infinities<DT>(w[4 * c]), no_infinities<DT>(w[4 * c + 1]),
+                                                                                       no_infinities<DT>(w[4 * c + 2]), no_infinities<DT>(w[4 * c + 3])};
     }
     uint32_t mag = 0;
 #pragma unroll
@@ -269,7 +275,8 @@ __device__ __forceinline__ void append_keys(const AppendArgs &a, char *codes, co
 
 // Values: a wavefront to the 16 tokens 16 t + 4 wave + i, a lane to two channels of them (of every 128).
 template <int DT, int D>
-__device__ __forceinline__ void append_values(const AppendArgs &a, char *codes, const char *tail, float *scale_out, float held_scale, uint32_t *amax_s) {
+__device__ __forceinline__ void append_values(const AppendArgs &a, char *codes, const char *tail, char *keep, float *scale_out, float held_scale,
+                                              uint32_t *amax_s) {
     constexpr int TURNS = (D + 127) / 128;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int from = a.from();
@@ -298,6 +305,24 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, char *codes, 
                 }
             }
             w[turn][i] = x;
+        }
+    }
+    if (keep) {  // (a lane's four tokens of a channel lie side by side)
+        uint16_t *to = reinterpret_cast<uint16_t *>(keep);
+#pragma unroll
+        for (int turn = 0; turn < TURNS; ++turn) {
+            const int d = turn * 128 + 2 * lane;
+            if (d >= D) continue;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (16 * k + 4 * wave + 4 <= from && !a.reopened) continue;
+                uint32_t x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = no_infinities<DT>(w[turn][4 * k + i]);
+                uint16_t *at = to + tail_v_at(D, 16 * k + 4 * wave, d);
+                *reinterpret_cast<kv_w2 *>(at) = kv_w2{__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u)};
+                *reinterpret_cast<kv_w2 *>(at + 8) = kv_w2{__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
+            }
         }
     }
 #pragma unroll
@@ -341,13 +366,10 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, char *codes, 
     }
 }
 
-// grid (blocks touched, and one more if one of them becomes whole, BH, keys / values), 256 threads.  The last workgroup keeps the rows
-// of the last whole block as they came, from the caller's arrays; where some of them are there as codes only, the block's own
-// workgroup does, in front of the barrier behind which it writes the codes anew.  (All of it by the block's own workgroup: 512 rows of
-// 8 heads written and attended for 102 us, with one more 97.5; 4 x 8 heads x 8191 rows stored and read back 118 us and 83.5.)
-// Workgroups go to the eight dies in turn: where a pair has a multiple of eight of them, each pair begins with another block, since the
-// ones that write rows as they came, the slowest, would all be on one die (4 x 8 heads x 8127 rows: 56 us, and 45 so; other numbers
-// spread by themselves: 8191 rows, 129 workgroups a pair, 44.5, and 54.6 if shifted).
+// grid (blocks touched, BH, keys / values), 256 threads.  Workgroups go to the eight dies in turn: where a pair has a multiple of eight of
+// them, each pair begins with another block, since the ones that leave a block unfinished, the slowest, would all be on one die
+// (4 x 8 heads of float16, us, so / without: 2000 rows 15.8 / 17.4, 4063 rows 22.6 / 24.8, 8191 rows 45.4 / 53.9; 8127 and 8255 rows, 127 and
+// 129 workgroups a pair, spread by themselves: 44.3 and 44.6).
 template <int DT, int DK, int DV>
 __global__ void __launch_bounds__(256) block_append_kernel(BlockStore s, const char *keys, const char *values, int64_t pos0, int n, BlockKept to) {
     __shared__ __align__(16) uint32_t raw[64 * (DK / 2 + 4)];
@@ -361,26 +383,24 @@ __global__ void __launch_bounds__(256) block_append_kernel(BlockStore s, const c
     a.ud = v ? s.Dv_user : s.Dk_user;
     const int done = (int)((pos0 + n) / BLOCK_ROWS) - 1;
     a.blk = (int)(pos0 / BLOCK_ROWS) + (int)(gridDim.x % 8 == 0 ? (blockIdx.x + blockIdx.y) % gridDim.x : blockIdx.x);
-    const bool keeper = a.blk > (int)((pos0 + n - 1) / BLOCK_ROWS);
-    if (keeper) a.blk = done;
     a.bh = blockIdx.y;
     a.reopened = a.blk < s.coded && pos0 > a.lo();
     const PageEntry e = block_page(s, a.blk / BLOCK_PER_PAGE);
     const int in_page = a.blk % BLOCK_PER_PAGE, bh = a.bh;
     float *scales = reinterpret_cast<float *>(e.ksb + (size_t)bh * s.st.ksb_cell) + 2 * in_page + (v ? 1 : 0);
     const float held = a.reopened ? *scales : 1.f;
-    const bool whole = pos0 + n >= a.lo() + BLOCK_ROWS, keep = a.blk == done && keeper != a.reopened;
+    const bool whole = pos0 + n >= a.lo() + BLOCK_ROWS, keep = a.blk == done;  // (the last whole block is kept as it came, too)
     if (v) {
         const size_t at = (size_t)bh * BLOCK_ROWS * DV * 2;
         char *codes = e.v + (size_t)bh * s.st.v_cell + (size_t)in_page * BLOCK_ROWS * DV;
-        if (!whole || keep) append_tail<DT, DV, true>(a, codes, s.tail_v + at, (whole ? to.done_v : to.open_v) + at, held);
-        if (whole && !keeper) append_values<DT, DV>(a, codes, s.tail_v + at, scales, held, amax_s);
+        if (whole) append_values<DT, DV>(a, codes, s.tail_v + at, keep ? to.done_v + at : nullptr, scales, held, amax_s);
+        else append_tail<DT, DV, true>(a, codes, s.tail_v + at, to.open_v + at, held);
     } else {
         const size_t at = (size_t)bh * BLOCK_ROWS * DK * 2;
         char *codes = e.k + (size_t)bh * s.st.k_cell + (size_t)in_page * BLOCK_ROWS * DK;
         char *summary = e.vsb + (size_t)bh * s.st.vsb_cell + (size_t)in_page * 2 * DK;
-        if (!whole || keep) append_tail<DT, DK, false>(a, codes, s.tail_k + at, (whole ? to.done_k : to.open_k) + at, held);
-        if (whole && !keeper) append_keys<DT, DK>(a, codes, s.tail_k + at, scales, summary, held, raw, ends, amax_s);
+        if (whole) append_keys<DT, DK>(a, codes, s.tail_k + at, keep ? to.done_k + at : nullptr, scales, summary, held, raw, ends, amax_s);
+        else append_tail<DT, DK, false>(a, codes, s.tail_k + at, to.open_k + at, held);
     }
 }
 
@@ -450,7 +470,7 @@ template <int DT> __global__ void __launch_bounds__(256) block_fetch_kernel(Bloc
 hipError_t launch_block_append(const BlockStore &s, const void *keys, const void *values, int64_t pos0, int n, const BlockKept &to,
                                hipStream_t stream) {
     const int64_t first = pos0 / BLOCK_ROWS, last = (pos0 + n - 1) / BLOCK_ROWS;
-    const dim3 grid((unsigned)(last - first + 1) + ((pos0 + n) / BLOCK_ROWS > first ? 1 : 0), s.st.BH, 2), block(256);
+    const dim3 grid((unsigned)(last - first + 1), s.st.BH, 2), block(256);
     const char *k = static_cast<const char *>(keys), *v = static_cast<const char *>(values);
 #define KV_APPEND(DK, DV)                                                                                                                \
     if (s.st.Dk == DK && s.st.Dv == DV) {                                                                                                \
