@@ -165,11 +165,10 @@ __device__ __forceinline__ void append_tail(const AppendArgs &a, const char *cod
     }
 }
 
-// A block that is whole after this call: its rows (those held so far and the new ones) become codes, and, of the call's last such
-// block, stay in `keep` as they came.  A wavefront takes what
-// it can write out in whole lines, straight from registers; the largest magnitude meets in LDS.  Elements stay as they came,
-// two to a word: magnitudes and channel extremes are packed integer maxima, the division by the scale and the rounding one
-// conversion for two.  Elements past the largest that can be coded (infinities and NaN among them) are seen to where a
+// A block that is whole after this call: its rows (those held so far and the new ones) become codes and, of the call's last such
+// block, stay in `keep` as they came.  A wavefront takes what it can write out in whole lines, straight from registers; the
+// largest magnitude meets in LDS.  Elements are two to a word: magnitudes and channel extremes are packed integer maxima, the
+// division by the scale and the rounding one conversion for two.  Elements past the largest that can be coded (infinities and NaN among them) are seen to where a
 // thread has met one.  Bound by memory, 2 bytes read and 1 written an element: 8 x 8 heads x 2048 rows x 128 20 us, 5.0 TB/s;
 // 4 x 8 heads x 8191 rows 43 us, 4.7 TB/s, what a copy gives.
 //

@@ -481,7 +481,8 @@ class QuantizedKVCache(_Cache):
 
 class BlockScaledKVCache(KVCacheSimple):
     """A `KVCacheSimple` to its caller that holds its rows in 8 bits: blocks of 64 positions of one kv head as e4m3 codes with
-    a power of two as their scale, the rows behind the last whole block as they came.  No counterpart in the reference.
+    a power of two as their scale, the rows behind the last whole block as they came.  `trim` takes rows off as if they had never been
+    written (include/kvhip.h: back to where).  No counterpart in the reference.
     float16 and bfloat16, head sizes up to 256.  `update` and `fetch` hand out the rows as they are held; `state` likewise."""
     kind = L.KIND_BLOCK_SCALED
     block_rows = 64
