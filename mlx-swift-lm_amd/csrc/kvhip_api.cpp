@@ -1756,6 +1756,22 @@ kvhip_status kvhip_cache_update_attend_blocks(kvhip_cache *c, const void *q, con
         return ok;
     }
     hipStream_t s = S(c, stream);
+    // (and all the memory is there before: a call that cannot have it -- under capture, say -- has done nothing)
+    {
+        BlockAttend plan;
+        plan.a.st = c->st;
+        plan.a.Hq = Hq;
+        plan.a.Hkv = c->Hkv;
+        plan.a.L = L;
+        plan.a.T = (int)T;
+        plan.list = blocks;
+        plan.count = count;
+        KV_TRY(ensure_ws(c, align256(plan_block_attend(plan)) + block_select_workspace(x), s));
+        if (c->padded()) {
+            KV_TRY(ensure_pad_buf(c, 2, (size_t)B * Hq * L * c->st.Dk * c->st.es));
+            KV_TRY(ensure_pad_buf(c, 3, (size_t)B * Hq * L * c->st.Dv * c->st.es));
+        }
+    }
     const bool fuse = block_step_fuses(c, L);
     KV_TRY(update_blocks(c, k, v, L, s, !fuse));
     x.b = block_store(c);

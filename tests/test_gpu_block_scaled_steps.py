@@ -175,6 +175,37 @@ def test_prompt_chunks_of_keys_of_192(dtype, n, heads, pads):
     check(cache.attend(qd, 0.07, mask), *exact_and_bound(q, oracle, 0.07, causal(730, n, pads)))
 
 
+@pytest.mark.parametrize("sizes", [(128, 128), (50, 36)])
+@pytest.mark.parametrize("n", [1, 3])
+def test_a_step_over_blocks_without_memory_has_done_nothing(sizes, n):
+    """Scratch that would have to grow while a stream is being captured: the call fails before it counts its rows in, and made
+    again outside it is what it would have been."""
+    hip = C.CDLL("libamdhip64.so")
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    _, k, v = heads_of(gen, BF16, 20000, sizes, (8, 2))
+    cache, other = kvhip.BlockScaledKVCache(), kvhip.BlockScaledKVCache()
+    cache.reserve(2, 2, sizes[0], sizes[1], BF16, 21000)
+    for c in (cache, other):
+        c.update(k, v, fetch=False)
+    q, k, v = heads_of(gen, BF16, n, sizes, (8, 2))
+    out, blocks = torch.empty(2, 8, n, sizes[1], dtype=BF16, device="cuda"), torch.empty(2, 2, n, 40, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    stream, graph = torch.cuda.Stream(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(C.c_void_p(stream.cuda_stream), 0) == 0
+    status = kvhip.load().kvhip_cache_update_attend_blocks(cache._h, q.data_ptr(), k.data_ptr(), v.data_ptr(), 2, 8, 2, n, sizes[0], sizes[1], L.BF16, 0.1,
+                                                           40, 1, 2, None, blocks.data_ptr(), out.data_ptr(), stream.cuda_stream)
+    hip.hipStreamEndCapture(C.c_void_p(stream.cuda_stream), C.byref(graph))
+    hip.hipGetLastError()
+    if status == 0:  # (memory of freed caches was at hand: a captured call like any other, not replayed)
+        cache.trim(n)
+    assert cache.offset == 20000
+    got, chosen = cache.update_attend_blocks(q, k, v, 0.1, 40, 1, 2)
+    want, same = other.update_attend_blocks(q, k, v, 0.1, 40, 1, 2)
+    assert torch.equal(got, want) and torch.equal(chosen, same)
+    for a, b in zip(cache.fetch(), other.fetch()):
+        assert torch.equal(a, b)
+
+
 # ---- scores far from zero -----------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("sizes", [(64, 64), (128, 128), (256, 256)])
