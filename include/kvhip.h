@@ -355,6 +355,77 @@ kvhip_status kvhip_cache_update_attend_blocks(kvhip_cache *cache, const void *qu
                                               int32_t dtype, float scale, int32_t count, int32_t first, int32_t recent,
                                               const int32_t *left_pad, int32_t *blocks, void *out, void *stream);
 
+/* ---- recurrent layers' state ----------------------------------------------- */
+/*
+ * Hybrid models put recurrent layers beside their attention layers; what those remember of a sequence is two dense arrays of
+ * fixed size (the reference keeps them in an ArraysCache / MambaCache, KVCache.swift:1307-1726): the last inputs of a short convolution
+ * and the state of the gated delta rule.  Both belong to the caller, who passes the old and the new one: the same array
+ * (updated in place) or two (the old one stays for a rejected draft); they overlap in no other way, and outputs overlap no input.
+ * Sequence b's tokens are those at left_pad[b] <= l < lengths[b] (device [B] or NULL: 0, L); the others are not there: they
+ * change no state, what stands in their place is never used, and their outputs are zero.
+ *
+ * y_l = f(bias + sum_w weight[:, w] e_{l + w}), by channel, e the window's W - 1 rows and then the sequence's tokens; f is x sigmoid(x)
+ * when `silu`.  The new window is the last W - 1 rows of e.  x [B,L,C], sequences and tokens x_stride_b / x_stride_l elements
+ * apart; weight [C,W], bias [C] or NULL, window [B,W-1,C], out [B,L,C], all of `dtype`, sums in float32.  window_in NULL: zeros.
+ * 1 <= W <= 8.
+ */
+kvhip_status kvhip_short_convolution(const void *x, int64_t x_stride_b, int64_t x_stride_l, const void *weight, const void *bias,
+                                     int32_t B, int32_t L, int32_t C, int32_t W, int32_t dtype, int32_t silu, const int32_t *left_pad,
+                                     const int32_t *lengths, const void *window_in, void *window_out, void *out, void *stream);
+/*
+ * The gated delta rule (`gatedDeltaUpdate`, GatedDelta.swift:112).  For each sequence and value head a state S [Dv,Dk] in float32,
+ * key head h / (Hv / Hk) serving value head h:
+ *     q^ = scale q / sqrt(sum q^2 + norm_eps),  k^ = k / sqrt(sum k^2 + norm_eps)      (norm_eps 0: q^ = scale q, k^ = k)
+ *     g = exp(-exp(a_log) softplus(a + dt_bias)),  beta = sigmoid(b)                   (a_log NULL: g = exp(a), beta = b)
+ *     S <- g S;  u = beta (v - S k^);  S <- S + u k^T;  out = S q^
+ * q, k [B,L,Hk,Dk] and v [B,L,Hv,Dv] of `dtype`: heads and channels dense, sequences and tokens by strides in elements, so that they may be
+ * parts of one array.  a, b [B,L,Hv] of gate_dtype, likewise.  a_log, dt_bias (or NULL) [Hv] float32.  state [B,Hv,Dv,Dk]
+ * float32 (state_in NULL: zeros), out [B,L,Hv,Dv] of `dtype`.  Dk up to 256.
+ * States, sums and decays are float32 (a prompt's decays are summed in float64); only outputs are rounded to `dtype`.
+ * `workspace`: device memory of kvhip_gated_delta_workspace bytes (16-byte aligned; NULL if that is 0), of no content before or after; calls that
+ * can overlap need one each.
+ */
+typedef struct kvhip_gated_delta_args {
+    const void *q, *k, *v, *a, *b;
+    int64_t q_stride_b, q_stride_l, k_stride_b, k_stride_l, v_stride_b, v_stride_l, a_stride_b, a_stride_l, b_stride_b, b_stride_l;
+    const float *a_log, *dt_bias;
+    const int32_t *left_pad, *lengths;
+    const float *state_in;
+    float *state_out;
+    void *out;
+    int32_t B, L, Hk, Hv, Dk, Dv;
+    int32_t dtype, gate_dtype;
+    float scale, norm_eps;
+} kvhip_gated_delta_args;
+size_t kvhip_gated_delta_workspace(const kvhip_gated_delta_args *args);
+kvhip_status kvhip_gated_delta(const kvhip_gated_delta_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- beam search ------------------------------------------------------------ */
+/*
+ * The `count` best continuations of each of `groups` groups of `beams` rows of logits [groups * beams, vocabulary] (rows `stride`
+ * elements apart).  Row r continued by token t scores scores[r] + x[r,t] - log sum_j exp x[r,j] (scores NULL: 0), in float64
+ * from float32 sums.  Best first; among equals the lower beam, then the higher logit, then the lower token.  A row whose `done` (bytes, or
+ * NULL) is set offers pad_token alone, at scores[r].  A logit that is no number counts as minus infinity, infinity as the
+ * largest float32; a score that is no number as minus infinity.  rows (numbers of logits rows: an order for kvhip_cache_reorder), tokens, best:
+ * [groups, count]; where fewer candidates are there, -1, -1 and minus infinity behind them.
+ * beams and count up to 64, groups * beams up to 65535.  `workspace`: device memory of kvhip_beam_select_workspace bytes, 16-byte
+ * aligned, of no content before or after; calls that can overlap need one each.
+ */
+size_t kvhip_beam_select_workspace(int32_t groups, int32_t beams, int32_t vocabulary, int32_t dtype, int32_t count);
+kvhip_status kvhip_beam_select(const void *logits, int64_t stride, int32_t groups, int32_t beams, int32_t vocabulary, int32_t dtype,
+                               const float *scores, const uint8_t *done, int32_t count, int32_t pad_token, int32_t *rows,
+                               int32_t *tokens, float *best, void *workspace, size_t workspace_bytes, void *stream);
+/*
+ * Batch row b of the cache becomes what row order[b] was (device [B] int32; an entry outside [0, B) leaves its row).  `shared`: leading
+ * positions that rows and those they take from are known to have in common (a prompt's): the tiles of 64 positions that lie
+ * wholly in them are not moved (a RotatingKVCache moves whatever it holds).  In place, without scratch; rows that
+ * stay are not touched.  B up to 2048.  KVHIP_ERR_STATE while a round is staged.
+ */
+kvhip_status kvhip_cache_reorder(kvhip_cache *cache, const int32_t *order, int64_t shared, void *stream);
+/* The same for up to 8 dense arrays of `rows` rows, row_bytes[i] bytes each (a recurrent layer's window and state). */
+kvhip_status kvhip_reorder_rows(int32_t count, void *const *arrays, const size_t *row_bytes, int32_t rows, const int32_t *order,
+                                void *stream);
+
 /* `makeMask(n:windowSize:returnArray:)`; window_size <= 0 stands for nil. */
 kvhip_status kvhip_cache_mask_plan(const kvhip_cache *cache, int32_t n, int32_t window_size,
                                    int32_t return_array, kvhip_mask_plan_t *out_plan);

@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "kvhip_block.hpp"
+#include "kvhip_delta.hpp"
 #include "kvhip_internal.hpp"
 
 using namespace kvhip;
@@ -1778,6 +1779,166 @@ kvhip_status kvhip_cache_update_attend_blocks(kvhip_cache *c, const void *q, con
     const kvhip_status st = attend_blocks_impl(c, q, B, Hq, L, Dk, scale, blocks, count, left_pad, out, fuse ? k : nullptr, fuse ? v : nullptr, s, &x);
     if (st != KVHIP_OK && fuse) cut_blocks(c, c->offset - 1);  // nothing was written: take the row back
     return st;
+}
+
+// ---- recurrent layers' state ------------------------------------------------------
+static bool float_dtype(int32_t dtype) { return dtype == KVHIP_F16 || dtype == KVHIP_BF16 || dtype == KVHIP_F32; }
+
+kvhip_status kvhip_short_convolution(const void *x, int64_t x_stride_b, int64_t x_stride_l, const void *weight, const void *bias, int32_t B,
+                                     int32_t L, int32_t C, int32_t W, int32_t dtype, int32_t silu, const int32_t *left_pad,
+                                     const int32_t *lengths, const void *window_in, void *window_out, void *out, void *stream) {
+    if (!x || !weight || !out) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
+    if (B <= 0 || L <= 0 || C <= 0 || W <= 0 || x_stride_b < 0 || x_stride_l < 0) return fail(KVHIP_ERR_INVALID_ARG, "non-positive shape");
+    if (W > 1 && !window_out) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
+    if (!float_dtype(dtype)) return fail(KVHIP_ERR_INVALID_ARG, "convolutions are float16, bfloat16 or float32");
+    if (W > 8) return fail(KVHIP_ERR_UNSUPPORTED, "convolutions of more than 8 taps");
+    if (B > 65535 || L > (1 << 20) || C > (1 << 28)) return fail(KVHIP_ERR_UNSUPPORTED, "more than 65535 sequences, 2^20 tokens or 2^28 channels");
+    ConvArgs a;
+    a.x = static_cast<const char *>(x);
+    a.x_sb = x_stride_b;
+    a.x_sl = x_stride_l;
+    a.weight = static_cast<const char *>(weight);
+    a.bias = static_cast<const char *>(bias);
+    a.left_pad = left_pad;
+    a.lengths = lengths;
+    a.window_in = static_cast<const char *>(window_in);
+    a.window_out = static_cast<char *>(window_out);
+    a.out = static_cast<char *>(out);
+    a.B = B;
+    a.L = L;
+    a.C = C;
+    a.W = W;
+    a.dtype = dtype;
+    a.silu = silu != 0;
+    KV_HIP(launch_short_conv(a, S(stream)));
+    return KVHIP_OK;
+}
+
+static kvhip_status delta_args(const kvhip_gated_delta_args *p, DeltaArgs &x) {
+    if (!p) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
+    if (!p->q || !p->k || !p->v || !p->a || !p->b || !p->state_out || !p->out) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
+    if (p->B <= 0 || p->L <= 0 || p->Hk <= 0 || p->Hv <= 0 || p->Dk <= 0 || p->Dv <= 0) return fail(KVHIP_ERR_INVALID_ARG, "non-positive shape");
+    for (int64_t s : {p->q_stride_b, p->q_stride_l, p->k_stride_b, p->k_stride_l, p->v_stride_b, p->v_stride_l, p->a_stride_b, p->a_stride_l,
+                      p->b_stride_b, p->b_stride_l})
+        if (s < 0) return fail(KVHIP_ERR_INVALID_ARG, "negative stride");
+    if (p->Hv % p->Hk) return fail(KVHIP_ERR_INVALID_ARG, "value heads are no multiple of key heads");
+    if (!float_dtype(p->dtype) || !float_dtype(p->gate_dtype)) return fail(KVHIP_ERR_INVALID_ARG, "the gated delta rule takes float16, bfloat16 or float32");
+    if (!(p->norm_eps >= 0.f)) return fail(KVHIP_ERR_INVALID_ARG, "norm_eps is negative");
+    if (p->Dk > 256) return fail(KVHIP_ERR_UNSUPPORTED, "the gated delta rule takes keys of up to 256 channels");
+    if (p->B > 65535 || p->Hv > 65535 || p->L > (1 << 24) || p->Dv > (1 << 20))
+        return fail(KVHIP_ERR_UNSUPPORTED, "more than 65535 sequences or heads, 2^24 tokens or 2^20 value channels");
+    x.q = static_cast<const char *>(p->q);
+    x.k = static_cast<const char *>(p->k);
+    x.v = static_cast<const char *>(p->v);
+    x.a = static_cast<const char *>(p->a);
+    x.b = static_cast<const char *>(p->b);
+    x.q_sb = p->q_stride_b, x.q_sl = p->q_stride_l, x.k_sb = p->k_stride_b, x.k_sl = p->k_stride_l, x.v_sb = p->v_stride_b, x.v_sl = p->v_stride_l;
+    x.a_sb = p->a_stride_b, x.a_sl = p->a_stride_l, x.b_sb = p->b_stride_b, x.b_sl = p->b_stride_l;
+    x.a_log = p->a_log;
+    x.dt_bias = p->dt_bias;
+    x.left_pad = p->left_pad;
+    x.lengths = p->lengths;
+    x.state_in = p->state_in;
+    x.state_out = p->state_out;
+    x.out = static_cast<char *>(p->out);
+    x.B = p->B, x.L = p->L, x.Hk = p->Hk, x.Hv = p->Hv, x.Dk = p->Dk, x.Dv = p->Dv;
+    x.dtype = p->dtype, x.gate_dtype = p->gate_dtype;
+    x.scale = p->scale, x.eps = p->norm_eps;
+    return KVHIP_OK;
+}
+size_t kvhip_gated_delta_workspace(const kvhip_gated_delta_args *p) {
+    (void)p;
+    return 0;
+}
+kvhip_status kvhip_gated_delta(const kvhip_gated_delta_args *p, void *workspace, size_t workspace_bytes, void *stream) {
+    DeltaArgs x;
+    KV_TRY(delta_args(p, x));
+    (void)workspace, (void)workspace_bytes;
+    KV_HIP(launch_delta_steps(x, S(stream)));
+    return KVHIP_OK;
+}
+
+// ---- beam search --------------------------------------------------------------------
+static kvhip_status beam_args(int32_t groups, int32_t beams, int32_t vocabulary, int32_t dtype, int32_t count, BeamArgs &x) {
+    if (groups <= 0 || beams <= 0 || vocabulary <= 0 || count <= 0) return fail(KVHIP_ERR_INVALID_ARG, "non-positive shape");
+    if (!float_dtype(dtype)) return fail(KVHIP_ERR_INVALID_ARG, "logits are float16, bfloat16 or float32");
+    if (beams > 64 || count > 64 || (int64_t)groups * beams > 65535)
+        return fail(KVHIP_ERR_UNSUPPORTED, "more than 64 beams or candidates, or 65535 rows");
+    if (vocabulary > (1 << 24)) return fail(KVHIP_ERR_UNSUPPORTED, "a vocabulary of more than 2^24");
+    x.groups = groups;
+    x.beams = beams;
+    x.vocabulary = vocabulary;
+    x.dtype = dtype;
+    x.count = count;
+    return KVHIP_OK;
+}
+size_t kvhip_beam_select_workspace(int32_t groups, int32_t beams, int32_t vocabulary, int32_t dtype, int32_t count) {
+    BeamArgs x;
+    return beam_args(groups, beams, vocabulary, dtype, count, x) == KVHIP_OK ? beam_workspace(x) : 0;
+}
+kvhip_status kvhip_beam_select(const void *logits, int64_t stride, int32_t groups, int32_t beams, int32_t vocabulary, int32_t dtype,
+                               const float *scores, const uint8_t *done, int32_t count, int32_t pad_token, int32_t *rows, int32_t *tokens,
+                               float *best, void *workspace, size_t workspace_bytes, void *stream) {
+    BeamArgs x;
+    KV_TRY(beam_args(groups, beams, vocabulary, dtype, count, x));
+    if (!logits || !rows || !tokens || !best || !workspace) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
+    if (stride < 0) return fail(KVHIP_ERR_INVALID_ARG, "negative stride");
+    if (done && (pad_token < 0 || pad_token >= vocabulary)) return fail(KVHIP_ERR_INVALID_ARG, "pad_token lies outside the vocabulary");
+    if (workspace_bytes < beam_workspace(x) || (uintptr_t)workspace % 16) return fail(KVHIP_ERR_INVALID_ARG, "workspace too small or not 16-byte aligned");
+    x.logits = static_cast<const char *>(logits);
+    x.stride = stride;
+    x.scores = scores;
+    x.done = done;
+    x.pad_token = pad_token;
+    x.rows = rows;
+    x.tokens = tokens;
+    x.best = best;
+    KV_HIP(launch_beam_select(x, workspace, S(stream)));
+    return KVHIP_OK;
+}
+
+kvhip_status kvhip_reorder_rows(int32_t count, void *const *arrays, const size_t *row_bytes, int32_t rows, const int32_t *order, void *stream) {
+    if (count < 0 || rows <= 0 || !order || (count > 0 && (!arrays || !row_bytes))) return fail(KVHIP_ERR_INVALID_ARG, "null argument or non-positive shape");
+    if (count > REORDER_ARRAYS || rows > REORDER_ROWS) return fail(KVHIP_ERR_UNSUPPORTED, "more than 8 arrays or 2048 rows");
+    ReorderArrays x;
+    x.n = count;
+    for (int i = 0; i < count; ++i) {
+        if (!arrays[i]) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
+        if (row_bytes[i] > ((size_t)1 << 32)) return fail(KVHIP_ERR_UNSUPPORTED, "rows of more than 4 GiB");
+        x.at[i] = static_cast<char *>(arrays[i]);
+        x.bytes[i] = row_bytes[i];
+    }
+    KV_HIP(launch_reorder_arrays(x, rows, order, S(stream)));
+    return KVHIP_OK;
+}
+kvhip_status kvhip_cache_reorder(kvhip_cache *c, const int32_t *order, int64_t shared, void *stream) {
+    if (!c || !order || shared < 0) return fail(KVHIP_ERR_INVALID_ARG, "null argument or negative number of shared positions");
+    if (c->staging) return fail(KVHIP_ERR_STATE, "a cache cannot be reordered while a round is staged");
+    if (!c->has_geom || !c->has_buffers) return KVHIP_OK;
+    if (c->B > REORDER_ROWS) return fail(KVHIP_ERR_UNSUPPORTED, "more than 2048 sequences");
+    hipStream_t s = S(c, stream);
+    int64_t rows = std::max(c->offset, c->presented);
+    if (c->kind == KVHIP_KIND_ROTATING) {
+        shared = rows = 0;
+        for (int32_t slot : c->rows) rows = std::max<int64_t>(rows, slot + 1);
+    }
+    rows = std::min(rows, c->cap_slots());
+    if (shared < rows) KV_HIP(launch_reorder_pages(c->st, c->Hkv, (int)(shared / TILE), (int)((rows + TILE - 1) / TILE), order, s));
+    if (c->kind == KVHIP_KIND_BLOCK_SCALED && c->tail) {
+        ReorderArrays x;
+        for (int i = 0; i < BLOCK_KEPT; ++i) {
+            if (c->kept[i].block < 0) continue;
+            char *k, *v;
+            tail_at(c, i, k, v);
+            const size_t pair = (size_t)c->Hkv * BLOCK_ROWS * c->st.es;
+            x.at[x.n] = k;
+            x.bytes[x.n++] = pair * c->st.Dk;
+            x.at[x.n] = v;
+            x.bytes[x.n++] = pair * c->st.Dv;
+        }
+        KV_HIP(launch_reorder_arrays(x, c->B, order, s));
+    }
+    return KVHIP_OK;
 }
 
 kvhip_status kvhip_cache_mask_plan(const kvhip_cache *c, int32_t n, int32_t window, int32_t return_array,

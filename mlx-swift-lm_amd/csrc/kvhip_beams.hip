@@ -1,0 +1,491 @@
+// Beam search: the selection over beams and vocabulary, and the rows of caches trading places by what it selects.
+//
+// The selection reads the logits once.  beam_rows_kernel: a workgroup holds a segment of one row in registers, takes its maximum
+// M and sum exp(x - M), and the `count` best of it.  A wavefront's count-th largest lane maximum is a bound that at least `count` of its
+// elements reach (found bit by bit by counting lanes, in whole numbers that are ordered as the values are); the largest of the
+// wavefronts' bounds leaves hardly more than `count` elements of the segment, which are put down in LDS and ranked against one
+// another by value, then index.  beam_merge_kernel does the same for a batch row's candidates by their scores,
+//   s[beam] + ((x - M) - log sum),
+// in 64 bits, so that a sum's rounding does not decide between beams.  Where a list would overflow (thousands of equal values)
+// the best is taken out `count` times instead.
+#include "kvhip_delta.hpp"
+#include "kvhip_device.hpp"
+#include "kvhip_wave.hpp"
+
+namespace kvhip {
+namespace {
+
+typedef float kv_f4 __attribute__((ext_vector_type(4)));
+
+constexpr int BEAM_LIST = 512;  // elements that are ranked
+constexpr float NEVER = -__builtin_inff();
+
+// whole numbers in the order of the values (no NaN)
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t u = __float_as_uint(v + 0.f);  // (-0 as 0)
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+// the largest whole number that at least `count` (1 to 64) of the wavefront's lanes reach
+__device__ __forceinline__ uint32_t reached(uint32_t key, int count) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t up = t | (1u << bit);
+        if (__popcll(__ballot(key >= up)) >= count) t = up;
+    }
+    return t;
+}
+// a logit as it counts: what is no number never, infinity as the largest number
+__device__ __forceinline__ float logit(float v) { return v != v ? NEVER : fminf(v, 3.4028234663852886e38f); }
+
+// Scratch: for each row and segment its `count` best (value, index; -1 behind the last) and (maximum, sum).
+struct BeamScratch {
+    float *value;
+    int32_t *index;
+    float2 *sums;
+    int32_t segments, segment;
+};
+__host__ __device__ inline int64_t beam_at(const BeamScratch &w, int64_t row, int seg) { return row * w.segments + seg; }
+
+template <int NV> constexpr int beam_segment(int vec) { return 256 * NV * vec; }
+
+// NV: 16-byte vectors to a thread
+template <int DT, int NV, bool WIDE>
+__global__ void __launch_bounds__(256) beam_rows_kernel(BeamArgs x, BeamScratch w) {
+    constexpr int VEC = DT == 2 ? 4 : 8, ES = DT == 2 ? 4 : 2, E = NV * VEC;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seg = blockIdx.x;
+    const int64_t row = blockIdx.y, at = beam_at(w, row, seg);
+    const int count = x.count;
+    __shared__ uint32_t wave_key[4];
+    __shared__ float wave_top[4], wave_sum4s[4];
+    __shared__ float list_v[BEAM_LIST];
+    __shared__ int32_t list_i[BEAM_LIST];
+    __shared__ int listed;
+    float *value = w.value + at * count;
+    int32_t *index = w.index + at * count;
+    if (x.done && x.done[row]) {  // one candidate, of the score that the beam has
+        if (tid < count) {
+            value[tid] = seg == 0 && tid == 0 ? 0.f : NEVER;
+            index[tid] = seg == 0 && tid == 0 ? x.pad_token : -1;
+        }
+        if (tid == 0) w.sums[at] = make_float2(0.f, seg == 0 ? 1.f : 0.f);
+        return;
+    }
+    const char *p = x.logits + row * x.stride * ES;
+    const int base = seg * w.segment;
+    float v[E];
+    if (tid == 0) listed = 0;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+        const int i = base + (n * 256 + tid) * VEC;
+        if (WIDE && i + VEC <= x.vocabulary) {
+            const kv_u4 u = *reinterpret_cast<const kv_u4 *>(p + (int64_t)i * ES);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                if constexpr (DT == 2) {
+                    v[n * 4 + m] = logit(__uint_as_float(u[m]));
+                } else if constexpr (DT == 1) {
+                    v[n * 8 + 2 * m] = logit(__uint_as_float(u[m] << 16));
+                    v[n * 8 + 2 * m + 1] = logit(__uint_as_float(u[m] & 0xffff0000u));
+                } else {
+                    const kv_h2 h = as_h2(u[m]);
+                    v[n * 8 + 2 * m] = logit((float)h.x);
+                    v[n * 8 + 2 * m + 1] = logit((float)h.y);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int m = 0; m < VEC; ++m) v[n * VEC + m] = i + m < x.vocabulary ? logit(Elem<DT>::load(p, i + m)) : NEVER;
+        }
+    }
+    float top = NEVER;
+#pragma unroll
+    for (int e = 0; e < E; ++e) top = fmaxf(top, v[e]);
+    const uint32_t bound = reached(ordered(top), count);
+    const float wtop = wave_max(top);
+    if (lane == 0) {
+        wave_key[wave] = bound;
+        wave_top[wave] = wtop;
+    }
+    __syncthreads();
+    const uint32_t least = max(max(wave_key[0], wave_key[1]), max(wave_key[2], wave_key[3]));
+    const float all = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
+    float sum = 0.f;
+    if (all != NEVER) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum += fast_exp2((v[e] - all) * LOG2E);
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) wave_sum4s[wave] = sum;
+    if (ordered(top) >= least) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (ordered(v[e]) >= least) {
+                const int i = base + ((e / VEC) * 256 + tid) * VEC + e % VEC;
+                if (i < x.vocabulary) {
+                    const int n = atomicAdd(&listed, 1);
+                    if (n < BEAM_LIST) {
+                        list_v[n] = v[e];
+                        list_i[n] = i;
+                    }
+                }
+            }
+    }
+    __syncthreads();
+    const int n = listed;
+    if (tid == 0) w.sums[at] = make_float2(all, wave_sum4s[0] + wave_sum4s[1] + wave_sum4s[2] + wave_sum4s[3]);
+    if (n <= BEAM_LIST) {
+        for (int i = tid; i < n; i += 256) {
+            const float mine = list_v[i];
+            const int32_t id = list_i[i];
+            int rank = 0;
+            for (int m = 0; m < n; ++m) rank += list_v[m] > mine || (list_v[m] == mine && list_i[m] < id);
+            if (rank < count) {
+                value[rank] = mine;
+                index[rank] = id;
+            }
+        }
+        for (int i = n + tid; i < count; i += 256) {
+            value[i] = NEVER;
+            index[i] = -1;
+        }
+        return;
+    }
+    // thousands of equal values: the best behind the last one taken, `count` times
+    float last_v = __builtin_inff();
+    int32_t last_i = -1;
+    for (int c = 0; c < count; ++c) {
+        float best = NEVER;
+        int32_t id = 0x7fffffff;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int i = base + ((e / VEC) * 256 + tid) * VEC + e % VEC;
+            const bool behind = v[e] < last_v || (v[e] == last_v && i > last_i);
+            if (i < x.vocabulary && behind && (v[e] > best || (v[e] == best && i < id))) {
+                best = v[e];
+                id = i;
+            }
+        }
+        __syncthreads();
+        list_v[tid] = best;
+        list_i[tid] = id;
+        __syncthreads();
+        for (int half = 128; half > 0; half >>= 1) {
+            if (tid < half) {
+                const float o = list_v[tid + half];
+                const int32_t oi = list_i[tid + half];
+                if (o > list_v[tid] || (o == list_v[tid] && oi < list_i[tid])) {
+                    list_v[tid] = o;
+                    list_i[tid] = oi;
+                }
+            }
+            __syncthreads();
+        }
+        last_v = list_v[0];
+        last_i = list_i[0];
+        if (tid == 0) {
+            value[c] = last_v;
+            index[c] = last_i;
+        }
+    }
+}
+
+// A candidate of the merge, and whether it comes before another.
+struct Candidate {
+    double score;
+    float value;
+    int32_t beam, token;
+};
+__device__ __forceinline__ bool before(const Candidate &a, const Candidate &b) {
+    if (a.score != b.score) return a.score > b.score;
+    if (a.beam != b.beam) return a.beam < b.beam;
+    if (a.value != b.value) return a.value > b.value;
+    return a.token < b.token;
+}
+
+constexpr int MERGE_THREADS = 256, MERGE_BEAMS = 64;
+__global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(BeamArgs x, BeamScratch w) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = blockIdx.x, count = x.count;
+    __shared__ double beam_score[MERGE_BEAMS], beam_log[MERGE_BEAMS];
+    __shared__ float beam_top[MERGE_BEAMS];
+    __shared__ uint32_t wave_key[4];
+    __shared__ double list_s[BEAM_LIST];
+    __shared__ float list_v[BEAM_LIST];
+    __shared__ int32_t list_b[BEAM_LIST], list_t[BEAM_LIST];
+    __shared__ int listed;
+    if (tid == 0) listed = 0;
+    if (tid < x.beams) {
+        const int64_t row = (int64_t)g * x.beams + tid;
+        float top = NEVER;
+        for (int s = 0; s < w.segments; ++s) top = fmaxf(top, w.sums[beam_at(w, row, s)].x);
+        if (x.done && x.done[row]) top = 0.f;
+        double sum = 0.;
+        for (int s = 0; s < w.segments; ++s) {
+            const float2 t = w.sums[beam_at(w, row, s)];
+            if (t.x != NEVER) sum += (double)t.y * exp((double)t.x - (double)top);
+        }
+        const float own = x.scores ? x.scores[row] : 0.f;
+        // (a beam none of whose tokens counts, or whose score is no number: candidates that come last)
+        beam_score[tid] = own == own && top != NEVER ? (double)own : -__builtin_inf();
+        beam_top[tid] = top;
+        beam_log[tid] = log(sum);
+    }
+    __syncthreads();
+    const int per = w.segments * count, total = x.beams * per;
+    const int64_t first = (int64_t)g * x.beams * per;
+    auto candidate = [&](int i) {
+        Candidate c;
+        c.beam = i / per;
+        c.value = w.value[first + i];
+        c.token = w.index[first + i];
+        const double own = beam_score[c.beam];
+        // (the difference first: a logit may be so large that the others are lost in it)
+        c.score = own == -__builtin_inf() || c.value == NEVER ? -__builtin_inf() : own + (((double)c.value - (double)beam_top[c.beam]) - beam_log[c.beam]);
+        return c;
+    };
+    // scores for the bound, in 32 bits: rounding keeps their order
+    uint32_t top = 0;
+    for (int i = tid; i < total; i += MERGE_THREADS) {
+        const Candidate c = candidate(i);
+        if (c.token >= 0) top = max(top, ordered((float)c.score));
+    }
+    const uint32_t bound = reached(top, count);
+    if (lane == 0) wave_key[wave] = bound;
+    __syncthreads();
+    const uint32_t least = max(max(wave_key[0], wave_key[1]), max(wave_key[2], wave_key[3]));
+    if (top >= least) {
+        for (int i = tid; i < total; i += MERGE_THREADS) {
+            const Candidate c = candidate(i);
+            if (c.token < 0 || ordered((float)c.score) < least) continue;
+            const int n = atomicAdd(&listed, 1);
+            if (n < BEAM_LIST) {
+                list_s[n] = c.score;
+                list_v[n] = c.value;
+                list_b[n] = c.beam;
+                list_t[n] = c.token;
+            }
+        }
+    }
+    __syncthreads();
+    const int n = listed;
+    auto put = [&](int at, const Candidate &c) {
+        const int64_t o = (int64_t)g * count + at;
+        x.rows[o] = g * x.beams + c.beam;
+        x.tokens[o] = c.token;
+        x.best[o] = (float)c.score;
+    };
+    auto held = [&](int i) { return Candidate{list_s[i], list_v[i], list_b[i], list_t[i]}; };
+    if (n <= BEAM_LIST) {
+        for (int i = tid; i < n; i += MERGE_THREADS) {
+            const Candidate mine = held(i);
+            int rank = 0;
+            for (int m = 0; m < n; ++m) rank += before(held(m), mine);
+            if (rank < count) put(rank, mine);
+        }
+        for (int i = n + tid; i < count; i += MERGE_THREADS) {
+            const int64_t o = (int64_t)g * count + i;
+            x.rows[o] = x.tokens[o] = -1;
+            x.best[o] = NEVER;
+        }
+        return;
+    }
+    Candidate last{__builtin_inf(), __builtin_inff(), -1, -1};
+    for (int c = 0; c < count; ++c) {
+        Candidate best{-__builtin_inf(), NEVER, 0x7fffffff, 0x7fffffff};
+        for (int i = tid; i < total; i += MERGE_THREADS) {
+            const Candidate o = candidate(i);
+            if (o.token >= 0 && before(last, o) && before(o, best)) best = o;
+        }
+        __syncthreads();
+        list_s[tid] = best.score;
+        list_v[tid] = best.value;
+        list_b[tid] = best.beam;
+        list_t[tid] = best.token;
+        __syncthreads();
+        for (int half = MERGE_THREADS / 2; half > 0; half >>= 1) {
+            if (tid < half && before(held(tid + half), held(tid))) {
+                list_s[tid] = list_s[tid + half];
+                list_v[tid] = list_v[tid + half];
+                list_b[tid] = list_b[tid + half];
+                list_t[tid] = list_t[tid + half];
+            }
+            __syncthreads();
+        }
+        last = held(0);
+        if (tid == 0) put(c, last);
+    }
+}
+
+// 16-byte vectors to a thread: the fewest that leave the chip four workgroups a compute unit, at most 8 (float32: 16, the same elements)
+inline int beam_vectors(const BeamArgs &x) {
+    const int vec = x.dtype == KVHIP_F32 ? 4 : 8;
+    const int64_t rows = (int64_t)x.groups * x.beams;
+    int nv = 8;
+    while (nv > 1 && rows * ((x.vocabulary + 256 * nv * vec - 1) / (256 * nv * vec)) < 1024) nv >>= 1;
+    return nv;
+}
+inline BeamScratch beam_scratch(const BeamArgs &x, void *workspace, size_t *bytes) {
+    const int vec = x.dtype == KVHIP_F32 ? 4 : 8;
+    BeamScratch w;
+    w.segment = 256 * beam_vectors(x) * vec;
+    w.segments = (int32_t)(((int64_t)x.vocabulary + w.segment - 1) / w.segment);
+    const size_t parts = (size_t)x.groups * x.beams * w.segments;
+    char *p = static_cast<char *>(workspace);
+    w.sums = reinterpret_cast<float2 *>(p);
+    w.value = reinterpret_cast<float *>(p + parts * sizeof(float2));
+    w.index = reinterpret_cast<int32_t *>(w.value + parts * x.count);
+    if (bytes) *bytes = parts * (sizeof(float2) + x.count * 8);
+    return w;
+}
+
+// ---- rows that trade places -----------------------------------------------------------------------------------------
+// A workgroup holds one piece of every row that moves: all of them are read before any is written, so no row needs a second
+// place, and a row that several take is read once from memory.  Rows that stay are not touched.
+constexpr int REORDER_REGS = 8, REORDER_THREADS = 256;
+static_assert(REORDER_REGS * REORDER_THREADS == REORDER_ROWS, "a unit of every row to a workgroup at least");
+
+// units of U in [0, n) of each row, `stride` bytes apart; rows * n <= REORDER_ROWS
+template <class U> __device__ __forceinline__ void reorder_piece(char *base, uint64_t stride, int n, int rows, const int32_t *order) {
+    U held[REORDER_REGS];
+    bool moves[REORDER_REGS];
+#pragma unroll
+    for (int r = 0; r < REORDER_REGS; ++r) {
+        const int i = r * REORDER_THREADS + threadIdx.x, row = i / n;
+        moves[r] = false;
+        if (row >= rows) continue;
+        const int32_t from = order[row];
+        moves[r] = from != row && from >= 0 && from < rows;
+        if (moves[r]) held[r] = *reinterpret_cast<const U *>(base + (uint64_t)from * stride + (uint64_t)(i - row * n) * sizeof(U));
+    }
+    // (what another wavefront stores below must not overtake a load in flight)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < REORDER_REGS; ++r) {
+        const int i = r * REORDER_THREADS + threadIdx.x, row = i / n;
+        if (moves[r]) *reinterpret_cast<U *>(base + (uint64_t)row * stride + (uint64_t)(i - row * n) * sizeof(U)) = held[r];
+    }
+}
+// units of every row that a piece has: whole rows of workgroups' threads where it can
+__host__ __device__ inline int reorder_units(int rows) {
+    int n = REORDER_ROWS / rows;
+    for (int p = REORDER_ROWS; p > 1; p >>= 1)  // (a power of two: pieces then start on whole lines)
+        if (p <= n) return p;
+    return 1;
+}
+
+struct ReorderFlat {
+    ReorderArrays x;
+    uint32_t first[REORDER_ARRAYS + 1];  // pieces before each array's
+};
+template <class U> __global__ void __launch_bounds__(REORDER_THREADS) reorder_arrays_kernel(ReorderFlat f, int rows, const int32_t *order) {
+    int a = 0;
+    while (a + 1 < f.x.n && blockIdx.x >= f.first[a + 1]) ++a;
+    const int n = reorder_units(rows);
+    const uint64_t at = (uint64_t)(blockIdx.x - f.first[a]) * n, units = f.x.bytes[a] / sizeof(U);
+    if (at >= units) return;
+    reorder_piece<U>(f.x.at[a] + at * sizeof(U), f.x.bytes[a], (int)min((uint64_t)n, units - at), rows, order);
+}
+
+// planes: 0 K, 1 V, 2 K's pairs or scales, 3 V's pairs or extremes
+template <class U>
+__global__ void __launch_bounds__(REORDER_THREADS) reorder_pages_kernel(Store st, int Hkv, int tile0, int planes, const int32_t *order) {
+    const int tile = tile0 + blockIdx.y, h = blockIdx.z % Hkv;
+    int plane = 0;
+    for (int skip = blockIdx.z / Hkv;; ++plane) {  // the skip-th plane of the mask
+        if (!(planes >> plane & 1)) continue;
+        if (skip-- == 0) break;
+    }
+    const PageEntry e = st.pt[tile / (PAGE / TILE)];
+    const uint32_t cell = plane == 0 ? st.k_cell : plane == 1 ? st.v_cell : plane == 2 ? st.ksb_cell : st.vsb_cell;
+    char *base = plane == 0 ? e.k : plane == 1 ? e.v : plane == 2 ? e.ksb : e.vsb;
+    const uint32_t part = cell / (PAGE / TILE), units = part / sizeof(U);
+    const int rows = st.BH / Hkv, n = reorder_units(rows);
+    const uint32_t at = blockIdx.x * n;
+    if (at >= units) return;
+    base += (uint64_t)h * cell + (uint64_t)(tile % (PAGE / TILE)) * part + (uint64_t)at * sizeof(U);
+    reorder_piece<U>(base, (uint64_t)Hkv * cell, (int)min((uint32_t)n, units - at), rows, order);
+}
+
+}  // namespace
+
+size_t beam_workspace(const BeamArgs &x) {
+    size_t bytes = 0;
+    beam_scratch(x, nullptr, &bytes);
+    return bytes;
+}
+
+hipError_t launch_beam_select(const BeamArgs &x, void *workspace, hipStream_t s) {
+    const BeamScratch w = beam_scratch(x, workspace, nullptr);
+    const int nv = beam_vectors(x), es = x.dtype == KVHIP_F32 ? 4 : 2;
+    const bool wide = ((uintptr_t)x.logits | (uint64_t)(x.stride * es)) % 16 == 0;
+    const dim3 grid(w.segments, x.groups * x.beams), block(256);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, x, w); };
+#define KV_GO(DT, NV) (wide ? go(beam_rows_kernel<DT, NV, true>) : go(beam_rows_kernel<DT, NV, false>))
+#define KV_SIZE(DT) (nv == 8 ? KV_GO(DT, 8) : nv == 4 ? KV_GO(DT, 4) : nv == 2 ? KV_GO(DT, 2) : KV_GO(DT, 1))
+    if (x.dtype == KVHIP_F16) KV_SIZE(0);
+    else if (x.dtype == KVHIP_BF16) KV_SIZE(1);
+    else KV_SIZE(2);
+#undef KV_SIZE
+#undef KV_GO
+    hipLaunchKernelGGL(beam_merge_kernel, dim3(x.groups), dim3(MERGE_THREADS), 0, s, x, w);
+    return hipGetLastError();
+}
+
+hipError_t launch_reorder_arrays(const ReorderArrays &x, int rows, const int32_t *order, hipStream_t s) {
+    // one launch for the arrays of whole 16-byte units, one each for those of 4, 2 and 1 bytes
+    for (int unit : {16, 4, 2, 1}) {
+        ReorderFlat f{};
+        uint64_t pieces = 0;
+        for (int i = 0; i < x.n; ++i) {
+            const uint64_t low = (uintptr_t)x.at[i] | x.bytes[i];
+            const int own = low % 16 == 0 ? 16 : low % 4 == 0 ? 4 : low % 2 == 0 ? 2 : 1;
+            if (own != unit || x.bytes[i] == 0) continue;
+            const uint64_t units = x.bytes[i] / unit, n = reorder_units(rows);
+            f.first[f.x.n] = (uint32_t)pieces;
+            f.x.at[f.x.n] = x.at[i];
+            f.x.bytes[f.x.n++] = x.bytes[i];
+            pieces += (units + n - 1) / n;
+        }
+        if (f.x.n == 0) continue;
+        if (pieces > 0x7fffffffu) return hipErrorInvalidValue;
+        f.first[f.x.n] = (uint32_t)pieces;
+        const dim3 grid((unsigned)pieces), block(REORDER_THREADS);
+        if (unit == 16) hipLaunchKernelGGL((reorder_arrays_kernel<kv_u4>), grid, block, 0, s, f, rows, order);
+        else if (unit == 4) hipLaunchKernelGGL((reorder_arrays_kernel<uint32_t>), grid, block, 0, s, f, rows, order);
+        else if (unit == 2) hipLaunchKernelGGL((reorder_arrays_kernel<uint16_t>), grid, block, 0, s, f, rows, order);
+        else hipLaunchKernelGGL((reorder_arrays_kernel<uint8_t>), grid, block, 0, s, f, rows, order);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+hipError_t launch_reorder_pages(const Store &st, int Hkv, int tile0, int tile1, const int32_t *order, hipStream_t s) {
+    if (tile1 <= tile0) return hipSuccess;
+    const int rows = st.BH / Hkv, n = reorder_units(rows);
+    const uint32_t cells[4] = {st.k_cell, st.v_cell, st.ksb_cell, st.vsb_cell};
+    for (int unit : {16, 4}) {  // (a block-scaled cache's scales are 8 bytes to a tile)
+        int planes = 0, number = 0;
+        uint32_t most = 0;
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t part = cells[i] / (PAGE / TILE);
+            if (part == 0 || (part % 16 == 0) != (unit == 16)) continue;
+            planes |= 1 << i;
+            ++number;
+            most = part > most ? part : most;
+        }
+        if (!number) continue;
+        // (65535 tiles to a launch: the grid's limit)
+        for (int t = tile0; t < tile1; t += 65535) {
+            const dim3 grid((most / unit + n - 1) / n, tile1 - t < 65535 ? tile1 - t : 65535, Hkv * number), block(REORDER_THREADS);
+            if (unit == 16) hipLaunchKernelGGL((reorder_pages_kernel<kv_u4>), grid, block, 0, s, st, Hkv, t, planes, order);
+            else hipLaunchKernelGGL((reorder_pages_kernel<uint32_t>), grid, block, 0, s, st, Hkv, t, planes, order);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+    }
+    return hipSuccess;
+}
+
+}  // namespace kvhip

@@ -13,3 +13,5 @@ from .rounds import (AppendOnlyRoundStrategy, KVCacheRound, KVCacheRoundCommit, 
 from .rope import RoPE, apply_rotary_position, attention_with_rope_and_cache_update  # noqa: F401
 from .prefill import PrefillParameters  # noqa: F401
 from .prompt_cache import KVCacheError, load_prompt_cache, save_prompt_cache  # noqa: F401
+from .recurrent import GatedDeltaCache, causal_convolution, gated_delta_update  # noqa: F401
+from .beams import beam_select  # noqa: F401

@@ -46,8 +46,16 @@ class MaskPlan(C.Structure):
                 ("roll_shift", C.c_int32), ("roll_window", C.c_int32)]
 
 
+class GatedDelta(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "a", "b")] +
+                [(f"{n}_stride_{x}", C.c_int64) for n in ("q", "k", "v", "a", "b") for x in ("b", "l")] +
+                [(n, C.c_void_p) for n in ("a_log", "dt_bias", "left_pad", "lengths", "state_in", "state_out", "out")] +
+                [(n, C.c_int32) for n in ("B", "L", "Hk", "Hv", "Dk", "Dv", "dtype", "gate_dtype")] +
+                [("scale", C.c_float), ("norm_eps", C.c_float)])
+
+
 # name -> (restype, argtypes); every symbol include/kvhip.h declares
-_P, _I32, _I64, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_float
+_P, _I32, _I64, _F, _SZ = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
 SIGNATURES = {
     "kvhip_version": (C.c_char_p, []),
     "kvhip_last_error_message": (C.c_char_p, []),
@@ -88,6 +96,13 @@ SIGNATURES = {
     "kvhip_cache_attend_blocks": (_I32, [_P, _P, _I32, _I32, _I32, _I32, _F, _P, _I32, _P, _P, _P]),
     "kvhip_cache_update_attend_blocks": (_I32, [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F, _I32, _I32, _I32,
                                                 _P, _P, _P, _P]),
+    "kvhip_short_convolution": (_I32, [_P, _I64, _I64, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P]),
+    "kvhip_gated_delta_workspace": (_SZ, [C.POINTER(GatedDelta)]),
+    "kvhip_gated_delta": (_I32, [C.POINTER(GatedDelta), _P, _SZ, _P]),
+    "kvhip_beam_select_workspace": (_SZ, [_I32, _I32, _I32, _I32, _I32]),
+    "kvhip_beam_select": (_I32, [_P, _I64, _I32, _I32, _I32, _I32, _P, _P, _I32, _I32, _P, _P, _P, _P, _SZ, _P]),
+    "kvhip_cache_reorder": (_I32, [_P, _P, _I64, _P]),
+    "kvhip_reorder_rows": (_I32, [_I32, C.POINTER(_P), C.POINTER(_SZ), _I32, _P, _P]),
     "kvhip_cache_mask_plan": (_I32, [_P, _I32, _I32, _I32, C.POINTER(MaskPlan)]),
     "kvhip_mask_materialize": (_I32, [C.POINTER(MaskPlan), _P, _P]),
     "kvhip_cache_state_count": (_I32, [_P]),

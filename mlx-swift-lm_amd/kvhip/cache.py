@@ -329,6 +329,21 @@ class _Cache:
         L.check(self._lib.kvhip_mask_materialize(C.byref(p), _ptr(buf), _stream()))
         return MaskMode.from_array(buf.bool())
 
+    def reorder(self, order, shared=0):
+        """Sequence b of the batch becomes what sequence order[b] was (`beam_select`'s rows, on the device); an entry outside the batch
+        leaves its own.  `shared`: leading positions that sequences and those they take from have in common, which need not move."""
+        if self._shape is None:
+            if self.offset:
+                raise ValueError("how many sequences this cache has is not known here: it was made from a handle")
+            return
+        if order.dtype not in (torch.int32, torch.int64) or tuple(order.shape) != (self._shape[0],):
+            raise ValueError(f"an order is one row number to each of {self._shape[0]} sequences, not {order.dtype} {tuple(order.shape)}")
+        dev = torch._C._cuda_getDevice()
+        if not order.is_cuda or order.device.index != dev:
+            raise ValueError(f"the order lies on {order.device}, the current device is cuda:{dev}")
+        order = order.to(torch.int32).contiguous()
+        L.check(self._lib.kvhip_cache_reorder(self._h, _ptr(order), int(shared), _stream()))
+
     # ---- state / metaState ---------------------------------------------------
     @property
     def state(self):
