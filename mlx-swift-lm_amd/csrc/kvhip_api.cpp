@@ -1847,14 +1847,19 @@ static kvhip_status delta_args(const kvhip_gated_delta_args *p, DeltaArgs &x) {
     return KVHIP_OK;
 }
 size_t kvhip_gated_delta_workspace(const kvhip_gated_delta_args *p) {
-    (void)p;
-    return 0;
+    DeltaArgs x;
+    return delta_args(p, x) == KVHIP_OK && delta_takes_chunks(x) ? delta_chunk_workspace(x) : 0;
 }
 kvhip_status kvhip_gated_delta(const kvhip_gated_delta_args *p, void *workspace, size_t workspace_bytes, void *stream) {
     DeltaArgs x;
     KV_TRY(delta_args(p, x));
-    (void)workspace, (void)workspace_bytes;
-    KV_HIP(launch_delta_steps(x, S(stream)));
+    if (delta_takes_chunks(x)) {
+        if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < delta_chunk_workspace(x))
+            return fail(KVHIP_ERR_INVALID_ARG, "workspace missing, too small or not 16-byte aligned");
+        KV_HIP(launch_delta_chunks(x, workspace, S(stream)));
+    } else {
+        KV_HIP(launch_delta_steps(x, S(stream)));
+    }
     return KVHIP_OK;
 }
 

@@ -25,6 +25,10 @@ struct DeltaArgs {
     float scale = 1.f, eps = 0.f;
 };
 hipError_t launch_delta_steps(const DeltaArgs &x, hipStream_t s);
+// Prompts in chunks on the matrix cores: whether a call goes that way, the scratch it takes, and the call.
+bool delta_takes_chunks(const DeltaArgs &x);
+size_t delta_chunk_workspace(const DeltaArgs &x);
+hipError_t launch_delta_chunks(const DeltaArgs &x, void *workspace, hipStream_t s);
 
 struct ConvArgs {
     const char *x = nullptr, *weight = nullptr, *bias = nullptr;

@@ -1,0 +1,565 @@
+// The gated delta rule over prompts, 64 tokens at a time on the matrix cores.
+//
+// With G_i the logarithms of a chunk's decays summed up to token i, K^ and Q^ the normed rows and S0 the state in front of it,
+//     A_ij = beta_i e^(G_i - G_j) k^_i k^_j  (j < i),   T = (I + A)^-1 diag(beta)
+//     U = T (V - diag(e^G) K^ S0^T)
+//     O = diag(e^G) Q^ S0^T + P U,   P_ij = e^(G_i - G_j) q^_i k^_j  (j <= i)
+//     S1^T = e^(G_63) S0^T + K^^T diag(e^(G_63 - G)) U
+// T and P need no state: chunk_prep_kernel makes them for all chunks at once.  chunk_scan_kernel walks the chunks of one head, 16 NT columns
+// of the values to a workgroup (columns never meet), the state in its accumulators: wavefront w holds rows of dk of S^T and does
+// rows 16 w .. of every product.
+//
+// Numbers.  The state is returned in float32, so everything that it is made from keeps float32's accuracy.  Norms are factors
+// of rows, put on in float32 behind the products: the operands Q and K stay what they came as, exact in one part of bfloat16
+// (float16: two).  S, U are split into three parts of bfloat16 each (24 bits, float32's whole range); T is float32 and so is
+// its product.  Decays are summed in float64: e^-1000 beside e^-0.001 loses nothing.  The output, which is rounded to 16 bits,
+// takes two parts of S, U and P.
+//
+// Operands lie in the workspace as the lanes take them, 1 KB to an instruction: contractions may be summed in any
+// order, so that lane (n, g)'s eight elements of a step are those at 4 g and 16 + 4 g of it -- which is where a product leaves them: S, U
+// go from accumulators to operands without crossing lanes, only from wavefront to wavefront through LDS.
+#include "kvhip_delta.hpp"
+#include "kvhip_device.hpp"
+
+namespace kvhip {
+namespace {
+
+typedef float kv_f4 __attribute__((ext_vector_type(4)));
+typedef __bf16 kv_b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 kv_h8 __attribute__((ext_vector_type(8)));
+
+constexpr int CHUNK = 64;
+
+__device__ __forceinline__ kv_f4 mfma_bf16(const kv_u4 &a, const kv_u4 &b, const kv_f4 &c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kv_b8, a), __builtin_bit_cast(kv_b8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ kv_f4 mfma_f16(const kv_u4 &a, const kv_u4 &b, const kv_f4 &c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(kv_h8, a), __builtin_bit_cast(kv_h8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ kv_f4 mfma_f32(float a, float b, const kv_f4 &c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// two values' parts of bfloat16, the largest first; what is left in x, y
+__device__ __forceinline__ uint32_t take_part(float &x, float &y) {
+    const uint32_t w = pk_bf2(x, y);
+    x -= __uint_as_float(w << 16);
+    y -= __uint_as_float(w & 0xffff0000u);
+    return w;
+}
+
+// Where a call's chunks keep what the scan takes.  All offsets in bytes, per key head or value head and chunk.
+struct ChunkSpace {
+    char *base;
+    uint64_t q, kt;             // behind k of a key head's chunk
+    uint64_t key, head;         // a key head's chunk, a value head's (T, P, factors)
+    uint64_t heads;             // where the value heads' begin
+    int32_t chunk0, chunks;     // the chunks that are laid out
+};
+__device__ __forceinline__ char *key_at(const ChunkSpace &w, int64_t bh, int c) { return w.base + (bh * w.chunks + c) * w.key; }
+__device__ __forceinline__ char *head_at(const ChunkSpace &w, int64_t bh, int c) { return w.base + w.heads + (bh * w.chunks + c) * w.head; }
+constexpr int T_BYTES = CHUNK * CHUNK * 4, P_BYTES = CHUNK * CHUNK * 4;
+// factors: e^G r_k (what K S is worth), scale e^G r_q, e^(G_63 - G) r_k, and e^G_63
+constexpr int FACTOR_BYTES = (3 * CHUNK + 64) * 4;
+
+struct ChunkSpan {
+    int from, end;  // the sequence's tokens
+    __device__ __forceinline__ ChunkSpan(const DeltaArgs &x, int b) {
+        from = x.left_pad ? min(max(x.left_pad[b], 0), x.L) : 0;
+        end = x.lengths ? min(max(x.lengths[b], from), x.L) : x.L;
+    }
+    __device__ __forceinline__ bool any(int chunk) const { return chunk * CHUNK < end && (chunk + 1) * CHUNK > from; }
+};
+
+// KD: channels of a key as they are laid out (zeros behind Dk); WIDE: rows of whole 16-byte pieces
+template <int DT, int KD, bool WIDE>
+__global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace w) {
+    constexpr int PITCH = KD + 8, KP = DT == 0 ? 2 : 1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, per = x.Hv / x.Hk, hk = h / per;
+    const ChunkSpan span(x, b);
+    const int t0 = (w.chunk0 + c) * CHUNK;
+    if (!span.any(w.chunk0 + c)) return;
+    __shared__ __align__(16) uint16_t ks[CHUNK * PITCH], qs[CHUNK * PITCH];
+    __shared__ float rk[CHUNK], rq[CHUNK], beta[CHUNK];
+    __shared__ __align__(16) float As[CHUNK][CHUNK + 4], Ts[CHUNK][CHUNK + 4];
+    __shared__ double total[CHUNK];
+    {  // rows, and their norms: four threads to a row
+        const int row = tid >> 2, t = t0 + row;
+        const bool there = t >= span.from && t < span.end;
+        const uint16_t *kp = reinterpret_cast<const uint16_t *>(x.k) + (int64_t)b * x.k_sb + (int64_t)t * x.k_sl + (int64_t)hk * x.Dk;
+        const uint16_t *qp = reinterpret_cast<const uint16_t *>(x.q) + (int64_t)b * x.q_sb + (int64_t)t * x.q_sl + (int64_t)hk * x.Dk;
+        float sk = 0.f, sq = 0.f;
+#pragma unroll
+        for (int i = 0; i < KD / 32; ++i) {
+            const int d = 8 * ((tid & 3) + 4 * i);
+            kv_u4 kw = {0, 0, 0, 0}, qw = {0, 0, 0, 0};
+            if (WIDE) {
+                if (there && d < x.Dk) {
+                    kw = *reinterpret_cast<const kv_u4 *>(kp + d);
+                    qw = *reinterpret_cast<const kv_u4 *>(qp + d);
+                }
+            } else if (there) {
+#pragma unroll
+                for (int m = 0; m < 8; ++m)
+                    if (d + m < x.Dk) {
+                        kw[m >> 1] |= (uint32_t)kp[d + m] << (16 * (m & 1));
+                        qw[m >> 1] |= (uint32_t)qp[d + m] << (16 * (m & 1));
+                    }
+            }
+            *reinterpret_cast<kv_u4 *>(ks + row * PITCH + d) = kw;
+            *reinterpret_cast<kv_u4 *>(qs + row * PITCH + d) = qw;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                float k0, k1, q0, q1;
+                if constexpr (DT == 1) {
+                    k0 = __uint_as_float(kw[m] << 16), k1 = __uint_as_float(kw[m] & 0xffff0000u);
+                    q0 = __uint_as_float(qw[m] << 16), q1 = __uint_as_float(qw[m] & 0xffff0000u);
+                } else {
+                    const kv_half2 a = as_h2(kw[m]), e = as_h2(qw[m]);
+                    k0 = (float)a.x, k1 = (float)a.y, q0 = (float)e.x, q1 = (float)e.y;
+                }
+                sk = fmaf(k1, k1, fmaf(k0, k0, sk));
+                sq = fmaf(q1, q1, fmaf(q0, q0, sq));
+            }
+        }
+        sk += __shfl_xor(sk, 1);
+        sk += __shfl_xor(sk, 2);
+        sq += __shfl_xor(sq, 1);
+        sq += __shfl_xor(sq, 2);
+        if ((tid & 3) == 0) {
+            rk[row] = x.eps > 0.f ? 1.f / sqrtf(sk + x.eps) : 1.f;
+            rq[row] = x.scale * (x.eps > 0.f ? 1.f / sqrtf(sq + x.eps) : 1.f);
+        }
+    }
+    if (wave == 0) {  // gates, and the decays summed up
+        const int t = t0 + lane;
+        const bool there = t >= span.from && t < span.end;
+        float decay = 0.f, rate = 0.f;
+        if (there) {
+            const int64_t ai = (int64_t)b * x.a_sb + (int64_t)t * x.a_sl + h, bi = (int64_t)b * x.b_sb + (int64_t)t * x.b_sl + h;
+            auto gate = [&](const char *p, int64_t i) {
+                return x.gate_dtype == KVHIP_F32 ? Elem<2>::load(p, i) : x.gate_dtype == KVHIP_BF16 ? Elem<1>::load(p, i) : Elem<0>::load(p, i);
+            };
+            decay = gate(x.a, ai);
+            rate = gate(x.b, bi);
+            if (x.a_log) {
+                const float s = decay + (x.dt_bias ? x.dt_bias[h] : 0.f);
+                decay = -expf(x.a_log[h]) * (fmaxf(s, 0.f) + log1pf(expf(-fabsf(s))));
+                rate = 1.f / (1.f + expf(-rate));
+            }
+            decay = fmaxf(decay, -1e5f);  // (e^-1e5 is nothing, and differences of sums stay numbers)
+        }
+        double sum = decay;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const double o = __shfl_up(sum, s);
+            if (lane >= s) sum += o;
+        }
+        total[lane] = sum;
+        beta[lane] = rate;
+    }
+    __syncthreads();
+    char *head = head_at(w, (int64_t)b * x.Hv + h, c);
+    if (tid < CHUNK) {
+        float *f = reinterpret_cast<float *>(head + T_BYTES + P_BYTES);
+        const float rise = expf((float)total[tid]);
+        f[tid] = rise * rk[tid];
+        f[CHUNK + tid] = rise * rq[tid];
+        f[2 * CHUNK + tid] = expf((float)(total[CHUNK - 1] - total[tid])) * rk[tid];
+        if (tid == 0) f[3 * CHUNK] = expf((float)total[CHUNK - 1]);
+    }
+    if (h % per == 0) {  // the rows as operands, once for the heads that share them
+        char *key = key_at(w, (int64_t)b * x.Hk + hk, c);
+        auto parts = [&](kv_u4 v, kv_u4 &low) {  // (float16: bfloat16's part of each element, and what is left)
+            if constexpr (DT == 1) return v;
+            kv_u4 r;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const kv_half2 e = as_h2(v[m]);
+                float a = (float)e.x, o = (float)e.y;
+                r[m] = take_part(a, o);
+                low[m] = pk_bf2(a, o);
+            }
+            return r;
+        };
+        for (int i = wave; i < 4 * (KD / 32); i += 4) {  // rows 16 mt + n, channels 32 s + 4 g and 16 on
+            const int mt = i & 3, s = i >> 2;
+            const uint16_t *kr = ks + (16 * mt + n) * PITCH + 32 * s + 4 * g, *qr = qs + (16 * mt + n) * PITCH + 32 * s + 4 * g;
+            const kv_u2 k0 = *reinterpret_cast<const kv_u2 *>(kr), k1 = *reinterpret_cast<const kv_u2 *>(kr + 16);
+            const kv_u2 q0 = *reinterpret_cast<const kv_u2 *>(qr), q1 = *reinterpret_cast<const kv_u2 *>(qr + 16);
+            kv_u4 low;
+            const int64_t at = ((int64_t)mt * (KD / 32) + s) * 1024 + lane * 16;
+            *reinterpret_cast<kv_u4 *>(key + at) = parts(kv_u4{k0.x, k0.y, k1.x, k1.y}, low);
+            if (KP == 2) *reinterpret_cast<kv_u4 *>(key + at + CHUNK * KD * 2) = low;
+            *reinterpret_cast<kv_u4 *>(key + w.q + at) = parts(kv_u4{q0.x, q0.y, q1.x, q1.y}, low);
+            if (KP == 2) *reinterpret_cast<kv_u4 *>(key + w.q + at + CHUNK * KD * 2) = low;
+        }
+        for (int i = wave; i < KD / 16 * 2; i += 4) {  // channels 16 mt + n, tokens 32 s + 4 g and 16 on
+            const int mt = i >> 1, s = i & 1;
+            kv_u4 v, low;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const uint16_t *p = ks + (32 * s + 16 * (m >> 1) + 4 * g + 2 * (m & 1)) * PITCH + 16 * mt + n;
+                v[m] = p[0] | (uint32_t)p[PITCH] << 16;
+            }
+            const int64_t at = (int64_t)i * 1024 + lane * 16;
+            *reinterpret_cast<kv_u4 *>(key + w.kt + at) = parts(v, low);
+            if (KP == 2) *reinterpret_cast<kv_u4 *>(key + w.kt + at + CHUNK * KD * 2) = low;
+        }
+    }
+    {  // k k^T and q k^T: wavefront w rows 16 w on
+        kv_f4 kk[4], qk[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kk[j] = qk[j] = kv_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KD / 32; ++s) {
+            const kv_u4 ka = *reinterpret_cast<const kv_u4 *>(ks + (16 * wave + n) * PITCH + 32 * s + 8 * g);
+            const kv_u4 qa = *reinterpret_cast<const kv_u4 *>(qs + (16 * wave + n) * PITCH + 32 * s + 8 * g);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const kv_u4 kb = *reinterpret_cast<const kv_u4 *>(ks + (16 * j + n) * PITCH + 32 * s + 8 * g);
+                kk[j] = DT == 1 ? mfma_bf16(ka, kb, kk[j]) : mfma_f16(ka, kb, kk[j]);
+                qk[j] = DT == 1 ? mfma_bf16(qa, kb, qk[j]) : mfma_f16(qa, kb, qk[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = 16 * wave + 4 * g + r, col = 16 * j + n;
+                const float fade = col <= row ? expf((float)(total[row] - total[col])) * rk[col] : 0.f;
+                As[row][col] = col < row ? beta[row] * rk[row] * fade * kk[j][r] : 0.f;
+                Ts[row][col] = col <= row ? rq[row] * fade * qk[j][r] : 0.f;  // (P, until it is put away)
+            }
+    }
+    __syncthreads();
+    {  // P in two parts: rows 16 w + n, tokens 32 s + 4 g and 16 on
+        char *p = head + T_BYTES;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const kv_f4 a = *reinterpret_cast<const kv_f4 *>(&Ts[16 * wave + n][32 * s + 4 * g]), e = *reinterpret_cast<const kv_f4 *>(&Ts[16 * wave + n][32 * s + 16 + 4 * g]);
+            float v[8] = {a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
+            kv_u4 high, low;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                high[m] = take_part(v[2 * m], v[2 * m + 1]);
+                low[m] = pk_bf2(v[2 * m], v[2 * m + 1]);
+            }
+            *reinterpret_cast<kv_u4 *>(p + (wave * 2 + s) * 1024 + lane * 16) = high;
+            *reinterpret_cast<kv_u4 *>(p + 8192 + (wave * 2 + s) * 1024 + lane * 16) = low;
+        }
+    }
+    __syncthreads();
+    // (I + A)^-1 in blocks of 16: those of the diagonal by substitution, a column to a lane ...
+    if (lane < 16) {
+        float t[16];
+        const int o = 16 * wave;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float s = i == lane ? 1.f : 0.f;
+#pragma unroll
+            for (int j = 0; j < i; ++j) s = fmaf(-As[o + i][o + j], t[j], s);
+            t[i] = s;
+            Ts[o + i][o + lane] = s;
+        }
+    }
+    __syncthreads();
+    // ... those at distance d below it from  T_ij = -T_ii sum_k A_ik T_kj
+#pragma unroll
+    for (int d = 1; d < 4; ++d) {
+        const int i = wave, j = wave - d;
+        if (j >= 0) {
+            kv_f4 y = {0.f, 0.f, 0.f, 0.f}, z = {0.f, 0.f, 0.f, 0.f};
+            for (int k = j; k < i; ++k)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) y = mfma_f32(As[16 * i + n][16 * k + 4 * s + g], Ts[16 * k + 4 * s + g][16 * j + n], y);
+            const kv_f4 a = *reinterpret_cast<const kv_f4 *>(&Ts[16 * i + n][16 * i + 4 * g]);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) z = mfma_f32(-a[s], y[s], z);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) Ts[16 * i + 4 * g + r][16 * j + n] = z[r];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+        if (kt > wave) break;
+        kv_f4 t = *reinterpret_cast<const kv_f4 *>(&Ts[16 * wave + n][16 * kt + 4 * g]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[r] *= beta[16 * kt + 4 * g + r];
+        *reinterpret_cast<kv_f4 *>(head + (wave * 4 + kt) * 1024 + lane * 16) = t;
+    }
+}
+
+// KP: parts of a key's element;  NT: tiles of 16 value channels to a workgroup
+template <int DT, int KD, int NT>
+__global__ void __launch_bounds__(256) chunk_scan_kernel(DeltaArgs x, ChunkSpace w, const float *state_in) {
+    constexpr int KP = DT == 0 ? 2 : 1, KS = KD / 32, TPW = KD / 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    // (a head's workgroups on one die, where their operands meet in its cache: 8 dies take workgroups in turn)
+    const int heads = x.B * x.Hv, bh = blockIdx.x % heads, col0 = blockIdx.x / heads * (16 * NT);
+    const int b = bh / x.Hv, h = bh % x.Hv;
+    const ChunkSpan span(x, b);
+    const int64_t bk = (int64_t)b * x.Hk + h / (x.Hv / x.Hk);
+    __shared__ __align__(16) char sS[3 * KS * NT * 1024];
+    __shared__ __align__(16) char sX[4 * NT * 1024];
+    __shared__ __align__(16) char sU[5 * 2 * NT * 1024];  // parts of e^(G_63 - G) r_k U: 0 to 2; of U: 3, 4
+    kv_f4 S[TPW][NT];
+    const bool wide = x.Dk % 4 == 0 && ((uintptr_t)state_in | (uintptr_t)x.state_out) % 16 == 0;
+#pragma unroll
+    for (int i = 0; i < TPW; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int d = 16 * (wave * TPW + i) + 4 * g, col = col0 + 16 * t + n;
+            S[i][t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+            if (!state_in || col >= x.Dv) continue;
+            const float *p = state_in + ((int64_t)bh * x.Dv + col) * x.Dk + d;
+            if (wide) {
+                if (d < x.Dk) S[i][t] = *reinterpret_cast<const kv_f4 *>(p);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (d + r < x.Dk) S[i][t][r] = p[r];
+            }
+        }
+    const uint16_t *vp = reinterpret_cast<const uint16_t *>(x.v) + (int64_t)b * x.v_sb + (int64_t)h * x.Dv + col0;
+    uint16_t *op = reinterpret_cast<uint16_t *>(x.out) + ((int64_t)b * x.L * x.Hv + h) * x.Dv + col0;
+    const int64_t o_sl = (int64_t)x.Hv * x.Dv;
+    for (int c = 0; c < w.chunks; ++c) {
+        const int row0 = (w.chunk0 + c) * CHUNK + 16 * wave + 4 * g;
+        if (!span.any(w.chunk0 + c)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (row0 + r < x.L && col0 + 16 * t + n < x.Dv) op[(row0 + r) * o_sl + 16 * t + n] = 0;
+            continue;
+        }
+        const char *key = key_at(w, bk, c) + lane * 16, *head = head_at(w, bh, c) + lane * 16;
+        const float *factor = reinterpret_cast<const float *>(head_at(w, bh, c) + T_BYTES + P_BYTES);
+        kv_u4 K[KP][KS], Q[KP][KS], KT[KP][TPW][2], P[2][2];
+        kv_f4 T[4];
+#pragma unroll
+        for (int p = 0; p < KP; ++p) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                K[p][s] = *reinterpret_cast<const kv_u4 *>(key + p * CHUNK * KD * 2 + (wave * KS + s) * 1024);
+                Q[p][s] = *reinterpret_cast<const kv_u4 *>(key + w.q + p * CHUNK * KD * 2 + (wave * KS + s) * 1024);
+            }
+#pragma unroll
+            for (int i = 0; i < TPW; ++i)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) KT[p][i][s] = *reinterpret_cast<const kv_u4 *>(key + w.kt + p * CHUNK * KD * 2 + ((wave * TPW + i) * 2 + s) * 1024);
+        }
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+            T[kt] = kv_f4{0.f, 0.f, 0.f, 0.f};
+            if (kt <= wave) T[kt] = *reinterpret_cast<const kv_f4 *>(head + (wave * 4 + kt) * 1024);
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) P[p][s] = *reinterpret_cast<const kv_u4 *>(head + T_BYTES + p * 8192 + (wave * 2 + s) * 1024);
+        const kv_f4 rise_k = *reinterpret_cast<const kv_f4 *>(factor + 16 * wave + 4 * g), rise_q = *reinterpret_cast<const kv_f4 *>(factor + CHUNK + 16 * wave + 4 * g);
+        const kv_f4 fall = *reinterpret_cast<const kv_f4 *>(factor + 2 * CHUNK + 16 * wave + 4 * g);
+        const float last = factor[3 * CHUNK];
+        float V[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = row0 + r;
+                V[t][r] = row >= span.from && row < span.end && col0 + 16 * t + n < x.Dv ? Elem<DT>::load(vp, (int64_t)row * x.v_sl + 16 * t + n) : 0.f;
+            }
+        // the state as an operand
+#pragma unroll
+        for (int i = 0; i < TPW; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int tile = wave * TPW + i;
+                kv_f4 s = S[i][t];
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {
+                    float s0 = s[0], s1 = s[1], s2 = s[2], s3 = s[3];
+                    const uint32_t lo = take_part(s0, s1), hi = take_part(s2, s3);
+                    s = kv_f4{s0, s1, s2, s3};
+                    *reinterpret_cast<kv_u2 *>(sS + ((p * KS + (tile >> 1)) * NT + t) * 1024 + lane * 16 + (tile & 1) * 8) = kv_u2{lo, hi};
+                }
+            }
+        __syncthreads();
+        kv_f4 R[NT], O[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) R[t] = O[t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                kv_u4 part[3];
+#pragma unroll
+                for (int p = 0; p < 3; ++p) part[p] = *reinterpret_cast<const kv_u4 *>(sS + ((p * KS + s) * NT + t) * 1024 + lane * 16);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) R[t] = mfma_bf16(K[0][s], part[p], R[t]);
+                O[t] = mfma_bf16(Q[0][s], part[0], O[t]);
+                O[t] = mfma_bf16(Q[0][s], part[1], O[t]);
+                if constexpr (KP == 2) {
+                    R[t] = mfma_bf16(K[1][s], part[0], R[t]);
+                    R[t] = mfma_bf16(K[1][s], part[1], R[t]);
+                    O[t] = mfma_bf16(Q[1][s], part[0], O[t]);
+                }
+            }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            kv_f4 X;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                X[r] = fmaf(-rise_k[r], R[t][r], V[t][r]);
+                O[t][r] *= rise_q[r];
+            }
+            *reinterpret_cast<kv_f4 *>(sX + (wave * NT + t) * 1024 + lane * 16) = X;
+        }
+        __syncthreads();
+        kv_f4 U[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) U[t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+            if (kt > wave) break;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const kv_f4 X = *reinterpret_cast<const kv_f4 *>(sX + (kt * NT + t) * 1024 + lane * 16);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) U[t] = mfma_f32(T[kt][r], X[r], U[t]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float u[4], f[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                u[r] = U[t][r];
+                f[r] = fall[r] * u[r];
+            }
+            char *at = sU + ((wave >> 1) * NT + t) * 1024 + lane * 16 + (wave & 1) * 8;
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<kv_u2 *>(at + p * 2 * NT * 1024) = kv_u2{take_part(f[0], f[1]), take_part(f[2], f[3])};
+#pragma unroll
+            for (int p = 3; p < 5; ++p) *reinterpret_cast<kv_u2 *>(at + p * 2 * NT * 1024) = kv_u2{take_part(u[0], u[1]), take_part(u[2], u[3])};
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TPW; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[i][t][r] *= last;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                kv_u4 part[5];
+#pragma unroll
+                for (int p = 0; p < 5; ++p) part[p] = *reinterpret_cast<const kv_u4 *>(sU + ((p * 2 + s) * NT + t) * 1024 + lane * 16);
+#pragma unroll
+                for (int i = 0; i < TPW; ++i) {
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) S[i][t] = mfma_bf16(KT[0][i][s], part[p], S[i][t]);
+                    if constexpr (KP == 2) {
+                        S[i][t] = mfma_bf16(KT[1][i][s], part[0], S[i][t]);
+                        S[i][t] = mfma_bf16(KT[1][i][s], part[1], S[i][t]);
+                    }
+                }
+                O[t] = mfma_bf16(P[0][s], part[3], O[t]);
+                O[t] = mfma_bf16(P[0][s], part[4], O[t]);
+                O[t] = mfma_bf16(P[1][s], part[3], O[t]);
+            }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = row0 + r;
+                if (row < x.L && col0 + 16 * t + n < x.Dv)
+                    Elem<DT>::store(op, row * o_sl + 16 * t + n, row >= span.from && row < span.end ? O[t][r] : 0.f);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < TPW; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int d = 16 * (wave * TPW + i) + 4 * g, col = col0 + 16 * t + n;
+            if (col >= x.Dv) continue;
+            float *p = x.state_out + ((int64_t)bh * x.Dv + col) * x.Dk + d;
+            if (wide) {
+                if (d < x.Dk) *reinterpret_cast<kv_f4 *>(p) = S[i][t];
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (d + r < x.Dk) p[r] = S[i][t][r];
+            }
+        }
+}
+
+inline int chunk_key_dim(const DeltaArgs &x) { return x.Dk <= 64 ? 64 : x.Dk <= 128 ? 128 : 256; }
+// What a chunk of all sequences and heads takes, and how many chunks are laid out at a time: what they take is to stay in the
+// last-level cache between the two kernels.
+constexpr uint64_t CHUNK_SPACE = (uint64_t)192 << 20;
+inline ChunkSpace chunk_space(const DeltaArgs &x, void *workspace, uint64_t *bytes) {
+    ChunkSpace w{};
+    const uint64_t rows = (uint64_t)CHUNK * chunk_key_dim(x) * 2 * (x.dtype == KVHIP_F16 ? 2 : 1);
+    w.base = static_cast<char *>(workspace);
+    w.q = rows;
+    w.kt = 2 * rows;
+    w.key = 3 * rows;
+    w.head = T_BYTES + P_BYTES + FACTOR_BYTES;
+    const uint64_t one = (uint64_t)x.B * (x.Hk * w.key + x.Hv * w.head);
+    const int all = (x.L + CHUNK - 1) / CHUNK;
+    const uint64_t fit = CHUNK_SPACE / one;
+    w.chunks = (int32_t)(fit < 4 ? 4 : fit);
+    if (w.chunks > all) w.chunks = all;
+    w.heads = (uint64_t)x.B * x.Hk * w.chunks * w.key;
+    *bytes = one * w.chunks;
+    return w;
+}
+
+template <int DT, int KD> hipError_t launch_chunks(const DeltaArgs &x, ChunkSpace w, hipStream_t s) {
+    auto even = [&](const char *p, int64_t sb, int64_t sl) { return ((uintptr_t)p | (uint64_t)(sb * 2) | (uint64_t)(sl * 2)) % 16 == 0; };
+    const bool wide = x.Dk % 8 == 0 && even(x.q, x.q_sb, x.q_sl) && even(x.k, x.k_sb, x.k_sl);
+    const int all = (x.L + CHUNK - 1) / CHUNK, most = w.chunks;
+    const float *state = x.state_in;
+    for (int c = 0; c < all; c += most) {
+        w.chunk0 = c;
+        w.chunks = all - c < most ? all - c : most;
+        const dim3 prep(w.chunks, x.Hv, x.B);
+        if (wide) hipLaunchKernelGGL((chunk_prep_kernel<DT, KD, true>), prep, dim3(256), 0, s, x, w);
+        else hipLaunchKernelGGL((chunk_prep_kernel<DT, KD, false>), prep, dim3(256), 0, s, x, w);
+        const int64_t heads = (int64_t)x.B * x.Hv, one = (x.Dv + 15) / 16, two = (x.Dv + 31) / 32;
+        bool wider = false;
+        if constexpr (KD < 256) {
+            wider = heads * one > 512;
+            if (wider) hipLaunchKernelGGL((chunk_scan_kernel<DT, KD, 2>), dim3((unsigned)(heads * two)), dim3(256), 0, s, x, w, state);
+        }
+        if (!wider) hipLaunchKernelGGL((chunk_scan_kernel<DT, KD, 1>), dim3((unsigned)(heads * one)), dim3(256), 0, s, x, w, state);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        state = x.state_out;
+    }
+    return hipSuccess;
+}
+
+}  // namespace
+
+bool delta_takes_chunks(const DeltaArgs &x) { return x.dtype != KVHIP_F32 && x.L > 16 && (int64_t)x.B * x.Hv * ((x.Dv + 15) / 16) < ((int64_t)1 << 31); }
+
+size_t delta_chunk_workspace(const DeltaArgs &x) {
+    uint64_t bytes = 0;
+    (void)chunk_space(x, nullptr, &bytes);
+    return bytes;
+}
+
+hipError_t launch_delta_chunks(const DeltaArgs &x, void *workspace, hipStream_t s) {
+    uint64_t bytes = 0;
+    const ChunkSpace w = chunk_space(x, workspace, &bytes);
+    const int kd = chunk_key_dim(x);
+    if (x.dtype == KVHIP_F16) return kd == 64 ? launch_chunks<0, 64>(x, w, s) : kd == 128 ? launch_chunks<0, 128>(x, w, s) : launch_chunks<0, 256>(x, w, s);
+    return kd == 64 ? launch_chunks<1, 64>(x, w, s) : kd == 128 ? launch_chunks<1, 128>(x, w, s) : launch_chunks<1, 256>(x, w, s);
+}
+
+}  // namespace kvhip
