@@ -46,6 +46,9 @@ __device__ __forceinline__ uint32_t take_part(float &x, float &y) {
     return w;
 }
 
+// what wavefronts hand one another through LDS; requests past it stay in flight
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // Where a call's chunks keep what the scan takes.  All offsets in bytes, per key head or value head and chunk.
 struct ChunkSpace {
     char *base;
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
 
 // KP: parts of a key's element;  NT: tiles of 16 value channels to a workgroup
 template <int DT, int KD, int NT>
-__global__ void __launch_bounds__(256) chunk_scan_kernel(DeltaArgs x, ChunkSpace w, const float *state_in) {
+__global__ void __launch_bounds__(256, KD * (DT == 0 ? 2 : 1) > 256 ? 1 : 2) chunk_scan_kernel(DeltaArgs x, ChunkSpace w, const float *state_in) {
     constexpr int KP = DT == 0 ? 2 : 1, KS = KD / 32, TPW = KD / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
     // (a head's workgroups on one die, where their operands meet in its cache: 8 dies take workgroups in turn)
@@ -324,71 +327,104 @@ __global__ void __launch_bounds__(256) chunk_scan_kernel(DeltaArgs x, ChunkSpace
     const uint16_t *vp = reinterpret_cast<const uint16_t *>(x.v) + (int64_t)b * x.v_sb + (int64_t)h * x.Dv + col0;
     uint16_t *op = reinterpret_cast<uint16_t *>(x.out) + ((int64_t)b * x.L * x.Hv + h) * x.Dv + col0;
     const int64_t o_sl = (int64_t)x.Hv * x.Dv;
+    // the sequence's chunks among those that are laid out; rows of the others are zero
+    const int c0 = max(span.from / CHUNK - w.chunk0, 0), c1 = min((span.end + CHUNK - 1) / CHUNK - w.chunk0, w.chunks);
+    const bool none = span.from >= span.end || c0 >= c1;
     for (int c = 0; c < w.chunks; ++c) {
+        if (!none && c >= c0 && c < c1) continue;
         const int row0 = (w.chunk0 + c) * CHUNK + 16 * wave + 4 * g;
-        if (!span.any(w.chunk0 + c)) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (row0 + r < x.L && col0 + 16 * t + n < x.Dv) op[(row0 + r) * o_sl + 16 * t + n] = 0;
-            continue;
-        }
-        const char *key = key_at(w, bk, c) + lane * 16, *head = head_at(w, bh, c) + lane * 16;
-        const float *factor = reinterpret_cast<const float *>(head_at(w, bh, c) + T_BYTES + P_BYTES);
-        kv_u4 K[KP][KS], Q[KP][KS], KT[KP][TPW][2], P[2][2];
-        kv_f4 T[4];
-#pragma unroll
-        for (int p = 0; p < KP; ++p) {
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                K[p][s] = *reinterpret_cast<const kv_u4 *>(key + p * CHUNK * KD * 2 + (wave * KS + s) * 1024);
-                Q[p][s] = *reinterpret_cast<const kv_u4 *>(key + w.q + p * CHUNK * KD * 2 + (wave * KS + s) * 1024);
-            }
-#pragma unroll
-            for (int i = 0; i < TPW; ++i)
-#pragma unroll
-                for (int s = 0; s < 2; ++s) KT[p][i][s] = *reinterpret_cast<const kv_u4 *>(key + w.kt + p * CHUNK * KD * 2 + ((wave * TPW + i) * 2 + s) * 1024);
-        }
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-            T[kt] = kv_f4{0.f, 0.f, 0.f, 0.f};
-            if (kt <= wave) T[kt] = *reinterpret_cast<const kv_f4 *>(head + (wave * 4 + kt) * 1024);
-        }
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) P[p][s] = *reinterpret_cast<const kv_u4 *>(head + T_BYTES + p * 8192 + (wave * 2 + s) * 1024);
-        const kv_f4 rise_k = *reinterpret_cast<const kv_f4 *>(factor + 16 * wave + 4 * g), rise_q = *reinterpret_cast<const kv_f4 *>(factor + CHUNK + 16 * wave + 4 * g);
-        const kv_f4 fall = *reinterpret_cast<const kv_f4 *>(factor + 2 * CHUNK + 16 * wave + 4 * g);
-        const float last = factor[3 * CHUNK];
-        float V[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = row0 + r;
-                V[t][r] = row >= span.from && row < span.end && col0 + 16 * t + n < x.Dv ? Elem<DT>::load(vp, (int64_t)row * x.v_sl + 16 * t + n) : 0.f;
-            }
-        // the state as an operand
+            for (int r = 0; r < 4; ++r)
+                if (row0 + r < x.L && col0 + 16 * t + n < x.Dv) op[(row0 + r) * o_sl + 16 * t + n] = 0;
+    }
+    // A chunk's operands are requested as soon as the last chunk's have been used, in the order in which they will be.
+    kv_u4 K[KP][KS], Q[KP][KS], KT[KP][TPW][2], P[2][2];
+    kv_f4 T[4], rise_k, rise_q, fall;
+    float last;
+    uint16_t V[NT][4];
+    const char *key = key_at(w, bk, c0) + lane * 16 + wave * KS * 1024, *key_t = key_at(w, bk, c0) + w.kt + lane * 16 + wave * TPW * 2048;
+    const char *head = head_at(w, bh, c0) + lane * 16, *factor = head_at(w, bh, c0) + T_BYTES + P_BYTES + (16 * wave + 4 * g) * 4;
+    const char *factor0 = head_at(w, bh, c0) + T_BYTES + P_BYTES;
+    const int rows0 = (w.chunk0 + c0) * CHUNK + 16 * wave + 4 * g;
+    const uint16_t *v = vp + (int64_t)rows0 * x.v_sl + n;
+    uint16_t *o = op + rows0 * o_sl + n;
+    auto request_rows = [&](int64_t at) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int p = 0; p < KP; ++p) K[p][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + p * CHUNK * KD * 2 + s * 1024);
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int p = 0; p < KP; ++p) Q[p][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + w.q + p * CHUNK * KD * 2 + s * 1024);
+    };
+    // whether a chunk has all its tokens, and a workgroup all its columns
+    auto whole = [&](int c) { return (w.chunk0 + c) * CHUNK >= span.from && (w.chunk0 + c + 1) * CHUNK <= span.end && col0 + 16 * NT <= x.Dv; };
+    auto request_values = [&](int64_t at, bool all) {
+        rise_k = *reinterpret_cast<const kv_f4 *>(factor + at * w.head);
+        rise_q = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + CHUNK * 4);
+        if (all) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) V[t][r] = v[(at * CHUNK + r) * x.v_sl + 16 * t];
+        } else {  // (a token that is there in place of one that is not)
+            const int row0 = rows0 + (int)at * CHUNK;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) V[t][r] = vp[(int64_t)min(max(row0 + r, span.from), span.end - 1) * x.v_sl + min(16 * t + n, x.Dv - 1 - col0)];
+        }
+    };
+    auto request_system = [&](int64_t at) {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+            if (kt <= wave) T[kt] = *reinterpret_cast<const kv_f4 *>(head + at * w.head + (wave * 4 + kt) * 1024);
+        fall = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + 2 * CHUNK * 4);
+    };
+    auto request_rest = [&](int64_t at) {
+        last = *reinterpret_cast<const float *>(factor0 + at * w.head + 3 * CHUNK * 4);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < TPW; ++i)
+#pragma unroll
+                for (int p = 0; p < KP; ++p) KT[p][i][s] = *reinterpret_cast<const kv_u4 *>(key_t + at * w.key + p * CHUNK * KD * 2 + (i * 2 + s) * 1024);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) P[p][s] = *reinterpret_cast<const kv_u4 *>(head + at * w.head + T_BYTES + p * 8192 + (wave * 2 + s) * 1024);
+    };
+    // the state as an operand, for all wavefronts
+    auto share_state = [&]() {
 #pragma unroll
         for (int i = 0; i < TPW; ++i)
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const int tile = wave * TPW + i;
-                kv_f4 s = S[i][t];
+                float s0 = S[i][t][0], s1 = S[i][t][1], s2 = S[i][t][2], s3 = S[i][t][3];
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {
-                    float s0 = s[0], s1 = s[1], s2 = s[2], s3 = s[3];
-                    const uint32_t lo = take_part(s0, s1), hi = take_part(s2, s3);
-                    s = kv_f4{s0, s1, s2, s3};
-                    *reinterpret_cast<kv_u2 *>(sS + ((p * KS + (tile >> 1)) * NT + t) * 1024 + lane * 16 + (tile & 1) * 8) = kv_u2{lo, hi};
-                }
+                for (int p = 0; p < 3; ++p)
+                    *reinterpret_cast<kv_u2 *>(sS + ((p * KS + (tile >> 1)) * NT + t) * 1024 + lane * 16 + (tile & 1) * 8) = kv_u2{take_part(s0, s1), take_part(s2, s3)};
             }
-        __syncthreads();
-        kv_f4 R[NT], O[NT];
+    };
+    if (!none) {
+        request_rows(0);
+        request_values(0, whole(c0));
+        request_system(0);
+        request_rest(0);
+        share_state();
+    }
+    bool all = whole(c0);
+    for (int c = c0; !none && c < c1; ++c) {
+        const int next = min(c + 1, c1 - 1) - c0;
+        const bool all_next = whole(next + c0);
+        lds_barrier();
+        kv_f4 R[NT][2], O[NT][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) R[t] = O[t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < NT; ++t) R[t][0] = R[t][1] = O[t][0] = O[t][1] = kv_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -396,14 +432,15 @@ __global__ void __launch_bounds__(256) chunk_scan_kernel(DeltaArgs x, ChunkSpace
                 kv_u4 part[3];
 #pragma unroll
                 for (int p = 0; p < 3; ++p) part[p] = *reinterpret_cast<const kv_u4 *>(sS + ((p * KS + s) * NT + t) * 1024 + lane * 16);
-#pragma unroll
-                for (int p = 0; p < 3; ++p) R[t] = mfma_bf16(K[0][s], part[p], R[t]);
-                O[t] = mfma_bf16(Q[0][s], part[0], O[t]);
-                O[t] = mfma_bf16(Q[0][s], part[1], O[t]);
+                R[t][0] = mfma_bf16(K[0][s], part[0], R[t][0]);
+                R[t][1] = mfma_bf16(K[0][s], part[1], R[t][1]);
+                if constexpr (KP == 2) R[t][0] = mfma_bf16(K[1][s], part[0], R[t][0]);
+                O[t][0] = mfma_bf16(Q[0][s], part[0], O[t][0]);
+                R[t][1] = mfma_bf16(K[0][s], part[2], R[t][1]);
+                O[t][1] = mfma_bf16(Q[0][s], part[1], O[t][1]);
                 if constexpr (KP == 2) {
-                    R[t] = mfma_bf16(K[1][s], part[0], R[t]);
-                    R[t] = mfma_bf16(K[1][s], part[1], R[t]);
-                    O[t] = mfma_bf16(Q[1][s], part[0], O[t]);
+                    R[t][1] = mfma_bf16(K[1][s], part[1], R[t][1]);
+                    O[t][0] = mfma_bf16(Q[1][s], part[0], O[t][0]);
                 }
             }
 #pragma unroll
@@ -411,15 +448,22 @@ __global__ void __launch_bounds__(256) chunk_scan_kernel(DeltaArgs x, ChunkSpace
             kv_f4 X;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                X[r] = fmaf(-rise_k[r], R[t][r], V[t][r]);
-                O[t][r] *= rise_q[r];
+                float value = Elem<DT>::load(&V[t][r], 0);
+                if (!all) {
+                    const int row = rows0 + (c - c0) * CHUNK + r;
+                    value = row >= span.from && row < span.end ? value : 0.f;
+                }
+                X[r] = fmaf(-rise_k[r], R[t][0][r] + R[t][1][r], value);
+                O[t][0][r] = rise_q[r] * (O[t][0][r] + O[t][1][r]);
             }
             *reinterpret_cast<kv_f4 *>(sX + (wave * NT + t) * 1024 + lane * 16) = X;
         }
-        __syncthreads();
-        kv_f4 U[NT];
+        request_rows(next);
+        request_values(next, all_next);
+        lds_barrier();
+        kv_f4 U[NT][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) U[t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < NT; ++t) U[t][0] = U[t][1] = kv_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
             if (kt > wave) break;
@@ -427,7 +471,7 @@ __global__ void __launch_bounds__(256) chunk_scan_kernel(DeltaArgs x, ChunkSpace
             for (int t = 0; t < NT; ++t) {
                 const kv_f4 X = *reinterpret_cast<const kv_f4 *>(sX + (kt * NT + t) * 1024 + lane * 16);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) U[t] = mfma_f32(T[kt][r], X[r], U[t]);
+                for (int r = 0; r < 4; ++r) U[t][r & 1] = mfma_f32(T[kt][r], X[r], U[t][r & 1]);
             }
         }
 #pragma unroll
@@ -435,7 +479,7 @@ __global__ void __launch_bounds__(256) chunk_scan_kernel(DeltaArgs x, ChunkSpace
             float u[4], f[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                u[r] = U[t][r];
+                u[r] = U[t][0][r] + U[t][1][r];
                 f[r] = fall[r] * u[r];
             }
             char *at = sU + ((wave >> 1) * NT + t) * 1024 + lane * 16 + (wave & 1) * 8;
@@ -444,7 +488,8 @@ __global__ void __launch_bounds__(256) chunk_scan_kernel(DeltaArgs x, ChunkSpace
 #pragma unroll
             for (int p = 3; p < 5; ++p) *reinterpret_cast<kv_u2 *>(at + p * 2 * NT * 1024) = kv_u2{take_part(u[0], u[1]), take_part(u[2], u[3])};
         }
-        __syncthreads();
+        request_system(next);
+        lds_barrier();
 #pragma unroll
         for (int i = 0; i < TPW; ++i)
 #pragma unroll
@@ -459,26 +504,40 @@ __global__ void __launch_bounds__(256) chunk_scan_kernel(DeltaArgs x, ChunkSpace
 #pragma unroll
                 for (int p = 0; p < 5; ++p) part[p] = *reinterpret_cast<const kv_u4 *>(sU + ((p * 2 + s) * NT + t) * 1024 + lane * 16);
 #pragma unroll
-                for (int i = 0; i < TPW; ++i) {
+                for (int p = 0; p < 3; ++p) {
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) S[i][t] = mfma_bf16(KT[0][i][s], part[p], S[i][t]);
-                    if constexpr (KP == 2) {
-                        S[i][t] = mfma_bf16(KT[1][i][s], part[0], S[i][t]);
-                        S[i][t] = mfma_bf16(KT[1][i][s], part[1], S[i][t]);
+                    for (int i = 0; i < TPW; ++i) {
+                        S[i][t] = mfma_bf16(KT[0][i][s], part[p], S[i][t]);
+                        if (KP == 2 && p < 2) S[i][t] = mfma_bf16(KT[KP - 1][i][s], part[p], S[i][t]);
                     }
+                    if (p < 2) O[t][0] = mfma_bf16(P[0][s], part[3 + p], O[t][0]);
+                    else O[t][0] = mfma_bf16(P[1][s], part[3], O[t][0]);
                 }
-                O[t] = mfma_bf16(P[0][s], part[3], O[t]);
-                O[t] = mfma_bf16(P[0][s], part[4], O[t]);
-                O[t] = mfma_bf16(P[1][s], part[3], O[t]);
             }
+        share_state();  // (its last readers are behind two barriers)
+        request_rest(next);
+        if (all) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = row0 + r;
-                if (row < x.L && col0 + 16 * t + n < x.Dv)
-                    Elem<DT>::store(op, row * o_sl + 16 * t + n, row >= span.from && row < span.end ? O[t][r] : 0.f);
+            for (int t = 0; t < NT; ++t) {
+                const uint32_t a = DT == 1 ? pk_bf2(O[t][0][0], O[t][0][1]) : pk_h2(O[t][0][0], O[t][0][1]);
+                const uint32_t e = DT == 1 ? pk_bf2(O[t][0][2], O[t][0][3]) : pk_h2(O[t][0][2], O[t][0][3]);
+                o[16 * t] = (uint16_t)a;
+                o[o_sl + 16 * t] = (uint16_t)(a >> 16);
+                o[2 * o_sl + 16 * t] = (uint16_t)e;
+                o[3 * o_sl + 16 * t] = (uint16_t)(e >> 16);
             }
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = rows0 + (c - c0) * CHUNK + r;
+                    if (row < x.L && col0 + 16 * t + n < x.Dv)
+                        Elem<DT>::store(o, r * o_sl + 16 * t, row >= span.from && row < span.end ? O[t][0][r] : 0.f);
+                }
+        }
+        o += CHUNK * o_sl;
+        all = all_next;
     }
 #pragma unroll
     for (int i = 0; i < TPW; ++i)
