@@ -11,8 +11,8 @@
 //
 // Numbers.  The state is returned in float32, so everything that it is made from keeps float32's accuracy.  Norms are factors
 // of rows, put on in float32 behind the products: the operands Q and K stay what they came as, exact in one part of bfloat16
-// (float16: two).  S, U are split into three parts of bfloat16 each (24 bits, float32's whole range); T is float32 and so is
-// its product.  Decays are summed in float64: e^-1000 beside e^-0.001 loses nothing.  The output, which is rounded to 16 bits,
+// (float16: two).  S, T, U and what T is multiplied with are split into three parts of bfloat16 each (24 bits, float32's whole
+// range), of which the products below 2^-24 are left out.  Decays are summed in float64: e^-1000 beside e^-0.001 loses nothing.  The output, which is rounded to 16 bits,
 // takes two parts of S, U and P.
 //
 // Operands lie in the workspace as the lanes take them, 1 KB to an instruction: contractions may be summed in any
@@ -59,7 +59,7 @@ struct ChunkSpace {
 };
 __device__ __forceinline__ char *key_at(const ChunkSpace &w, int64_t bh, int c) { return w.base + (bh * w.chunks + c) * w.key; }
 __device__ __forceinline__ char *head_at(const ChunkSpace &w, int64_t bh, int c) { return w.base + w.heads + (bh * w.chunks + c) * w.head; }
-constexpr int T_BYTES = CHUNK * CHUNK * 4, P_BYTES = CHUNK * CHUNK * 4;
+constexpr int T_BYTES = CHUNK * CHUNK * 6, P_BYTES = CHUNK * CHUNK * 4;  // three and two parts
 // factors: e^G r_k (what K S is worth), scale e^G r_q, e^(G_63 - G) r_k, and e^G_63
 constexpr int FACTOR_BYTES = (3 * CHUNK + 64) * 4;
 
@@ -75,49 +75,66 @@ struct ChunkSpan {
 // KD: channels of a key as they are laid out (zeros behind Dk); WIDE: rows of whole 16-byte pieces
 template <int DT, int KD, bool WIDE>
 __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace w) {
-    constexpr int PITCH = KD + 8, KP = DT == 0 ? 2 : 1;
+    constexpr int PITCH = KD + 8, KP = DT == 0 ? 2 : 1, ROW = CHUNK + 4, BYTES = CHUNK * PITCH * 2;
+    constexpr double LOG2E_64 = 1.4426950408889634074;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
     const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, per = x.Hv / x.Hk, hk = h / per;
     const ChunkSpan span(x, b);
     const int t0 = (w.chunk0 + c) * CHUNK;
     if (!span.any(w.chunk0 + c)) return;
-    __shared__ __align__(16) uint16_t ks[CHUNK * PITCH], qs[CHUNK * PITCH];
+    __shared__ __align__(16) char keys[BYTES], queries[BYTES > CHUNK * ROW * 4 ? BYTES : CHUNK * ROW * 4];
+    __shared__ __align__(16) float Ts[CHUNK][ROW];  // P, then T
     __shared__ float rk[CHUNK], rq[CHUNK], beta[CHUNK];
-    __shared__ __align__(16) float As[CHUNK][CHUNK + 4], Ts[CHUNK][CHUNK + 4];
-    __shared__ double total[CHUNK];
+    __shared__ double total[CHUNK];  // decays summed up, as powers of two
+    uint16_t *ks = reinterpret_cast<uint16_t *>(keys), *qs = reinterpret_cast<uint16_t *>(queries);
+    float(*As)[ROW] = reinterpret_cast<float(*)[ROW]>(queries);  // (in the queries' place behind their product)
+    float decay = 0.f, rate = 0.f;
+    if (wave == 0 && t0 + lane >= span.from && t0 + lane < span.end) {
+        const int64_t t = t0 + lane, ai = (int64_t)b * x.a_sb + t * x.a_sl + h, bi = (int64_t)b * x.b_sb + t * x.b_sl + h;
+        auto gate = [&](const char *p, int64_t i) {
+            return x.gate_dtype == KVHIP_F32 ? Elem<2>::load(p, i) : x.gate_dtype == KVHIP_BF16 ? Elem<1>::load(p, i) : Elem<0>::load(p, i);
+        };
+        decay = gate(x.a, ai);
+        rate = gate(x.b, bi);
+    }
     {  // rows, and their norms: four threads to a row
         const int row = tid >> 2, t = t0 + row;
         const bool there = t >= span.from && t < span.end;
         const uint16_t *kp = reinterpret_cast<const uint16_t *>(x.k) + (int64_t)b * x.k_sb + (int64_t)t * x.k_sl + (int64_t)hk * x.Dk;
         const uint16_t *qp = reinterpret_cast<const uint16_t *>(x.q) + (int64_t)b * x.q_sb + (int64_t)t * x.q_sl + (int64_t)hk * x.Dk;
         float sk = 0.f, sq = 0.f;
+        kv_u4 kw[KD / 32], qw[KD / 32];
 #pragma unroll
         for (int i = 0; i < KD / 32; ++i) {
             const int d = 8 * ((tid & 3) + 4 * i);
-            kv_u4 kw = {0, 0, 0, 0}, qw = {0, 0, 0, 0};
+            kw[i] = qw[i] = kv_u4{0, 0, 0, 0};
             if (WIDE) {
                 if (there && d < x.Dk) {
-                    kw = *reinterpret_cast<const kv_u4 *>(kp + d);
-                    qw = *reinterpret_cast<const kv_u4 *>(qp + d);
+                    kw[i] = *reinterpret_cast<const kv_u4 *>(kp + d);
+                    qw[i] = *reinterpret_cast<const kv_u4 *>(qp + d);
                 }
             } else if (there) {
 #pragma unroll
                 for (int m = 0; m < 8; ++m)
                     if (d + m < x.Dk) {
-                        kw[m >> 1] |= (uint32_t)kp[d + m] << (16 * (m & 1));
-                        qw[m >> 1] |= (uint32_t)qp[d + m] << (16 * (m & 1));
+                        kw[i][m >> 1] |= (uint32_t)kp[d + m] << (16 * (m & 1));
+                        qw[i][m >> 1] |= (uint32_t)qp[d + m] << (16 * (m & 1));
                     }
             }
-            *reinterpret_cast<kv_u4 *>(ks + row * PITCH + d) = kw;
-            *reinterpret_cast<kv_u4 *>(qs + row * PITCH + d) = qw;
+        }
+#pragma unroll
+        for (int i = 0; i < KD / 32; ++i) {
+            const int d = 8 * ((tid & 3) + 4 * i);
+            *reinterpret_cast<kv_u4 *>(ks + row * PITCH + d) = kw[i];
+            *reinterpret_cast<kv_u4 *>(qs + row * PITCH + d) = qw[i];
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 float k0, k1, q0, q1;
                 if constexpr (DT == 1) {
-                    k0 = __uint_as_float(kw[m] << 16), k1 = __uint_as_float(kw[m] & 0xffff0000u);
-                    q0 = __uint_as_float(qw[m] << 16), q1 = __uint_as_float(qw[m] & 0xffff0000u);
+                    k0 = __uint_as_float(kw[i][m] << 16), k1 = __uint_as_float(kw[i][m] & 0xffff0000u);
+                    q0 = __uint_as_float(qw[i][m] << 16), q1 = __uint_as_float(qw[i][m] & 0xffff0000u);
                 } else {
-                    const kv_half2 a = as_h2(kw[m]), e = as_h2(qw[m]);
+                    const kv_half2 a = as_h2(kw[i][m]), e = as_h2(qw[i][m]);
                     k0 = (float)a.x, k1 = (float)a.y, q0 = (float)e.x, q1 = (float)e.y;
                 }
                 sk = fmaf(k1, k1, fmaf(k0, k0, sk));
@@ -134,83 +151,48 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
         }
     }
     if (wave == 0) {  // gates, and the decays summed up
-        const int t = t0 + lane;
-        const bool there = t >= span.from && t < span.end;
-        float decay = 0.f, rate = 0.f;
-        if (there) {
-            const int64_t ai = (int64_t)b * x.a_sb + (int64_t)t * x.a_sl + h, bi = (int64_t)b * x.b_sb + (int64_t)t * x.b_sl + h;
-            auto gate = [&](const char *p, int64_t i) {
-                return x.gate_dtype == KVHIP_F32 ? Elem<2>::load(p, i) : x.gate_dtype == KVHIP_BF16 ? Elem<1>::load(p, i) : Elem<0>::load(p, i);
-            };
-            decay = gate(x.a, ai);
-            rate = gate(x.b, bi);
-            if (x.a_log) {
-                const float s = decay + (x.dt_bias ? x.dt_bias[h] : 0.f);
-                decay = -expf(x.a_log[h]) * (fmaxf(s, 0.f) + log1pf(expf(-fabsf(s))));
-                rate = 1.f / (1.f + expf(-rate));
-            }
-            decay = fmaxf(decay, -1e5f);  // (e^-1e5 is nothing, and differences of sums stay numbers)
+        if (x.a_log && t0 + lane >= span.from && t0 + lane < span.end) {
+            const float s = decay + (x.dt_bias ? x.dt_bias[h] : 0.f);
+            decay = -expf(x.a_log[h]) * (fmaxf(s, 0.f) + log1pf(expf(-fabsf(s))));
+            rate = 1.f / (1.f + expf(-rate));
         }
-        double sum = decay;
+        double sum = fmaxf(decay, -1e5f);  // (e^-1e5 is nothing, and differences of sums stay numbers)
 #pragma unroll
         for (int s = 1; s < 64; s <<= 1) {
             const double o = __shfl_up(sum, s);
             if (lane >= s) sum += o;
         }
-        total[lane] = sum;
+        total[lane] = sum * LOG2E_64;
         beta[lane] = rate;
     }
     __syncthreads();
-    char *head = head_at(w, (int64_t)b * x.Hv + h, c);
-    if (tid < CHUNK) {
-        float *f = reinterpret_cast<float *>(head + T_BYTES + P_BYTES);
-        const float rise = expf((float)total[tid]);
-        f[tid] = rise * rk[tid];
-        f[CHUNK + tid] = rise * rq[tid];
-        f[2 * CHUNK + tid] = expf((float)(total[CHUNK - 1] - total[tid])) * rk[tid];
-        if (tid == 0) f[3 * CHUNK] = expf((float)total[CHUNK - 1]);
-    }
-    if (h % per == 0) {  // the rows as operands, once for the heads that share them
-        char *key = key_at(w, (int64_t)b * x.Hk + hk, c);
-        auto parts = [&](kv_u4 v, kv_u4 &low) {  // (float16: bfloat16's part of each element, and what is left)
-            if constexpr (DT == 1) return v;
-            kv_u4 r;
+    char *head = head_at(w, (int64_t)b * x.Hv + h, c), *key = key_at(w, (int64_t)b * x.Hk + hk, c);
+    const bool lays_rows = h % per == 0;  // the rows as operands, once for the heads that share them
+    auto parts = [&](kv_u4 v, kv_u4 &low) {  // (float16: bfloat16's part of each element, and what is left)
+        if constexpr (DT == 1) return v;
+        kv_u4 r;
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const kv_half2 e = as_h2(v[m]);
-                float a = (float)e.x, o = (float)e.y;
-                r[m] = take_part(a, o);
-                low[m] = pk_bf2(a, o);
-            }
-            return r;
-        };
-        for (int i = wave; i < 4 * (KD / 32); i += 4) {  // rows 16 mt + n, channels 32 s + 4 g and 16 on
-            const int mt = i & 3, s = i >> 2;
-            const uint16_t *kr = ks + (16 * mt + n) * PITCH + 32 * s + 4 * g, *qr = qs + (16 * mt + n) * PITCH + 32 * s + 4 * g;
-            const kv_u2 k0 = *reinterpret_cast<const kv_u2 *>(kr), k1 = *reinterpret_cast<const kv_u2 *>(kr + 16);
-            const kv_u2 q0 = *reinterpret_cast<const kv_u2 *>(qr), q1 = *reinterpret_cast<const kv_u2 *>(qr + 16);
-            kv_u4 low;
-            const int64_t at = ((int64_t)mt * (KD / 32) + s) * 1024 + lane * 16;
-            *reinterpret_cast<kv_u4 *>(key + at) = parts(kv_u4{k0.x, k0.y, k1.x, k1.y}, low);
-            if (KP == 2) *reinterpret_cast<kv_u4 *>(key + at + CHUNK * KD * 2) = low;
-            *reinterpret_cast<kv_u4 *>(key + w.q + at) = parts(kv_u4{q0.x, q0.y, q1.x, q1.y}, low);
-            if (KP == 2) *reinterpret_cast<kv_u4 *>(key + w.q + at + CHUNK * KD * 2) = low;
+        for (int m = 0; m < 4; ++m) {
+            const kv_half2 e = as_h2(v[m]);
+            float a = (float)e.x, o = (float)e.y;
+            r[m] = take_part(a, o);
+            low[m] = pk_bf2(a, o);
         }
-        for (int i = wave; i < KD / 16 * 2; i += 4) {  // channels 16 mt + n, tokens 32 s + 4 g and 16 on
-            const int mt = i >> 1, s = i & 1;
-            kv_u4 v, low;
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const uint16_t *p = ks + (32 * s + 16 * (m >> 1) + 4 * g + 2 * (m & 1)) * PITCH + 16 * mt + n;
-                v[m] = p[0] | (uint32_t)p[PITCH] << 16;
-            }
-            const int64_t at = (int64_t)i * 1024 + lane * 16;
-            *reinterpret_cast<kv_u4 *>(key + w.kt + at) = parts(v, low);
-            if (KP == 2) *reinterpret_cast<kv_u4 *>(key + w.kt + at + CHUNK * KD * 2) = low;
-        }
-    }
-    {  // k k^T and q k^T: wavefront w rows 16 w on
-        kv_f4 kk[4], qk[4];
+        return r;
+    };
+    auto lay = [&](char *to, kv_u4 v) {
+        kv_u4 low;
+        *reinterpret_cast<kv_u4 *>(to) = parts(v, low);
+        if (KP == 2) *reinterpret_cast<kv_u4 *>(to + CHUNK * KD * 2) = low;
+    };
+    // rows 16 mt + n, channels 32 s + 4 g and 16 on
+    auto lay_rows = [&](const uint16_t *rows, char *to, int mt, int s) {
+        const uint16_t *p = rows + (16 * mt + n) * PITCH + 32 * s + 4 * g;
+        const kv_u2 a = *reinterpret_cast<const kv_u2 *>(p), e = *reinterpret_cast<const kv_u2 *>(p + 16);
+        lay(to + ((int64_t)mt * (KD / 32) + s) * 1024 + lane * 16, kv_u4{a.x, a.y, e.x, e.y});
+    };
+    kv_f4 kk[4], qk[4];
+    {  // k k^T and q k^T on and below the diagonal: wavefront w rows 16 w on
 #pragma unroll
         for (int j = 0; j < 4; ++j) kk[j] = qk[j] = kv_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -219,23 +201,46 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
             const kv_u4 qa = *reinterpret_cast<const kv_u4 *>(qs + (16 * wave + n) * PITCH + 32 * s + 8 * g);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
+                if (j > wave) break;
                 const kv_u4 kb = *reinterpret_cast<const kv_u4 *>(ks + (16 * j + n) * PITCH + 32 * s + 8 * g);
                 kk[j] = DT == 1 ? mfma_bf16(ka, kb, kk[j]) : mfma_f16(ka, kb, kk[j]);
                 qk[j] = DT == 1 ? mfma_bf16(qa, kb, qk[j]) : mfma_f16(qa, kb, qk[j]);
             }
         }
+        if (lays_rows)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+            for (int s = 0; s < KD / 32; ++s) lay_rows(qs, key + w.q, wave, s);
+    }
+    __syncthreads();  // (the queries have been read)
+    {
+        double mine[4];
+        float b0[4], q0[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = 16 * wave + 4 * g + r;
+            mine[r] = total[row];
+            b0[r] = beta[row] * rk[row];
+            q0[r] = rq[row];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int col = 16 * j + n;
+            const double other = total[col];
+            const float k0 = rk[col];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int row = 16 * wave + 4 * g + r, col = 16 * j + n;
-                const float fade = col <= row ? expf((float)(total[row] - total[col])) * rk[col] : 0.f;
-                As[row][col] = col < row ? beta[row] * rk[row] * fade * kk[j][r] : 0.f;
-                Ts[row][col] = col <= row ? rq[row] * fade * qk[j][r] : 0.f;  // (P, until it is put away)
+                const int row = 16 * wave + 4 * g + r;
+                if (j > wave) {
+                    Ts[row][col] = 0.f;
+                    continue;
+                }
+                const float fade = col <= row ? __builtin_amdgcn_exp2f((float)(mine[r] - other)) * k0 : 0.f;
+                As[row][col] = col < row ? b0[r] * fade * kk[j][r] : 0.f;
+                Ts[row][col] = q0[r] * fade * qk[j][r];
             }
+        }
     }
-    __syncthreads();
-    {  // P in two parts: rows 16 w + n, tokens 32 s + 4 g and 16 on
+    {  // P in two parts: rows 16 w + n, tokens 32 s + 4 g and 16 on (rows that this wavefront wrote)
         char *p = head + T_BYTES;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -252,17 +257,46 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
         }
     }
     __syncthreads();
-    // (I + A)^-1 in blocks of 16: those of the diagonal by substitution, a column to a lane ...
-    if (lane < 16) {
+    // (I + A)^-1 in blocks of 16: those of the diagonal by substitution, a column of a block to a lane of the first wavefront,
+    // while the others put away what is left ...
+    if (wave == 0) {
         float t[16];
-        const int o = 16 * wave;
+        const int o = 16 * g;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            float s = i == lane ? 1.f : 0.f;
+            float part[4] = {i == n ? 1.f : 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < i; ++j) s = fmaf(-As[o + i][o + j], t[j], s);
-            t[i] = s;
-            Ts[o + i][o + lane] = s;
+            for (int j = 0; j < i; j += 4) {
+                const kv_f4 a = *reinterpret_cast<const kv_f4 *>(&As[o + i][o + j]);
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+                    if (j + m < i) part[m] = fmaf(-a[m], t[j + m], part[m]);
+            }
+            t[i] = (part[0] + part[1]) + (part[2] + part[3]);
+            Ts[o + i][o + n] = t[i];
+        }
+    } else {
+        if (lays_rows) {
+            for (int i = wave - 1; i < 4 * (KD / 32); i += 3) lay_rows(ks, key, i & 3, i >> 2);
+            for (int i = wave - 1; i < KD / 16 * 2; i += 3) {  // channels 16 mt + n, tokens 32 s + 4 g and 16 on
+                const int mt = i >> 1, s = i & 1;
+                kv_u4 v;
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const uint16_t *p = ks + (32 * s + 16 * (m >> 1) + 4 * g + 2 * (m & 1)) * PITCH + 16 * mt + n;
+                    v[m] = p[0] | (uint32_t)p[PITCH] << 16;
+                }
+                lay(key + w.kt + (int64_t)i * 1024 + lane * 16, v);
+            }
+        }
+        if (wave == 1) {
+            float *f = reinterpret_cast<float *>(head + T_BYTES + P_BYTES);
+            const double mine = total[lane], last = total[CHUNK - 1];
+            const float rise = __builtin_amdgcn_exp2f((float)mine);
+            f[lane] = rise * rk[lane];
+            f[CHUNK + lane] = rise * rq[lane];
+            f[2 * CHUNK + lane] = __builtin_amdgcn_exp2f((float)(last - mine)) * rk[lane];
+            if (lane == 0) f[3 * CHUNK] = __builtin_amdgcn_exp2f((float)last);
         }
     }
     __syncthreads();
@@ -271,41 +305,160 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
     for (int d = 1; d < 4; ++d) {
         const int i = wave, j = wave - d;
         if (j >= 0) {
-            kv_f4 y = {0.f, 0.f, 0.f, 0.f}, z = {0.f, 0.f, 0.f, 0.f};
-            for (int k = j; k < i; ++k)
+            kv_f4 y[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = 0; s < 4; ++s) y = mfma_f32(As[16 * i + n][16 * k + 4 * s + g], Ts[16 * k + 4 * s + g][16 * j + n], y);
+            for (int m = 0; m < d; ++m) {
+                const int k = j + m;
+                const kv_f4 a = *reinterpret_cast<const kv_f4 *>(&As[16 * i + n][16 * k + 4 * g]);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) y[s & 1] = mfma_f32(a[s], Ts[16 * k + 4 * g + s][16 * j + n], y[s & 1]);
+            }
             const kv_f4 a = *reinterpret_cast<const kv_f4 *>(&Ts[16 * i + n][16 * i + 4 * g]);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) z = mfma_f32(-a[s], y[s], z);
+            for (int s = 0; s < 4; ++s) z = mfma_f32(-a[s], y[0][s] + y[1][s], z);
 #pragma unroll
             for (int r = 0; r < 4; ++r) Ts[16 * i + 4 * g + r][16 * j + n] = z[r];
         }
         __syncthreads();
     }
+    // T in three parts: rows 16 w + n, tokens 32 s + 4 g and 16 on (zero above the diagonal)
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-        if (kt > wave) break;
-        kv_f4 t = *reinterpret_cast<const kv_f4 *>(&Ts[16 * wave + n][16 * kt + 4 * g]);
+    for (int s = 0; s < 2; ++s) {
+        if (2 * s > wave) break;
+        float t[8];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t[r] *= beta[16 * kt + 4 * g + r];
-        *reinterpret_cast<kv_f4 *>(head + (wave * 4 + kt) * 1024 + lane * 16) = t;
+        for (int m = 0; m < 8; ++m) {
+            const int col = 32 * s + 16 * (m >> 2) + 4 * g + (m & 3);
+            t[m] = col / 16 <= wave ? Ts[16 * wave + n][col] * beta[col] : 0.f;
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            kv_u4 part;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) part[m] = take_part(t[2 * m], t[2 * m + 1]);
+            *reinterpret_cast<kv_u4 *>(head + p * 8192 + (wave * 2 + s) * 1024 + lane * 16) = part;
+        }
     }
 }
 
-// KP: parts of a key's element;  NT: tiles of 16 value channels to a workgroup
+// NT: tiles of 16 value channels to a workgroup.  Wavefronts 0 to 3 carry the state, 4 to 7 make the outputs: what a chunk's outputs
+// need is off the way from one state to the next, and fills the other's waits on the same SIMDs.  (KP: parts of a key's element)
 template <int DT, int KD, int NT>
-__global__ void __launch_bounds__(256, KD * (DT == 0 ? 2 : 1) > 256 ? 1 : 2) chunk_scan_kernel(DeltaArgs x, ChunkSpace w, const float *state_in) {
-    constexpr int KP = DT == 0 ? 2 : 1, KS = KD / 32, TPW = KD / 64;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+__global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSpace w, const float *state_in) {
+    constexpr int KP = DT == 0 ? 2 : 1, KS = KD / 32, TPW = KD / 64, LOW = CHUNK * KD * 2;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6 & 3, n = lane & 15, g = lane >> 4;
     // (a head's workgroups on one die, where their operands meet in its cache: 8 dies take workgroups in turn)
     const int heads = x.B * x.Hv, bh = blockIdx.x % heads, col0 = blockIdx.x / heads * (16 * NT);
     const int b = bh / x.Hv, h = bh % x.Hv;
     const ChunkSpan span(x, b);
     const int64_t bk = (int64_t)b * x.Hk + h / (x.Hv / x.Hk);
-    __shared__ __align__(16) char sS[3 * KS * NT * 1024];
-    __shared__ __align__(16) char sX[4 * NT * 1024];
-    __shared__ __align__(16) char sU[5 * 2 * NT * 1024];  // parts of e^(G_63 - G) r_k U: 0 to 2; of U: 3, 4
+    __shared__ __align__(16) char sS[3 * KS * NT * 1024];  // the state's parts, an operand a step
+    __shared__ __align__(16) char sX[3 * 2 * NT * 1024];   // X's parts
+    __shared__ __align__(16) char sF[3 * 2 * NT * 1024];   // parts of diag(e^(G_63 - G) r_k) U
+    __shared__ __align__(16) char sU[4 * NT * 1024];       // U, in float32
+    // the sequence's chunks among those that are laid out
+    const int c0 = max(span.from / CHUNK - w.chunk0, 0), c1 = min((span.end + CHUNK - 1) / CHUNK - w.chunk0, w.chunks);
+    const bool none = span.from >= span.end || c0 >= c1;
+    // whether a chunk has all its tokens, and a workgroup all its columns
+    auto whole = [&](int c) { return (w.chunk0 + c) * CHUNK >= span.from && (w.chunk0 + c + 1) * CHUNK <= span.end && col0 + 16 * NT <= x.Dv; };
+    const int rows0 = (w.chunk0 + c0) * CHUNK + 16 * wave + 4 * g;
+    const char *key = key_at(w, bk, c0) + lane * 16, *head = head_at(w, bh, c0) + lane * 16;
+    const char *factors = head_at(w, bh, c0) + T_BYTES + P_BYTES, *factor = factors + (16 * wave + 4 * g) * 4;
+    auto part_of = [&](char *base, int p, int steps, int s, int t) { return base + ((p * steps + s) * NT + t) * 1024 + lane * 16; };
+    // A chunk's operands are requested as soon as the last chunk's have been used, in the order in which they will be.
+    if (threadIdx.x >= 256) {
+        uint16_t *op = reinterpret_cast<uint16_t *>(x.out) + ((int64_t)b * x.L * x.Hv + h) * x.Dv + col0 + n;
+        const int64_t o_sl = (int64_t)x.Hv * x.Dv;
+        for (int c = 0; c < w.chunks; ++c) {  // rows of chunks without tokens
+            if (!none && c >= c0 && c < c1) continue;
+            const int row0 = (w.chunk0 + c) * CHUNK + 16 * wave + 4 * g;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (row0 + r < x.L && col0 + 16 * t + n < x.Dv) op[(row0 + r) * o_sl + 16 * t] = 0;
+        }
+        if (none) return;
+        kv_u4 Q[KP][KS], P[2][2];
+        kv_f4 rise;
+        uint16_t *o = op + rows0 * o_sl;
+        auto request_rows = [&](int64_t at) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int p = 0; p < KP; ++p) Q[p][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + w.q + p * LOW + (wave * KS + s) * 1024);
+        };
+        auto request_rest = [&](int64_t at) {
+            rise = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + CHUNK * 4);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) P[p][s] = *reinterpret_cast<const kv_u4 *>(head + at * w.head + T_BYTES + p * 8192 + (wave * 2 + s) * 1024);
+        };
+        request_rows(0);
+        request_rest(0);
+        for (int c = c0; c < c1; ++c) {
+            const int next = min(c + 1, c1 - 1) - c0;
+            kv_f4 O[NT], I[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) O[t] = I[t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+            lds_barrier();
+            lds_barrier();  // (the state's wavefronts read it first)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const kv_u4 s0 = *reinterpret_cast<const kv_u4 *>(part_of(sS, 0, KS, s, t)), s1 = *reinterpret_cast<const kv_u4 *>(part_of(sS, 1, KS, s, t));
+                    O[t] = mfma_bf16(Q[0][s], s0, O[t]);
+                    O[t] = mfma_bf16(Q[0][s], s1, O[t]);
+                    if constexpr (KP == 2) O[t] = mfma_bf16(Q[1][s], s0, O[t]);
+                }
+            request_rows(next);
+            lds_barrier();
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const kv_f4 a = *reinterpret_cast<const kv_f4 *>(sU + (2 * s * NT + t) * 1024 + lane * 16);
+                    const kv_f4 e = *reinterpret_cast<const kv_f4 *>(sU + ((2 * s + 1) * NT + t) * 1024 + lane * 16);
+                    float u[8] = {a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
+                    kv_u4 u0, u1;
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        u0[m] = take_part(u[2 * m], u[2 * m + 1]);
+                        u1[m] = pk_bf2(u[2 * m], u[2 * m + 1]);
+                    }
+                    I[t] = mfma_bf16(P[0][s], u0, I[t]);
+                    I[t] = mfma_bf16(P[0][s], u1, I[t]);
+                    I[t] = mfma_bf16(P[1][s], u0, I[t]);
+                }
+            const bool all = whole(c);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float y[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = fmaf(rise[r], O[t][r], I[t][r]);
+                if (all) {
+                    const uint32_t a = DT == 1 ? pk_bf2(y[0], y[1]) : pk_h2(y[0], y[1]), e = DT == 1 ? pk_bf2(y[2], y[3]) : pk_h2(y[2], y[3]);
+                    o[16 * t] = (uint16_t)a;
+                    o[o_sl + 16 * t] = (uint16_t)(a >> 16);
+                    o[2 * o_sl + 16 * t] = (uint16_t)e;
+                    o[3 * o_sl + 16 * t] = (uint16_t)(e >> 16);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int row = rows0 + (c - c0) * CHUNK + r;
+                        if (row < x.L && col0 + 16 * t + n < x.Dv)
+                            Elem<DT>::store(o, r * o_sl + 16 * t, row >= span.from && row < span.end ? y[r] : 0.f);
+                    }
+                }
+            }
+            o += CHUNK * o_sl;
+            request_rest(next);
+        }
+        return;
+    }
+    __builtin_amdgcn_s_setprio(2);
     kv_f4 S[TPW][NT];
     const bool wide = x.Dk % 4 == 0 && ((uintptr_t)state_in | (uintptr_t)x.state_out) % 16 == 0;
 #pragma unroll
@@ -324,220 +477,157 @@ __global__ void __launch_bounds__(256, KD * (DT == 0 ? 2 : 1) > 256 ? 1 : 2) chu
                     if (d + r < x.Dk) S[i][t][r] = p[r];
             }
         }
-    const uint16_t *vp = reinterpret_cast<const uint16_t *>(x.v) + (int64_t)b * x.v_sb + (int64_t)h * x.Dv + col0;
-    uint16_t *op = reinterpret_cast<uint16_t *>(x.out) + ((int64_t)b * x.L * x.Hv + h) * x.Dv + col0;
-    const int64_t o_sl = (int64_t)x.Hv * x.Dv;
-    // the sequence's chunks among those that are laid out; rows of the others are zero
-    const int c0 = max(span.from / CHUNK - w.chunk0, 0), c1 = min((span.end + CHUNK - 1) / CHUNK - w.chunk0, w.chunks);
-    const bool none = span.from >= span.end || c0 >= c1;
-    for (int c = 0; c < w.chunks; ++c) {
-        if (!none && c >= c0 && c < c1) continue;
-        const int row0 = (w.chunk0 + c) * CHUNK + 16 * wave + 4 * g;
+    if (!none) {
+        const uint16_t *vp = reinterpret_cast<const uint16_t *>(x.v) + (int64_t)b * x.v_sb + (int64_t)h * x.Dv + col0, *v = vp + (int64_t)rows0 * x.v_sl + n;
+        const int steps = wave < 2 ? 1 : 2;  // of T's rows that are not zero
+        kv_u4 K[KP][KS], KT[KP][TPW][2], T[3][2];
+        kv_f4 rise, fall;
+        float last;
+        uint16_t V[NT][4];
+        auto request_rows = [&](int64_t at) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (row0 + r < x.L && col0 + 16 * t + n < x.Dv) op[(row0 + r) * o_sl + 16 * t + n] = 0;
-    }
-    // A chunk's operands are requested as soon as the last chunk's have been used, in the order in which they will be.
-    kv_u4 K[KP][KS], Q[KP][KS], KT[KP][TPW][2], P[2][2];
-    kv_f4 T[4], rise_k, rise_q, fall;
-    float last;
-    uint16_t V[NT][4];
-    const char *key = key_at(w, bk, c0) + lane * 16 + wave * KS * 1024, *key_t = key_at(w, bk, c0) + w.kt + lane * 16 + wave * TPW * 2048;
-    const char *head = head_at(w, bh, c0) + lane * 16, *factor = head_at(w, bh, c0) + T_BYTES + P_BYTES + (16 * wave + 4 * g) * 4;
-    const char *factor0 = head_at(w, bh, c0) + T_BYTES + P_BYTES;
-    const int rows0 = (w.chunk0 + c0) * CHUNK + 16 * wave + 4 * g;
-    const uint16_t *v = vp + (int64_t)rows0 * x.v_sl + n;
-    uint16_t *o = op + rows0 * o_sl + n;
-    auto request_rows = [&](int64_t at) {
+                for (int p = 0; p < KP; ++p) K[p][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + p * LOW + (wave * KS + s) * 1024);
+        };
+        auto request_values = [&](int64_t at, bool all) {
+            rise = *reinterpret_cast<const kv_f4 *>(factor + at * w.head);
+            if (all) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int p = 0; p < KP; ++p) K[p][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + p * CHUNK * KD * 2 + s * 1024);
+                    for (int t = 0; t < NT; ++t) V[t][r] = v[(at * CHUNK + r) * x.v_sl + 16 * t];
+            } else {  // (a token that is there in place of one that is not)
+                const int row0 = rows0 + (int)at * CHUNK;
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int p = 0; p < KP; ++p) Q[p][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + w.q + p * CHUNK * KD * 2 + s * 1024);
-    };
-    // whether a chunk has all its tokens, and a workgroup all its columns
-    auto whole = [&](int c) { return (w.chunk0 + c) * CHUNK >= span.from && (w.chunk0 + c + 1) * CHUNK <= span.end && col0 + 16 * NT <= x.Dv; };
-    auto request_values = [&](int64_t at, bool all) {
-        rise_k = *reinterpret_cast<const kv_f4 *>(factor + at * w.head);
-        rise_q = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + CHUNK * 4);
-        if (all) {
+                    for (int t = 0; t < NT; ++t) V[t][r] = vp[(int64_t)min(max(row0 + r, span.from), span.end - 1) * x.v_sl + min(16 * t + n, x.Dv - 1 - col0)];
+            }
+        };
+        auto request_system = [&](int64_t at) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int s = 0; s < 2; ++s)
+                if (s < steps)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) V[t][r] = v[(at * CHUNK + r) * x.v_sl + 16 * t];
-        } else {  // (a token that is there in place of one that is not)
-            const int row0 = rows0 + (int)at * CHUNK;
+                    for (int p = 0; p < 3; ++p) T[p][s] = *reinterpret_cast<const kv_u4 *>(head + at * w.head + p * 8192 + (wave * 2 + s) * 1024);
+            fall = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + 2 * CHUNK * 4);
+        };
+        auto request_rest = [&](int64_t at) {
+            last = *reinterpret_cast<const float *>(factors + at * w.head + 3 * CHUNK * 4);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) V[t][r] = vp[(int64_t)min(max(row0 + r, span.from), span.end - 1) * x.v_sl + min(16 * t + n, x.Dv - 1 - col0)];
-        }
-    };
-    auto request_system = [&](int64_t at) {
+                for (int i = 0; i < TPW; ++i)
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-            if (kt <= wave) T[kt] = *reinterpret_cast<const kv_f4 *>(head + at * w.head + (wave * 4 + kt) * 1024);
-        fall = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + 2 * CHUNK * 4);
-    };
-    auto request_rest = [&](int64_t at) {
-        last = *reinterpret_cast<const float *>(factor0 + at * w.head + 3 * CHUNK * 4);
+                    for (int p = 0; p < KP; ++p) KT[p][i][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + w.kt + p * LOW + ((wave * TPW + i) * 2 + s) * 1024);
+        };
+        // four neighbouring elements of a column as parts of half an operand
+        auto share = [&](char *base, int steps_, int tile, int t, float v0, float v1, float v2, float v3) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+            for (int p = 0; p < 3; ++p)
+                *reinterpret_cast<kv_u2 *>(part_of(base, p, steps_, tile >> 1, t) + (tile & 1) * 8) = kv_u2{take_part(v0, v1), take_part(v2, v3)};
+        };
+        auto share_state = [&]() {
 #pragma unroll
             for (int i = 0; i < TPW; ++i)
 #pragma unroll
-                for (int p = 0; p < KP; ++p) KT[p][i][s] = *reinterpret_cast<const kv_u4 *>(key_t + at * w.key + p * CHUNK * KD * 2 + (i * 2 + s) * 1024);
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int p = 0; p < 2; ++p) P[p][s] = *reinterpret_cast<const kv_u4 *>(head + at * w.head + T_BYTES + p * 8192 + (wave * 2 + s) * 1024);
-    };
-    // the state as an operand, for all wavefronts
-    auto share_state = [&]() {
-#pragma unroll
-        for (int i = 0; i < TPW; ++i)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const int tile = wave * TPW + i;
-                float s0 = S[i][t][0], s1 = S[i][t][1], s2 = S[i][t][2], s3 = S[i][t][3];
-#pragma unroll
-                for (int p = 0; p < 3; ++p)
-                    *reinterpret_cast<kv_u2 *>(sS + ((p * KS + (tile >> 1)) * NT + t) * 1024 + lane * 16 + (tile & 1) * 8) = kv_u2{take_part(s0, s1), take_part(s2, s3)};
-            }
-    };
-    if (!none) {
+                for (int t = 0; t < NT; ++t) share(sS, KS, wave * TPW + i, t, S[i][t][0], S[i][t][1], S[i][t][2], S[i][t][3]);
+        };
+        bool all = whole(c0);
         request_rows(0);
-        request_values(0, whole(c0));
+        request_values(0, all);
         request_system(0);
         request_rest(0);
         share_state();
-    }
-    bool all = whole(c0);
-    for (int c = c0; !none && c < c1; ++c) {
-        const int next = min(c + 1, c1 - 1) - c0;
-        const bool all_next = whole(next + c0);
-        lds_barrier();
-        kv_f4 R[NT][2], O[NT][2];
+        for (int c = c0; c < c1; ++c) {
+            const int next = min(c + 1, c1 - 1) - c0;
+            const bool all_next = whole(next + c0);
+            kv_f4 R[NT][2], U[NT][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) R[t][0] = R[t][1] = O[t][0] = O[t][1] = kv_f4{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < NT; ++t) R[t][0] = R[t][1] = U[t][0] = U[t][1] = kv_f4{0.f, 0.f, 0.f, 0.f};
+            lds_barrier();
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                kv_u4 part[3];
+                for (int t = 0; t < NT; ++t) {
+                    kv_u4 part[3];
 #pragma unroll
-                for (int p = 0; p < 3; ++p) part[p] = *reinterpret_cast<const kv_u4 *>(sS + ((p * KS + s) * NT + t) * 1024 + lane * 16);
-                R[t][0] = mfma_bf16(K[0][s], part[0], R[t][0]);
-                R[t][1] = mfma_bf16(K[0][s], part[1], R[t][1]);
-                if constexpr (KP == 2) R[t][0] = mfma_bf16(K[1][s], part[0], R[t][0]);
-                O[t][0] = mfma_bf16(Q[0][s], part[0], O[t][0]);
-                R[t][1] = mfma_bf16(K[0][s], part[2], R[t][1]);
-                O[t][1] = mfma_bf16(Q[0][s], part[1], O[t][1]);
-                if constexpr (KP == 2) {
-                    R[t][1] = mfma_bf16(K[1][s], part[1], R[t][1]);
-                    O[t][0] = mfma_bf16(Q[1][s], part[0], O[t][0]);
-                }
-            }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            kv_f4 X;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float value = Elem<DT>::load(&V[t][r], 0);
-                if (!all) {
-                    const int row = rows0 + (c - c0) * CHUNK + r;
-                    value = row >= span.from && row < span.end ? value : 0.f;
-                }
-                X[r] = fmaf(-rise_k[r], R[t][0][r] + R[t][1][r], value);
-                O[t][0][r] = rise_q[r] * (O[t][0][r] + O[t][1][r]);
-            }
-            *reinterpret_cast<kv_f4 *>(sX + (wave * NT + t) * 1024 + lane * 16) = X;
-        }
-        request_rows(next);
-        request_values(next, all_next);
-        lds_barrier();
-        kv_f4 U[NT][2];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) U[t][0] = U[t][1] = kv_f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-            if (kt > wave) break;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const kv_f4 X = *reinterpret_cast<const kv_f4 *>(sX + (kt * NT + t) * 1024 + lane * 16);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) U[t][r & 1] = mfma_f32(T[kt][r], X[r], U[t][r & 1]);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float u[4], f[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                u[r] = U[t][0][r] + U[t][1][r];
-                f[r] = fall[r] * u[r];
-            }
-            char *at = sU + ((wave >> 1) * NT + t) * 1024 + lane * 16 + (wave & 1) * 8;
-#pragma unroll
-            for (int p = 0; p < 3; ++p) *reinterpret_cast<kv_u2 *>(at + p * 2 * NT * 1024) = kv_u2{take_part(f[0], f[1]), take_part(f[2], f[3])};
-#pragma unroll
-            for (int p = 3; p < 5; ++p) *reinterpret_cast<kv_u2 *>(at + p * 2 * NT * 1024) = kv_u2{take_part(u[0], u[1]), take_part(u[2], u[3])};
-        }
-        request_system(next);
-        lds_barrier();
-#pragma unroll
-        for (int i = 0; i < TPW; ++i)
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) S[i][t][r] *= last;
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                kv_u4 part[5];
-#pragma unroll
-                for (int p = 0; p < 5; ++p) part[p] = *reinterpret_cast<const kv_u4 *>(sU + ((p * 2 + s) * NT + t) * 1024 + lane * 16);
-#pragma unroll
-                for (int p = 0; p < 3; ++p) {
-#pragma unroll
-                    for (int i = 0; i < TPW; ++i) {
-                        S[i][t] = mfma_bf16(KT[0][i][s], part[p], S[i][t]);
-                        if (KP == 2 && p < 2) S[i][t] = mfma_bf16(KT[KP - 1][i][s], part[p], S[i][t]);
+                    for (int p = 0; p < 3; ++p) part[p] = *reinterpret_cast<const kv_u4 *>(part_of(sS, p, KS, s, t));
+                    R[t][0] = mfma_bf16(K[0][s], part[0], R[t][0]);
+                    R[t][1] = mfma_bf16(K[0][s], part[1], R[t][1]);
+                    if constexpr (KP == 2) {
+                        R[t][0] = mfma_bf16(K[1][s], part[0], R[t][0]);
+                        R[t][1] = mfma_bf16(K[1][s], part[1], R[t][1]);
                     }
-                    if (p < 2) O[t][0] = mfma_bf16(P[0][s], part[3 + p], O[t][0]);
-                    else O[t][0] = mfma_bf16(P[1][s], part[3], O[t][0]);
+                    R[t][s & 1] = mfma_bf16(K[0][s], part[2], R[t][s & 1]);
                 }
-            }
-        share_state();  // (its last readers are behind two barriers)
-        request_rest(next);
-        if (all) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const uint32_t a = DT == 1 ? pk_bf2(O[t][0][0], O[t][0][1]) : pk_h2(O[t][0][0], O[t][0][1]);
-                const uint32_t e = DT == 1 ? pk_bf2(O[t][0][2], O[t][0][3]) : pk_h2(O[t][0][2], O[t][0][3]);
-                o[16 * t] = (uint16_t)a;
-                o[o_sl + 16 * t] = (uint16_t)(a >> 16);
-                o[2 * o_sl + 16 * t] = (uint16_t)e;
-                o[3 * o_sl + 16 * t] = (uint16_t)(e >> 16);
-            }
-        } else {
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
+                float X[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int row = rows0 + (c - c0) * CHUNK + r;
-                    if (row < x.L && col0 + 16 * t + n < x.Dv)
-                        Elem<DT>::store(o, r * o_sl + 16 * t, row >= span.from && row < span.end ? O[t][0][r] : 0.f);
+                    float value = Elem<DT>::load(&V[t][r], 0);
+                    if (!all) {
+                        const int row = rows0 + (c - c0) * CHUNK + r;
+                        value = row >= span.from && row < span.end ? value : 0.f;
+                    }
+                    X[r] = fmaf(-rise[r], R[t][0][r] + R[t][1][r], value);
                 }
+                share(sX, 2, wave, t, X[0], X[1], X[2], X[3]);
+            }
+            request_rows(next);
+            request_values(next, all_next);
+            lds_barrier();
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s >= steps) break;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    kv_u4 part[3];
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) part[p] = *reinterpret_cast<const kv_u4 *>(part_of(sX, p, 2, s, t));
+                    U[t][0] = mfma_bf16(T[0][s], part[0], U[t][0]);
+                    U[t][1] = mfma_bf16(T[0][s], part[1], U[t][1]);
+                    U[t][0] = mfma_bf16(T[1][s], part[0], U[t][0]);
+                    U[t][1] = mfma_bf16(T[1][s], part[1], U[t][1]);
+                    U[t][0] = mfma_bf16(T[0][s], part[2], U[t][0]);
+                    U[t][1] = mfma_bf16(T[2][s], part[0], U[t][1]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                kv_f4 u;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) u[r] = U[t][0][r] + U[t][1][r];
+                *reinterpret_cast<kv_f4 *>(sU + (wave * NT + t) * 1024 + lane * 16) = u;
+                share(sF, 2, wave, t, fall[0] * u[0], fall[1] * u[1], fall[2] * u[2], fall[3] * u[3]);
+            }
+            request_system(next);
+            lds_barrier();
+#pragma unroll
+            for (int i = 0; i < TPW; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[i][t][r] *= last;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) {
+                        const kv_u4 part = *reinterpret_cast<const kv_u4 *>(part_of(sF, p, 2, s, t));
+#pragma unroll
+                        for (int i = 0; i < TPW; ++i) {
+                            S[i][t] = mfma_bf16(KT[0][i][s], part, S[i][t]);
+                            if (KP == 2 && p < 2) S[i][t] = mfma_bf16(KT[KP - 1][i][s], part, S[i][t]);
+                        }
+                    }
+            request_rest(next);
+            share_state();  // (its last readers are behind a barrier)
+            all = all_next;
         }
-        o += CHUNK * o_sl;
-        all = all_next;
     }
 #pragma unroll
     for (int i = 0; i < TPW; ++i)
@@ -593,9 +683,9 @@ template <int DT, int KD> hipError_t launch_chunks(const DeltaArgs &x, ChunkSpac
         bool wider = false;
         if constexpr (KD < 256) {
             wider = heads * one > 512;
-            if (wider) hipLaunchKernelGGL((chunk_scan_kernel<DT, KD, 2>), dim3((unsigned)(heads * two)), dim3(256), 0, s, x, w, state);
+            if (wider) hipLaunchKernelGGL((chunk_scan_kernel<DT, KD, 2>), dim3((unsigned)(heads * two)), dim3(512), 0, s, x, w, state);
         }
-        if (!wider) hipLaunchKernelGGL((chunk_scan_kernel<DT, KD, 1>), dim3((unsigned)(heads * one)), dim3(256), 0, s, x, w, state);
+        if (!wider) hipLaunchKernelGGL((chunk_scan_kernel<DT, KD, 1>), dim3((unsigned)(heads * one)), dim3(512), 0, s, x, w, state);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         state = x.state_out;
