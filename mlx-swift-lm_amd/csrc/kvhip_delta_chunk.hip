@@ -13,7 +13,7 @@
 // of rows, put on in float32 behind the products: the operands Q and K stay what they came as, exact in one part of bfloat16
 // (float16: two).  S, T, U and what T is multiplied with are split into three parts of bfloat16 each (24 bits, float32's whole
 // range), of which the products below 2^-24 are left out.  Decays are summed in float64: e^-1000 beside e^-0.001 loses nothing.  The output, which is rounded to 16 bits,
-// takes two parts of S, U and P.
+// takes two parts of S and one of U and P, in float16 over powers of two for each row and column (float16: two).
 //
 // Operands lie in the workspace as the lanes take them, 1 KB to an instruction: contractions may be summed in any
 // order, so that lane (n, g)'s eight elements of a step are those at 4 g and 16 + 4 g of it -- which is where a product leaves them: S, U
@@ -46,6 +46,29 @@ __device__ __forceinline__ uint32_t take_part(float &x, float &y) {
     return w;
 }
 
+// two values' parts of float16: 11 bits, and the next 11
+__device__ __forceinline__ kv_u2 split2(float x, float y, float f) {  // of x f and y f, f a power of two
+    kv_half2 h, l;
+    h.x = (_Float16)(x * f);
+    h.y = (_Float16)(y * f);
+    l.x = (_Float16)fmaf(x, f, -(float)h.x);
+    l.y = (_Float16)fmaf(y, f, -(float)h.y);
+    return kv_u2{__builtin_bit_cast(uint32_t, h), __builtin_bit_cast(uint32_t, l)};
+}
+// The power of two over which a row's or column's elements are laid out in float16, by the largest: they end below 2^14.
+__device__ __forceinline__ float unit_of(float top) {
+    const uint32_t e = __float_as_uint(top) >> 23;  // (infinity and NaN: some unit; they stay what they are)
+    return __uint_as_float((min(max(e, 27u), 240u) - 13) << 23);
+}
+__device__ __forceinline__ float over(float unit) { return __uint_as_float(0x7f000000u - __float_as_uint(unit)); }  // 1 / unit
+// the largest of the four lanes that hold a column
+__device__ __forceinline__ float column_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // what wavefronts hand one another through LDS; requests past it stay in flight
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -59,9 +82,10 @@ struct ChunkSpace {
 };
 __device__ __forceinline__ char *key_at(const ChunkSpace &w, int64_t bh, int c) { return w.base + (bh * w.chunks + c) * w.key; }
 __device__ __forceinline__ char *head_at(const ChunkSpace &w, int64_t bh, int c) { return w.base + w.heads + (bh * w.chunks + c) * w.head; }
-constexpr int T_BYTES = CHUNK * CHUNK * 6, P_BYTES = CHUNK * CHUNK * 4;  // three and two parts
-// factors: e^G r_k (what K S is worth), scale e^G r_q, e^(G_63 - G) r_k, and e^G_63
-constexpr int FACTOR_BYTES = (3 * CHUNK + 64) * 4;
+constexpr int T_BYTES = CHUNK * CHUNK * 6, P_BYTES = CHUNK * CHUNK * 4;  // three parts, and two (bfloat16: one is used)
+// factors of rows: e^G r_k (what K S is worth), scale e^G r_q, e^(G_63 - G) r_k, P's units, and e^G_63
+constexpr int RISE_K = 0, RISE_Q = CHUNK, FALL = 2 * CHUNK, P_UNIT = 3 * CHUNK, LAST = 4 * CHUNK;
+constexpr int FACTOR_BYTES = 5 * CHUNK * 4;
 
 struct ChunkSpan {
     int from, end;  // the sequence's tokens
@@ -84,7 +108,7 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
     if (!span.any(w.chunk0 + c)) return;
     __shared__ __align__(16) char keys[BYTES], queries[BYTES > CHUNK * ROW * 4 ? BYTES : CHUNK * ROW * 4];
     __shared__ __align__(16) float Ts[CHUNK][ROW];  // P, then T
-    __shared__ float rk[CHUNK], rq[CHUNK], beta[CHUNK];
+    __shared__ float rk[CHUNK], rq[CHUNK], beta[CHUNK], p_unit[CHUNK];
     __shared__ double total[CHUNK];  // decays summed up, as powers of two
     uint16_t *ks = reinterpret_cast<uint16_t *>(keys), *qs = reinterpret_cast<uint16_t *>(queries);
     float(*As)[ROW] = reinterpret_cast<float(*)[ROW]>(queries);  // (in the queries' place behind their product)
@@ -240,20 +264,29 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
             }
         }
     }
-    {  // P in two parts: rows 16 w + n, tokens 32 s + 4 g and 16 on (rows that this wavefront wrote)
+    {  // P in float16 over a unit of each row: rows 16 w + n (that this wavefront wrote), tokens 32 s + 4 g and 16 on
+        float v[2][8], top = 0.f;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int m = 0; m < 8; ++m) {
+                v[s][m] = Ts[16 * wave + n][32 * s + 16 * (m >> 2) + 4 * g + (m & 3)];
+                top = fmaxf(top, fabsf(v[s][m]));
+            }
+        const float unit = unit_of(column_max(top)), f = over(unit);
+        if (g == 0) p_unit[16 * wave + n] = unit;
         char *p = head + T_BYTES;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const kv_f4 a = *reinterpret_cast<const kv_f4 *>(&Ts[16 * wave + n][32 * s + 4 * g]), e = *reinterpret_cast<const kv_f4 *>(&Ts[16 * wave + n][32 * s + 16 + 4 * g]);
-            float v[8] = {a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
+            if (2 * s > wave) break;
             kv_u4 high, low;
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                high[m] = take_part(v[2 * m], v[2 * m + 1]);
-                low[m] = pk_bf2(v[2 * m], v[2 * m + 1]);
+                const kv_u2 part = split2(v[s][2 * m], v[s][2 * m + 1], f);
+                high[m] = part.x, low[m] = part.y;
             }
             *reinterpret_cast<kv_u4 *>(p + (wave * 2 + s) * 1024 + lane * 16) = high;
-            *reinterpret_cast<kv_u4 *>(p + 8192 + (wave * 2 + s) * 1024 + lane * 16) = low;
+            if (DT == 0) *reinterpret_cast<kv_u4 *>(p + 8192 + (wave * 2 + s) * 1024 + lane * 16) = low;
         }
     }
     __syncthreads();
@@ -293,10 +326,11 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
             float *f = reinterpret_cast<float *>(head + T_BYTES + P_BYTES);
             const double mine = total[lane], last = total[CHUNK - 1];
             const float rise = __builtin_amdgcn_exp2f((float)mine);
-            f[lane] = rise * rk[lane];
-            f[CHUNK + lane] = rise * rq[lane];
-            f[2 * CHUNK + lane] = __builtin_amdgcn_exp2f((float)(last - mine)) * rk[lane];
-            if (lane == 0) f[3 * CHUNK] = __builtin_amdgcn_exp2f((float)last);
+            f[RISE_K + lane] = rise * rk[lane];
+            f[RISE_Q + lane] = rise * rq[lane];
+            f[FALL + lane] = __builtin_amdgcn_exp2f((float)(last - mine)) * rk[lane];
+            f[P_UNIT + lane] = p_unit[lane];
+            if (lane == 0) f[LAST] = __builtin_amdgcn_exp2f((float)last);
         }
     }
     __syncthreads();
@@ -345,7 +379,8 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
 // need is off the way from one state to the next, and fills the other's waits on the same SIMDs.  (KP: parts of a key's element)
 template <int DT, int KD, int NT>
 __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSpace w, const float *state_in) {
-    constexpr int KP = DT == 0 ? 2 : 1, KS = KD / 32, TPW = KD / 64, LOW = CHUNK * KD * 2;
+    constexpr int KP = DT == 0 ? 2 : 1, SP = KP, KS = KD / 32, TPW = KD / 64, LOW = CHUNK * KD * 2;  // SP: parts of P and U in the outputs
+    static_assert(KD % 64 == 0, "whole tiles to a wavefront");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6 & 3, n = lane & 15, g = lane >> 4;
     // (a head's workgroups on one die, where their operands meet in its cache: 8 dies take workgroups in turn)
     const int heads = x.B * x.Hv, bh = blockIdx.x % heads, col0 = blockIdx.x / heads * (16 * NT);
@@ -379,8 +414,9 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                     if (row0 + r < x.L && col0 + 16 * t + n < x.Dv) op[(row0 + r) * o_sl + 16 * t] = 0;
         }
         if (none) return;
-        kv_u4 Q[KP][KS], P[2][2];
-        kv_f4 rise;
+        kv_u4 Q[KP][KS], P[SP][2];
+        kv_f4 rise, unit;
+        const int steps = wave < 2 ? 1 : 2;  // of P's rows that are not zero
         uint16_t *o = op + rows0 * o_sl;
         auto request_rows = [&](int64_t at) {
 #pragma unroll
@@ -389,11 +425,13 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                 for (int p = 0; p < KP; ++p) Q[p][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + w.q + p * LOW + (wave * KS + s) * 1024);
         };
         auto request_rest = [&](int64_t at) {
-            rise = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + CHUNK * 4);
+            rise = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + RISE_Q * 4);
+            unit = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + P_UNIT * 4);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
+                if (s < steps)
 #pragma unroll
-                for (int p = 0; p < 2; ++p) P[p][s] = *reinterpret_cast<const kv_u4 *>(head + at * w.head + T_BYTES + p * 8192 + (wave * 2 + s) * 1024);
+                    for (int p = 0; p < SP; ++p) P[p][s] = *reinterpret_cast<const kv_u4 *>(head + at * w.head + T_BYTES + p * 8192 + (wave * 2 + s) * 1024);
         };
         request_rows(0);
         request_rest(0);
@@ -403,7 +441,6 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
 #pragma unroll
             for (int t = 0; t < NT; ++t) O[t] = I[t] = kv_f4{0.f, 0.f, 0.f, 0.f};
             lds_barrier();
-            lds_barrier();  // (the state's wavefronts read it first)
 #pragma unroll
             for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -415,29 +452,42 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                 }
             request_rows(next);
             lds_barrier();
+            lds_barrier();
+            float u_unit[NT];
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+            for (int t = 0; t < NT; ++t) {
+                kv_f4 u[4];
+                float top = 0.f;
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const kv_f4 a = *reinterpret_cast<const kv_f4 *>(sU + (2 * s * NT + t) * 1024 + lane * 16);
-                    const kv_f4 e = *reinterpret_cast<const kv_f4 *>(sU + ((2 * s + 1) * NT + t) * 1024 + lane * 16);
-                    float u[8] = {a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
-                    kv_u4 u0, u1;
+                for (int k = 0; k < 4; ++k) {
+                    if (k >= 2 * steps) break;
+                    u[k] = *reinterpret_cast<const kv_f4 *>(sU + (k * NT + t) * 1024 + lane * 16);
+                    top = fmaxf(top, fmaxf(fmaxf(fabsf(u[k][0]), fabsf(u[k][1])), fmaxf(fabsf(u[k][2]), fabsf(u[k][3]))));
+                }
+                u_unit[t] = unit_of(column_max(top));
+                const float f = over(u_unit[t]);
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    if (s >= steps) break;
+                    kv_u4 high, low;
 #pragma unroll
                     for (int m = 0; m < 4; ++m) {
-                        u0[m] = take_part(u[2 * m], u[2 * m + 1]);
-                        u1[m] = pk_bf2(u[2 * m], u[2 * m + 1]);
+                        const kv_u2 part = split2(u[2 * s + (m >> 1)][2 * (m & 1)], u[2 * s + (m >> 1)][2 * (m & 1) + 1], f);
+                        high[m] = part.x, low[m] = part.y;
                     }
-                    I[t] = mfma_bf16(P[0][s], u0, I[t]);
-                    I[t] = mfma_bf16(P[0][s], u1, I[t]);
-                    I[t] = mfma_bf16(P[1][s], u0, I[t]);
+                    I[t] = mfma_f16(P[0][s], high, I[t]);
+                    if constexpr (SP == 2) {
+                        I[t] = mfma_f16(P[SP - 1][s], high, I[t]);
+                        I[t] = mfma_f16(P[0][s], low, I[t]);
+                    }
                 }
+            }
             const bool all = whole(c);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 float y[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = fmaf(rise[r], O[t][r], I[t][r]);
+                for (int r = 0; r < 4; ++r) y[r] = fmaf(rise[r], O[t][r], unit[r] * u_unit[t] * I[t][r]);
                 if (all) {
                     const uint32_t a = DT == 1 ? pk_bf2(y[0], y[1]) : pk_h2(y[0], y[1]), e = DT == 1 ? pk_bf2(y[2], y[3]) : pk_h2(y[2], y[3]);
                     o[16 * t] = (uint16_t)a;
@@ -458,7 +508,6 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
         }
         return;
     }
-    __builtin_amdgcn_s_setprio(2);
     kv_f4 S[TPW][NT];
     const bool wide = x.Dk % 4 == 0 && ((uintptr_t)state_in | (uintptr_t)x.state_out) % 16 == 0;
 #pragma unroll
@@ -491,7 +540,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                 for (int p = 0; p < KP; ++p) K[p][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + p * LOW + (wave * KS + s) * 1024);
         };
         auto request_values = [&](int64_t at, bool all) {
-            rise = *reinterpret_cast<const kv_f4 *>(factor + at * w.head);
+            rise = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + RISE_K * 4);
             if (all) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
@@ -511,10 +560,10 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                 if (s < steps)
 #pragma unroll
                     for (int p = 0; p < 3; ++p) T[p][s] = *reinterpret_cast<const kv_u4 *>(head + at * w.head + p * 8192 + (wave * 2 + s) * 1024);
-            fall = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + 2 * CHUNK * 4);
+            fall = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + FALL * 4);
         };
         auto request_rest = [&](int64_t at) {
-            last = *reinterpret_cast<const float *>(factors + at * w.head + 3 * CHUNK * 4);
+            last = *reinterpret_cast<const float *>(factors + at * w.head + LAST * 4);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -679,11 +728,11 @@ template <int DT, int KD> hipError_t launch_chunks(const DeltaArgs &x, ChunkSpac
         const dim3 prep(w.chunks, x.Hv, x.B);
         if (wide) hipLaunchKernelGGL((chunk_prep_kernel<DT, KD, true>), prep, dim3(256), 0, s, x, w);
         else hipLaunchKernelGGL((chunk_prep_kernel<DT, KD, false>), prep, dim3(256), 0, s, x, w);
-        const int64_t heads = (int64_t)x.B * x.Hv, one = (x.Dv + 15) / 16, two = (x.Dv + 31) / 32;
+        const int64_t heads = (int64_t)x.B * x.Hv, one = (x.Dv + 15) / 16, four = (x.Dv + 63) / 64;
         bool wider = false;
         if constexpr (KD < 256) {
             wider = heads * one > 512;
-            if (wider) hipLaunchKernelGGL((chunk_scan_kernel<DT, KD, 2>), dim3((unsigned)(heads * two)), dim3(512), 0, s, x, w, state);
+            if (wider) hipLaunchKernelGGL((chunk_scan_kernel<DT, KD, 4>), dim3((unsigned)(heads * four)), dim3(512), 0, s, x, w, state);
         }
         if (!wider) hipLaunchKernelGGL((chunk_scan_kernel<DT, KD, 1>), dim3((unsigned)(heads * one)), dim3(512), 0, s, x, w, state);
         const hipError_t e = hipGetLastError();
