@@ -8,6 +8,8 @@
 //   s[beam] + ((x - M) - log sum),
 // in 64 bits, so that a sum's rounding does not decide between beams.  Where a list would overflow (thousands of equal values)
 // the best is taken out `count` times instead.
+#include <type_traits>
+
 #include "kvhip_delta.hpp"
 #include "kvhip_device.hpp"
 #include "kvhip_wave.hpp"
@@ -25,16 +27,19 @@ __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t u = __float_as_uint(v + 0.f);  // (-0 as 0)
     return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
-// the largest whole number that at least `count` (1 to 64) of the wavefront's lanes reach
+__device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
+// the largest whole number of sixteen bits above sixteen zeros that at least `count` (1 to 64) of the wavefront's lanes reach
 __device__ __forceinline__ uint32_t reached(uint32_t key, int count) {
     uint32_t t = 0;
 #pragma unroll
-    for (int bit = 31; bit >= 0; --bit) {
+    for (int bit = 31; bit >= 16; --bit) {
         const uint32_t up = t | (1u << bit);
         if (__popcll(__ballot(key >= up)) >= count) t = up;
     }
     return t;
 }
+// a value and its index as one whole number: the larger value first, then the lower index
+__device__ __forceinline__ uint64_t rank_key(float v, int i) { return (uint64_t)ordered(v) << 32 | (uint32_t)~i; }
 // a logit as it counts: what is no number never, infinity as the largest number
 __device__ __forceinline__ float logit(float v) { return v != v ? NEVER : fminf(v, 3.4028234663852886e38f); }
 
@@ -51,15 +56,14 @@ template <int NV> constexpr int beam_segment(int vec) { return 256 * NV * vec; }
 
 // NV: 16-byte vectors to a thread
 template <int DT, int NV, bool WIDE>
-__global__ void __launch_bounds__(256) beam_rows_kernel(BeamArgs x, BeamScratch w) {
-    constexpr int VEC = DT == 2 ? 4 : 8, ES = DT == 2 ? 4 : 2, E = NV * VEC;
+__global__ void __launch_bounds__(256, WIDE ? 6 : 4) beam_rows_kernel(BeamArgs x, BeamScratch w) {
+    constexpr int VEC = DT == 2 ? 4 : 8, ES = DT == 2 ? 4 : 2;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seg = blockIdx.x;
     const int64_t row = blockIdx.y, at = beam_at(w, row, seg);
     const int count = x.count;
     __shared__ uint32_t wave_key[4];
     __shared__ float wave_top[4], wave_sum4s[4];
-    __shared__ float list_v[BEAM_LIST];
-    __shared__ int32_t list_i[BEAM_LIST];
+    __shared__ uint64_t list[BEAM_LIST];  // (value, index) as one whole number, the larger the better
     __shared__ int listed;
     float *value = w.value + at * count;
     int32_t *index = w.index + at * count;
@@ -73,76 +77,111 @@ __global__ void __launch_bounds__(256) beam_rows_kernel(BeamArgs x, BeamScratch 
     }
     const char *p = x.logits + row * x.stride * ES;
     const int base = seg * w.segment;
-    float v[E];
+    // (kept as they came: what is held of a segment decides how many workgroups are there to wait for memory)
+    kv_u4 raw[NV];
     if (tid == 0) listed = 0;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
         const int i = base + (n * 256 + tid) * VEC;
         if (WIDE && i + VEC <= x.vocabulary) {
-            const kv_u4 u = *reinterpret_cast<const kv_u4 *>(p + (int64_t)i * ES);
+            raw[n] = *reinterpret_cast<const kv_u4 *>(p + (int64_t)i * ES);
+        } else {
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 if constexpr (DT == 2) {
-                    v[n * 4 + m] = logit(__uint_as_float(u[m]));
-                } else if constexpr (DT == 1) {
-                    v[n * 8 + 2 * m] = logit(__uint_as_float(u[m] << 16));
-                    v[n * 8 + 2 * m + 1] = logit(__uint_as_float(u[m] & 0xffff0000u));
+                    raw[n][m] = i + m < x.vocabulary ? reinterpret_cast<const uint32_t *>(p)[i + m] : 0xff800000u;
                 } else {
-                    const kv_h2 h = as_h2(u[m]);
-                    v[n * 8 + 2 * m] = logit((float)h.x);
-                    v[n * 8 + 2 * m + 1] = logit((float)h.y);
+                    constexpr uint32_t none = DT == 1 ? 0xff80u : 0xfc00u;  // (minus infinity)
+                    const uint16_t *q = reinterpret_cast<const uint16_t *>(p);
+                    const uint32_t lo = i + 2 * m < x.vocabulary ? q[i + 2 * m] : none, hi = i + 2 * m + 1 < x.vocabulary ? q[i + 2 * m + 1] : none;
+                    raw[n][m] = lo | hi << 16;
                 }
             }
-        } else {
-#pragma unroll
-            for (int m = 0; m < VEC; ++m) v[n * VEC + m] = i + m < x.vocabulary ? logit(Elem<DT>::load(p, i + m)) : NEVER;
         }
     }
-    float top = NEVER;
+    // a thread's element e, as it counts
+    auto element = [&](auto looked_at, int n, int m) {
+        float v;
+        if constexpr (DT == 2) v = __uint_as_float(raw[n][m]);
+        else if constexpr (DT == 1) v = __uint_as_float(m & 1 ? raw[n][m >> 1] & 0xffff0000u : raw[n][m >> 1] << 16);
+        else v = m & 1 ? (float)as_h2(raw[n][m >> 1]).y : (float)as_h2(raw[n][m >> 1]).x;
+        return decltype(looked_at)::value ? logit(v) : v;
+    };
+    // (converted anew from here on: the elements of a whole pass held as floats are twice the registers)
+    auto anew = [&]() {
 #pragma unroll
-    for (int e = 0; e < E; ++e) top = fmaxf(top, v[e]);
-    const uint32_t bound = reached(ordered(top), count);
-    const float wtop = wave_max(top);
-    if (lane == 0) {
-        wave_key[wave] = bound;
-        wave_top[wave] = wtop;
-    }
-    __syncthreads();
-    const uint32_t least = max(max(wave_key[0], wave_key[1]), max(wave_key[2], wave_key[3]));
-    const float all = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
-    float sum = 0.f;
-    if (all != NEVER) {
+        for (int n = 0; n < NV; ++n) asm volatile("" : "+v"(raw[n]));
+    };
+    float all, sum, least, tops[NV];
+    auto pass = [&](auto looked_at) {
+        float top = NEVER;
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum += fast_exp2((v[e] - all) * LOG2E);
-    }
-    sum = wave_sum(sum);
-    if (lane == 0) wave_sum4s[wave] = sum;
-    if (ordered(top) >= least) {
+        for (int n = 0; n < NV; ++n) {
+            tops[n] = NEVER;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (ordered(v[e]) >= least) {
-                const int i = base + ((e / VEC) * 256 + tid) * VEC + e % VEC;
-                if (i < x.vocabulary) {
-                    const int n = atomicAdd(&listed, 1);
-                    if (n < BEAM_LIST) {
-                        list_v[n] = v[e];
-                        list_i[n] = i;
+            for (int m = 0; m < VEC; ++m) tops[n] = fmaxf(tops[n], element(looked_at, n, m));
+            top = fmaxf(top, tops[n]);
+        }
+        const uint32_t bound = reached(ordered(top), count);
+        const float wtop = wave_max(top);
+        if (lane == 0) {
+            wave_key[wave] = bound;
+            wave_top[wave] = wtop;
+        }
+        __syncthreads();
+        least = unordered(max(max(max(wave_key[0], wave_key[1]), max(wave_key[2], wave_key[3])), 0x007fffffu));  // (-inf at least)
+        all = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
+        sum = 0.f;
+        anew();
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+            for (int m = 0; m < VEC; ++m) sum += fast_exp2((element(looked_at, n, m) - all) * LOG2E);  // (the largest's is one, exactly)
+        sum = wave_sum(sum);
+        if (lane == 0) wave_sum4s[wave] = sum;
+        __syncthreads();
+        sum = wave_sum4s[0] + wave_sum4s[1] + wave_sum4s[2] + wave_sum4s[3];
+    };
+    auto put_down = [&](auto looked_at) {
+        anew();
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+            if (tops[n] >= least) {
+#pragma unroll
+                for (int m = 0; m < VEC; ++m) {
+                    const float v = element(looked_at, n, m);
+                    const int i = base + (n * 256 + tid) * VEC + m;
+                    if (v >= least && i < x.vocabulary) {
+                        const int k = atomicAdd(&listed, 1);
+                        if (k < BEAM_LIST) list[k] = rank_key(v, i);
                     }
                 }
             }
+    };
+    // Logits are taken as they are; where one is no number or infinite, which the sum or the maximum shows, all are looked at
+    // and the pass is made again.
+    pass(std::false_type{});
+    const bool looked = !(sum == sum && all < __builtin_inff());
+    if (!looked) {
+        put_down(std::false_type{});
+    } else {
+        __syncthreads();
+        pass(std::true_type{});
+        if (all == NEVER) sum = 0.f;  // (a segment without a logit that counts)
+        put_down(std::true_type{});
     }
     __syncthreads();
     const int n = listed;
-    if (tid == 0) w.sums[at] = make_float2(all, wave_sum4s[0] + wave_sum4s[1] + wave_sum4s[2] + wave_sum4s[3]);
+    if (tid == 0) w.sums[at] = make_float2(all, sum);
     if (n <= BEAM_LIST) {
         for (int i = tid; i < n; i += 256) {
-            const float mine = list_v[i];
-            const int32_t id = list_i[i];
+            const uint64_t mine = list[i];
             int rank = 0;
-            for (int m = 0; m < n; ++m) rank += list_v[m] > mine || (list_v[m] == mine && list_i[m] < id);
+#pragma unroll 4
+            for (int m = 0; m < n; ++m) rank += list[m] > mine;
             if (rank < count) {
-                value[rank] = mine;
-                index[rank] = id;
+                value[rank] = unordered((uint32_t)(mine >> 32));
+                index[rank] = (int32_t)~(uint32_t)mine;
             }
         }
         for (int i = n + tid; i < count; i += 256) {
@@ -151,136 +190,141 @@ __global__ void __launch_bounds__(256) beam_rows_kernel(BeamArgs x, BeamScratch 
         }
         return;
     }
-    // thousands of equal values: the best behind the last one taken, `count` times
-    float last_v = __builtin_inff();
-    int32_t last_i = -1;
+    // thousands of equal values: the best behind the last one taken, `count` times (from the caches, as often)
+    uint64_t last = ~0ull;
     for (int c = 0; c < count; ++c) {
-        float best = NEVER;
-        int32_t id = 0x7fffffff;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = base + ((e / VEC) * 256 + tid) * VEC + e % VEC;
-            const bool behind = v[e] < last_v || (v[e] == last_v && i > last_i);
-            if (i < x.vocabulary && behind && (v[e] > best || (v[e] == best && i < id))) {
-                best = v[e];
-                id = i;
-            }
+        uint64_t best = 0;
+        for (int i = base + tid; i < min(base + w.segment, x.vocabulary); i += 256) {
+            const uint64_t key = rank_key(logit(Elem<DT>::load(p, i)), i);
+            if (key < last && key > best) best = key;
         }
         __syncthreads();
-        list_v[tid] = best;
-        list_i[tid] = id;
+        list[tid] = best;
         __syncthreads();
         for (int half = 128; half > 0; half >>= 1) {
-            if (tid < half) {
-                const float o = list_v[tid + half];
-                const int32_t oi = list_i[tid + half];
-                if (o > list_v[tid] || (o == list_v[tid] && oi < list_i[tid])) {
-                    list_v[tid] = o;
-                    list_i[tid] = oi;
-                }
-            }
+            if (tid < half && list[tid + half] > list[tid]) list[tid] = list[tid + half];
             __syncthreads();
         }
-        last_v = list_v[0];
-        last_i = list_i[0];
+        last = list[0];
         if (tid == 0) {
-            value[c] = last_v;
-            index[c] = last_i;
+            value[c] = unordered((uint32_t)(last >> 32));
+            index[c] = (int32_t)~(uint32_t)last;
         }
     }
 }
 
-// A candidate of the merge, and whether it comes before another.
+// A candidate of the merge as whole numbers in the order of what they stand for: its score, the larger the better; then beam,
+// logit and token, the smaller the better (6, 32 and 24 bits).
 struct Candidate {
-    double score;
-    float value;
-    int32_t beam, token;
+    uint64_t score, tie;
 };
-__device__ __forceinline__ bool before(const Candidate &a, const Candidate &b) {
-    if (a.score != b.score) return a.score > b.score;
-    if (a.beam != b.beam) return a.beam < b.beam;
-    if (a.value != b.value) return a.value > b.value;
-    return a.token < b.token;
+__device__ __forceinline__ bool before(const Candidate &a, const Candidate &b) { return a.score > b.score || (a.score == b.score && a.tie < b.tie); }
+__device__ __forceinline__ uint64_t ordered64(double v) {
+    const uint64_t u = __double_as_longlong(v + 0.);
+    return u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
 }
+__device__ __forceinline__ double unordered64(uint64_t u) { return __longlong_as_double(u & 0x8000000000000000ull ? u ^ 0x8000000000000000ull : ~u); }
 
-constexpr int MERGE_THREADS = 256, MERGE_BEAMS = 64;
+constexpr int MERGE_THREADS = 512, MERGE_BEAMS = 64, MERGE_HELD = 4;
+static_assert(MERGE_THREADS <= BEAM_LIST, "a place in the list for each thread");
 __global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(BeamArgs x, BeamScratch w) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = blockIdx.x, count = x.count;
     __shared__ double beam_score[MERGE_BEAMS], beam_log[MERGE_BEAMS];
     __shared__ float beam_top[MERGE_BEAMS];
-    __shared__ uint32_t wave_key[4];
-    __shared__ double list_s[BEAM_LIST];
-    __shared__ float list_v[BEAM_LIST];
-    __shared__ int32_t list_b[BEAM_LIST], list_t[BEAM_LIST];
+    __shared__ uint32_t wave_key[MERGE_THREADS / 64];
+    __shared__ __align__(16) Candidate list[BEAM_LIST];
     __shared__ int listed;
     if (tid == 0) listed = 0;
-    if (tid < x.beams) {
-        const int64_t row = (int64_t)g * x.beams + tid;
-        float top = NEVER;
-        for (int s = 0; s < w.segments; ++s) top = fmaxf(top, w.sums[beam_at(w, row, s)].x);
-        if (x.done && x.done[row]) top = 0.f;
-        double sum = 0.;
-        for (int s = 0; s < w.segments; ++s) {
-            const float2 t = w.sums[beam_at(w, row, s)];
-            if (t.x != NEVER) sum += (double)t.y * exp((double)t.x - (double)top);
-        }
-        const float own = x.scores ? x.scores[row] : 0.f;
-        // (a beam none of whose tokens counts, or whose score is no number: candidates that come last)
-        beam_score[tid] = own == own && top != NEVER ? (double)own : -__builtin_inf();
-        beam_top[tid] = top;
-        beam_log[tid] = log(sum);
-    }
-    __syncthreads();
     const int per = w.segments * count, total = x.beams * per;
     const int64_t first = (int64_t)g * x.beams * per;
-    auto candidate = [&](int i) {
-        Candidate c;
-        c.beam = i / per;
-        c.value = w.value[first + i];
-        c.token = w.index[first + i];
-        const double own = beam_score[c.beam];
-        // (the difference first: a logit may be so large that the others are lost in it)
-        c.score = own == -__builtin_inf() || c.value == NEVER ? -__builtin_inf() : own + (((double)c.value - (double)beam_top[c.beam]) - beam_log[c.beam]);
-        return c;
-    };
-    // scores for the bound, in 32 bits: rounding keeps their order
-    uint32_t top = 0;
-    for (int i = tid; i < total; i += MERGE_THREADS) {
-        const Candidate c = candidate(i);
-        if (c.token >= 0) top = max(top, ordered((float)c.score));
+    // a thread's first candidates, on their way while the sums are looked at
+    float value[MERGE_HELD];
+    int32_t token[MERGE_HELD];
+#pragma unroll
+    for (int j = 0; j < MERGE_HELD; ++j) {
+        const int i = j * MERGE_THREADS + tid;
+        token[j] = i < total ? w.index[first + i] : -1;
+        value[j] = i < total ? w.value[first + i] : NEVER;
     }
+    for (int k = tid >> 4; k < x.beams; k += MERGE_THREADS / 16) {  // sixteen lanes to a beam
+        const int64_t row = (int64_t)g * x.beams + k;
+        float top = NEVER, sum = 0.f;
+        for (int s = tid & 15; s < w.segments; s += 16) {
+            const float2 t = w.sums[beam_at(w, row, s)];
+            if (t.x == NEVER) continue;
+            const float high = fmaxf(top, t.x);
+            sum = sum * fast_exp2((top - high) * LOG2E) + t.y * fast_exp2((t.x - high) * LOG2E);
+            top = high;
+        }
+#pragma unroll
+        for (int m = 1; m < 16; m <<= 1) {
+            const float t = __shfl_xor(top, m), y = __shfl_xor(sum, m), high = fmaxf(top, t);
+            if (high == NEVER) continue;
+            sum = sum * fast_exp2((top - high) * LOG2E) + y * fast_exp2((t - high) * LOG2E);
+            top = high;
+        }
+        if ((tid & 15) == 0) {
+            const float own = x.scores ? x.scores[row] : 0.f;
+            // (a beam none of whose tokens counts, or whose score is no number: candidates that come last)
+            beam_score[k] = own == own && top != NEVER ? (double)own : -__builtin_inf();
+            beam_top[k] = top;
+            beam_log[k] = log((double)sum);
+        }
+    }
+    __syncthreads();
+    auto scored = [&](int i, float v, int32_t t) {
+        const int beam = i / per;
+        const double own = beam_score[beam];
+        // (the difference first: a logit may be so large that the others are lost in it)
+        const double score = own == -__builtin_inf() || v == NEVER ? -__builtin_inf() : own + (((double)v - (double)beam_top[beam]) - beam_log[beam]);
+        return Candidate{ordered64(score), (uint64_t)beam << 56 | (uint64_t)~ordered(v) << 24 | (uint32_t)t};
+    };
+    auto candidate = [&](int i) { return scored(i, w.value[first + i], w.index[first + i]); };
+    // scores for the bound: their leading 32 bits, rounded down, are in the same order
+    uint32_t top = 0, mine[MERGE_HELD];
+#pragma unroll
+    for (int j = 0; j < MERGE_HELD; ++j) {
+        const int i = j * MERGE_THREADS + tid;
+        mine[j] = token[j] >= 0 ? (uint32_t)(scored(i, value[j], token[j]).score >> 32) : 0;
+        top = max(top, mine[j]);
+    }
+    for (int i = MERGE_HELD * MERGE_THREADS + tid; i < total; i += MERGE_THREADS)
+        if (w.index[first + i] >= 0) top = max(top, (uint32_t)(candidate(i).score >> 32));
     const uint32_t bound = reached(top, count);
     if (lane == 0) wave_key[wave] = bound;
     __syncthreads();
-    const uint32_t least = max(max(wave_key[0], wave_key[1]), max(wave_key[2], wave_key[3]));
+    uint32_t least = 1;
+#pragma unroll
+    for (int i = 0; i < MERGE_THREADS / 64; ++i) least = max(least, wave_key[i]);
+    auto put_down = [&](const Candidate &c) {
+        const int n = atomicAdd(&listed, 1);
+        if (n < BEAM_LIST) list[n] = c;
+    };
     if (top >= least) {
-        for (int i = tid; i < total; i += MERGE_THREADS) {
-            const Candidate c = candidate(i);
-            if (c.token < 0 || ordered((float)c.score) < least) continue;
-            const int n = atomicAdd(&listed, 1);
-            if (n < BEAM_LIST) {
-                list_s[n] = c.score;
-                list_v[n] = c.value;
-                list_b[n] = c.beam;
-                list_t[n] = c.token;
+#pragma unroll
+        for (int j = 0; j < MERGE_HELD; ++j)
+            if (mine[j] >= least) put_down(scored(j * MERGE_THREADS + tid, value[j], token[j]));
+        for (int i = MERGE_HELD * MERGE_THREADS + tid; i < total; i += MERGE_THREADS)
+            if (w.index[first + i] >= 0) {
+                const Candidate c = candidate(i);
+                if ((uint32_t)(c.score >> 32) >= least) put_down(c);
             }
-        }
     }
     __syncthreads();
     const int n = listed;
     auto put = [&](int at, const Candidate &c) {
         const int64_t o = (int64_t)g * count + at;
-        x.rows[o] = g * x.beams + c.beam;
-        x.tokens[o] = c.token;
-        x.best[o] = (float)c.score;
+        x.rows[o] = g * x.beams + (int)(c.tie >> 56);
+        x.tokens[o] = (int32_t)(c.tie & 0xffffffu);
+        x.best[o] = (float)unordered64(c.score);
     };
-    auto held = [&](int i) { return Candidate{list_s[i], list_v[i], list_b[i], list_t[i]}; };
     if (n <= BEAM_LIST) {
         for (int i = tid; i < n; i += MERGE_THREADS) {
-            const Candidate mine = held(i);
+            const Candidate own = list[i];
             int rank = 0;
-            for (int m = 0; m < n; ++m) rank += before(held(m), mine);
-            if (rank < count) put(rank, mine);
+#pragma unroll 4
+            for (int m = 0; m < n; ++m) rank += before(list[m], own);
+            if (rank < count) put(rank, own);
         }
         for (int i = n + tid; i < count; i += MERGE_THREADS) {
             const int64_t o = (int64_t)g * count + i;
@@ -289,38 +333,32 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(BeamArgs x, B
         }
         return;
     }
-    Candidate last{__builtin_inf(), __builtin_inff(), -1, -1};
+    Candidate last{~0ull, 0};
     for (int c = 0; c < count; ++c) {
-        Candidate best{-__builtin_inf(), NEVER, 0x7fffffff, 0x7fffffff};
+        Candidate best{0, ~0ull};
         for (int i = tid; i < total; i += MERGE_THREADS) {
+            if (w.index[first + i] < 0) continue;
             const Candidate o = candidate(i);
-            if (o.token >= 0 && before(last, o) && before(o, best)) best = o;
+            if (before(last, o) && before(o, best)) best = o;
         }
         __syncthreads();
-        list_s[tid] = best.score;
-        list_v[tid] = best.value;
-        list_b[tid] = best.beam;
-        list_t[tid] = best.token;
+        list[tid] = best;
         __syncthreads();
         for (int half = MERGE_THREADS / 2; half > 0; half >>= 1) {
-            if (tid < half && before(held(tid + half), held(tid))) {
-                list_s[tid] = list_s[tid + half];
-                list_v[tid] = list_v[tid + half];
-                list_b[tid] = list_b[tid + half];
-                list_t[tid] = list_t[tid + half];
-            }
+            if (tid < half && before(list[tid + half], list[tid])) list[tid] = list[tid + half];
             __syncthreads();
         }
-        last = held(0);
+        last = list[0];
         if (tid == 0) put(c, last);
     }
 }
 
-// 16-byte vectors to a thread: the fewest that leave the chip four workgroups a compute unit, at most 8 (float32: 16, the same elements)
+// 16-byte vectors to a thread: the most, up to 4, that leave the chip four workgroups a compute unit.  (8: fewer wavefronts fit to
+// wait for memory, 256 bfloat16 rows of 152 064: 28 us, and 24.4 with 4; 2: 26.9, and twice the candidates to merge)
 inline int beam_vectors(const BeamArgs &x) {
     const int vec = x.dtype == KVHIP_F32 ? 4 : 8;
     const int64_t rows = (int64_t)x.groups * x.beams;
-    int nv = 8;
+    int nv = 4;
     while (nv > 1 && rows * ((x.vocabulary + 256 * nv * vec - 1) / (256 * nv * vec)) < 1024) nv >>= 1;
     return nv;
 }
@@ -422,7 +460,7 @@ hipError_t launch_beam_select(const BeamArgs &x, void *workspace, hipStream_t s)
     const dim3 grid(w.segments, x.groups * x.beams), block(256);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, x, w); };
 #define KV_GO(DT, NV) (wide ? go(beam_rows_kernel<DT, NV, true>) : go(beam_rows_kernel<DT, NV, false>))
-#define KV_SIZE(DT) (nv == 8 ? KV_GO(DT, 8) : nv == 4 ? KV_GO(DT, 4) : nv == 2 ? KV_GO(DT, 2) : KV_GO(DT, 1))
+#define KV_SIZE(DT) (nv == 4 ? KV_GO(DT, 4) : nv == 2 ? KV_GO(DT, 2) : KV_GO(DT, 1))
     if (x.dtype == KVHIP_F16) KV_SIZE(0);
     else if (x.dtype == KVHIP_BF16) KV_SIZE(1);
     else KV_SIZE(2);

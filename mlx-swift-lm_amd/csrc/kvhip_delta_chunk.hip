@@ -698,7 +698,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
 inline int chunk_key_dim(const DeltaArgs &x) { return x.Dk <= 64 ? 64 : x.Dk <= 128 ? 128 : 256; }
 // What a chunk of all sequences and heads takes, and how many chunks are laid out at a time: what they take is to stay in the
 // last-level cache between the two kernels.
-constexpr uint64_t CHUNK_SPACE = (uint64_t)192 << 20;
+constexpr uint64_t CHUNK_SPACE = (uint64_t)384 << 20;
 inline ChunkSpace chunk_space(const DeltaArgs &x, void *workspace, uint64_t *bytes) {
     ChunkSpace w{};
     const uint64_t rows = (uint64_t)CHUNK * chunk_key_dim(x) * 2 * (x.dtype == KVHIP_F16 ? 2 : 1);
@@ -744,7 +744,13 @@ template <int DT, int KD> hipError_t launch_chunks(const DeltaArgs &x, ChunkSpac
 
 }  // namespace
 
-bool delta_takes_chunks(const DeltaArgs &x) { return x.dtype != KVHIP_F32 && x.L > 16 && (int64_t)x.B * x.Hv * ((x.Dv + 15) / 16) < ((int64_t)1 << 31); }
+// From how many tokens on, by the rows of all states (a token costs the other kernel what they take to pass through the vector
+// units, a chunk costs much the same whatever it holds).  32 heads x 128 x 128, us by chunks / by tokens: one sequence, 6 tokens 14.8 / 14.0, 8: 14.8 /
+// 17.5; 8 sequences, 10: 34.4 / 28.9, 12: 34.5 / 33.7, 16: 34.5 / 42.4; 64 sequences, 12: 200 / 189, 16: 204 / 242.
+bool delta_takes_chunks(const DeltaArgs &x) {
+    const int64_t rows = (int64_t)x.B * x.Hv * x.Dv;
+    return x.dtype != KVHIP_F32 && x.L > (rows <= 8192 ? 7 : rows <= 65536 ? 11 : 15) && rows < ((int64_t)1 << 31);
+}
 
 size_t delta_chunk_workspace(const DeltaArgs &x) {
     uint64_t bytes = 0;

@@ -10,6 +10,7 @@
 // eight lanes (three permutes each) run side by side.  Every lane makes the token's norms and gates for itself.
 #include "kvhip_delta.hpp"
 #include "kvhip_device.hpp"
+#include "kvhip_wave.hpp"
 
 namespace kvhip {
 namespace {
@@ -71,7 +72,7 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs x) {
             s[r][c] = x.state_in && row < Dv ? load4<2, WIDE>(p + 4 * d, Dk - d) : kv_f4{0.f, 0.f, 0.f, 0.f};
         }
     }
-    const float rate = x.a_log ? expf(x.a_log[h]) : 0.f, dt = x.a_log && x.dt_bias ? x.dt_bias[h] : 0.f;
+    const float rate = x.a_log ? LOG2E * expf(x.a_log[h]) : 0.f, dt = x.a_log && x.dt_bias ? x.dt_bias[h] : 0.f;
     const char *qp = x.q + ((int64_t)b * x.q_sb + (int64_t)hk * Dk) * ES, *kp = x.k + ((int64_t)b * x.k_sb + (int64_t)hk * Dk) * ES;
     const char *vp = x.v + ((int64_t)b * x.v_sb + (int64_t)h * Dv) * ES;
     char *op = x.out + ((int64_t)b * x.L * x.Hv + h) * Dv * ES;
@@ -126,17 +127,17 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs x) {
         float g, beta;
         if (x.a_log) {
             const float t = ga + dt;
-            g = expf(-rate * (fmaxf(t, 0.f) + log1pf(expf(-fabsf(t)))));
-            beta = 1.f / (1.f + expf(-gb));
+            g = fast_exp2(-rate * (fmaxf(t, 0.f) + log1pf(fast_exp2(-LOG2E * fabsf(t)))));
+            beta = __builtin_amdgcn_rcpf(1.f + fast_exp2(-LOG2E * gb));
         } else {
-            g = expf(ga);
+            g = fast_exp2(LOG2E * ga);
             beta = gb;
         }
         if (l + 1 < end) request(l + 1);
         qq = sum8(qq);
         kk = sum8(kk);
         qk = sum8(qk);
-        const float kf = x.eps > 0.f ? 1.f / sqrtf(kk + x.eps) : 1.f, qf = x.scale * (x.eps > 0.f ? 1.f / sqrtf(qq + x.eps) : 1.f);
+        const float kf = x.eps > 0.f ? __builtin_amdgcn_rsqf(kk + x.eps) : 1.f, qf = x.scale * (x.eps > 0.f ? __builtin_amdgcn_rsqf(qq + x.eps) : 1.f);
         const float qkf = qk * kf * qf;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs x) {
 // neighbouring channels (16 bytes) of CONV_TOKENS tokens: a token is read once, the taps slide through registers.  Tiles of
 // tokens start at the sequence's first one (left_pad), so that the first tile alone reads the window -- and can write the new
 // one over it.
-constexpr int CONV_TOKENS = 32, CONV_AHEAD = 8;
+constexpr int CONV_TOKENS = 32, CONV_AHEAD = 4;
 
 template <int DT, int V> struct ConvRow {
     float v[V];
@@ -290,7 +291,7 @@ __global__ void __launch_bounds__(256) short_conv_kernel(ConvArgs x) {
                 float s = bias[i];
 #pragma unroll
                 for (int m = 0; m < WT; ++m) s = fmaf(w[m][i], e[t + m].v[i], s);
-                y.v[i] = x.silu ? s / (1.f + expf(-s)) : s;
+                y.v[i] = x.silu ? s * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * -LOG2E)) : s;
             }
             y.store(op + (l + t) * cs);
         }
@@ -302,18 +303,21 @@ __global__ void __launch_bounds__(256) short_conv_kernel(ConvArgs x) {
 }  // namespace
 
 hipError_t launch_delta_steps(const DeltaArgs &x, hipStream_t s) {
-    // Rows of S to a lane: as many as leave every compute unit two wavefronts; a lane's operands are then shared by more rows.
+    // Rows of S to a lane: a token's norms and gates, which every wavefront makes for itself, then serve more rows, but fewer
+    // wavefronts wait for memory.  32 heads x 128 x 128, us with 1 / 2 / 4 rows: 4 sequences 6.8 / 7.0 / 8.2, 8: 9.4 / 8.9 / 10.1, 16:
+    // 18.5 / 16.9 / 12.9, 64: 65.9 / 57.3 / 55.0; 5 float32 tokens of 16: 33.3 / 26.0 / 21.8.  Keys of 256, 4 heads of 512, 32
+    // sequences: 40.0 / 32.5 / 34.4.
     const int64_t rows = (int64_t)x.B * x.Hv * x.Dv;
     const int es = x.dtype == KVHIP_F32 ? 4 : 2;
     auto even = [&](const char *p, int64_t sb, int64_t sl) { return ((uintptr_t)p | (uint64_t)(sb * es) | (uint64_t)(sl * es)) % (4 * es) == 0; };
     const bool wide = x.Dk % 4 == 0 && even(x.q, x.q_sb, x.q_sl) && even(x.k, x.k_sb, x.k_sl) &&
                       ((uintptr_t)x.state_in | (uintptr_t)x.state_out) % 16 == 0;
-    const int R = rows >= 16384 ? 4 : 1;
+    const int R = rows < 32768 ? 1 : rows < 65536 || x.Dk > 128 ? 2 : 4;
     const int waves = 4, per = waves * 8 * R;
     const dim3 grid((x.Dv + per - 1) / per, x.Hv, x.B), block(64 * waves);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, x); };
 #define KV_GO(DT, NC, RR) (wide ? go(delta_steps_kernel<DT, NC, RR, true>) : go(delta_steps_kernel<DT, NC, RR, false>))
-#define KV_ROWS(DT, NC) (R == 4 ? KV_GO(DT, NC, 4) : KV_GO(DT, NC, 1))
+#define KV_ROWS(DT, NC) (R == 4 ? KV_GO(DT, NC, (NC < 8 ? 4 : 2)) : R == 2 ? KV_GO(DT, NC, 2) : KV_GO(DT, NC, 1))
 #define KV_SIZE(DT)                                 \
     do {                                            \
         if (x.Dk <= 64) KV_ROWS(DT, 2);             \
