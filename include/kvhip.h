@@ -397,6 +397,7 @@ typedef struct kvhip_gated_delta_args {
     int32_t dtype, gate_dtype;
     float scale, norm_eps;
 } kvhip_gated_delta_args;
+/* (of the sizes and types in args alone) */
 size_t kvhip_gated_delta_workspace(const kvhip_gated_delta_args *args);
 kvhip_status kvhip_gated_delta(const kvhip_gated_delta_args *args, void *workspace, size_t workspace_bytes, void *stream);
 

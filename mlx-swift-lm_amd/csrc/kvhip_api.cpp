@@ -1814,9 +1814,10 @@ kvhip_status kvhip_short_convolution(const void *x, int64_t x_stride_b, int64_t 
     return KVHIP_OK;
 }
 
-static kvhip_status delta_args(const kvhip_gated_delta_args *p, DeltaArgs &x) {
+// `arrays` false: the sizes alone (what a call would take)
+static kvhip_status delta_args(const kvhip_gated_delta_args *p, DeltaArgs &x, bool arrays = true) {
     if (!p) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
-    if (!p->q || !p->k || !p->v || !p->a || !p->b || !p->state_out || !p->out) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
+    if (arrays && (!p->q || !p->k || !p->v || !p->a || !p->b || !p->state_out || !p->out)) return fail(KVHIP_ERR_INVALID_ARG, "null argument");
     if (p->B <= 0 || p->L <= 0 || p->Hk <= 0 || p->Hv <= 0 || p->Dk <= 0 || p->Dv <= 0) return fail(KVHIP_ERR_INVALID_ARG, "non-positive shape");
     for (int64_t s : {p->q_stride_b, p->q_stride_l, p->k_stride_b, p->k_stride_l, p->v_stride_b, p->v_stride_l, p->a_stride_b, p->a_stride_l,
                       p->b_stride_b, p->b_stride_l})
@@ -1848,7 +1849,7 @@ static kvhip_status delta_args(const kvhip_gated_delta_args *p, DeltaArgs &x) {
 }
 size_t kvhip_gated_delta_workspace(const kvhip_gated_delta_args *p) {
     DeltaArgs x;
-    return delta_args(p, x) == KVHIP_OK && delta_takes_chunks(x) ? delta_chunk_workspace(x) : 0;
+    return delta_args(p, x, false) == KVHIP_OK && delta_takes_chunks(x) ? delta_chunk_workspace(x) : 0;
 }
 kvhip_status kvhip_gated_delta(const kvhip_gated_delta_args *p, void *workspace, size_t workspace_bytes, void *stream) {
     DeltaArgs x;

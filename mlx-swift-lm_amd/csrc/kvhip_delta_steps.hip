@@ -242,6 +242,23 @@ __global__ void __launch_bounds__(256) short_conv_kernel(ConvArgs x) {
     const int l0 = from + tile, l1 = min(l0 + CONV_TOKENS, end);
     for (int l = max(l0, end); l < min(l0 + CONV_TOKENS, x.L); ++l) none.store(op + l * cs);
     if (l0 >= l1 && tile > 0) return;
+    float w[WT][V], bias[V];
+    if (WT == 4 && V > 1 && x.W == 4 && (uintptr_t)x.weight % 16 == 0) {  // (four taps of V channels: 64 bytes side by side)
+        ConvRow<DT, V> packed[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) packed[m].load(x.weight + (int64_t)c * 4 * ES + m * 16);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) w[t][i] = packed[(i * 4 + t) / V].v[(i * 4 + t) % V];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int t = 0; t < WT; ++t) w[t][i] = t >= skip ? Elem<DT>::load(x.weight, (int64_t)(c + i) * x.W + t - skip) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) bias[i] = x.bias ? Elem<DT>::load(x.bias, c + i) : 0.f;
     ConvRow<DT, V> e[WT - 1 + CONV_AHEAD];  // rows l - (WT - 1) on
     // (row i of the window is e's row skip + i)
 #pragma unroll
@@ -268,13 +285,6 @@ __global__ void __launch_bounds__(256) short_conv_kernel(ConvArgs x) {
             }
             r.store(wout + (i - skip) * cs);
         }
-    }
-    float w[WT][V], bias[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bias[i] = x.bias ? Elem<DT>::load(x.bias, c + i) : 0.f;
-#pragma unroll
-        for (int t = 0; t < WT; ++t) w[t][i] = t >= skip ? Elem<DT>::load(x.weight, (int64_t)(c + i) * x.W + t - skip) : 0.f;
     }
     for (int l = l0; l < l1; l += CONV_AHEAD) {
 #pragma unroll

@@ -167,11 +167,24 @@ def step():
         from .rope import RoPE
 
         module.bind(torch.Tensor, RoPE, (torch.float16, torch.bfloat16, torch.float32), torch._C._cuda_getDevice,
-                    torch._C._cuda_getCurrentRawStream)
+                    torch._C._cuda_getCurrentRawStream, {"dtype": torch.int32})
         lib = load()
         at = [C.cast(getattr(lib, name), C.c_void_p).value for name in ("kvhip_cache_update_attend", "kvhip_cache_update_attend_rope")]
         _step = (module, at[0], at[1])
     return _step
+
+
+_native = {}
+
+
+def native(name, entry):
+    """The extension's call `name` for an entry point that takes a workspace: (the call, or None where it is not built, the entry
+    point's address, and that of its `_workspace`)."""
+    if name not in _native:
+        module, lib = step()[0], load()
+        at = [C.cast(getattr(lib, e), C.c_void_p).value for e in (entry, entry + "_workspace")]
+        _native[name] = (getattr(module, name) if module else None, *at)
+    return _native[name]
 
 
 def check(status):

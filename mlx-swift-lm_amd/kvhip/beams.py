@@ -14,6 +14,14 @@ def beam_select(logits, scores=None, count=None, done=None, pad_token=0):
     `pad_token` alone, at their own score.  `rows` are rows of the B K logits (int32), an order for `cache.reorder` when count
     is K; a continuation scores scores + log softmax(logits); among equals the lower beam, then the higher logit, then the lower
     token.  Where there are fewer candidates: -1, -1 and minus infinity."""
+    if scores is not None and done is None and logits.is_cuda:
+        L.init()
+        native, entry, workspace = L.native("select", "kvhip_beam_select")  # (of the ordinary form, as one native call)
+        out = native(entry, workspace, logits, scores, logits.shape[1] if count is None else count, pad_token) if native and logits.dim() == 3 else None
+        if type(out) is int:
+            L.check(out)
+        if out is not None:
+            return out
     if logits.dim() != 3 or logits.dtype not in _DT:
         raise ValueError(f"logits are [B, K, V] in float16, bfloat16 or float32, not {logits.dtype} {tuple(logits.shape)}")
     B, K, V = logits.shape

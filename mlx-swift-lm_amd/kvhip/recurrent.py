@@ -200,6 +200,15 @@ class GatedDeltaCache:
         """The gated delta rule over q, k [B, L, Hk, Dk] and v [B, L, Hv, Dv] from this cache's state on, which moves on: [B, L, Hv, Dv].
         a, b [B, L, Hv]: with a_log [Hv] what the decays exp(-exp(a_log) softplus(a + dt_bias)) and the rates sigmoid(b) come from, without
         it the decays' logarithms and the rates themselves.  `scale` defaults to Dk^-0.5; norm_eps 0 leaves q and k as they are."""
+        state = self._held("_state")
+        if state is not None and left_pad is None and lengths is None and a_log is not None and dt_bias is not None:
+            native, entry, workspace = L.native("delta", "kvhip_gated_delta")  # (a step of the ordinary form, as one native call)
+            out = native(entry, workspace, q, k, v, a, b, a_log, dt_bias, state, scale, norm_eps) if native else None
+            if type(out) is int:
+                L.check(out)
+            if out is not None:
+                self.offset += out.shape[1]
+                return out
         if any(t.dim() != 4 for t in (q, k, v)) or q.shape != k.shape or q.shape[:2] != v.shape[:2]:
             raise ValueError(f"queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not go together")
         B, n, Hk, Dk = k.shape
@@ -213,7 +222,6 @@ class GatedDeltaCache:
                 raise ValueError(f"{name} is one number to each of {Hv} heads, not {tuple(t.shape)}")
         if dt_bias is not None and a_log is None:
             raise ValueError("dt_bias goes with a_log")
-        state = self._held("_state")
         if state is not None and tuple(state.shape) != (B, Hv, Dv, Dk):
             raise ValueError(f"keys {tuple(k.shape)} and values {tuple(v.shape)} do not go with the state {tuple(state.shape)}")
         _on_current_device(q, k, v, a, b, a_log, dt_bias, state)
