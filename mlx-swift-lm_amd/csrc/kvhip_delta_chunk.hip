@@ -98,7 +98,7 @@ struct ChunkSpan {
 
 // KD: channels of a key as they are laid out (zeros behind Dk); WIDE: rows of whole 16-byte pieces
 template <int DT, int KD, bool WIDE>
-__global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace w) {
+__global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(DeltaArgs x, ChunkSpace w) {
     constexpr int PITCH = KD + 8, KP = DT == 0 ? 2 : 1, ROW = CHUNK + 4, BYTES = CHUNK * PITCH * 2;
     constexpr double LOG2E_64 = 1.4426950408889634074;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
@@ -106,12 +106,13 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
     const ChunkSpan span(x, b);
     const int t0 = (w.chunk0 + c) * CHUNK;
     if (!span.any(w.chunk0 + c)) return;
-    __shared__ __align__(16) char keys[BYTES], queries[BYTES > CHUNK * ROW * 4 ? BYTES : CHUNK * ROW * 4];
-    __shared__ __align__(16) float Ts[CHUNK][ROW];  // P, then T
+    constexpr int PLACE = BYTES > CHUNK * ROW * 4 ? BYTES : CHUNK * ROW * 4;
+    __shared__ __align__(16) char keys[PLACE], queries[PLACE];
     __shared__ float rk[CHUNK], rq[CHUNK], beta[CHUNK], p_unit[CHUNK];
     __shared__ double total[CHUNK];  // decays summed up, as powers of two
     uint16_t *ks = reinterpret_cast<uint16_t *>(keys), *qs = reinterpret_cast<uint16_t *>(queries);
-    float(*As)[ROW] = reinterpret_cast<float(*)[ROW]>(queries);  // (in the queries' place behind their product)
+    // behind their products, in the rows' places: A in the queries' (in front of it P, a wavefront's rows at a time), T in the keys'
+    float(*As)[ROW] = reinterpret_cast<float(*)[ROW]>(queries), (*Ts)[ROW] = reinterpret_cast<float(*)[ROW]>(keys);
     float decay = 0.f, rate = 0.f;
     if (wave == 0 && t0 + lane >= span.from && t0 + lane < span.end) {
         const int64_t t = t0 + lane, ai = (int64_t)b * x.a_sb + t * x.a_sl + h, bi = (int64_t)b * x.b_sb + t * x.b_sl + h;
@@ -231,11 +232,26 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
                 qk[j] = DT == 1 ? mfma_bf16(qa, kb, qk[j]) : mfma_f16(qa, kb, qk[j]);
             }
         }
-        if (lays_rows)
+        if (lays_rows) {
 #pragma unroll
-            for (int s = 0; s < KD / 32; ++s) lay_rows(qs, key + w.q, wave, s);
+            for (int s = 0; s < KD / 32; ++s) {
+                lay_rows(qs, key + w.q, wave, s);
+                lay_rows(ks, key, wave, s);
+            }
+#pragma unroll 2
+            for (int i = wave; i < KD / 16 * 2; i += 4) {  // channels 16 mt + n, tokens 32 s + 4 g and 16 on
+                const int mt = i >> 1, s = i & 1;
+                kv_u4 v;
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const uint16_t *p = ks + (32 * s + 16 * (m >> 1) + 4 * g + 2 * (m & 1)) * PITCH + 16 * mt + n;
+                    v[m] = p[0] | (uint32_t)p[PITCH] << 16;
+                }
+                lay(key + w.kt + (int64_t)i * 1024 + lane * 16, v);
+            }
+        }
     }
-    __syncthreads();  // (the queries have been read)
+    __syncthreads();  // (the rows have been read)
     {
         double mine[4];
         float b0[4], q0[4];
@@ -254,13 +270,9 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int row = 16 * wave + 4 * g + r;
-                if (j > wave) {
-                    Ts[row][col] = 0.f;
-                    continue;
-                }
-                const float fade = col <= row ? __builtin_amdgcn_exp2f((float)(mine[r] - other)) * k0 : 0.f;
-                As[row][col] = col < row ? b0[r] * fade * kk[j][r] : 0.f;
-                Ts[row][col] = q0[r] * fade * qk[j][r];
+                const float fade = j <= wave && col <= row ? __builtin_amdgcn_exp2f((float)(mine[r] - other)) * k0 : 0.f;
+                kk[j][r] *= col < row ? b0[r] * fade : 0.f;
+                As[row][col] = q0[r] * fade * qk[j][r];  // (P)
             }
         }
     }
@@ -270,7 +282,7 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int m = 0; m < 8; ++m) {
-                v[s][m] = Ts[16 * wave + n][32 * s + 16 * (m >> 2) + 4 * g + (m & 3)];
+                v[s][m] = As[16 * wave + n][32 * s + 16 * (m >> 2) + 4 * g + (m & 3)];
                 top = fmaxf(top, fabsf(v[s][m]));
             }
         const float unit = unit_of(column_max(top)), f = over(unit);
@@ -289,9 +301,13 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
             if (DT == 0) *reinterpret_cast<kv_u4 *>(p + 8192 + (wave * 2 + s) * 1024 + lane * 16) = low;
         }
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) As[16 * wave + 4 * g + r][16 * j + n] = kk[j][r];
     __syncthreads();
-    // (I + A)^-1 in blocks of 16: those of the diagonal by substitution, a column of a block to a lane of the first wavefront,
-    // while the others put away what is left ...
+    // (I + A)^-1 in blocks of 16: those of the diagonal by substitution, a column of a block to a lane of the first wavefront
+    // ...
     if (wave == 0) {
         float t[16];
         const int o = 16 * g;
@@ -309,19 +325,6 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(DeltaArgs x, ChunkSpace
             Ts[o + i][o + n] = t[i];
         }
     } else {
-        if (lays_rows) {
-            for (int i = wave - 1; i < 4 * (KD / 32); i += 3) lay_rows(ks, key, i & 3, i >> 2);
-            for (int i = wave - 1; i < KD / 16 * 2; i += 3) {  // channels 16 mt + n, tokens 32 s + 4 g and 16 on
-                const int mt = i >> 1, s = i & 1;
-                kv_u4 v;
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    const uint16_t *p = ks + (32 * s + 16 * (m >> 1) + 4 * g + 2 * (m & 1)) * PITCH + 16 * mt + n;
-                    v[m] = p[0] | (uint32_t)p[PITCH] << 16;
-                }
-                lay(key + w.kt + (int64_t)i * 1024 + lane * 16, v);
-            }
-        }
         if (wave == 1) {
             float *f = reinterpret_cast<float *>(head + T_BYTES + P_BYTES);
             const double mine = total[lane], last = total[CHUNK - 1];

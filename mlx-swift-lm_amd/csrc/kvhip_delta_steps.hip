@@ -6,7 +6,7 @@
 // delta_steps_kernel keeps S in registers over all tokens of a call: eight lanes hold a row of S (one channel of the values),
 // four neighbouring elements in every 32 each, so that a wavefront's load is eight whole cache lines.  Rows never meet: a
 // wavefront needs no other, nothing goes through LDS, and a head's rows are spread over as many wavefronts as fill the chip.  With
-// o = g (S k-free) written out,  o = g (S q^) + u (k^ q^),  both products of a token read the same S and their sums over the
+// o written as  g (S q^) + u (k^ q^),  both products of a token read the same S and their sums over the
 // eight lanes (three permutes each) run side by side.  Every lane makes the token's norms and gates for itself.
 #include "kvhip_delta.hpp"
 #include "kvhip_device.hpp"
@@ -69,7 +69,10 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs x) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d = 32 * c + 4 * j;
-            s[r][c] = x.state_in && row < Dv ? load4<2, WIDE>(p + 4 * d, Dk - d) : kv_f4{0.f, 0.f, 0.f, 0.f};
+            s[r][c] = kv_f4{0.f, 0.f, 0.f, 0.f};
+            if (!x.state_in || row >= Dv) continue;
+            if constexpr (!WIDE) s[r][c] = load4<2, false>(p + 4 * d, Dk - d);
+            else if (d < Dk) s[r][c] = __builtin_nontemporal_load(reinterpret_cast<const kv_f4 *>(p + 4 * d));
         }
     }
     const float rate = x.a_log ? LOG2E * expf(x.a_log[h]) : 0.f, dt = x.a_log && x.dt_bias ? x.dt_bias[h] : 0.f;
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs x) {
         for (int c = 0; c < NC; ++c) {
             const int d = 32 * c + 4 * j;
             if constexpr (WIDE) {
-                if (d < Dk) *reinterpret_cast<kv_f4 *>(p + d) = s[r][c];
+                if (d < Dk) __builtin_nontemporal_store(s[r][c], reinterpret_cast<kv_f4 *>(p + d));
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
