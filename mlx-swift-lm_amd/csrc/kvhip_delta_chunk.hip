@@ -9,15 +9,19 @@
 // of the values to a workgroup (columns never meet), the state in its accumulators: wavefront w holds rows of dk of S^T and does
 // rows 16 w .. of every product.
 //
-// Numbers.  The state is returned in float32, so everything that it is made from keeps float32's accuracy.  Norms are factors
-// of rows, put on in float32 behind the products: the operands Q and K stay what they came as, exact in one part of bfloat16
-// (float16: two).  S, T, U and what T is multiplied with are split into three parts of bfloat16 each (24 bits, float32's whole
-// range), of which the products below 2^-24 are left out.  Decays are summed in float64: e^-1000 beside e^-0.001 loses nothing.  The output, which is rounded to 16 bits,
-// takes two parts of S and one of U and P, in float16 over powers of two for each row and column (float16: two).
+// Numbers.  The state is returned in float32, so everything that it is made from keeps float32's accuracy on 16-bit operands.  Norms are
+// factors of rows, put on in float32 behind the products: Q and K stay what they came as, in float16 over a power of two for
+// each row (exact, but for elements below 2^-28 of the row's largest).  The state and what is added to it are two parts of float16
+// (22 bits) over powers of two for each column: of a wavefront's rows of the state the largest is at hand, of
+// diag(e^(G_63 - G)) U it is bounded by that of X and the largest sum over a row of T.  T and X are three parts of bfloat16 (24 bits, float32's
+// range), of which the products below 2^-24 are left out.  Decays are summed in float64: e^-1000 beside e^-0.001 loses
+// nothing.  The outputs, rounded to 16 bits, take one part of S, P and U each (float16: two).
 //
 // Operands lie in the workspace as the lanes take them, 1 KB to an instruction: contractions may be summed in any
 // order, so that lane (n, g)'s eight elements of a step are those at 4 g and 16 + 4 g of it -- which is where a product leaves them: S, U
 // go from accumulators to operands without crossing lanes, only from wavefront to wavefront through LDS.
+#include <type_traits>
+
 #include "kvhip_delta.hpp"
 #include "kvhip_device.hpp"
 
@@ -83,8 +87,9 @@ struct ChunkSpace {
 __device__ __forceinline__ char *key_at(const ChunkSpace &w, int64_t bh, int c) { return w.base + (bh * w.chunks + c) * w.key; }
 __device__ __forceinline__ char *head_at(const ChunkSpace &w, int64_t bh, int c) { return w.base + w.heads + (bh * w.chunks + c) * w.head; }
 constexpr int T_BYTES = CHUNK * CHUNK * 6, P_BYTES = CHUNK * CHUNK * 4;  // three parts, and two (bfloat16: one is used)
-// factors of rows: e^G r_k (what K S is worth), scale e^G r_q, e^(G_63 - G) r_k, P's units, and e^G_63
-constexpr int RISE_K = 0, RISE_Q = CHUNK, FALL = 2 * CHUNK, P_UNIT = 3 * CHUNK, LAST = 4 * CHUNK;
+// Factors of rows, the units of their operands among them: e^G r_k (what K S is worth), scale e^G r_q, e^(G_63 - G) r_k, P's units; then
+// e^G_63, and the bound of |diag(e^(G_63 - G)) U| over the largest |X| of a column.
+constexpr int RISE_K = 0, RISE_Q = CHUNK, FALL = 2 * CHUNK, P_UNIT = 3 * CHUNK, LAST = 4 * CHUNK, GAIN = 4 * CHUNK + 1;
 constexpr int FACTOR_BYTES = 5 * CHUNK * 4;
 
 struct ChunkSpan {
@@ -99,7 +104,7 @@ struct ChunkSpan {
 // KD: channels of a key as they are laid out (zeros behind Dk); WIDE: rows of whole 16-byte pieces
 template <int DT, int KD, bool WIDE>
 __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(DeltaArgs x, ChunkSpace w) {
-    constexpr int PITCH = KD + 8, KP = DT == 0 ? 2 : 1, ROW = CHUNK + 4, BYTES = CHUNK * PITCH * 2;
+    constexpr int PITCH = KD + 8, ROW = CHUNK + 4, BYTES = CHUNK * PITCH * 2;
     constexpr double LOG2E_64 = 1.4426950408889634074;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
     const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, per = x.Hv / x.Hk, hk = h / per;
@@ -108,7 +113,7 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
     if (!span.any(w.chunk0 + c)) return;
     constexpr int PLACE = BYTES > CHUNK * ROW * 4 ? BYTES : CHUNK * ROW * 4;
     __shared__ __align__(16) char keys[PLACE], queries[PLACE];
-    __shared__ float rk[CHUNK], rq[CHUNK], beta[CHUNK], p_unit[CHUNK];
+    __shared__ float rk[CHUNK], rq[CHUNK], beta[CHUNK], p_unit[CHUNK], key_unit[CHUNK], query_unit[CHUNK], falls[CHUNK], tops[4];
     __shared__ double total[CHUNK];  // decays summed up, as powers of two
     uint16_t *ks = reinterpret_cast<uint16_t *>(keys), *qs = reinterpret_cast<uint16_t *>(queries);
     // behind their products, in the rows' places: A in the queries' (in front of it P, a wavefront's rows at a time), T in the keys'
@@ -127,7 +132,7 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
         const bool there = t >= span.from && t < span.end;
         const uint16_t *kp = reinterpret_cast<const uint16_t *>(x.k) + (int64_t)b * x.k_sb + (int64_t)t * x.k_sl + (int64_t)hk * x.Dk;
         const uint16_t *qp = reinterpret_cast<const uint16_t *>(x.q) + (int64_t)b * x.q_sb + (int64_t)t * x.q_sl + (int64_t)hk * x.Dk;
-        float sk = 0.f, sq = 0.f;
+        float sk = 0.f, sq = 0.f, mk = 0.f, mq = 0.f;
         kv_u4 kw[KD / 32], qw[KD / 32];
 #pragma unroll
         for (int i = 0; i < KD / 32; ++i) {
@@ -164,15 +169,22 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
                 }
                 sk = fmaf(k1, k1, fmaf(k0, k0, sk));
                 sq = fmaf(q1, q1, fmaf(q0, q0, sq));
+                mk = fmaxf(mk, fmaxf(fabsf(k0), fabsf(k1)));
+                mq = fmaxf(mq, fmaxf(fabsf(q0), fabsf(q1)));
             }
         }
-        sk += __shfl_xor(sk, 1);
-        sk += __shfl_xor(sk, 2);
-        sq += __shfl_xor(sq, 1);
-        sq += __shfl_xor(sq, 2);
+#pragma unroll
+        for (int m = 1; m < 4; m <<= 1) {
+            sk += __shfl_xor(sk, m);
+            sq += __shfl_xor(sq, m);
+            mk = fmaxf(mk, __shfl_xor(mk, m));
+            mq = fmaxf(mq, __shfl_xor(mq, m));
+        }
         if ((tid & 3) == 0) {
-            rk[row] = x.eps > 0.f ? 1.f / sqrtf(sk + x.eps) : 1.f;
-            rq[row] = x.scale * (x.eps > 0.f ? 1.f / sqrtf(sq + x.eps) : 1.f);
+            rk[row] = x.eps > 0.f ? __builtin_amdgcn_rsqf(sk + x.eps) : 1.f;
+            rq[row] = x.scale * (x.eps > 0.f ? __builtin_amdgcn_rsqf(sq + x.eps) : 1.f);
+            key_unit[row] = unit_of(mk);
+            query_unit[row] = unit_of(mq);
         }
     }
     if (wave == 0) {  // gates, and the decays summed up
@@ -193,28 +205,17 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
     __syncthreads();
     char *head = head_at(w, (int64_t)b * x.Hv + h, c), *key = key_at(w, (int64_t)b * x.Hk + hk, c);
     const bool lays_rows = h % per == 0;  // the rows as operands, once for the heads that share them
-    auto parts = [&](kv_u4 v, kv_u4 &low) {  // (float16: bfloat16's part of each element, and what is left)
-        if constexpr (DT == 1) return v;
-        kv_u4 r;
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const kv_half2 e = as_h2(v[m]);
-            float a = (float)e.x, o = (float)e.y;
-            r[m] = take_part(a, o);
-            low[m] = pk_bf2(a, o);
-        }
-        return r;
-    };
-    auto lay = [&](char *to, kv_u4 v) {
-        kv_u4 low;
-        *reinterpret_cast<kv_u4 *>(to) = parts(v, low);
-        if (KP == 2) *reinterpret_cast<kv_u4 *>(to + CHUNK * KD * 2) = low;
+    // 16-bit elements of rows as float16, each over its row's unit
+    auto scaled = [&](uint32_t v, float f0, float f1) {
+        if constexpr (DT == 1) return pk_h2(__uint_as_float(v << 16) * f0, __uint_as_float(v & 0xffff0000u) * f1);
+        const kv_half2 e = as_h2(v);
+        return pk_h2((float)e.x * f0, (float)e.y * f1);
     };
     // rows 16 mt + n, channels 32 s + 4 g and 16 on
-    auto lay_rows = [&](const uint16_t *rows, char *to, int mt, int s) {
+    auto lay_rows = [&](const uint16_t *rows, float f, char *to, int mt, int s) {
         const uint16_t *p = rows + (16 * mt + n) * PITCH + 32 * s + 4 * g;
         const kv_u2 a = *reinterpret_cast<const kv_u2 *>(p), e = *reinterpret_cast<const kv_u2 *>(p + 16);
-        lay(to + ((int64_t)mt * (KD / 32) + s) * 1024 + lane * 16, kv_u4{a.x, a.y, e.x, e.y});
+        *reinterpret_cast<kv_u4 *>(to + ((int64_t)mt * (KD / 32) + s) * 1024 + lane * 16) = kv_u4{scaled(a.x, f, f), scaled(a.y, f, f), scaled(e.x, f, f), scaled(e.y, f, f)};
     };
     kv_f4 kk[4], qk[4];
     {  // k k^T and q k^T on and below the diagonal: wavefront w rows 16 w on
@@ -233,21 +234,25 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
             }
         }
         if (lays_rows) {
+            const float fq = over(query_unit[16 * wave + n]), fk = over(key_unit[16 * wave + n]);
 #pragma unroll
             for (int s = 0; s < KD / 32; ++s) {
-                lay_rows(qs, key + w.q, wave, s);
-                lay_rows(ks, key, wave, s);
+                lay_rows(qs, fq, key + w.q, wave, s);
+                lay_rows(ks, fk, key, wave, s);
             }
+            const int s = wave & 1;  // channels 16 mt + n, tokens 32 s + 4 g and 16 on
+            float f[8];
+#pragma unroll
+            for (int m = 0; m < 8; ++m) f[m] = over(key_unit[32 * s + 16 * (m >> 2) + 4 * g + (m & 3)]);
 #pragma unroll 2
-            for (int i = wave; i < KD / 16 * 2; i += 4) {  // channels 16 mt + n, tokens 32 s + 4 g and 16 on
-                const int mt = i >> 1, s = i & 1;
+            for (int mt = wave >> 1; mt < KD / 16; mt += 2) {
                 kv_u4 v;
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     const uint16_t *p = ks + (32 * s + 16 * (m >> 1) + 4 * g + 2 * (m & 1)) * PITCH + 16 * mt + n;
-                    v[m] = p[0] | (uint32_t)p[PITCH] << 16;
+                    v[m] = scaled(p[0] | (uint32_t)p[PITCH] << 16, f[2 * m], f[2 * m + 1]);
                 }
-                lay(key + w.kt + (int64_t)i * 1024 + lane * 16, v);
+                *reinterpret_cast<kv_u4 *>(key + w.kt + (mt * 2 + s) * 1024 + lane * 16) = v;
             }
         }
     }
@@ -329,9 +334,9 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
             float *f = reinterpret_cast<float *>(head + T_BYTES + P_BYTES);
             const double mine = total[lane], last = total[CHUNK - 1];
             const float rise = __builtin_amdgcn_exp2f((float)mine);
-            f[RISE_K + lane] = rise * rk[lane];
-            f[RISE_Q + lane] = rise * rq[lane];
-            f[FALL + lane] = __builtin_amdgcn_exp2f((float)(last - mine)) * rk[lane];
+            f[RISE_K + lane] = rise * rk[lane] * key_unit[lane];
+            f[RISE_Q + lane] = rise * rq[lane] * query_unit[lane];
+            f[FALL + lane] = falls[lane] = __builtin_amdgcn_exp2f((float)(last - mine)) * rk[lane] * key_unit[lane];
             f[P_UNIT + lane] = p_unit[lane];
             if (lane == 0) f[LAST] = __builtin_amdgcn_exp2f((float)last);
         }
@@ -358,7 +363,9 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
         }
         __syncthreads();
     }
-    // T in three parts: rows 16 w + n, tokens 32 s + 4 g and 16 on (zero above the diagonal)
+    // T in three parts: rows 16 w + n, tokens 32 s + 4 g and 16 on (zero above the diagonal); and how much of X's largest can come
+    // to be added to the state
+    float sum = 0.f;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         if (2 * s > wave) break;
@@ -367,6 +374,7 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
         for (int m = 0; m < 8; ++m) {
             const int col = 32 * s + 16 * (m >> 2) + 4 * g + (m & 3);
             t[m] = col / 16 <= wave ? Ts[16 * wave + n][col] * beta[col] : 0.f;
+            sum += fabsf(t[m]);
         }
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
@@ -376,13 +384,21 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
             *reinterpret_cast<kv_u4 *>(head + p * 8192 + (wave * 2 + s) * 1024 + lane * 16) = part;
         }
     }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    sum *= falls[16 * wave + n];
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) sum = fmaxf(sum, __shfl_xor(sum, m));
+    if (lane == 0) tops[wave] = sum;
+    __syncthreads();
+    if (tid == 0) reinterpret_cast<float *>(head + T_BYTES + P_BYTES)[GAIN] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 }
 
 // NT: tiles of 16 value channels to a workgroup.  Wavefronts 0 to 3 carry the state, 4 to 7 make the outputs: what a chunk's outputs
-// need is off the way from one state to the next, and fills the other's waits on the same SIMDs.  (KP: parts of a key's element)
+// need is off the way from one state to the next, and fills the other's waits on the same SIMDs.
 template <int DT, int KD, int NT>
 __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSpace w, const float *state_in) {
-    constexpr int KP = DT == 0 ? 2 : 1, SP = KP, KS = KD / 32, TPW = KD / 64, LOW = CHUNK * KD * 2;  // SP: parts of P and U in the outputs
+    constexpr int SP = DT == 0 ? 2 : 1, KS = KD / 32, TPW = KD / 64;  // SP: parts that outputs take; TPW: a wavefront's tiles of the state
     static_assert(KD % 64 == 0, "whole tiles to a wavefront");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6 & 3, n = lane & 15, g = lane >> 4;
     // (a head's workgroups on one die, where their operands meet in its cache: 8 dies take workgroups in turn)
@@ -390,10 +406,12 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
     const int b = bh / x.Hv, h = bh % x.Hv;
     const ChunkSpan span(x, b);
     const int64_t bk = (int64_t)b * x.Hk + h / (x.Hv / x.Hk);
-    __shared__ __align__(16) char sS[3 * KS * NT * 1024];  // the state's parts, an operand a step
+    __shared__ __align__(16) char sS[2 * KS * NT * 1024];  // the state's parts, an operand a step
     __shared__ __align__(16) char sX[3 * 2 * NT * 1024];   // X's parts
-    __shared__ __align__(16) char sF[3 * 2 * NT * 1024];   // parts of diag(e^(G_63 - G) r_k) U
+    __shared__ __align__(16) char sF[2 * 2 * NT * 1024];   // parts of diag(e^(G_63 - G) r_k) U
     __shared__ __align__(16) char sU[4 * NT * 1024];       // U, in float32
+    // by column and wavefront: the units of its rows of the state, and the largest of its rows of X
+    __shared__ __align__(16) float state_unit[NT][16][4], x_top[NT][16][4];
     // the sequence's chunks among those that are laid out
     const int c0 = max(span.from / CHUNK - w.chunk0, 0), c1 = min((span.end + CHUNK - 1) / CHUNK - w.chunk0, w.chunks);
     const bool none = span.from >= span.end || c0 >= c1;
@@ -403,6 +421,36 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
     const char *key = key_at(w, bk, c0) + lane * 16, *head = head_at(w, bh, c0) + lane * 16;
     const char *factors = head_at(w, bh, c0) + T_BYTES + P_BYTES, *factor = factors + (16 * wave + 4 * g) * 4;
     auto part_of = [&](char *base, int p, int steps, int s, int t) { return base + ((p * steps + s) * NT + t) * 1024 + lane * 16; };
+    // What LDS holds of a step is asked for at once and in front of its products: left alone, the compiler asks for each operand where it
+    // is used, and waits for LDS as often.  Requests to memory, which take their time to be issued, stand behind it, where a wavefront waits
+    // anyway, and not in front of a barrier.
+    auto all_requested = []() { __builtin_amdgcn_sched_barrier(0); };
+    // rows [KS] times the state's columns 16 t on, in PARTS parts: each wavefront's rows of it apart, then put together by their units
+    auto times_state = [&](auto parts, const kv_u4 *rows, int t, auto &&meanwhile) {
+        kv_f4 y[4], sum;
+        kv_u4 part[decltype(parts)::value][KS];
+#pragma unroll
+        for (int p = 0; p < decltype(parts)::value; ++p)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) part[p][s] = *reinterpret_cast<const kv_u4 *>(part_of(sS, p, KS, s, t));
+        const kv_f4 units = *reinterpret_cast<const kv_f4 *>(state_unit[t][n]);
+        all_requested();
+        meanwhile();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = kv_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = 0; p < decltype(parts)::value; ++p)
+#pragma unroll
+            for (int i = 0; i < 4 * TPW; i += TPW > 1 ? 2 : 1) {  // tiles of 16 rows, two to a step; of KD 64 a wavefront has half a step
+                const int s = i >> 1, k = i / TPW;
+                const kv_u4 &v = part[p][s];
+                if constexpr (TPW > 1) y[k] = mfma_f16(rows[s], v, y[k]);
+                else y[k] = mfma_f16(rows[s], i & 1 ? kv_u4{0, 0, v.z, v.w} : kv_u4{v.x, v.y, 0, 0}, y[k]);
+            }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[r] = fmaf(units[3], y[3][r], fmaf(units[2], y[2][r], fmaf(units[1], y[1][r], units[0] * y[0][r])));
+        return sum;
+    };
     // A chunk's operands are requested as soon as the last chunk's have been used, in the order in which they will be.
     if (threadIdx.x >= 256) {
         uint16_t *op = reinterpret_cast<uint16_t *>(x.out) + ((int64_t)b * x.L * x.Hv + h) * x.Dv + col0 + n;
@@ -417,15 +465,13 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                     if (row0 + r < x.L && col0 + 16 * t + n < x.Dv) op[(row0 + r) * o_sl + 16 * t] = 0;
         }
         if (none) return;
-        kv_u4 Q[KP][KS], P[SP][2];
+        kv_u4 Q[KS], P[SP][2];
         kv_f4 rise, unit;
         const int steps = wave < 2 ? 1 : 2;  // of P's rows that are not zero
         uint16_t *o = op + rows0 * o_sl;
         auto request_rows = [&](int64_t at) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int p = 0; p < KP; ++p) Q[p][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + w.q + p * LOW + (wave * KS + s) * 1024);
+            for (int s = 0; s < KS; ++s) Q[s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + w.q + (wave * KS + s) * 1024);
         };
         auto request_rest = [&](int64_t at) {
             rise = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + RISE_Q * 4);
@@ -441,18 +487,12 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
         for (int c = c0; c < c1; ++c) {
             const int next = min(c + 1, c1 - 1) - c0;
             kv_f4 O[NT], I[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) O[t] = I[t] = kv_f4{0.f, 0.f, 0.f, 0.f};
             lds_barrier();
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const kv_u4 s0 = *reinterpret_cast<const kv_u4 *>(part_of(sS, 0, KS, s, t)), s1 = *reinterpret_cast<const kv_u4 *>(part_of(sS, 1, KS, s, t));
-                    O[t] = mfma_bf16(Q[0][s], s0, O[t]);
-                    O[t] = mfma_bf16(Q[0][s], s1, O[t]);
-                    if constexpr (KP == 2) O[t] = mfma_bf16(Q[1][s], s0, O[t]);
-                }
+            for (int t = 0; t < NT; ++t) {
+                O[t] = times_state(std::integral_constant<int, SP>{}, Q, t, []() {});
+                I[t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+            }
             request_rows(next);
             lds_barrier();
             lds_barrier();
@@ -465,6 +505,11 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                 for (int k = 0; k < 4; ++k) {
                     if (k >= 2 * steps) break;
                     u[k] = *reinterpret_cast<const kv_f4 *>(sU + (k * NT + t) * 1024 + lane * 16);
+                }
+                all_requested();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (k >= 2 * steps) break;
                     top = fmaxf(top, fmaxf(fmaxf(fabsf(u[k][0]), fabsf(u[k][1])), fmaxf(fabsf(u[k][2]), fabsf(u[k][3]))));
                 }
                 u_unit[t] = unit_of(column_max(top));
@@ -532,15 +577,13 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
     if (!none) {
         const uint16_t *vp = reinterpret_cast<const uint16_t *>(x.v) + (int64_t)b * x.v_sb + (int64_t)h * x.Dv + col0, *v = vp + (int64_t)rows0 * x.v_sl + n;
         const int steps = wave < 2 ? 1 : 2;  // of T's rows that are not zero
-        kv_u4 K[KP][KS], KT[KP][TPW][2], T[3][2];
+        kv_u4 K[KS], KT[TPW][2], T[3][2];
         kv_f4 rise, fall;
-        float last;
+        float last, gain;
         uint16_t V[NT][4];
         auto request_rows = [&](int64_t at) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int p = 0; p < KP; ++p) K[p][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + p * LOW + (wave * KS + s) * 1024);
+            for (int s = 0; s < KS; ++s) K[s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + (wave * KS + s) * 1024);
         };
         auto request_values = [&](int64_t at, bool all) {
             rise = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + RISE_K * 4);
@@ -564,27 +607,33 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
 #pragma unroll
                     for (int p = 0; p < 3; ++p) T[p][s] = *reinterpret_cast<const kv_u4 *>(head + at * w.head + p * 8192 + (wave * 2 + s) * 1024);
             fall = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + FALL * 4);
+            gain = *reinterpret_cast<const float *>(factors + at * w.head + GAIN * 4);
         };
         auto request_rest = [&](int64_t at) {
             last = *reinterpret_cast<const float *>(factors + at * w.head + LAST * 4);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int i = 0; i < TPW; ++i)
-#pragma unroll
-                    for (int p = 0; p < KP; ++p) KT[p][i][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + w.kt + p * LOW + ((wave * TPW + i) * 2 + s) * 1024);
+                for (int i = 0; i < TPW; ++i) KT[i][s] = *reinterpret_cast<const kv_u4 *>(key + at * w.key + w.kt + ((wave * TPW + i) * 2 + s) * 1024);
         };
-        // four neighbouring elements of a column as parts of half an operand
-        auto share = [&](char *base, int steps_, int tile, int t, float v0, float v1, float v2, float v3) {
-#pragma unroll
-            for (int p = 0; p < 3; ++p)
-                *reinterpret_cast<kv_u2 *>(part_of(base, p, steps_, tile >> 1, t) + (tile & 1) * 8) = kv_u2{take_part(v0, v1), take_part(v2, v3)};
+        // four neighbouring elements of a column, over a unit, as float16's parts of half an operand
+        auto share = [&](char *base, int steps_, int tile, int t, const kv_f4 &v, float f) {
+            const kv_u2 a = split2(v[0], v[1], f), e = split2(v[2], v[3], f);
+            *reinterpret_cast<kv_u2 *>(part_of(base, 0, steps_, tile >> 1, t) + (tile & 1) * 8) = kv_u2{a.x, e.x};
+            *reinterpret_cast<kv_u2 *>(part_of(base, 1, steps_, tile >> 1, t) + (tile & 1) * 8) = kv_u2{a.y, e.y};
         };
+        auto largest = [](const kv_f4 &v) { return fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))); };
         auto share_state = [&]() {
 #pragma unroll
-            for (int i = 0; i < TPW; ++i)
+            for (int t = 0; t < NT; ++t) {
+                float top = largest(S[0][t]);
 #pragma unroll
-                for (int t = 0; t < NT; ++t) share(sS, KS, wave * TPW + i, t, S[i][t][0], S[i][t][1], S[i][t][2], S[i][t][3]);
+                for (int i = 1; i < TPW; ++i) top = fmaxf(top, largest(S[i][t]));
+                const float unit = unit_of(column_max(top)), f = over(unit);
+                if (g == 0) state_unit[t][n][wave] = unit;
+#pragma unroll
+                for (int i = 0; i < TPW; ++i) share(sS, KS, wave * TPW + i, t, S[i][t], f);
+            }
         };
         bool all = whole(c0);
         request_rows(0);
@@ -593,30 +642,18 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
         request_rest(0);
         share_state();
         for (int c = c0; c < c1; ++c) {
-            const int next = min(c + 1, c1 - 1) - c0;
+            const int now = c - c0, next = min(c + 1, c1 - 1) - c0;
             const bool all_next = whole(next + c0);
-            kv_f4 R[NT][2], U[NT][2];
+            kv_f4 U[NT][2];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) R[t][0] = R[t][1] = U[t][0] = U[t][1] = kv_f4{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < NT; ++t) U[t][0] = U[t][1] = kv_f4{0.f, 0.f, 0.f, 0.f};
             lds_barrier();
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    kv_u4 part[3];
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) part[p] = *reinterpret_cast<const kv_u4 *>(part_of(sS, p, KS, s, t));
-                    R[t][0] = mfma_bf16(K[0][s], part[0], R[t][0]);
-                    R[t][1] = mfma_bf16(K[0][s], part[1], R[t][1]);
-                    if constexpr (KP == 2) {
-                        R[t][0] = mfma_bf16(K[1][s], part[0], R[t][0]);
-                        R[t][1] = mfma_bf16(K[1][s], part[1], R[t][1]);
-                    }
-                    R[t][s & 1] = mfma_bf16(K[0][s], part[2], R[t][s & 1]);
-                }
-#pragma unroll
             for (int t = 0; t < NT; ++t) {
-                float X[4];
+                const kv_f4 R = times_state(std::integral_constant<int, 2>{}, K, t, [&]() {
+                    if (t == 0 && c > c0) request_rest(now);
+                });
+                kv_f4 X;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float value = Elem<DT>::load(&V[t][r], 0);
@@ -624,27 +661,41 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                         const int row = rows0 + (c - c0) * CHUNK + r;
                         value = row >= span.from && row < span.end ? value : 0.f;
                     }
-                    X[r] = fmaf(-rise[r], R[t][0][r] + R[t][1][r], value);
+                    X[r] = fmaf(-rise[r], R[r], value);
                 }
-                share(sX, 2, wave, t, X[0], X[1], X[2], X[3]);
+                const float top = column_max(largest(X));
+                if (g == 0) x_top[t][n][wave] = top;
+                float x0 = X[0], x1 = X[1], x2 = X[2], x3 = X[3];
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    *reinterpret_cast<kv_u2 *>(part_of(sX, p, 2, wave >> 1, t) + (wave & 1) * 8) = kv_u2{take_part(x0, x1), take_part(x2, x3)};
             }
-            request_rows(next);
-            request_values(next, all_next);
             lds_barrier();
+            float f_unit[NT];
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (s >= steps) break;
+            for (int t = 0; t < NT; ++t) {
+                kv_u4 part[3][2];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    kv_u4 part[3];
+                for (int s = 0; s < 2; ++s)
+                    if (s < steps)
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) part[p] = *reinterpret_cast<const kv_u4 *>(part_of(sX, p, 2, s, t));
-                    U[t][0] = mfma_bf16(T[0][s], part[0], U[t][0]);
-                    U[t][1] = mfma_bf16(T[0][s], part[1], U[t][1]);
-                    U[t][0] = mfma_bf16(T[1][s], part[0], U[t][0]);
-                    U[t][1] = mfma_bf16(T[1][s], part[1], U[t][1]);
-                    U[t][0] = mfma_bf16(T[0][s], part[2], U[t][0]);
-                    U[t][1] = mfma_bf16(T[2][s], part[0], U[t][1]);
+                        for (int p = 0; p < 3; ++p) part[p][s] = *reinterpret_cast<const kv_u4 *>(part_of(sX, p, 2, s, t));
+                const kv_f4 tops = *reinterpret_cast<const kv_f4 *>(x_top[t][n]);
+                all_requested();
+                if (t == 0) {
+                    request_rows(next);
+                    request_values(next, all_next);
+                }
+                f_unit[t] = unit_of(gain * fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    if (s >= steps) break;
+                    U[t][0] = mfma_bf16(T[0][s], part[0][s], U[t][0]);
+                    U[t][1] = mfma_bf16(T[0][s], part[1][s], U[t][1]);
+                    U[t][0] = mfma_bf16(T[1][s], part[0][s], U[t][0]);
+                    U[t][1] = mfma_bf16(T[1][s], part[1][s], U[t][1]);
+                    U[t][0] = mfma_bf16(T[0][s], part[2][s], U[t][0]);
+                    U[t][1] = mfma_bf16(T[2][s], part[0][s], U[t][1]);
                 }
             }
 #pragma unroll
@@ -653,30 +704,38 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
 #pragma unroll
                 for (int r = 0; r < 4; ++r) u[r] = U[t][0][r] + U[t][1][r];
                 *reinterpret_cast<kv_f4 *>(sU + (wave * NT + t) * 1024 + lane * 16) = u;
-                share(sF, 2, wave, t, fall[0] * u[0], fall[1] * u[1], fall[2] * u[2], fall[3] * u[3]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) u[r] *= fall[r];
+                share(sF, 2, wave, t, u, over(f_unit[t]));
             }
-            request_system(next);
             lds_barrier();
+            kv_f4 D[TPW][NT];
+#pragma unroll
+            for (int i = 0; i < TPW; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) D[i][t] = kv_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                kv_u4 part[2][2];
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) part[p][s] = *reinterpret_cast<const kv_u4 *>(part_of(sF, p, 2, s, t));
+                all_requested();
+                if (t == 0) request_system(next);
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+#pragma unroll
+                        for (int i = 0; i < TPW; ++i) D[i][t] = mfma_f16(KT[i][s], part[p][s], D[i][t]);
+            }
 #pragma unroll
             for (int i = 0; i < TPW; ++i)
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) S[i][t][r] *= last;
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) {
-                        const kv_u4 part = *reinterpret_cast<const kv_u4 *>(part_of(sF, p, 2, s, t));
-#pragma unroll
-                        for (int i = 0; i < TPW; ++i) {
-                            S[i][t] = mfma_bf16(KT[0][i][s], part, S[i][t]);
-                            if (KP == 2 && p < 2) S[i][t] = mfma_bf16(KT[KP - 1][i][s], part, S[i][t]);
-                        }
-                    }
-            request_rest(next);
+                    for (int r = 0; r < 4; ++r) S[i][t][r] = fmaf(f_unit[t], D[i][t][r], last * S[i][t][r]);
             share_state();  // (its last readers are behind a barrier)
             all = all_next;
         }
@@ -704,7 +763,7 @@ inline int chunk_key_dim(const DeltaArgs &x) { return x.Dk <= 64 ? 64 : x.Dk <= 
 constexpr uint64_t CHUNK_SPACE = (uint64_t)384 << 20;
 inline ChunkSpace chunk_space(const DeltaArgs &x, void *workspace, uint64_t *bytes) {
     ChunkSpace w{};
-    const uint64_t rows = (uint64_t)CHUNK * chunk_key_dim(x) * 2 * (x.dtype == KVHIP_F16 ? 2 : 1);
+    const uint64_t rows = (uint64_t)CHUNK * chunk_key_dim(x) * 2;
     w.base = static_cast<char *>(workspace);
     w.q = rows;
     w.kt = 2 * rows;
@@ -731,13 +790,20 @@ template <int DT, int KD> hipError_t launch_chunks(const DeltaArgs &x, ChunkSpac
         const dim3 prep(w.chunks, x.Hv, x.B);
         if (wide) hipLaunchKernelGGL((chunk_prep_kernel<DT, KD, true>), prep, dim3(256), 0, s, x, w);
         else hipLaunchKernelGGL((chunk_prep_kernel<DT, KD, false>), prep, dim3(256), 0, s, x, w);
-        const int64_t heads = (int64_t)x.B * x.Hv, one = (x.Dv + 15) / 16, four = (x.Dv + 63) / 64;
-        bool wider = false;
-        if constexpr (KD < 256) {
-            wider = heads * one > 512;
-            if (wider) hipLaunchKernelGGL((chunk_scan_kernel<DT, KD, 4>), dim3((unsigned)(heads * four)), dim3(512), 0, s, x, w, state);
+        auto scan = [&](auto kernel, int columns) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)x.B * x.Hv * ((x.Dv + columns - 1) / columns))), dim3(512), 0, s, x, w, state);
+        };
+        const int64_t groups = (int64_t)x.B * x.Hv * ((x.Dv + 15) / 16);
+        // As few columns to a workgroup as give every compute unit one, else as many as its registers hold: all read a head's whole
+        // operands.  128 channels, 32 heads of 128, us with 16 / 32 / 64: 8192 tokens of one sequence 319 / 406 (the whole call); 2048 of
+        // two 146 / 127; 2048 of four - / 261 / 244; 2000 of eight - / 605 / 496.  256 channels, 4 heads of 512, 2048 of four: 167 / 137.
+        if (groups <= 256) {
+            scan(chunk_scan_kernel<DT, KD, 1>, 16);
+        } else if (KD > 128 || groups <= 512) {
+            scan(chunk_scan_kernel<DT, KD, 2>, 32);
+        } else if constexpr (KD <= 128) {
+            scan(chunk_scan_kernel<DT, KD, 4>, 64);
         }
-        if (!wider) hipLaunchKernelGGL((chunk_scan_kernel<DT, KD, 1>), dim3((unsigned)(heads * one)), dim3(512), 0, s, x, w, state);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         state = x.state_out;

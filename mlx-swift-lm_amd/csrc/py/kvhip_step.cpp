@@ -277,7 +277,8 @@ PyObject *select(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     if (!stream || !take_part(args[2], 3, dev, x) || !take_part(args[3], 2, dev, s) || !take_int(args[4], count) || !take_int(args[5], pad)) return none();
     const long long B = x.n[0], K = x.n[1], V = x.n[2];
     if (s.dtype != KVHIP_F32 || s.n[0] != B || s.n[1] != K || (B > 1 && s.stride_b != K) || (K > 1 && s.stride_l != 1)) return none();
-    if ((B > 1 && x.stride_b != K * x.stride_l) || x.stride_l < 0 || count <= 0 || count > INT32_MAX || pad < INT32_MIN || pad > INT32_MAX) return none();
+    const long long pitch = K > 1 ? x.stride_l : x.stride_b;  // elements from a row to the next
+    if ((B > 1 && x.stride_b != K * pitch) || count <= 0 || count > INT32_MAX || pad < INT32_MIN || pad > INT32_MAX) return none();
     void *entry = PyLong_AsVoidPtr(args[0]), *workspace = PyLong_AsVoidPtr(args[1]);
     if (PyErr_Occurred() || !entry || !workspace) return none();
     const size_t need = reinterpret_cast<decltype(&kvhip_beam_select_workspace)>(workspace)((int32_t)B, (int32_t)K, (int32_t)V, x.dtype, (int32_t)count);
@@ -299,7 +300,7 @@ PyObject *select(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     kvhip_status status = KVHIP_OK;
     if (ok) {
         Py_BEGIN_ALLOW_THREADS
-        status = reinterpret_cast<decltype(&kvhip_beam_select)>(entry)(x.p, x.stride_l, (int32_t)B, (int32_t)K, (int32_t)V, x.dtype,
+        status = reinterpret_cast<decltype(&kvhip_beam_select)>(entry)(x.p, pitch, (int32_t)B, (int32_t)K, (int32_t)V, x.dtype,
                                                                        static_cast<const float *>(s.p), nullptr, (int32_t)count, (int32_t)pad,
                                                                        static_cast<int32_t *>(at[0]), static_cast<int32_t *>(at[1]),
                                                                        static_cast<float *>(at[2]), at[3], need, st);

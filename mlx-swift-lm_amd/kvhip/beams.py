@@ -30,8 +30,10 @@ def beam_select(logits, scores=None, count=None, done=None, pad_token=0):
         raise ValueError(f"scores are float32 {(B, K)}, not {scores.dtype} {tuple(scores.shape)}")
     if done is not None and (tuple(done.shape) != (B, K) or done.dtype not in (torch.bool, torch.uint8)):
         raise ValueError(f"done is bool {(B, K)}, not {done.dtype} {tuple(done.shape)}")
-    if (V > 1 and logits.stride(2) != 1) or (B > 1 and logits.stride(0) != K * logits.stride(1)) or logits.stride(1) < 0:
+    pitch = logits.stride(1 if K > 1 else 0)  # elements from a row to the next
+    if (V > 1 and logits.stride(2) != 1) or (B > 1 and logits.stride(0) != K * pitch):
         logits = logits.contiguous()
+        pitch = V
     scores, done = (None if t is None else t.contiguous() for t in (scores, done))
     _on_current_device(logits, scores, done)
     L.init()
@@ -40,7 +42,7 @@ def beam_select(logits, scores=None, count=None, done=None, pad_token=0):
     rows, tokens, best = out[0], out[1], out[2].view(torch.float32)
     need = lib.kvhip_beam_select_workspace(B, K, V, _DT[logits.dtype], count)
     scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
-    L.check(lib.kvhip_beam_select(_ptr(logits), logits.stride(1), B, K, V, _DT[logits.dtype], None if scores is None else _ptr(scores),
+    L.check(lib.kvhip_beam_select(_ptr(logits), pitch, B, K, V, _DT[logits.dtype], None if scores is None else _ptr(scores),
                                   None if done is None else _ptr(done), count, int(pad_token), _ptr(rows), _ptr(tokens), _ptr(best),
                                   _ptr(scratch) if need else None, need, _stream()))
     return rows, tokens, best

@@ -39,6 +39,27 @@ def test_gated_delta_refuses(given, status):
     assert lib.kvhip_last_error_message()
 
 
+@pytest.mark.parametrize("workspace, less, status", [(None, 0, INVALID), (P, 1, INVALID), (C.c_void_p(4104), 0, INVALID)])
+def test_prompts_refuse_a_workspace_that_is_none(workspace, less, status):
+    lib = kvhip.load()
+    x = delta(L=64)
+    need = lib.kvhip_gated_delta_workspace(C.byref(x))
+    assert need > 0
+    assert lib.kvhip_gated_delta(C.byref(x), workspace, need - less, None) == status
+
+
+def test_workspaces_go_by_sizes_alone():
+    """No array has to be there to ask; single tokens and float32 need none; long prompts are laid out a stretch at a time."""
+    lib = kvhip.load()
+
+    def need(**given):
+        return lib.kvhip_gated_delta_workspace(C.byref(delta(**given)))
+
+    assert need(L=64, q=None, k=None, v=None, a=None, b=None, state_out=None, out=None) == need(L=64) > 0
+    assert need(L=1) == need(L=4) == need(L=5000, dtype=L.F32) == need(L=64, Dk=300) == 0
+    assert need(L=65) > need(L=64) and need(L=2 ** 20, B=8, Hk=16, Hv=32, Dk=128, Dv=128) < 2 ** 30
+
+
 def test_gated_delta_refuses_nothing():
     lib = kvhip.load()
     assert lib.kvhip_gated_delta(None, None, 0, None) == INVALID
