@@ -17,6 +17,12 @@
 // range), of which the products below 2^-24 are left out.  Decays are summed in float64: e^-1000 beside e^-0.001 loses
 // nothing.  The outputs, rounded to 16 bits, take one part of S, P and U each (float16: two).
 //
+// 8192 tokens x 32 heads x 128 x 128 in bfloat16, one sequence: 74 us of preparation and 234 of the scan, whose 128 chunks follow one
+// another, 1.8 us each: about 1.1 are the chain of products and barriers from state to state, the rest the arrival of the
+// 80 KB of operands that each of the 256 workgroups takes a chunk (11 TB/s, from the L2s).  Widths and splits of
+// the work were tried: one wavefront to 16 columns in place of one to 16 rows took 151 us for half the tokens.
+// 2000 tokens of 8 sequences in float16: 103 and 323 us, in two rounds of the workspace.
+//
 // Operands lie in the workspace as the lanes take them, 1 KB to an instruction: contractions may be summed in any
 // order, so that lane (n, g)'s eight elements of a step are those at 4 g and 16 + 4 g of it -- which is where a product leaves them: S, U
 // go from accumulators to operands without crossing lanes, only from wavefront to wavefront through LDS.
@@ -758,8 +764,10 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
 }
 
 inline int chunk_key_dim(const DeltaArgs &x) { return x.Dk <= 64 ? 64 : x.Dk <= 128 ? 128 : 256; }
-// What a chunk of all sequences and heads takes, and how many chunks are laid out at a time: what they take is to stay in the
-// last-level cache between the two kernels.
+// What a chunk of all sequences and heads takes, and how many chunks are laid out at a time: what they take is to stay near the
+// last-level cache between the two kernels, and a round is to be long enough to pay for its start.  96 / 192 / 384 / 768 MiB, 32 heads of
+// 128 x 128 in bfloat16, us: 8 x 2000 tokens 649 / 564 / 553 / 548; 16 x 4096 2225 / 2112 / 1920 / 1813; 32768 of one 1175 / 1106 /
+// 1181 / 1159.  More than 384 gains little for twice the memory.
 constexpr uint64_t CHUNK_SPACE = (uint64_t)384 << 20;
 inline ChunkSpace chunk_space(const DeltaArgs &x, void *workspace, uint64_t *bytes) {
     ChunkSpace w{};
@@ -794,9 +802,10 @@ template <int DT, int KD> hipError_t launch_chunks(const DeltaArgs &x, ChunkSpac
             hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)x.B * x.Hv * ((x.Dv + columns - 1) / columns))), dim3(512), 0, s, x, w, state);
         };
         const int64_t groups = (int64_t)x.B * x.Hv * ((x.Dv + 15) / 16);
-        // As few columns to a workgroup as give every compute unit one, else as many as its registers hold: all read a head's whole
-        // operands.  128 channels, 32 heads of 128, us with 16 / 32 / 64: 8192 tokens of one sequence 319 / 406 (the whole call); 2048 of
-        // two 146 / 127; 2048 of four - / 261 / 244; 2000 of eight - / 605 / 496.  256 channels, 4 heads of 512, 2048 of four: 167 / 137.
+        // Every workgroup of a head reads the head's whole operands: few columns to each fill the chip, many read less.  Whole calls in
+        // us with 16 / 32 / 64 columns, 32 heads of 128 x 128 in bfloat16: 8192 tokens (256 groups) 316 / 404 / 635; 2 x 2048 (512)
+        // 152 / 126 / 190; 4 x 2048 (1024) 342 / 256 / 238; 8 x 2000 in float16 (2048) 1124 / 660 / 538.  256 channels have no
+        // registers for 64; 4 heads of 512 x 256: 4096 tokens (128) 147 / 215; 4 x 2048 (512) 162 / 138.
         if (groups <= 256) {
             scan(chunk_scan_kernel<DT, KD, 1>, 16);
         } else if (KD > 128 || groups <= 512) {
