@@ -154,17 +154,19 @@ __global__ void __launch_bounds__(256, WIDE ? 6 : 4) beam_rows_kernel(BeamArgs x
                 for (int m = 0; m < VEC; ++m) {
                     const float v = element(looked_at, n, m);
                     const int i = base + (n * 256 + tid) * VEC + m;
-                    if (v >= least && i < x.vocabulary) {
+                    if (v >= least && i < x.vocabulary && (!decltype(looked_at)::value || v > NEVER || i - base < 2 * count)) {
                         const int k = atomicAdd(&listed, 1);
                         if (k < BEAM_LIST) list[k] = rank_key(v, i);
                     }
                 }
             }
     };
-    // Logits are taken as they are; where one is no number or infinite, which the sum or the maximum shows, all are looked at
-    // and the pass is made again.
+    // Logits are taken as they are; where one is no number or infinite, which the sum or the maximum shows, or less than `count` lanes
+    // of each wavefront hold one that counts, all are looked at and the pass is made again.  Of what is masked the first `count` are
+    // listed then, which lie among the first 2 count where less than `count` others are: 256 bfloat16 rows of 152 064 with 100 left
+    // 53 us the whole call, 311 with all of them listed and the best taken out one by one.
     pass(std::false_type{});
-    const bool looked = !(sum == sum && all < __builtin_inff());
+    const bool looked = !(sum == sum && all < __builtin_inff() && least > NEVER);
     if (!looked) {
         put_down(std::false_type{});
     } else {
