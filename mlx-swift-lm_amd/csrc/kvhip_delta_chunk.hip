@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
             decay = -expf(x.a_log[h]) * (fmaxf(s, 0.f) + log1pf(expf(-fabsf(s))));
             rate = 1.f / (1.f + expf(-rate));
         }
-        double sum = fmaxf(decay, -1e5f);  // (e^-1e5 is nothing, and differences of sums stay numbers)
+        double sum = decay < -1e5f ? -1e5f : decay;  // (e^-1e5 is nothing, and differences of sums stay numbers)
 #pragma unroll
         for (int s = 1; s < 64; s <<= 1) {
             const double o = __shfl_up(sum, s);

@@ -341,7 +341,9 @@ class _Cache:
         dev = torch._C._cuda_getDevice()
         if not order.is_cuda or order.device.index != dev:
             raise ValueError(f"the order lies on {order.device}, the current device is cuda:{dev}")
-        order = order.to(torch.int32).contiguous()
+        if order.dtype == torch.int64:  # (an entry beyond int32 stays one outside the batch)
+            order = order.clamp(-1, self._shape[0]).to(torch.int32)
+        order = order.contiguous()
         L.check(self._lib.kvhip_cache_reorder(self._h, _ptr(order), int(shared), _stream()))
 
     # ---- state / metaState ---------------------------------------------------

@@ -25,14 +25,21 @@ def _per_sequence(t, batch, name):
         return None
     if tuple(t.shape) != (batch,):
         raise ValueError(f"{name} is one number to each of {batch} sequences, not {tuple(t.shape)}")
-    return t.to(device="cuda", dtype=torch.int32).contiguous()
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} is int32 or int64, not {t.dtype}")
+    return _int32(t).to("cuda").contiguous()
+
+
+def _int32(t):
+    """Whole numbers as int32, those beyond its ends as its ends."""
+    return t if t.dtype == torch.int32 else t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
 
 
 def _order(order, rows):
     if order.dtype not in (torch.int32, torch.int64) or tuple(order.shape) != (rows,):
         raise ValueError(f"an order is one row number to each of {rows} sequences, not {order.dtype} {tuple(order.shape)}")
     _on_current_device(order)
-    return order.to(torch.int32).contiguous()
+    return _int32(order).contiguous()
 
 
 def _dense_rows(t):

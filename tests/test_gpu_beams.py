@@ -104,6 +104,20 @@ def test_rows_of_a_wider_array(dtype, shift):
     check_select(part.transpose(0, 1), None, 4)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_that_lie_apart_and_rows_that_are_one(dtype):
+    """One beam to a batch row out of wider rows, rows that several beams share, and a prompt's one row as every beam's."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    whole = torch.randn(6, 1, 2100, generator=gen, device="cuda").to(dtype)
+    for part in (whole[..., :2003], whole[:, :, 3:1900], whole[::2, :, :700], whole[:1].expand(5, 1, 2100), whole[:1].expand(1, 4, 2100),
+                 whole.expand(6, 3, 2100)):
+        B, K = part.shape[:2]
+        scores = -torch.arange(B * K, device="cuda", dtype=torch.float32).reshape(B, K)
+        check_select(part, scores, 3)
+        check_select(part, scores, 3, torch.zeros(B, K, dtype=torch.bool, device="cuda"))
+        check_select(part, None, 2)
+
+
 def test_many_rows_and_offsets_beyond_32_bits():
     gen = torch.Generator(device="cuda").manual_seed(4)
     x = torch.empty(140, 64, 262144, dtype=torch.bfloat16, device="cuda")
@@ -332,6 +346,18 @@ def test_reordered_recurrent_states(dtype, rows, width):
         before = rows_of(cache)
         cache.reorder(order.cuda())
         assert all(torch.equal(a, moved(b, order)) for a, b in zip(rows_of(cache), before))
+
+
+def test_entries_beyond_32_bits_leave_a_row_its_own():
+    order = torch.tensor([2 ** 32 + 1, -2 ** 40, 2 ** 31], device="cuda")
+    cache = kvhip.GatedDeltaCache()
+    cache.delta_state = torch.randn(3, 1, 2, 8, device="cuda")
+    simple = kvhip.KVCacheSimple()
+    write(simple, *(torch.randn(3, 2, 5, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2)))
+    for c in (cache, simple):
+        before = rows_of(c)
+        c.reorder(order)
+        assert all(torch.equal(a, b) for a, b in zip(rows_of(c), before))
 
 
 def test_reorder_in_a_graph():

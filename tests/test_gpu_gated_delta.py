@@ -135,6 +135,95 @@ def test_padded_batches(dtype, n):
             assert torch.equal(cache.delta_state[i], state[i])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompts_beyond_one_stretch_of_the_workspace(dtype):
+    """Prompts that are laid out in two stretches, with sequences that end in the first, begin in the second, or have no token."""
+    rng = np.random.default_rng(3)
+    B, H, n = 32, 32, 400
+    x, state = make(rng, B, n, H, H, 8, 4, dtype)
+    sizes = dict(B=B, Hk=H, Hv=H, Dk=8, Dv=4, dtype={torch.float16: L.F16, torch.bfloat16: L.BF16}[dtype], gate_dtype=L.F32)
+    need = [L.load().kvhip_gated_delta_workspace(C.byref(L.GatedDelta(L=m, **sizes))) for m in (n, 2 * n)]
+    assert need[0] == need[1]
+    pad = torch.from_numpy(rng.integers(0, 70, B).astype(np.int32))
+    ends = torch.from_numpy(rng.integers(300, n + 1, B).astype(np.int32))
+    pad[3], ends[4], ends[5], pad[6] = 333, 100, 0, n
+    cache = kvhip.GatedDeltaCache()
+    cache.delta_state = state
+    out = kvhip.gated_delta_update(**x, cache=cache, left_pad=pad, lengths=ends)
+    check(out, cache.delta_state, expect(x, state, left_pad=pad, lengths=ends), n, dtype)
+    assert not out[5].any() and torch.equal(cache.delta_state[5], state[5]) and torch.equal(cache.delta_state[6], state[6])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [3, 150])
+def test_what_is_no_number_stays_in_its_sequence(dtype, n):
+    rng = np.random.default_rng(n)
+    x, state = make(rng, 4, n, 2, 4, 64, 48, dtype)
+    cache = kvhip.GatedDeltaCache()
+    cache.delta_state = state
+    fine = kvhip.gated_delta_update(**x, cache=cache)
+    at = n - 2
+    x["k"][0, at, 1, 5] = float("inf")
+    x["a"][1, at, 2] = float("nan")
+    x["v"][2, at, 3, 7] = float("nan")
+    other = kvhip.GatedDeltaCache()
+    other.delta_state = state
+    out = kvhip.gated_delta_update(**x, cache=other)
+    assert torch.equal(out[3], fine[3]) and torch.equal(other.delta_state[3], cache.delta_state[3])
+    for b, head, rows in ((0, (2, 3), slice(None)), (1, (2,), slice(None)), (2, (3,), slice(7, 8))):
+        for h in range(4):
+            if h not in head:
+                assert torch.equal(out[b, :, h], fine[b, :, h]) and torch.equal(other.delta_state[b, h], cache.delta_state[b, h])
+        for h in head:
+            assert not torch.isfinite(other.delta_state[b, h, rows]).all() and torch.isnan(out[b, at:, h, rows]).any()
+    assert torch.isnan(other.delta_state[1, 2]).all() and torch.isnan(out[1, at:, 2]).all()
+    still = [c for c in range(48) if c != 7]
+    assert torch.equal(out[2, :, 3, still], fine[2, :, 3, still]) and torch.equal(other.delta_state[2, 3, still], cache.delta_state[2, 3, still])
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_gates_of_other_types(n):
+    """Gates in float32 beside 16-bit rows, their parameters in any type, with no bias, and the same by either way into the library."""
+    rng = np.random.default_rng(n)
+    dtype = torch.bfloat16
+    x, state = make(rng, 2, n, 2, 4, 64, 64, dtype, gate_dtype=torch.float32)
+    x["a_log"], x["dt_bias"] = x["a_log"].to(dtype), x["dt_bias"].to(dtype)
+    plain = dict(x, a_log=x["a_log"].float(), dt_bias=x["dt_bias"].float())
+    results = []
+    for given in (x, plain, dict(plain, left_pad=torch.zeros(2, dtype=torch.int64))):
+        cache = kvhip.GatedDeltaCache()
+        cache.delta_state = state
+        out = kvhip.gated_delta_update(**given, cache=cache)
+        check(out, cache.delta_state, expect(plain, state), n, dtype)
+        results.append((out, cache.delta_state))
+    assert all(torch.equal(a, b) for r in results[1:] for a, b in zip(r, results[0]))
+    none = dict(plain, dt_bias=torch.zeros(4, device="cuda"))
+    cache = kvhip.GatedDeltaCache()
+    cache.delta_state = state
+    out = kvhip.gated_delta_update(**dict(none, dt_bias=None), cache=cache)
+    check(out, cache.delta_state, expect(none, state), n, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_small_values_behind_large_ones_that_fade(dtype):
+    """What a chunk adds to the state is laid out by a bound that large values in front raise: a state that is a thousandth of them
+    loses nothing."""
+    rng = np.random.default_rng(8)
+    n = 64
+    x, state = make(rng, 2, n, 1, 2, 128, 32, dtype, gate_dtype=torch.float32)
+    x["v"][:, :20] *= 1000
+    x["a"] = torch.full((2, n, 2), -0.01, device="cuda")
+    x["a"][:, 24:32] = -3.0  # (e^-24 of what was there is left)
+    x["b"] = torch.sigmoid(x["b"])
+    given = dict(x, a_log=None, dt_bias=None)
+    cache = kvhip.GatedDeltaCache()
+    cache.delta_state = state
+    out = kvhip.gated_delta_update(**given, cache=cache)
+    want = R.gated_delta(*(f64(x[k]) for k in ("q", "k", "v", "a", "b")), None, None, f64(state))
+    new = cache.delta_state.double().cpu().numpy()
+    assert np.linalg.norm(new - want[1]) <= 4e-6 * np.linalg.norm(want[1]) and torch.isfinite(out.float()).all()
+
+
 @pytest.mark.parametrize("n", [4, 96])
 def test_parts_of_one_array(n):
     """Queries, keys and values as the convolution hands them on, side by side; gates side by side; from an odd element on."""

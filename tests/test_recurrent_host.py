@@ -8,6 +8,7 @@ import torch
 
 import kvhip
 from kvhip import _lib as L
+from kvhip import recurrent
 from oracle import recurrent as R
 from oracle import beams as OB
 
@@ -154,6 +155,9 @@ def test_cache_refuses_arrays_that_do_not_go_together():
     with pytest.raises(ValueError):
         cache.meta_state = ["3", "0"]
     with pytest.raises(ValueError):
+        recurrent._per_sequence(torch.zeros(2), 2, "lengths")
+    assert recurrent._int32(torch.tensor([2 ** 40, -2 ** 40, 7])).tolist() == [2 ** 31 - 1, -2 ** 31, 7]
+    with pytest.raises(ValueError):
         kvhip.beam_select(torch.zeros(2, 5))
     with pytest.raises(ValueError):
         kvhip.beam_select(torch.zeros(2, 5, 7), scores=torch.zeros(2, 4))
@@ -161,6 +165,15 @@ def test_cache_refuses_arrays_that_do_not_go_together():
         kvhip.beam_select(torch.zeros(2, 5, 7), done=torch.zeros(2, 5))
     with pytest.raises(ValueError):
         kvhip.beam_select(torch.zeros(2, 5, 7))
+
+
+def test_a_hybrid_models_caches_where_all_have_to_go_back():
+    """A recurrent state cannot go back: rounds and trims refuse the list and touch nothing, its file format too."""
+    caches = [kvhip.GatedDeltaCache(), kvhip.GatedDeltaCache(2)]
+    assert kvhip.KVCacheStorage(caches).begin_round(4) is None
+    assert not kvhip.can_trim_prompt_cache(caches) and kvhip.trim_prompt_cache(caches, 3) == 0
+    with pytest.raises((ValueError, TypeError)):
+        kvhip.save_prompt_cache("/nonexistent/file.safetensors", caches)
 
 
 def test_oracle_state_is_what_was_written():
