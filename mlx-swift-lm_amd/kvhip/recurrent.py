@@ -156,8 +156,9 @@ class GatedDeltaCache:
         new.offset, new.window, new.delta_state = self.offset, self._held("_window"), self._held("_state")
         return new
 
-    def reorder(self, order):
-        """Sequence b becomes what sequence order[b] was (`beam_select`'s rows); an entry outside the batch leaves its own."""
+    def reorder(self, order, shared=0):
+        """Sequence b becomes what sequence order[b] was (`beam_select`'s rows); an entry outside the batch leaves its own.  (A state has
+        no positions that sequences could share: whatever `shared` says, all of it moves.)"""
         arrays = [t for t in (self._held("_window"), self._held("_state")) if t is not None and t.numel()]
         if not arrays:
             return

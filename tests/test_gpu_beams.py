@@ -356,7 +356,7 @@ def test_entries_beyond_32_bits_leave_a_row_its_own():
     write(simple, *(torch.randn(3, 2, 5, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2)))
     for c in (cache, simple):
         before = rows_of(c)
-        c.reorder(order)
+        c.reorder(order, shared=2)
         assert all(torch.equal(a, b) for a, b in zip(rows_of(c), before))
 
 
