@@ -1,6 +1,6 @@
 // CPython extension `kvhip._step`: one call of a layer -- `attentionWithCacheUpdate`, with or without the rotary
-// positions in front, a gated delta layer's update, or a beam
-// search's selection -- from its tensors to the C entry point in one native call.  A short decode step takes the device less
+// positions in front, a gated delta layer's update, or a beam search's selection -- from its tensors to the C entry point in one
+// native call.  A short decode step takes the device less
 // time than the interpreter took to look the tensors' shapes, types and addresses up and to convert twenty arguments
 // (16 layers over 512 keys of one sequence: 149 us a pass, 130 from here).  Handles the ordinary form of the call; for
 // everything else (other masks, arrays that are not contiguous, shapes or types that do not go together, numbers that are
@@ -274,7 +274,7 @@ PyObject *select(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     Py_XDECREF(device);
     Py_XDECREF(stream);
     Part x, s;
-    if (!stream || !take_part(args[2], 3, dev, x) || !take_part(args[3], 2, dev, s) || !take_int(args[4], count) || !take_int(args[5], pad)) return none();
+    if (!g_int32 || !stream || !take_part(args[2], 3, dev, x) || !take_part(args[3], 2, dev, s) || !take_int(args[4], count) || !take_int(args[5], pad)) return none();
     const long long B = x.n[0], K = x.n[1], V = x.n[2];
     if (s.dtype != KVHIP_F32 || s.n[0] != B || s.n[1] != K || (B > 1 && s.stride_b != K) || (K > 1 && s.stride_l != 1)) return none();
     const long long pitch = K > 1 ? x.stride_l : x.stride_b;  // elements from a row to the next
@@ -311,10 +311,11 @@ PyObject *select(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     return r;
 }
 
-// bind(Tensor, RoPE, (float16, bfloat16, float32), current device, its raw stream, {"dtype": int32})
+// bind(Tensor, RoPE, (float16, bfloat16, float32), current device, its raw stream[, {"dtype": int32}: without it `select` takes no call])
 PyObject *bind(PyObject *, PyObject *args) {
     PyObject *types;
-    if (!PyArg_ParseTuple(args, "OOO!OOO!", &g_tensor_type, &g_rope_type, &PyTuple_Type, &types, &g_device, &g_raw_stream, &PyDict_Type, &g_int32)) return nullptr;
+    g_int32 = nullptr;
+    if (!PyArg_ParseTuple(args, "OOO!OO|O!", &g_tensor_type, &g_rope_type, &PyTuple_Type, &types, &g_device, &g_raw_stream, &PyDict_Type, &g_int32)) return nullptr;
     if (PyTuple_GET_SIZE(types) != 3) {
         PyErr_SetString(PyExc_TypeError, "three dtypes");
         return nullptr;
@@ -323,7 +324,7 @@ PyObject *bind(PyObject *, PyObject *args) {
     Py_INCREF(g_rope_type);
     Py_INCREF(g_device);
     Py_INCREF(g_raw_stream);
-    Py_INCREF(g_int32);
+    Py_XINCREF(g_int32);
     for (int i = 0; i < 3; ++i) {
         g_dtypes[i] = PyTuple_GET_ITEM(types, i);
         Py_INCREF(g_dtypes[i]);
