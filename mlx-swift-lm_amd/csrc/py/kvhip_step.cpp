@@ -1,5 +1,5 @@
 // CPython extension `kvhip._step`: one call of a layer -- `attentionWithCacheUpdate`, with or without the rotary
-// positions in front, a gated delta layer's update, or a beam search's selection -- from its tensors to the C entry point in one
+// positions in front, a gated delta layer's convolution or update, or a beam search's selection -- from its tensors to the C entry point in one
 // native call.  A short decode step takes the device less
 // time than the interpreter took to look the tensors' shapes, types and addresses up and to convert twenty arguments
 // (16 layers over 512 keys of one sequence: 149 us a pass, 130 from here).  Handles the ordinary form of the call; for
@@ -258,6 +258,53 @@ PyObject *delta(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     return PyLong_FromLong(status);
 }
 
+// convolve(entry, x, weight, bias or None, window, silu)
+//   entry    address of kvhip_short_convolution
+//   window   the cache's, dense, updated in place
+// Handles calls without paddings; returns as attend does.
+PyObject *convolve(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    if (nargs != 6) {
+        PyErr_SetString(PyExc_TypeError, "convolve takes 6 arguments");
+        return nullptr;
+    }
+    PyObject *device = PyObject_CallNoArgs(g_device);
+    long long dev = -1;
+    const bool known = device && take_int(device, dev);
+    PyObject *stream = known ? PyObject_CallOneArg(g_raw_stream, device) : nullptr;
+    void *st = stream ? PyLong_AsVoidPtr(stream) : nullptr;
+    Py_XDECREF(device);
+    Py_XDECREF(stream);
+    Part x, w, bias{}, s;
+    const bool biased = args[3] != Py_None;
+    if (!stream || !take_part(args[1], 3, dev, x) || !take_part(args[2], 2, dev, w) || (biased && !take_part(args[3], 1, dev, bias)) ||
+        !take_part(args[4], 3, dev, s))
+        return none();
+    const long long B = x.n[0], L = x.n[1], C = x.n[2], W = w.n[1];
+    if (w.n[0] != C || (C > 1 && w.stride_b != W) || (W > 1 && w.stride_l != 1) || (biased && bias.n[0] != C)) return none();
+    if (s.n[0] != B || s.n[1] != W - 1 || s.n[2] != C || (B > 1 && s.stride_b != (W - 1) * C) || (W > 2 && s.stride_l != C)) return none();
+    if (w.dtype != x.dtype || s.dtype != x.dtype || (biased && bias.dtype != x.dtype)) return none();
+    const int silu = PyObject_IsTrue(args[5]);
+    void *entry = PyLong_AsVoidPtr(args[0]);
+    if (PyErr_Occurred() || !entry) return none();
+    PyObject *size = Py_BuildValue("(LLL)", B, L, C), *out = size ? PyObject_CallMethodOneArg(args[1], s_new_empty, size) : nullptr;
+    Py_XDECREF(size);
+    PyObject *ptr = out ? PyObject_CallMethodNoArgs(out, s_data_ptr) : nullptr;
+    void *p = ptr ? PyLong_AsVoidPtr(ptr) : nullptr;
+    Py_XDECREF(ptr);
+    if (PyErr_Occurred()) {
+        Py_XDECREF(out);
+        return nullptr;
+    }
+    kvhip_status status;
+    Py_BEGIN_ALLOW_THREADS
+    status = reinterpret_cast<decltype(&kvhip_short_convolution)>(entry)(x.p, x.stride_b, x.stride_l, w.p, bias.p, (int32_t)B, (int32_t)L,
+                                                                         (int32_t)C, (int32_t)W, x.dtype, silu, nullptr, nullptr, s.p, s.p, p, st);
+    Py_END_ALLOW_THREADS
+    if (status >= KVHIP_OK) return out;
+    Py_DECREF(out);
+    return PyLong_FromLong(status);
+}
+
 // select(entry, workspace, logits, scores, count, pad_token)
 //   entry, workspace   addresses of kvhip_beam_select and kvhip_beam_select_workspace
 // Handles dense [B, K, V] logits with dense float32 [B, K] scores and no beam done: (rows, tokens, scores), None or a status.
@@ -334,6 +381,7 @@ PyObject *bind(PyObject *, PyObject *args) {
 
 PyMethodDef g_methods[] = {{"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(attend)), METH_FASTCALL, nullptr},
                            {"delta", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(delta)), METH_FASTCALL, nullptr},
+                           {"convolve", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(convolve)), METH_FASTCALL, nullptr},
                            {"select", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(select)), METH_FASTCALL, nullptr},
                            {"bind", bind, METH_VARARGS, nullptr},
                            {nullptr, nullptr, 0, nullptr}};

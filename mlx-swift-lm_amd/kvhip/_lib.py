@@ -178,11 +178,11 @@ _native = {}
 
 
 def native(name, entry):
-    """The extension's call `name` for an entry point that takes a workspace: (the call, or None where it is not built, the entry
-    point's address, and that of its `_workspace`)."""
+    """The extension's call `name` for an entry point: (the call, or None where it is not built, the entry point's address and, where it
+    takes a workspace, that of its `_workspace`)."""
     if name not in _native:
         module, lib = step()[0], load()
-        at = [C.cast(getattr(lib, e), C.c_void_p).value for e in (entry, entry + "_workspace")]
+        at = [C.cast(getattr(lib, e), C.c_void_p).value for e in (entry, entry + "_workspace") if e in SIGNATURES]
         _native[name] = (getattr(module, name) if module else None, *at)
     return _native[name]
 

@@ -176,6 +176,14 @@ class GatedDeltaCache:
     # ---- the operators ------------------------------------------------------
     def convolve(self, x, weight, bias=None, silu=True, left_pad=None, lengths=None):
         """The short convolution of x [B, L, C] with weight [C, W] behind this cache's window, which moves on: [B, L, C]."""
+        window = self._held("_window")
+        if window is not None and left_pad is None and lengths is None:
+            native, entry = L.native("convolve", "kvhip_short_convolution")  # (a step of the ordinary form, as one native call)
+            out = native(entry, x, weight, bias, window, silu) if native else None
+            if type(out) is int:
+                L.check(out)
+            if out is not None:
+                return out
         if x.dim() != 3 or x.dtype not in _DT:
             raise ValueError(f"x is [B, L, C] in float16, bfloat16 or float32, not {x.dtype} {tuple(x.shape)}")
         B, n, c = x.shape
@@ -184,7 +192,6 @@ class GatedDeltaCache:
             raise ValueError(f"weight is {x.dtype} {(c, W)}, not {weight.dtype} {tuple(weight.shape)}")
         if bias is not None and (tuple(bias.shape) != (c,) or bias.dtype != x.dtype):
             raise ValueError(f"bias is {x.dtype} {(c,)}, not {bias.dtype} {tuple(bias.shape)}")
-        window = self._held("_window")
         if window is not None and (tuple(window.shape) != (B, W - 1, c) or window.dtype != x.dtype):
             raise ValueError(f"x {x.dtype} {tuple(x.shape)} does not go with the window {window.dtype} {tuple(window.shape)}")
         _on_current_device(x, weight, bias, window)

@@ -477,6 +477,31 @@ def test_convolution_of_parts_and_calls_that_join(dtype):
         check_conv(y, cache, x, w, bias, window, dtype)
 
 
+@pytest.mark.parametrize("n", [1, 40])
+def test_convolution_with_weights_that_lie_otherwise(n):
+    """Weights of another layer's layout, a strided bias and a column of a wider batch give what dense ones give, by either way in."""
+    rng = np.random.default_rng(n)
+    dtype = torch.bfloat16
+    x, w, bias, window = conv_inputs(rng, 3, n, 24, 4, dtype)
+    taps, wide = w.t().contiguous().t(), torch.stack([bias, bias], -1)[:, 0]
+    part = torch.stack([x, x], 1)[:, 1]
+    results = []
+    for given in (dict(x=x, weight=w, bias=bias), dict(x=x, weight=taps, bias=wide), dict(x=part, weight=w, bias=bias),
+                  dict(x=x, weight=w, bias=bias, left_pad=torch.zeros(3, dtype=torch.int32))):
+        cache = kvhip.GatedDeltaCache(4)
+        cache.window = window
+        y = kvhip.causal_convolution(cache=cache, **given)
+        check_conv(y, cache, x, w, bias, window, dtype)
+        results.append((y, cache.window))
+    assert all(torch.equal(a, b) for r in results[1:] for a, b in zip(r, results[0]))
+    with pytest.raises(ValueError):
+        cache.convolve(x, w[:, :3])
+    with pytest.raises(ValueError):
+        cache.convolve(x[:2], w)
+    with pytest.raises(ValueError):
+        cache.convolve(x, w, bias.float())
+
+
 def test_a_layers_calls_together():
     """Convolution, its parts as queries, keys and values, the delta rule: a prompt and two tokens, as a layer makes them."""
     rng = np.random.default_rng(12)
