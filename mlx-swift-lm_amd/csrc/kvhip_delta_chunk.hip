@@ -11,17 +11,17 @@
 //
 // Numbers.  The state is returned in float32, so everything that it is made from keeps float32's accuracy on 16-bit operands.  Norms are
 // factors of rows, put on in float32 behind the products: Q and K stay what they came as, in float16 over a power of two for
-// each row (exact, but for elements below 2^-28 of the row's largest).  The state and what is added to it are two parts of float16
-// (22 bits) over powers of two for each column: of a wavefront's rows of the state the largest is at hand, of
-// diag(e^(G_63 - G)) U it is bounded by that of X and the largest sum over a row of T.  T and X are three parts of bfloat16 (24 bits, float32's
-// range), of which the products below 2^-24 are left out.  Decays are summed in float64: e^-1000 beside e^-0.001 loses
+// each row (exact, but for elements below 2^-28 of the row's largest).  T, X, the state and what is added to it are two parts of float16
+// (22 bits; 1.4e-7 against 64 bits, as with three parts of bfloat16 for T and X) over powers of two: T's for each row, the others' for
+// each column.  Of a wavefront's rows of X or of the state the largest is at hand, of diag(e^(G_63 - G)) U it is bounded by X's
+// units and the largest sum over a row of T.  Decays are summed in float64: e^-1000 beside e^-0.001 loses
 // nothing.  The outputs, rounded to 16 bits, take one part of S, P and U each (float16: two).
 //
-// 8192 tokens x 32 heads x 128 x 128 in bfloat16, one sequence: 74 us of preparation and 234 of the scan, whose 128 chunks follow one
-// another, 1.8 us each: about 1.1 are the chain of products and barriers from state to state, the rest the arrival of the
-// 80 KB of operands that each of the 256 workgroups takes a chunk (11 TB/s, from the L2s).  Widths and splits of
-// the work were tried: one wavefront to 16 columns in place of one to 16 rows took 151 us for half the tokens.
-// 2000 tokens of 8 sequences in float16: 103 and 323 us, in two rounds of the workspace.
+// 8192 tokens x 32 heads x 128 x 128 in bfloat16, one sequence: 72 us of preparation (its writes and reads, 5 TB/s) and 234 of the
+// scan, whose 128 chunks follow one another, 1.8 us each: about 1.1 are the chain of products and barriers from state to state, the
+// rest comes with the 74 KB of operands and with the outputs of a chunk, wherever they lie (two chunks' operands again and again, in the
+// L2, take as long).  One wavefront to 16 columns in place of one to 16 rows took 151 us for half the tokens.
+// 2000 tokens of 8 sequences in float16: 101 and 310 us, in two stretches of the workspace.
 //
 // Operands lie in the workspace as the lanes take them, 1 KB to an instruction: contractions may be summed in any
 // order, so that lane (n, g)'s eight elements of a step are those at 4 g and 16 + 4 g of it -- which is where a product leaves them: S, U
@@ -37,6 +37,7 @@ namespace {
 typedef float kv_f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 kv_b8 __attribute__((ext_vector_type(8)));
 typedef _Float16 kv_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 kv_h4 __attribute__((ext_vector_type(4)));
 
 constexpr int CHUNK = 64;
 
@@ -46,15 +47,10 @@ __device__ __forceinline__ kv_f4 mfma_bf16(const kv_u4 &a, const kv_u4 &b, const
 __device__ __forceinline__ kv_f4 mfma_f16(const kv_u4 &a, const kv_u4 &b, const kv_f4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(kv_h8, a), __builtin_bit_cast(kv_h8, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ kv_f4 mfma_f32(float a, float b, const kv_f4 &c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-
-// two values' parts of bfloat16, the largest first; what is left in x, y
-__device__ __forceinline__ uint32_t take_part(float &x, float &y) {
-    const uint32_t w = pk_bf2(x, y);
-    x -= __uint_as_float(w << 16);
-    y -= __uint_as_float(w & 0xffff0000u);
-    return w;
+__device__ __forceinline__ kv_f4 mfma_f16(const kv_u2 &a, const kv_u2 &b, const kv_f4 &c) {  // (half the terms)
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(kv_h4, a), __builtin_bit_cast(kv_h4, b), c, 0, 0, 0);
 }
+__device__ __forceinline__ kv_f4 mfma_f32(float a, float b, const kv_f4 &c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 // two values' parts of float16: 11 bits, and the next 11
 __device__ __forceinline__ kv_u2 split2(float x, float y, float f) {  // of x f and y f, f a power of two
@@ -92,11 +88,11 @@ struct ChunkSpace {
 };
 __device__ __forceinline__ char *key_at(const ChunkSpace &w, int64_t bh, int c) { return w.base + (bh * w.chunks + c) * w.key; }
 __device__ __forceinline__ char *head_at(const ChunkSpace &w, int64_t bh, int c) { return w.base + w.heads + (bh * w.chunks + c) * w.head; }
-constexpr int T_BYTES = CHUNK * CHUNK * 6, P_BYTES = CHUNK * CHUNK * 4;  // three parts, and two (bfloat16: one is used)
-// Factors of rows, the units of their operands among them: e^G r_k (what K S is worth), scale e^G r_q, e^(G_63 - G) r_k, P's units; then
+constexpr int T_BYTES = CHUNK * CHUNK * 4, P_BYTES = CHUNK * CHUNK * 4;  // two parts (of P in bfloat16 one is used)
+// Factors of rows, the units of their operands among them: e^G r_k (what K S is worth), scale e^G r_q, e^(G_63 - G) r_k, P's units, T's; then
 // e^G_63, and the bound of |diag(e^(G_63 - G)) U| over the largest |X| of a column.
-constexpr int RISE_K = 0, RISE_Q = CHUNK, FALL = 2 * CHUNK, P_UNIT = 3 * CHUNK, LAST = 4 * CHUNK, GAIN = 4 * CHUNK + 1;
-constexpr int FACTOR_BYTES = 5 * CHUNK * 4;
+constexpr int RISE_K = 0, RISE_Q = CHUNK, FALL = 2 * CHUNK, P_UNIT = 3 * CHUNK, T_UNIT = 4 * CHUNK, LAST = 5 * CHUNK, GAIN = 5 * CHUNK + 1;
+constexpr int FACTOR_BYTES = 6 * CHUNK * 4;
 
 struct ChunkSpan {
     int from, end;  // the sequence's tokens
@@ -369,26 +365,33 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
         }
         __syncthreads();
     }
-    // T in three parts: rows 16 w + n, tokens 32 s + 4 g and 16 on (zero above the diagonal); and how much of X's largest can come
-    // to be added to the state
-    float sum = 0.f;
+    // T in two parts over a unit of each row: rows 16 w + n, tokens 32 s + 4 g and 16 on (zero above the diagonal); and how much of X's
+    // largest can come to be added to the state
+    float sum = 0.f, t[2][8], top = 0.f;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         if (2 * s > wave) break;
-        float t[8];
 #pragma unroll
         for (int m = 0; m < 8; ++m) {
             const int col = 32 * s + 16 * (m >> 2) + 4 * g + (m & 3);
-            t[m] = col / 16 <= wave ? Ts[16 * wave + n][col] * beta[col] : 0.f;
-            sum += fabsf(t[m]);
+            t[s][m] = col / 16 <= wave ? Ts[16 * wave + n][col] * beta[col] : 0.f;
+            sum += fabsf(t[s][m]);
+            top = fmaxf(top, fabsf(t[s][m]));
         }
+    }
+    const float unit = unit_of(column_max(top)), f = over(unit);
+    if (g == 0) reinterpret_cast<float *>(head + T_BYTES + P_BYTES)[T_UNIT + 16 * wave + n] = unit;
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {
-            kv_u4 part;
+    for (int s = 0; s < 2; ++s) {
+        if (2 * s > wave) break;
+        kv_u4 high, low;
 #pragma unroll
-            for (int m = 0; m < 4; ++m) part[m] = take_part(t[2 * m], t[2 * m + 1]);
-            *reinterpret_cast<kv_u4 *>(head + p * 8192 + (wave * 2 + s) * 1024 + lane * 16) = part;
+        for (int m = 0; m < 4; ++m) {
+            const kv_u2 part = split2(t[s][2 * m], t[s][2 * m + 1], f);
+            high[m] = part.x, low[m] = part.y;
         }
+        *reinterpret_cast<kv_u4 *>(head + (wave * 2 + s) * 1024 + lane * 16) = high;
+        *reinterpret_cast<kv_u4 *>(head + 8192 + (wave * 2 + s) * 1024 + lane * 16) = low;
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -413,11 +416,11 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
     const ChunkSpan span(x, b);
     const int64_t bk = (int64_t)b * x.Hk + h / (x.Hv / x.Hk);
     __shared__ __align__(16) char sS[2 * KS * NT * 1024];  // the state's parts, an operand a step
-    __shared__ __align__(16) char sX[3 * 2 * NT * 1024];   // X's parts
+    __shared__ __align__(16) char sX[2 * 2 * NT * 1024];   // X's parts
     __shared__ __align__(16) char sF[2 * 2 * NT * 1024];   // parts of diag(e^(G_63 - G) r_k) U
     __shared__ __align__(16) char sU[4 * NT * 1024];       // U, in float32
-    // by column and wavefront: the units of its rows of the state, and the largest of its rows of X
-    __shared__ __align__(16) float state_unit[NT][16][4], x_top[NT][16][4];
+    // by column and wavefront: the units of its rows of the state, and of X
+    __shared__ __align__(16) float state_unit[NT][16][4], x_unit[NT][16][4];
     // the sequence's chunks among those that are laid out
     const int c0 = max(span.from / CHUNK - w.chunk0, 0), c1 = min((span.end + CHUNK - 1) / CHUNK - w.chunk0, w.chunks);
     const bool none = span.from >= span.end || c0 >= c1;
@@ -583,8 +586,8 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
     if (!none) {
         const uint16_t *vp = reinterpret_cast<const uint16_t *>(x.v) + (int64_t)b * x.v_sb + (int64_t)h * x.Dv + col0, *v = vp + (int64_t)rows0 * x.v_sl + n;
         const int steps = wave < 2 ? 1 : 2;  // of T's rows that are not zero
-        kv_u4 K[KS], KT[TPW][2], T[3][2];
-        kv_f4 rise, fall;
+        kv_u4 K[KS], KT[TPW][2], T[2][2];
+        kv_f4 rise, fall, row_unit;
         float last, gain;
         uint16_t V[NT][4];
         auto request_rows = [&](int64_t at) {
@@ -611,7 +614,8 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
             for (int s = 0; s < 2; ++s)
                 if (s < steps)
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) T[p][s] = *reinterpret_cast<const kv_u4 *>(head + at * w.head + p * 8192 + (wave * 2 + s) * 1024);
+                    for (int p = 0; p < 2; ++p) T[p][s] = *reinterpret_cast<const kv_u4 *>(head + at * w.head + p * 8192 + (wave * 2 + s) * 1024);
+            row_unit = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + T_UNIT * 4);
             fall = *reinterpret_cast<const kv_f4 *>(factor + at * w.head + FALL * 4);
             gain = *reinterpret_cast<const float *>(factors + at * w.head + GAIN * 4);
         };
@@ -650,9 +654,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
         for (int c = c0; c < c1; ++c) {
             const int now = c - c0, next = min(c + 1, c1 - 1) - c0;
             const bool all_next = whole(next + c0);
-            kv_f4 U[NT][2];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) U[t][0] = U[t][1] = kv_f4{0.f, 0.f, 0.f, 0.f};
+            kv_f4 U[NT];
             lds_barrier();
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -669,46 +671,48 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                     }
                     X[r] = fmaf(-rise[r], R[r], value);
                 }
-                const float top = column_max(largest(X));
-                if (g == 0) x_top[t][n][wave] = top;
-                float x0 = X[0], x1 = X[1], x2 = X[2], x3 = X[3];
-#pragma unroll
-                for (int p = 0; p < 3; ++p)
-                    *reinterpret_cast<kv_u2 *>(part_of(sX, p, 2, wave >> 1, t) + (wave & 1) * 8) = kv_u2{take_part(x0, x1), take_part(x2, x3)};
+                const float unit = unit_of(column_max(largest(X)));
+                if (g == 0) x_unit[t][n][wave] = unit;
+                share(sX, 2, wave, t, X, over(unit));
             }
             lds_barrier();
             float f_unit[NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                kv_u4 part[3][2];
+                kv_u4 part[2][2];
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
                     if (s < steps)
 #pragma unroll
-                        for (int p = 0; p < 3; ++p) part[p][s] = *reinterpret_cast<const kv_u4 *>(part_of(sX, p, 2, s, t));
-                const kv_f4 tops = *reinterpret_cast<const kv_f4 *>(x_top[t][n]);
+                        for (int p = 0; p < 2; ++p) part[p][s] = *reinterpret_cast<const kv_u4 *>(part_of(sX, p, 2, s, t));
+                const kv_f4 units = *reinterpret_cast<const kv_f4 *>(x_unit[t][n]);
                 all_requested();
                 if (t == 0) {
                     request_rows(next);
                     request_values(next, all_next);
                 }
-                f_unit[t] = unit_of(gain * fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+                f_unit[t] = unit_of(gain * 16384.f * fmaxf(fmaxf(units[0], units[1]), fmaxf(units[2], units[3])));
+                U[t] = kv_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
+                for (int s = 0; s < 2; ++s) {  // each wavefront's rows of X apart, half a step, then put together by their units
                     if (s >= steps) break;
-                    U[t][0] = mfma_bf16(T[0][s], part[0][s], U[t][0]);
-                    U[t][1] = mfma_bf16(T[0][s], part[1][s], U[t][1]);
-                    U[t][0] = mfma_bf16(T[1][s], part[0][s], U[t][0]);
-                    U[t][1] = mfma_bf16(T[1][s], part[1][s], U[t][1]);
-                    U[t][0] = mfma_bf16(T[0][s], part[2][s], U[t][0]);
-                    U[t][1] = mfma_bf16(T[2][s], part[0][s], U[t][1]);
+                    auto half = [](const kv_u4 &v, int k) { return k ? kv_u2{v.z, v.w} : kv_u2{v.x, v.y}; };
+                    kv_f4 y[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        y[k] = mfma_f16(half(T[0][s], k), half(part[0][s], k), kv_f4{0.f, 0.f, 0.f, 0.f});
+                        y[k] = mfma_f16(half(T[0][s], k), half(part[1][s], k), y[k]);
+                        y[k] = mfma_f16(half(T[1][s], k), half(part[0][s], k), y[k]);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) U[t][r] = fmaf(units[2 * s + 1], y[1][r], fmaf(units[2 * s], y[0][r], U[t][r]));
                 }
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 kv_f4 u;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) u[r] = U[t][0][r] + U[t][1][r];
+                for (int r = 0; r < 4; ++r) u[r] = row_unit[r] * U[t][r];
                 *reinterpret_cast<kv_f4 *>(sU + (wave * NT + t) * 1024 + lane * 16) = u;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) u[r] *= fall[r];
@@ -766,8 +770,8 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
 inline int chunk_key_dim(const DeltaArgs &x) { return x.Dk <= 64 ? 64 : x.Dk <= 128 ? 128 : 256; }
 // What a chunk of all sequences and heads takes, and how many chunks are laid out at a time: what they take is to stay near the
 // last-level cache between the two kernels, and a round is to be long enough to pay for its start.  96 / 192 / 384 / 768 MiB, 32 heads of
-// 128 x 128 in bfloat16, us: 8 x 2000 tokens 649 / 564 / 553 / 548; 16 x 4096 2225 / 2112 / 1920 / 1813; 32768 of one 1175 / 1106 /
-// 1181 / 1159.  More than 384 gains little for twice the memory.
+// 128 x 128 in bfloat16, us: 8 x 2000 tokens 637 / 574 / 576 / 558; 16 x 4096 2224 / 2061 / 1910 / 1840; 32768 of one 1165 / 1111 /
+// 1154 / 1139.  More than 384 gains little for twice the memory.
 constexpr uint64_t CHUNK_SPACE = (uint64_t)384 << 20;
 inline ChunkSpace chunk_space(const DeltaArgs &x, void *workspace, uint64_t *bytes) {
     ChunkSpace w{};
@@ -803,9 +807,9 @@ template <int DT, int KD> hipError_t launch_chunks(const DeltaArgs &x, ChunkSpac
         };
         const int64_t groups = (int64_t)x.B * x.Hv * ((x.Dv + 15) / 16);
         // Every workgroup of a head reads the head's whole operands: few columns to each fill the chip, many read less.  Whole calls in
-        // us with 16 / 32 / 64 columns, 32 heads of 128 x 128 in bfloat16: 8192 tokens (256 groups) 316 / 404 / 635; 2 x 2048 (512)
-        // 152 / 126 / 190; 4 x 2048 (1024) 342 / 256 / 238; 8 x 2000 in float16 (2048) 1124 / 660 / 538.  256 channels have no
-        // registers for 64; 4 heads of 512 x 256: 4096 tokens (128) 147 / 215; 4 x 2048 (512) 162 / 138.
+        // us with 16 / 32 / 64 columns, 32 heads of 128 x 128 in bfloat16: 8192 tokens (256 groups) 319 / 415 / 652; 2 x 2048 (512)
+        // 152 / 129 / 191; 4 x 2048 (1024) 318 / 264 / 245; 8 x 2000 in float16 (2048) 1073 / 656 / 545 (but 6 x 2048, 1536, 590 / 395 / 410).
+        // 256 channels have no registers for 64; 4 heads of 512 x 256: 4096 tokens (128) 151 / 224; 4 x 2048 (512) 166 / 143.
         if (groups <= 256) {
             scan(chunk_scan_kernel<DT, KD, 1>, 16);
         } else if (KD > 128 || groups <= 512) {

@@ -5,7 +5,9 @@ arithmetic adds is never enlarged by a later one and errors add up over tokens. 
 of v) that is met, a token adds: two products of Dk terms, each off by at most (Dk / 8 + 3 + 4) half units of float32 of M
 (eight lanes' chains, three permutes, the norms' roots and quotients), the decay (its exponent is off by a few
 units of itself: x e^-x <= 0.37, so at most four units), the update and the sums.  96 units of 2^-24 M a token hold all of it
-for Dk <= 256.  Operands of the matrix cores are split into three parts of 8 bits, which is another unit.  The output is rounded once: half a step of its type.
+for Dk <= 256.  Operands of the matrix cores are split into two parts of 11 bits: the state, what is added to it, the triangular system and
+its right side are each off by at most two units of the largest in their row or column, eight units a token, where the sums over 32 terms
+at a time are off by less than the chains of Dk / 8.  The output is rounded once: half a step of its type.
 Convolution: at most 8 products and sums of terms no larger than sum |w e| = A, then x sigmoid(x), whose slope is below 1.1: 16 units of A, and
 the output's rounding.
 """
