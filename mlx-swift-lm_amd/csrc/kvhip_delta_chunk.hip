@@ -64,8 +64,11 @@ __device__ __forceinline__ kv_u2 split2(float x, float y, float f) {  // of x f 
 // The power of two over which a row's or column's elements are laid out in float16, by the largest: they end below 2^14.
 __device__ __forceinline__ float unit_of(float top) {
     const uint32_t e = __float_as_uint(top) >> 23;  // (infinity and NaN: some unit; they stay what they are)
-    return __uint_as_float((min(max(e, 27u), 240u) - 13) << 23);
+    return __uint_as_float((min(max(e, 28u), 254u) - 13) << 23);  // (2^-112 to 2^114)
 }
+// Products of two such operands are up to 2^28 of their units' product, and one unit may be as large as float32 goes: columns' units stand
+// for SHIFT of what they are, rows' for the rest.
+constexpr float SHIFT = 1.f / 16384;
 __device__ __forceinline__ float over(float unit) { return __uint_as_float(0x7f000000u - __float_as_uint(unit)); }  // 1 / unit
 // the largest of the four lanes that hold a column
 __device__ __forceinline__ float column_max(float v) {
@@ -336,8 +339,8 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
             float *f = reinterpret_cast<float *>(head + T_BYTES + P_BYTES);
             const double mine = total[lane], last = total[CHUNK - 1];
             const float rise = __builtin_amdgcn_exp2f((float)mine);
-            f[RISE_K + lane] = rise * rk[lane] * key_unit[lane];
-            f[RISE_Q + lane] = rise * rq[lane] * query_unit[lane];
+            f[RISE_K + lane] = rise * rk[lane] * key_unit[lane] / SHIFT;
+            f[RISE_Q + lane] = rise * rq[lane] * query_unit[lane] / SHIFT;
             f[FALL + lane] = falls[lane] = __builtin_amdgcn_exp2f((float)(last - mine)) * rk[lane] * key_unit[lane];
             f[P_UNIT + lane] = p_unit[lane];
             if (lane == 0) f[LAST] = __builtin_amdgcn_exp2f((float)last);
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
         }
     }
     const float unit = unit_of(column_max(top)), f = over(unit);
-    if (g == 0) reinterpret_cast<float *>(head + T_BYTES + P_BYTES)[T_UNIT + 16 * wave + n] = unit;
+    if (g == 0) reinterpret_cast<float *>(head + T_BYTES + P_BYTES)[T_UNIT + 16 * wave + n] = unit / SHIFT;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         if (2 * s > wave) break;
@@ -544,7 +547,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
             for (int t = 0; t < NT; ++t) {
                 float y[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = fmaf(rise[r], O[t][r], unit[r] * u_unit[t] * I[t][r]);
+                for (int r = 0; r < 4; ++r) y[r] = fmaf(rise[r], O[t][r], unit[r] * I[t][r] * u_unit[t]);
                 if (all) {
                     const uint32_t a = DT == 1 ? pk_bf2(y[0], y[1]) : pk_h2(y[0], y[1]), e = DT == 1 ? pk_bf2(y[2], y[3]) : pk_h2(y[2], y[3]);
                     o[16 * t] = (uint16_t)a;
@@ -640,7 +643,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
 #pragma unroll
                 for (int i = 1; i < TPW; ++i) top = fmaxf(top, largest(S[i][t]));
                 const float unit = unit_of(column_max(top)), f = over(unit);
-                if (g == 0) state_unit[t][n][wave] = unit;
+                if (g == 0) state_unit[t][n][wave] = unit * SHIFT;
 #pragma unroll
                 for (int i = 0; i < TPW; ++i) share(sS, KS, wave * TPW + i, t, S[i][t], f);
             }
@@ -672,7 +675,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                     X[r] = fmaf(-rise[r], R[r], value);
                 }
                 const float unit = unit_of(column_max(largest(X)));
-                if (g == 0) x_unit[t][n][wave] = unit;
+                if (g == 0) x_unit[t][n][wave] = unit * SHIFT;
                 share(sX, 2, wave, t, X, over(unit));
             }
             lds_barrier();
@@ -691,7 +694,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                     request_rows(next);
                     request_values(next, all_next);
                 }
-                f_unit[t] = unit_of(gain * 16384.f * fmaxf(fmaxf(units[0], units[1]), fmaxf(units[2], units[3])));
+                f_unit[t] = unit_of(gain * fmaxf(fmaxf(units[0], units[1]), fmaxf(units[2], units[3])) * (16384.f / SHIFT));
                 U[t] = kv_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {  // each wavefront's rows of X apart, half a step, then put together by their units

@@ -319,6 +319,20 @@ def test_values_of_other_sizes(dtype, size):
     check(out, cache.delta_state, expect(x, state), n, dtype)
 
 
+@pytest.mark.parametrize("n", [3, 100])
+@pytest.mark.parametrize("size", [2.0 ** 118, 2.0 ** -110])
+def test_values_at_the_ends_of_the_range(n, size):
+    """bfloat16 has float32's range, and so has what a prompt is made of."""
+    rng = np.random.default_rng(9)
+    x, state = make(rng, 2, n, 1, 2, 128, 64, torch.bfloat16)
+    x["v"] = x["v"] * size
+    state = state * size
+    cache = kvhip.GatedDeltaCache()
+    cache.delta_state = state
+    out = kvhip.gated_delta_update(**x, cache=cache)
+    check(out, cache.delta_state, expect(x, state), n, torch.bfloat16)
+
+
 def test_calls_join():
     """A prompt, a draft and tokens give what they give in one call, within the bound of both; a copy is what it was."""
     rng = np.random.default_rng(8)
