@@ -7,7 +7,7 @@
 // four neighbouring elements in every 32 each, so that a wavefront's load is eight whole cache lines.  Rows never meet: a
 // wavefront needs no other, nothing goes through LDS, and a head's rows are spread over as many wavefronts as fill the chip.
 // With o written as  g (S q^) + u (k^ q^),  both products of a token read the same S and their sums over the eight lanes (three
-// permutes each) run side by side.  Every lane makes the token's norms and gates for itself.
+// permutes each) run side by side.  Every lane makes the token's norms for itself.
 //
 // Memory bounds it: a state is read and written once, past the caches, which it would only sweep.  One token of 64 sequences x 32
 // heads x 128 x 128: 54 us, 5.0 TB/s (68 us through the caches).
@@ -63,6 +63,15 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs x) {
     const int Dk = x.Dk, Dv = x.Dv, hk = h / (x.Hv / x.Hk);
     const int from = x.left_pad ? min(max(x.left_pad[b], 0), x.L) : 0;
     const int end = x.lengths ? min(max(x.lengths[b], from), x.L) : x.L;
+    // Gates of 64 tokens at a time, a token to a lane; of the first ones, in front of the state.  (Every lane making every token's: 2048
+    // float32 tokens of 32 heads x 128 x 128 2115 us, and 1429 so; 64 single ones 54.2, and 55.6.)
+    float ga = 0.f, gb = 0.f;
+    auto request_gates = [&](int l) {
+        if (l + lane >= end) return;
+        ga = load_gate(x.gate_dtype, x.a, (int64_t)b * x.a_sb + (int64_t)(l + lane) * x.a_sl + h);
+        gb = load_gate(x.gate_dtype, x.b, (int64_t)b * x.b_sb + (int64_t)(l + lane) * x.b_sl + h);
+    };
+    request_gates(from);
     kv_f4 s[R][NC];
     const int64_t cell = ((int64_t)b * x.Hv + h) * Dv;
 #pragma unroll
@@ -85,7 +94,7 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs x) {
     const int64_t o_sl = (int64_t)x.Hv * Dv;
     // a token's operands, requested a token ahead
     kv_f4 q[NC], k[NC];
-    float v[R], ga = 0.f, gb = 0.f;
+    float v[R];
     auto request = [&](int l) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -95,9 +104,19 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs x) {
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) v[r] = row0 + 8 * r < Dv ? Elem<DT>::load(vp, (int64_t)l * x.v_sl + row0 + 8 * r) : 0.f;
-        ga = load_gate(x.gate_dtype, x.a, (int64_t)b * x.a_sb + (int64_t)l * x.a_sl + h);
-        gb = load_gate(x.gate_dtype, x.b, (int64_t)b * x.b_sb + (int64_t)l * x.b_sl + h);
     };
+    float decay = 1.f, beta_of = 0.f;
+    auto turn_gates = [&]() {
+        if (x.a_log) {
+            const float t = ga + dt;
+            decay = fast_exp2(-rate * (fmaxf(t, 0.f) + log1pf(fast_exp2(-LOG2E * fabsf(t)))));
+            beta_of = __builtin_amdgcn_rcpf(1.f + fast_exp2(-LOG2E * gb));
+        } else {
+            decay = fast_exp2(LOG2E * ga);
+            beta_of = gb;
+        }
+    };
+    auto of_lane = [](float v, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)); };
     if (from < end) request(from);
     auto store = [&](int l, int r, float o) {
         if (j == 0 && row0 + 8 * r < Dv) Elem<DT>::store(op, (int64_t)l * o_sl + row0 + 8 * r, o);
@@ -130,15 +149,12 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs x) {
         float vn[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) vn[r] = v[r];
-        float g, beta;
-        if (x.a_log) {
-            const float t = ga + dt;
-            g = fast_exp2(-rate * (fmaxf(t, 0.f) + log1pf(fast_exp2(-LOG2E * fabsf(t)))));
-            beta = __builtin_amdgcn_rcpf(1.f + fast_exp2(-LOG2E * gb));
-        } else {
-            g = fast_exp2(LOG2E * ga);
-            beta = gb;
+        const int at = (l - from) & 63;
+        if (at == 0) {
+            turn_gates();
+            request_gates(l + 64);
         }
+        const float g = of_lane(decay, at), beta = of_lane(beta_of, at);
         if (l + 1 < end) request(l + 1);
         qq = sum8(qq);
         kk = sum8(kk);
