@@ -15,7 +15,8 @@
 // (22 bits; 1.4e-7 against 64 bits, as with three parts of bfloat16 for T and X) over powers of two: T's for each row, the others' for
 // each column.  Of a wavefront's rows of X or of the state the largest is at hand, of diag(e^(G_63 - G)) U it is bounded by X's
 // units and the largest sum over a row of T.  Decays are summed in float64: e^-1000 beside e^-0.001 loses
-// nothing.  The outputs, rounded to 16 bits, take one part of S, P and U each (float16: two).
+// nothing.  The outputs take the same two parts of S, P and U: of one part, 11 bits, more than one in ten bfloat16 outputs would be
+// another value than the float32 arithmetic's.
 //
 // 8192 tokens x 32 heads x 128 x 128 in bfloat16, one sequence: 72 us of preparation (its writes and reads, 5 TB/s) and 234 of the
 // scan, whose 128 chunks follow one another, 1.8 us each: about 1.1 are the chain of products and barriers from state to state, the
@@ -26,8 +27,6 @@
 // Operands lie in the workspace as the lanes take them, 1 KB to an instruction: contractions may be summed in any
 // order, so that lane (n, g)'s eight elements of a step are those at 4 g and 16 + 4 g of it -- which is where a product leaves them: S, U
 // go from accumulators to operands without crossing lanes, only from wavefront to wavefront through LDS.
-#include <type_traits>
-
 #include "kvhip_delta.hpp"
 #include "kvhip_device.hpp"
 
@@ -91,7 +90,7 @@ struct ChunkSpace {
 };
 __device__ __forceinline__ char *key_at(const ChunkSpace &w, int64_t bh, int c) { return w.base + (bh * w.chunks + c) * w.key; }
 __device__ __forceinline__ char *head_at(const ChunkSpace &w, int64_t bh, int c) { return w.base + w.heads + (bh * w.chunks + c) * w.head; }
-constexpr int T_BYTES = CHUNK * CHUNK * 4, P_BYTES = CHUNK * CHUNK * 4;  // two parts (of P in bfloat16 one is used)
+constexpr int T_BYTES = CHUNK * CHUNK * 4, P_BYTES = CHUNK * CHUNK * 4;  // two parts
 // Factors of rows, the units of their operands among them: e^G r_k (what K S is worth), scale e^G r_q, e^(G_63 - G) r_k, P's units, T's; then
 // e^G_63, and the bound of |diag(e^(G_63 - G)) U| over the largest |X| of a column.
 constexpr int RISE_K = 0, RISE_Q = CHUNK, FALL = 2 * CHUNK, P_UNIT = 3 * CHUNK, T_UNIT = 4 * CHUNK, LAST = 5 * CHUNK, GAIN = 5 * CHUNK + 1;
@@ -308,7 +307,7 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
                 high[m] = part.x, low[m] = part.y;
             }
             *reinterpret_cast<kv_u4 *>(p + (wave * 2 + s) * 1024 + lane * 16) = high;
-            if (DT == 0) *reinterpret_cast<kv_u4 *>(p + 8192 + (wave * 2 + s) * 1024 + lane * 16) = low;
+            *reinterpret_cast<kv_u4 *>(p + 8192 + (wave * 2 + s) * 1024 + lane * 16) = low;
         }
     }
 #pragma unroll
@@ -410,7 +409,7 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
 // need is off the way from one state to the next, and fills the other's waits on the same SIMDs.
 template <int DT, int KD, int NT>
 __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSpace w, const float *state_in) {
-    constexpr int SP = DT == 0 ? 2 : 1, KS = KD / 32, TPW = KD / 64;  // SP: parts that outputs take; TPW: a wavefront's tiles of the state
+    constexpr int KS = KD / 32, TPW = KD / 64;  // TPW: a wavefront's tiles of the state
     static_assert(KD % 64 == 0, "whole tiles to a wavefront");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6 & 3, n = lane & 15, g = lane >> 4;
     // (a head's workgroups on one die, where their operands meet in its cache: 8 dies take workgroups in turn)
@@ -437,12 +436,12 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
     // is used, and waits for LDS as often.  Requests to memory, which take their time to be issued, stand behind it, where a wavefront waits
     // anyway, and not in front of a barrier.
     auto all_requested = []() { __builtin_amdgcn_sched_barrier(0); };
-    // rows [KS] times the state's columns 16 t on, in PARTS parts: each wavefront's rows of it apart, then put together by their units
-    auto times_state = [&](auto parts, const kv_u4 *rows, int t, auto &&meanwhile) {
+    // rows [KS] times the state's columns 16 t on, in its two parts: each wavefront's rows of it apart, then put together by their units
+    auto times_state = [&](const kv_u4 *rows, int t, auto &&meanwhile) {
         kv_f4 y[4], sum;
-        kv_u4 part[decltype(parts)::value][KS];
+        kv_u4 part[2][KS];
 #pragma unroll
-        for (int p = 0; p < decltype(parts)::value; ++p)
+        for (int p = 0; p < 2; ++p)
 #pragma unroll
             for (int s = 0; s < KS; ++s) part[p][s] = *reinterpret_cast<const kv_u4 *>(part_of(sS, p, KS, s, t));
         const kv_f4 units = *reinterpret_cast<const kv_f4 *>(state_unit[t][n]);
@@ -451,7 +450,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
 #pragma unroll
         for (int k = 0; k < 4; ++k) y[k] = kv_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int p = 0; p < decltype(parts)::value; ++p)
+        for (int p = 0; p < 2; ++p)
 #pragma unroll
             for (int i = 0; i < 4 * TPW; i += TPW > 1 ? 2 : 1) {  // tiles of 16 rows, two to a step; of KD 64 a wavefront has half a step
                 const int s = i >> 1, k = i / TPW;
@@ -477,7 +476,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                     if (row0 + r < x.L && col0 + 16 * t + n < x.Dv) op[(row0 + r) * o_sl + 16 * t] = 0;
         }
         if (none) return;
-        kv_u4 Q[KS], P[SP][2];
+        kv_u4 Q[KS], P[2][2];
         kv_f4 rise, unit;
         const int steps = wave < 2 ? 1 : 2;  // of P's rows that are not zero
         uint16_t *o = op + rows0 * o_sl;
@@ -492,7 +491,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
             for (int s = 0; s < 2; ++s)
                 if (s < steps)
 #pragma unroll
-                    for (int p = 0; p < SP; ++p) P[p][s] = *reinterpret_cast<const kv_u4 *>(head + at * w.head + T_BYTES + p * 8192 + (wave * 2 + s) * 1024);
+                    for (int p = 0; p < 2; ++p) P[p][s] = *reinterpret_cast<const kv_u4 *>(head + at * w.head + T_BYTES + p * 8192 + (wave * 2 + s) * 1024);
         };
         request_rows(0);
         request_rest(0);
@@ -502,7 +501,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
             lds_barrier();
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                O[t] = times_state(std::integral_constant<int, SP>{}, Q, t, []() {});
+                O[t] = times_state(Q, t, []() {});
                 I[t] = kv_f4{0.f, 0.f, 0.f, 0.f};
             }
             request_rows(next);
@@ -536,10 +535,8 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                         high[m] = part.x, low[m] = part.y;
                     }
                     I[t] = mfma_f16(P[0][s], high, I[t]);
-                    if constexpr (SP == 2) {
-                        I[t] = mfma_f16(P[SP - 1][s], high, I[t]);
-                        I[t] = mfma_f16(P[0][s], low, I[t]);
-                    }
+                    I[t] = mfma_f16(P[1][s], high, I[t]);
+                    I[t] = mfma_f16(P[0][s], low, I[t]);
                 }
             }
             const bool all = whole(c);
@@ -661,7 +658,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
             lds_barrier();
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const kv_f4 R = times_state(std::integral_constant<int, 2>{}, K, t, [&]() {
+                const kv_f4 R = times_state(K, t, [&]() {
                     if (t == 0 && c > c0) request_rest(now);
                 });
                 kv_f4 X;

@@ -1,0 +1,39 @@
+"""Accuracy of the gated delta rule where the bounds of a worst case say little.
+
+A 16-bit output is a float32 value y, rounded once: with o the definition's value, |out - o| <= |y - o| + half a step of the type at the larger of
+both.  What |out - o| has beyond that half step is therefore no more than |y - o|, which is held to what states are held to: errors
+that add up at random stay below 4e-6 of the 2-norm."""
+import numpy as np
+import pytest
+import torch
+
+import kvhip
+from tests.test_gpu_gated_delta import DTYPES, LAYOUTS, expect, f64, make
+
+pytestmark = pytest.mark.gpu
+
+
+def half_steps(out, o, dtype):
+    """Half the distance of `dtype`'s neighbouring values where `out` and `o` lie."""
+    info = torch.finfo(dtype)
+    size = np.maximum(np.maximum(np.abs(out), np.abs(o)), info.tiny)
+    return 2.0 ** np.floor(np.log2(size)) * info.eps / 2
+
+
+def beyond_rounding(out, o, dtype):
+    got = f64(out)
+    return np.maximum(np.abs(got - o) - (half_steps(got, o, dtype) if dtype != torch.float32 else 0.0), 0.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("n", [1, 5, 40, 200])
+def test_outputs_are_rounded_once(dtype, layout, n):
+    rng = np.random.default_rng(200 + n)
+    x, state = make(rng, 2, n, *layout, dtype)
+    cache = kvhip.GatedDeltaCache()
+    cache.delta_state = state
+    out = kvhip.gated_delta_update(**x, cache=cache)
+    o, s, _ = expect(x, state)
+    assert np.linalg.norm(f64(cache.delta_state) - s) <= 4e-6 * np.linalg.norm(s)
+    assert np.linalg.norm(beyond_rounding(out, o, dtype)) <= 4e-6 * np.linalg.norm(o)
