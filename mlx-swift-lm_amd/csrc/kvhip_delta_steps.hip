@@ -244,8 +244,9 @@ template <int DT, int V> struct ConvRow {
     }
 };
 
-// WT: taps that are laid out (4 or 8); the call's W <= WT are the last ones, the others weigh nothing and are not read
-template <int DT, int V, int WT>
+// W: taps.  (A kernel to each number of them: taps of weight zero behind a smaller one's would carry infinities and NaN on to tokens
+// that the convolution does not reach.)
+template <int DT, int V, int W>
 __global__ void __launch_bounds__(256) short_conv_kernel(ConvArgs x) {
     constexpr int ES = DT == 2 ? 4 : 2;
     const int c = (blockIdx.x * 256 + threadIdx.x) * V, b = blockIdx.z;
@@ -253,11 +254,10 @@ __global__ void __launch_bounds__(256) short_conv_kernel(ConvArgs x) {
     const int from = x.left_pad ? min(max(x.left_pad[b], 0), x.L) : 0;
     const int end = x.lengths ? min(max(x.lengths[b], from), x.L) : x.L;
     const char *xp = x.x + ((int64_t)b * x.x_sb + c) * ES;
-    const char *win = x.window_in ? x.window_in + ((int64_t)b * (x.W - 1) * x.C + c) * ES : nullptr;
-    char *wout = x.window_out + ((int64_t)b * (x.W - 1) * x.C + c) * ES;
+    const char *win = W > 1 && x.window_in ? x.window_in + ((int64_t)b * (W - 1) * x.C + c) * ES : nullptr;
+    char *wout = W > 1 ? x.window_out + ((int64_t)b * (W - 1) * x.C + c) * ES : nullptr;
     char *op = x.out + ((int64_t)b * x.L * x.C + c) * ES;
     const int64_t xs = x.x_sl * ES, cs = (int64_t)x.C * ES;
-    const int skip = WT - x.W;  // taps that are not there
     const int tile = blockIdx.y * CONV_TOKENS;
     ConvRow<DT, V> none;
     none.zero();
@@ -265,55 +265,52 @@ __global__ void __launch_bounds__(256) short_conv_kernel(ConvArgs x) {
     const int l0 = from + tile, l1 = min(l0 + CONV_TOKENS, end);
     for (int l = max(l0, end); l < min(l0 + CONV_TOKENS, x.L); ++l) none.store(op + l * cs);
     if (l0 >= l1 && tile > 0) return;
-    float w[WT][V], bias[V];
-    if (WT == 4 && V > 1 && x.W == 4 && (uintptr_t)x.weight % 16 == 0) {  // (four taps of V channels: 64 bytes side by side)
+    float w[W][V], bias[V];
+    if (W == 4 && V > 1 && (uintptr_t)x.weight % 16 == 0) {  // (four taps of V channels: 64 bytes side by side)
         ConvRow<DT, V> packed[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) packed[m].load(x.weight + (int64_t)c * 4 * ES + m * 16);
 #pragma unroll
         for (int i = 0; i < V; ++i)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) w[t][i] = packed[(i * 4 + t) / V].v[(i * 4 + t) % V];
+            for (int t = 0; t < W; ++t) w[t][i] = packed[(i * 4 + t) / V & 3].v[(i * 4 + t) % V];
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
 #pragma unroll
-            for (int t = 0; t < WT; ++t) w[t][i] = t >= skip ? Elem<DT>::load(x.weight, (int64_t)(c + i) * x.W + t - skip) : 0.f;
+            for (int t = 0; t < W; ++t) w[t][i] = Elem<DT>::load(x.weight, (int64_t)(c + i) * W + t);
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) bias[i] = x.bias ? Elem<DT>::load(x.bias, c + i) : 0.f;
-    ConvRow<DT, V> e[WT - 1 + CONV_AHEAD];  // rows l - (WT - 1) on
-    // (row i of the window is e's row skip + i)
+    ConvRow<DT, V> e[W - 1 + CONV_AHEAD];  // rows l - (W - 1) on
 #pragma unroll
-    for (int i = 0; i < WT - 1; ++i) {
+    for (int i = 0; i < W - 1; ++i) {
         e[i].zero();
-        if (i < skip) continue;
-        if (tile > 0) e[i].load(xp + (l0 - (WT - 1) + i) * xs);
-        else if (win) e[i].load(win + (i - skip) * cs);
+        if (tile > 0) e[i].load(xp + (l0 - (W - 1) + i) * xs);
+        else if (win) e[i].load(win + i * cs);
     }
-    if (tile == 0) {  // the new window: the last W - 1 of the old one's rows and the tokens
+    if (W > 1 && tile == 0) {  // the new window: the last W - 1 of the old one's rows and the tokens
         const int n = end - from;
 #pragma unroll
-        for (int i = 0; i < WT - 1; ++i) {
-            if (i < skip) continue;
+        for (int i = 0; i < W - 1; ++i) {
             const int at = i + n;  // as a row of e
             ConvRow<DT, V> r;
             r.zero();
-            if (at < WT - 1) {
+            if (at < W - 1) {
 #pragma unroll
-                for (int m = 0; m < WT - 1; ++m)
+                for (int m = 0; m < W - 1; ++m)
                     if (m == at) r = e[m];
             } else {
-                r.load(xp + (from + at - (WT - 1)) * xs);
+                r.load(xp + (from + at - (W - 1)) * xs);
             }
-            r.store(wout + (i - skip) * cs);
+            r.store(wout + i * cs);
         }
     }
     for (int l = l0; l < l1; l += CONV_AHEAD) {
 #pragma unroll
         for (int t = 0; t < CONV_AHEAD; ++t) {
-            if (l + t < l1) e[WT - 1 + t].load(xp + (l + t) * xs);
-            else e[WT - 1 + t].zero();
+            if (l + t < l1) e[W - 1 + t].load(xp + (l + t) * xs);
+            else e[W - 1 + t].zero();
         }
 #pragma unroll
         for (int t = 0; t < CONV_AHEAD; ++t) {
@@ -323,13 +320,13 @@ __global__ void __launch_bounds__(256) short_conv_kernel(ConvArgs x) {
             for (int i = 0; i < V; ++i) {
                 float s = bias[i];
 #pragma unroll
-                for (int m = 0; m < WT; ++m) s = fmaf(w[m][i], e[t + m].v[i], s);
+                for (int m = 0; m < W; ++m) s = fmaf(w[m][i], e[t + m].v[i], s);
                 y.v[i] = x.silu ? s * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * -LOG2E)) : s;
             }
             y.store(op + (l + t) * cs);
         }
 #pragma unroll
-        for (int i = 0; i < WT - 1; ++i) e[i] = e[i + CONV_AHEAD];
+        for (int i = 0; i < W - 1; ++i) e[i] = e[i + CONV_AHEAD];
     }
 }
 
@@ -374,11 +371,18 @@ hipError_t launch_short_conv(const ConvArgs &x, hipStream_t s) {
     const int per = 256 * (wide ? vec : 1);
     const dim3 grid((x.C + per - 1) / per, (x.L + CONV_TOKENS - 1) / CONV_TOKENS, x.B);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, x); };
-#define KV_GO(DT, V, WT) go(short_conv_kernel<DT, V, WT>)
-#define KV_TAPS(DT, V) (x.W <= 4 ? KV_GO(DT, V, 4) : KV_GO(DT, V, 8))
-    if (x.dtype == KVHIP_F16) wide ? KV_TAPS(0, 8) : KV_TAPS(0, 1);
-    else if (x.dtype == KVHIP_BF16) wide ? KV_TAPS(1, 8) : KV_TAPS(1, 1);
-    else wide ? KV_TAPS(2, 4) : KV_TAPS(2, 1);
+#define KV_GO(DT, V, W)                              \
+    case W:                                          \
+        wide ? go(short_conv_kernel<DT, V, W>) : go(short_conv_kernel<DT, 1, W>); \
+        break;
+#define KV_TAPS(DT, V)                                                                                                                  \
+    switch (x.W) {                                                                                                                      \
+        KV_GO(DT, V, 1) KV_GO(DT, V, 2) KV_GO(DT, V, 3) KV_GO(DT, V, 4) KV_GO(DT, V, 5) KV_GO(DT, V, 6) KV_GO(DT, V, 7) KV_GO(DT, V, 8) \
+        default: return hipErrorInvalidValue;                                                                                           \
+    }
+    if (x.dtype == KVHIP_F16) KV_TAPS(0, 8)
+    else if (x.dtype == KVHIP_BF16) KV_TAPS(1, 8)
+    else KV_TAPS(2, 4)
 #undef KV_TAPS
 #undef KV_GO
     return hipGetLastError();
