@@ -77,6 +77,11 @@ __device__ __forceinline__ float column_max(float v) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// A wavefront's number as what it is, the same in all its lanes: branches on it are a wavefront's.  (Matrix instructions heed no mask of lanes:
+// under a branch that the compiler takes for one of lanes, and leaves out because the masked way is short, they work on whatever their
+// registers hold.)
+__device__ __forceinline__ int wave_number() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // what wavefronts hand one another through LDS; requests past it stay in flight
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -110,7 +115,7 @@ template <int DT, int KD, bool WIDE>
 __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(DeltaArgs x, ChunkSpace w) {
     constexpr int PITCH = KD + 8, ROW = CHUNK + 4, BYTES = CHUNK * PITCH * 2;
     constexpr double LOG2E_64 = 1.4426950408889634074;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_number(), n = lane & 15, g = lane >> 4;
     const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, per = x.Hv / x.Hk, hk = h / per;
     const ChunkSpan span(x, b);
     const int t0 = (w.chunk0 + c) * CHUNK;
@@ -411,7 +416,7 @@ template <int DT, int KD, int NT>
 __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSpace w, const float *state_in) {
     constexpr int KS = KD / 32, TPW = KD / 64;  // TPW: a wavefront's tiles of the state
     static_assert(KD % 64 == 0, "whole tiles to a wavefront");
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6 & 3, n = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, number = wave_number(), wave = number & 3, n = lane & 15, g = lane >> 4;
     // (a head's workgroups on one die, where their operands meet in its cache: 8 dies take workgroups in turn)
     const int heads = x.B * x.Hv, bh = blockIdx.x % heads, col0 = blockIdx.x / heads * (16 * NT);
     const int b = bh / x.Hv, h = bh % x.Hv;
@@ -463,7 +468,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
         return sum;
     };
     // A chunk's operands are requested as soon as the last chunk's have been used, in the order in which they will be.
-    if (threadIdx.x >= 256) {
+    if (number >= 4) {
         uint16_t *op = reinterpret_cast<uint16_t *>(x.out) + ((int64_t)b * x.L * x.Hv + h) * x.Dv + col0 + n;
         const int64_t o_sl = (int64_t)x.Hv * x.Dv;
         for (int c = 0; c < w.chunks; ++c) {  // rows of chunks without tokens

@@ -37,3 +37,24 @@ def test_outputs_are_rounded_once(dtype, layout, n):
     o, s, _ = expect(x, state)
     assert np.linalg.norm(f64(cache.delta_state) - s) <= 4e-6 * np.linalg.norm(s)
     assert np.linalg.norm(beyond_rounding(out, o, dtype)) <= 4e-6 * np.linalg.norm(o)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("n", [20, 100, 200])
+def test_what_memory_held_before_is_nothing_to_a_prompt(dtype, layout, n):
+    """Workspace and registers are of no content: matrix instructions work on whole registers whatever lanes are masked, and what they
+    work on has to have been written."""
+    rng = np.random.default_rng(300 + n)
+    x, state = make(rng, 2, n, *layout, dtype)
+    results = []
+    for junk in (float("nan"), float("inf"), 0.0):
+        held = [torch.full((size,), junk, device="cuda") for size in (500, 8192, 13000, 16384, 60000, 200000)]
+        cache = kvhip.GatedDeltaCache()
+        cache.delta_state = state
+        del held
+        results.append((kvhip.gated_delta_update(**x, cache=cache), cache.delta_state))
+    assert all(torch.equal(a, b) for r in results[1:] for a, b in zip(r, results[0]))
+    o, s, _ = expect(x, state)
+    assert np.linalg.norm(f64(results[0][1]) - s) <= 4e-6 * np.linalg.norm(s)
+    assert np.linalg.norm(beyond_rounding(results[0][0], o, dtype)) <= 4e-6 * np.linalg.norm(o)
