@@ -9,14 +9,16 @@
 // of the values to a workgroup (columns never meet), the state in its accumulators: wavefront w holds rows of dk of S^T and does
 // rows 16 w .. of every product.
 //
-// Numbers.  The state is returned in float32, so everything that it is made from keeps float32's accuracy on 16-bit operands.  Norms are
+// Numbers.  The state is returned in float32, so what it is made from keeps float32's accuracy on 16-bit operands.  Norms are
 // factors of rows, put on in float32 behind the products: Q and K stay what they came as, in float16 over a power of two for
-// each row (exact, but for elements below 2^-28 of the row's largest).  T, X, the state and what is added to it are two parts of float16
-// (22 bits; 1.4e-7 against 64 bits, as with three parts of bfloat16 for T and X) over powers of two: T's for each row, the others' for
-// each column.  Of a wavefront's rows of X or of the state the largest is at hand, of diag(e^(G_63 - G)) U it is bounded by X's
-// units and the largest sum over a row of T.  Decays are summed in float64: e^-1000 beside e^-0.001 loses
-// nothing.  The outputs take the same two parts of S, P and U: of one part, 11 bits, more than one in ten bfloat16 outputs would be
-// another value than the float32 arithmetic's.
+// each row (exact, but for elements below 2^-28 of the row's largest).  T, P, X, the state and what is added to it are two parts of float16,
+// 22 bits together (1.4e-7 against 64 bits, as with three parts of bfloat16 for T and X), over powers of two: T's and P's for each row,
+// the others' for each column.  Of a wavefront's rows of X or of the state the largest is at hand, of diag(e^(G_63 - G)) U it is
+// bounded by X's units and the largest sum over a row of T.  The second parts are over 2^-11 of those units and summed up first, so that
+// all 22 bits are there down to 2^-28 of the largest, below which they go one by one.  (Over the same units as the first they went from 2^-16 on:
+// a chunk's values that its decays wipe out left 3e-6 of error in the others at a size of 1e6, 3e-4 at 6e7.)  Decays are summed in
+// float64: e^-1000 beside e^-0.001 loses nothing.  The outputs take the same parts: of one part, 11 bits, more than one in ten
+// bfloat16 outputs would be another value than the float32 arithmetic's.
 //
 // 8192 tokens x 32 heads x 128 x 128 in bfloat16, one sequence: 72 us of preparation (its writes and reads, 5 TB/s) and 234 of the
 // scan, whose 128 chunks follow one another, 1.8 us each: about 1.1 are the chain of products and barriers from state to state, the
@@ -51,15 +53,18 @@ __device__ __forceinline__ kv_f4 mfma_f16(const kv_u2 &a, const kv_u2 &b, const 
 }
 __device__ __forceinline__ kv_f4 mfma_f32(float a, float b, const kv_f4 &c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-// two values' parts of float16: 11 bits, and the next 11
+// two values' parts of float16: 11 bits, and the next 11 over LOW, so that these are there for all elements whose first ones are
+constexpr float LOW = 1.f / 2048;
 __device__ __forceinline__ kv_u2 split2(float x, float y, float f) {  // of x f and y f, f a power of two
     kv_half2 h, l;
     h.x = (_Float16)(x * f);
     h.y = (_Float16)(y * f);
-    l.x = (_Float16)fmaf(x, f, -(float)h.x);
-    l.y = (_Float16)fmaf(y, f, -(float)h.y);
+    l.x = (_Float16)(fmaf(x, f, -(float)h.x) * (1 / LOW));
+    l.y = (_Float16)(fmaf(y, f, -(float)h.y) * (1 / LOW));
     return kv_u2{__builtin_bit_cast(uint32_t, h), __builtin_bit_cast(uint32_t, l)};
 }
+// products with second parts, as the sum that those of the first parts are added to
+__device__ __forceinline__ kv_f4 lowered(const kv_f4 &v) { return v * LOW; }
 // The power of two over which a row's or column's elements are laid out in float16, by the largest: they end below 2^14.
 __device__ __forceinline__ float unit_of(float top) {
     const uint32_t e = __float_as_uint(top) >> 23;  // (infinity and NaN: some unit; they stay what they are)
@@ -455,7 +460,7 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
 #pragma unroll
         for (int k = 0; k < 4; ++k) y[k] = kv_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
+        for (int p = 1; p >= 0; --p) {
 #pragma unroll
             for (int i = 0; i < 4 * TPW; i += TPW > 1 ? 2 : 1) {  // tiles of 16 rows, two to a step; of KD 64 a wavefront has half a step
                 const int s = i >> 1, k = i / TPW;
@@ -463,6 +468,11 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                 if constexpr (TPW > 1) y[k] = mfma_f16(rows[s], v, y[k]);
                 else y[k] = mfma_f16(rows[s], i & 1 ? kv_u4{0, 0, v.z, v.w} : kv_u4{v.x, v.y, 0, 0}, y[k]);
             }
+            if (p == 1) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[k] = lowered(y[k]);
+            }
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) sum[r] = fmaf(units[3], y[3][r], fmaf(units[2], y[2][r], fmaf(units[1], y[1][r], units[0] * y[0][r])));
         return sum;
@@ -530,19 +540,22 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                 }
                 u_unit[t] = unit_of(column_max(top));
                 const float f = over(u_unit[t]);
+                kv_u4 high[2], low[2];
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     if (s >= steps) break;
-                    kv_u4 high, low;
 #pragma unroll
                     for (int m = 0; m < 4; ++m) {
                         const kv_u2 part = split2(u[2 * s + (m >> 1)][2 * (m & 1)], u[2 * s + (m >> 1)][2 * (m & 1) + 1], f);
-                        high[m] = part.x, low[m] = part.y;
+                        high[s][m] = part.x, low[s][m] = part.y;
                     }
-                    I[t] = mfma_f16(P[0][s], high, I[t]);
-                    I[t] = mfma_f16(P[1][s], high, I[t]);
-                    I[t] = mfma_f16(P[0][s], low, I[t]);
+                    I[t] = mfma_f16(P[1][s], high[s], I[t]);
+                    I[t] = mfma_f16(P[0][s], low[s], I[t]);
                 }
+                I[t] = lowered(I[t]);
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+                    if (s < steps) I[t] = mfma_f16(P[0][s], high[s], I[t]);
             }
             const bool all = whole(c);
 #pragma unroll
@@ -705,9 +718,9 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                     kv_f4 y[2];
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        y[k] = mfma_f16(half(T[0][s], k), half(part[0][s], k), kv_f4{0.f, 0.f, 0.f, 0.f});
-                        y[k] = mfma_f16(half(T[0][s], k), half(part[1][s], k), y[k]);
+                        y[k] = mfma_f16(half(T[0][s], k), half(part[1][s], k), kv_f4{0.f, 0.f, 0.f, 0.f});
                         y[k] = mfma_f16(half(T[1][s], k), half(part[0][s], k), y[k]);
+                        y[k] = mfma_f16(half(T[0][s], k), half(part[0][s], k), lowered(y[k]));
                     }
 #pragma unroll
                     for (int r = 0; r < 4; ++r) U[t][r] = fmaf(units[2 * s + 1], y[1][r], fmaf(units[2 * s], y[0][r], U[t][r]));
@@ -739,11 +752,16 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
                 all_requested();
                 if (t == 0) request_system(next);
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
+                for (int p = 1; p >= 0; --p) {
 #pragma unroll
-                    for (int p = 0; p < 2; ++p)
+                    for (int s = 0; s < 2; ++s)
 #pragma unroll
                         for (int i = 0; i < TPW; ++i) D[i][t] = mfma_f16(KT[i][s], part[p][s], D[i][t]);
+                    if (p == 1) {
+#pragma unroll
+                        for (int i = 0; i < TPW; ++i) D[i][t] = lowered(D[i][t]);
+                    }
+                }
             }
 #pragma unroll
             for (int i = 0; i < TPW; ++i)

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import kvhip
+from oracle import recurrent as R
 from tests.test_gpu_gated_delta import DTYPES, LAYOUTS, expect, f64, make
 
 pytestmark = pytest.mark.gpu
@@ -58,3 +59,27 @@ def test_what_memory_held_before_is_nothing_to_a_prompt(dtype, layout, n):
     o, s, _ = expect(x, state)
     assert np.linalg.norm(f64(results[0][1]) - s) <= 4e-6 * np.linalg.norm(s)
     assert np.linalg.norm(beyond_rounding(results[0][0], o, dtype)) <= 4e-6 * np.linalg.norm(o)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e6, 1e7, 6e7])
+@pytest.mark.parametrize("n, first, fade", [(64, 20, 24), (64, 3, 3), (150, 75, 80), (20, 5, 6)])
+def test_values_that_are_forgotten_cost_the_others_nothing(dtype, size, n, first, fade):
+    """Values of up to 6e7 times the others (float16 goes no further) that a chunk's decays wipe out: what stays keeps its accuracy, and so do
+    the outputs behind them."""
+    rng = np.random.default_rng(8)
+    x, state = make(rng, 2, n, 1, 2, 128, 32, dtype, gate_dtype=torch.float32)
+    low = min(1.0, 1e4 / size)
+    x["v"] = (x["v"].float() * low).to(dtype)
+    x["v"][:, :first] = (x["v"][:, :first].float() * size).to(dtype)
+    a = torch.full((2, n, 2), -0.01, device="cuda")
+    a[:, fade:fade + 8] = -8.0  # (e^-64 of what was there is left)
+    given = dict(x, a=a, b=torch.sigmoid(x["b"]), a_log=None, dt_bias=None)
+    assert torch.isfinite(x["v"].float()).all()
+    cache = kvhip.GatedDeltaCache()
+    cache.delta_state = state * low
+    out = kvhip.gated_delta_update(**given, cache=cache)
+    o, s, _ = R.gated_delta(*(f64(given[k]) for k in ("q", "k", "v", "a", "b")), None, None, f64(state * low))
+    assert np.linalg.norm(f64(cache.delta_state) - s) <= 4e-6 * np.linalg.norm(s)
+    behind = slice(fade + 8, n)
+    assert np.linalg.norm(beyond_rounding(out, o, dtype)[:, behind]) <= 4e-6 * np.linalg.norm(o[:, behind])
