@@ -2,15 +2,18 @@
 //
 // The selection reads the logits once.  beam_rows_kernel: a workgroup holds a segment of one row in registers, takes its maximum
 // M and sum exp(x - M), and the `count` best of it.  A wavefront's count-th largest lane maximum is a bound that at least `count` of its
-// elements reach (found bit by bit by counting lanes, in whole numbers that are ordered as the values are); the largest of the
-// wavefronts' bounds leaves hardly more than `count` elements of the segment, which are put down in LDS and ranked against one
+// elements reach (found bit by bit by counting lanes, in whole numbers that are ordered as the values are, by all the bits that tell them
+// apart: logits far from zero and close together are told apart as well as others); the largest of the
+// wavefronts' bounds leaves a few times `count` elements of the segment, which are put down in LDS and ranked against one
 // another by value, then index.  beam_merge_kernel does the same for a batch row's candidates by their scores,
 //   s[beam] + ((x - M) - log sum),
-// in 64 bits, so that a sum's rounding does not decide between beams.  Where a list would overflow (thousands of equal values)
-// the best is taken out `count` times instead.
+// in 64 bits, so that a sum's rounding does not decide between beams.  Where more reach the bound than the list holds (counts near 64, which
+// a wavefront's 64 lanes bound loosely; thousands of equal values) the bound is raised digit by digit, by counts of all that share the digits in
+// front, until no more do.  16 x 16 rows of 152 064 bfloat16 logits, us: count 8 32, 32 70, 64 246 (the best taken out one by one: 3393); 32 x 8
+// rows, scores of -5, -100 and -300, 30.8, 30.2 and 29.9 (by sixteen bits of a score 31.9, 46.1 and 45.6).
 //
-// Memory bounds the rows: 256 bfloat16 rows of 152 064 logits 21.5 us, 3.6 TB/s; the merge is one workgroup to a batch row and the
-// latency of its steps, 6.4 us.
+// Vector instructions bound the rows, sixteen to an element, 74 % of the SIMDs' cycles: 256 bfloat16 rows of 152 064 logits 25 us,
+// 3.1 TB/s; the merge is one workgroup to a batch row and the latency of its steps, 6.1 us.
 #include <type_traits>
 
 #include "kvhip_delta.hpp"
@@ -31,15 +34,52 @@ __device__ __forceinline__ uint32_t ordered(float v) {
     return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
-// the largest whole number of sixteen bits above sixteen zeros that at least `count` (1 to 64) of the wavefront's lanes reach
-__device__ __forceinline__ uint32_t reached(uint32_t key, int count) {
+// the largest whole number of BITS bits above zeros that at least `count` (1 to 64) of the wavefront's lanes reach
+template <int BITS> __device__ __forceinline__ uint32_t reached(uint32_t key, int count) {
     uint32_t t = 0;
 #pragma unroll
-    for (int bit = 31; bit >= 16; --bit) {
+    for (int bit = 31; bit >= 32 - BITS; --bit) {
         const uint32_t up = t | (1u << bit);
         if (__popcll(__ballot(key >= up)) >= count) t = up;
     }
     return t;
+}
+// Counts the lanes that `take` by their digit; in one step where all have the same.  (One by one, 8192 equal logits to each of 4864 workgroups took
+// 1017 us, and 329 so.)
+__device__ __forceinline__ void count_digit(uint32_t *counts, bool take, uint32_t digit, int lane) {
+    const uint64_t there = __ballot(take);
+    if (there == 0) return;
+    const int first = __builtin_ctzll(there);
+    const uint32_t of_first = __builtin_amdgcn_readlane(digit, first);
+    if (__ballot(take && digit == of_first) == there) {
+        if (lane == first) atomicAdd(&counts[of_first], (uint32_t)__popcll(there));
+    } else if (take) {
+        atomicAdd(&counts[digit], 1u);
+    }
+}
+// Of what `counts` has by 256 digits, `need` at least: the digit of the need-th largest, how many have larger ones, and how many this one.
+// (one wavefront's work)
+struct Digit {
+    uint32_t digit;
+    int above, inside;
+};
+__device__ __forceinline__ void digit_of(const uint32_t *counts, int need, int lane, Digit *to) {
+    int own[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += own[i] = (int)counts[255 - 4 * lane - i];
+    int upto = sum;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const int o = __shfl_up(upto, s);
+        if (lane >= s) upto += o;
+    }
+    int before = upto - sum;
+    if (before >= need || upto < need) return;  // (all lanes but one)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (before < need && before + own[i] >= need) *to = Digit{255u - 4 * lane - i, before, own[i]};
+        before += own[i];
+    }
 }
 // a value and its index as one whole number: the larger value first, then the lower index
 __device__ __forceinline__ uint64_t rank_key(float v, int i) { return (uint64_t)ordered(v) << 32 | (uint32_t)~i; }
@@ -55,8 +95,6 @@ struct BeamScratch {
 };
 __host__ __device__ inline int64_t beam_at(const BeamScratch &w, int64_t row, int seg) { return row * w.segments + seg; }
 
-template <int NV> constexpr int beam_segment(int vec) { return 256 * NV * vec; }
-
 // NV: 16-byte vectors to a thread
 template <int DT, int NV, bool WIDE>
 __global__ void __launch_bounds__(256, WIDE ? 6 : 4) beam_rows_kernel(BeamArgs x, BeamScratch w) {
@@ -68,6 +106,8 @@ __global__ void __launch_bounds__(256, WIDE ? 6 : 4) beam_rows_kernel(BeamArgs x
     __shared__ float wave_top[4], wave_sum4s[4];
     __shared__ uint64_t list[BEAM_LIST];  // (value, index) as one whole number, the larger the better
     __shared__ int listed;
+    __shared__ uint32_t digits[256];
+    __shared__ Digit found;
     float *value = w.value + at * count;
     int32_t *index = w.index + at * count;
     if (x.done && x.done[row]) {  // one candidate, of the score that the beam has
@@ -125,7 +165,7 @@ __global__ void __launch_bounds__(256, WIDE ? 6 : 4) beam_rows_kernel(BeamArgs x
             for (int m = 0; m < VEC; ++m) tops[n] = fmaxf(tops[n], element(looked_at, n, m));
             top = fmaxf(top, tops[n]);
         }
-        const uint32_t bound = reached(ordered(top), count);
+        const uint32_t bound = reached<DT == 1 ? 16 : DT == 0 ? 19 : 32>(ordered(top), count);  // (all the bits that tell values apart)
         const float wtop = wave_max(top);
         if (lane == 0) {
             wave_key[wave] = bound;
@@ -176,45 +216,56 @@ __global__ void __launch_bounds__(256, WIDE ? 6 : 4) beam_rows_kernel(BeamArgs x
         put_down(std::true_type{});
     }
     __syncthreads();
-    const int n = listed;
+    int n = listed;
     if (tid == 0) w.sums[at] = make_float2(all, sum);
-    if (n <= BEAM_LIST) {
-        for (int i = tid; i < n; i += 256) {
-            const uint64_t mine = list[i];
-            int rank = 0;
-#pragma unroll 4
-            for (int m = 0; m < n; ++m) rank += list[m] > mine;
-            if (rank < count) {
-                value[rank] = unordered((uint32_t)(mine >> 32));
-                index[rank] = (int32_t)~(uint32_t)mine;
+    if (n > BEAM_LIST) {
+        // too many reach the bound: digit by digit of (value, index) the one that no more than the list holds do
+        uint64_t least_key = 0;
+        int above = 0, shift = 64;
+        auto every = [&](auto &&take) {  // (from the caches, eight at a time: the registers have no room for keys)
+            const int end = min(base + w.segment, x.vocabulary);
+            for (int i0 = base + tid; i0 - tid < end; i0 += 8 * 256) {
+                float v[8];
+#pragma unroll
+                for (int m = 0; m < 8; ++m) v[m] = Elem<DT>::load(p, min(i0 + 256 * m, end - 1));
+#pragma unroll
+                for (int m = 0; m < 8; ++m) take(i0 + 256 * m < end, rank_key(logit(v[m]), i0 + 256 * m));
             }
-        }
-        for (int i = n + tid; i < count; i += 256) {
-            value[i] = NEVER;
-            index[i] = -1;
-        }
-        return;
-    }
-    // thousands of equal values: the best behind the last one taken, `count` times (from the caches, as often)
-    uint64_t last = ~0ull;
-    for (int c = 0; c < count; ++c) {
-        uint64_t best = 0;
-        for (int i = base + tid; i < min(base + w.segment, x.vocabulary); i += 256) {
-            const uint64_t key = rank_key(logit(Elem<DT>::load(p, i)), i);
-            if (key < last && key > best) best = key;
-        }
-        __syncthreads();
-        list[tid] = best;
-        __syncthreads();
-        for (int half = 128; half > 0; half >>= 1) {
-            if (tid < half && list[tid + half] > list[tid]) list[tid] = list[tid + half];
+        };
+        do {
+            shift -= 8;
+            digits[tid] = 0;
             __syncthreads();
+            every([&](bool there, uint64_t key) {
+                count_digit(digits, there && (shift == 56 || (key ^ least_key) >> (shift + 8) == 0), key >> shift & 255, lane);
+            });
+            __syncthreads();
+            if (wave == 0) digit_of(digits, count - above, lane, &found);
+            __syncthreads();
+            least_key |= (uint64_t)found.digit << shift;
+            above += found.above;
+            n = above + found.inside;
+        } while (n > BEAM_LIST);
+        if (tid == 0) listed = 0;
+        __syncthreads();
+        every([&](bool there, uint64_t key) {
+            if (there && key >= least_key) list[atomicAdd(&listed, 1)] = key;
+        });
+        __syncthreads();
+    }
+    for (int i = tid; i < n; i += 256) {
+        const uint64_t mine = list[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int m = 0; m < n; ++m) rank += list[m] > mine;
+        if (rank < count) {
+            value[rank] = unordered((uint32_t)(mine >> 32));
+            index[rank] = (int32_t)~(uint32_t)mine;
         }
-        last = list[0];
-        if (tid == 0) {
-            value[c] = unordered((uint32_t)(last >> 32));
-            index[c] = (int32_t)~(uint32_t)last;
-        }
+    }
+    for (int i = n + tid; i < count; i += 256) {
+        value[i] = NEVER;
+        index[i] = -1;
     }
 }
 
@@ -231,7 +282,9 @@ __device__ __forceinline__ uint64_t ordered64(double v) {
 __device__ __forceinline__ double unordered64(uint64_t u) { return __longlong_as_double(u & 0x8000000000000000ull ? u ^ 0x8000000000000000ull : ~u); }
 
 constexpr int MERGE_THREADS = 512, MERGE_BEAMS = 64, MERGE_HELD = 4;
-static_assert(MERGE_THREADS <= BEAM_LIST, "a place in the list for each thread");
+// The candidate that is a thread's j-th.  Those of a segment stand best first, so that a lane would see one rank of all: each time they move
+// on by nine (512 + 9 is prime, no count divides it).
+__device__ __forceinline__ int merge_place(int j, int tid) { return j * MERGE_THREADS + ((tid + 9 * j) & (MERGE_THREADS - 1)); }
 __global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(BeamArgs x, BeamScratch w) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = blockIdx.x, count = x.count;
     __shared__ double beam_score[MERGE_BEAMS], beam_log[MERGE_BEAMS];
@@ -239,6 +292,8 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(BeamArgs x, B
     __shared__ uint32_t wave_key[MERGE_THREADS / 64];
     __shared__ __align__(16) Candidate list[BEAM_LIST];
     __shared__ int listed;
+    __shared__ uint32_t digits[256];
+    __shared__ Digit found;
     if (tid == 0) listed = 0;
     const int per = w.segments * count, total = x.beams * per;
     const int64_t first = (int64_t)g * x.beams * per;
@@ -247,7 +302,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(BeamArgs x, B
     int32_t token[MERGE_HELD];
 #pragma unroll
     for (int j = 0; j < MERGE_HELD; ++j) {
-        const int i = j * MERGE_THREADS + tid;
+        const int i = merge_place(j, tid);
         token[j] = i < total ? w.index[first + i] : -1;
         value[j] = i < total ? w.value[first + i] : NEVER;
     }
@@ -285,17 +340,22 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(BeamArgs x, B
         return Candidate{ordered64(score), (uint64_t)beam << 56 | (uint64_t)~ordered(v) << 24 | (uint32_t)t};
     };
     auto candidate = [&](int i) { return scored(i, w.value[first + i], w.index[first + i]); };
-    // scores for the bound: their leading 32 bits, rounded down, are in the same order
+    // scores for the bound: their leading 32 bits, steps of 2^-20 of a score, rounded down, are in the same order
     uint32_t top = 0, mine[MERGE_HELD];
 #pragma unroll
     for (int j = 0; j < MERGE_HELD; ++j) {
-        const int i = j * MERGE_THREADS + tid;
-        mine[j] = token[j] >= 0 ? (uint32_t)(scored(i, value[j], token[j]).score >> 32) : 0;
+        mine[j] = token[j] >= 0 ? (uint32_t)(scored(merge_place(j, tid), value[j], token[j]).score >> 32) : 0;
         top = max(top, mine[j]);
     }
-    for (int i = MERGE_HELD * MERGE_THREADS + tid; i < total; i += MERGE_THREADS)
-        if (w.index[first + i] >= 0) top = max(top, (uint32_t)(candidate(i).score >> 32));
-    const uint32_t bound = reached(top, count);
+    // a thread's candidates from its j-th on
+    auto every = [&](int j, auto &&take) {
+        for (; j * MERGE_THREADS < total; ++j) {
+            const int i = merge_place(j, tid);
+            if (i < total && w.index[first + i] >= 0) take(candidate(i));
+        }
+    };
+    every(MERGE_HELD, [&](const Candidate &c) { top = max(top, (uint32_t)(c.score >> 32)); });
+    const uint32_t bound = reached<32>(top, count);
     if (lane == 0) wave_key[wave] = bound;
     __syncthreads();
     uint32_t least = 1;
@@ -308,53 +368,57 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(BeamArgs x, B
     if (top >= least) {
 #pragma unroll
         for (int j = 0; j < MERGE_HELD; ++j)
-            if (mine[j] >= least) put_down(scored(j * MERGE_THREADS + tid, value[j], token[j]));
-        for (int i = MERGE_HELD * MERGE_THREADS + tid; i < total; i += MERGE_THREADS)
-            if (w.index[first + i] >= 0) {
-                const Candidate c = candidate(i);
-                if ((uint32_t)(c.score >> 32) >= least) put_down(c);
-            }
+            if (mine[j] >= least) put_down(scored(merge_place(j, tid), value[j], token[j]));
+        every(MERGE_HELD, [&](const Candidate &c) {
+            if ((uint32_t)(c.score >> 32) >= least) put_down(c);
+        });
     }
     __syncthreads();
-    const int n = listed;
+    int n = listed;
+    if (n > BEAM_LIST) {
+        // too many reach the bound: digit by digit of (score, what is before in a tie) the one that no more than the list holds do
+        uint64_t high = 0, low = 0;
+        int above = 0;
+        auto digit_at = [](const Candidate &c, int d) { return (uint32_t)((d < 8 ? c.score >> (56 - 8 * d) : ~c.tie >> (120 - 8 * d)) & 255); };
+        for (int d = 0; n > BEAM_LIST; ++d) {
+            if (tid < 256) digits[tid] = 0;
+            __syncthreads();
+            every(0, [&](const Candidate &c) {  // (of those whose digits in front are the ones that were found)
+                const bool same = d == 0 ? true : d <= 8 ? (c.score ^ high) >> (64 - 8 * d) == 0 : c.score == high && (~c.tie ^ low) >> (128 - 8 * d) == 0;
+                count_digit(digits, same, digit_at(c, d), lane);
+            });
+            __syncthreads();
+            if (wave == 0) digit_of(digits, count - above, lane, &found);
+            __syncthreads();
+            if (d < 8) high |= (uint64_t)found.digit << (56 - 8 * d);
+            else low |= (uint64_t)found.digit << (120 - 8 * d);
+            above += found.above;
+            n = above + found.inside;
+        }
+        if (tid == 0) listed = 0;
+        __syncthreads();
+        every(0, [&](const Candidate &c) {
+            if (c.score > high || (c.score == high && ~c.tie >= low)) list[atomicAdd(&listed, 1)] = c;
+        });
+        __syncthreads();
+    }
     auto put = [&](int at, const Candidate &c) {
         const int64_t o = (int64_t)g * count + at;
         x.rows[o] = g * x.beams + (int)(c.tie >> 56);
         x.tokens[o] = (int32_t)(c.tie & 0xffffffu);
         x.best[o] = (float)unordered64(c.score);
     };
-    if (n <= BEAM_LIST) {
-        for (int i = tid; i < n; i += MERGE_THREADS) {
-            const Candidate own = list[i];
-            int rank = 0;
+    for (int i = tid; i < n; i += MERGE_THREADS) {
+        const Candidate own = list[i];
+        int rank = 0;
 #pragma unroll 4
-            for (int m = 0; m < n; ++m) rank += before(list[m], own);
-            if (rank < count) put(rank, own);
-        }
-        for (int i = n + tid; i < count; i += MERGE_THREADS) {
-            const int64_t o = (int64_t)g * count + i;
-            x.rows[o] = x.tokens[o] = -1;
-            x.best[o] = NEVER;
-        }
-        return;
+        for (int m = 0; m < n; ++m) rank += before(list[m], own);
+        if (rank < count) put(rank, own);
     }
-    Candidate last{~0ull, 0};
-    for (int c = 0; c < count; ++c) {
-        Candidate best{0, ~0ull};
-        for (int i = tid; i < total; i += MERGE_THREADS) {
-            if (w.index[first + i] < 0) continue;
-            const Candidate o = candidate(i);
-            if (before(last, o) && before(o, best)) best = o;
-        }
-        __syncthreads();
-        list[tid] = best;
-        __syncthreads();
-        for (int half = MERGE_THREADS / 2; half > 0; half >>= 1) {
-            if (tid < half && before(list[tid + half], list[tid])) list[tid] = list[tid + half];
-            __syncthreads();
-        }
-        last = list[0];
-        if (tid == 0) put(c, last);
+    for (int i = n + tid; i < count; i += MERGE_THREADS) {
+        const int64_t o = (int64_t)g * count + i;
+        x.rows[o] = x.tokens[o] = -1;
+        x.best[o] = NEVER;
     }
 }
 

@@ -16,7 +16,7 @@
 // the others' for each column.  Of a wavefront's rows of X or of the state the largest is at hand, of diag(e^(G_63 - G)) U it is
 // bounded by X's units and the largest sum over a row of T.  The second parts are over 2^-11 of those units and summed up first, so that
 // all 22 bits are there down to 2^-28 of the largest, below which they go one by one.  (Over the same units as the first they went from 2^-16 on:
-// a chunk's values that its decays wipe out left 3e-6 of error in the others at a size of 1e6, 3e-4 at 6e7.)  Decays are summed in
+// a chunk's values that its decays wipe out left 4e-6 of error in the others at a size of 1e6, 3e-4 at 6e7.)  Decays are summed in
 // float64: e^-1000 beside e^-0.001 loses nothing.  The outputs take the same parts: of one part, 11 bits, more than one in ten
 // bfloat16 outputs would be another value than the float32 arithmetic's.
 //
