@@ -197,8 +197,14 @@ def check(status):
 _inited = False
 
 
-def init(device: int = 0):
+def init(device=None):
+    """Binds the library to a device, once: to the current one (binding makes its device the current one: any other would turn the
+    caller's calls to it)."""
     global _inited
     if not _inited:
+        if device is None:
+            import torch
+
+            device = torch.cuda.current_device() if torch.cuda.is_available() else 0
         check(load().kvhip_init(device))
         _inited = True
