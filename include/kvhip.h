@@ -382,8 +382,8 @@ kvhip_status kvhip_short_convolution(const void *x, int64_t x_stride_b, int64_t 
  * parts of one array.  a, b [B,L,Hv] of gate_dtype, likewise.  a_log, dt_bias (or NULL) [Hv] float32.  state [B,Hv,Dv,Dk]
  * float32 (state_in NULL: zeros), out [B,L,Hv,Dv] of `dtype`.  Dk up to 256.
  * States, sums and decays are float32 (a prompt's decays are summed in float64); only outputs are rounded to `dtype`.
- * float16 and bfloat16 prompts go through the matrix cores in chunks of 64 tokens, counted from the call's first; calls of fewer than 8
- * to 16 tokens (by the size of the states) and float32 go token by token.  In a chunk, values keep float32's accuracy down to 2^-28 of the
+ * float16 and bfloat16 prompts go through the matrix cores in chunks of 64 tokens, counted from the call's first; calls of up to 7
+ * to 20 tokens (by heads and keys) and float32 go token by token.  In a chunk, values keep float32's accuracy down to 2^-28 of the
  * largest of their channel in it, whether that one is remembered or not, and lose it from there on.  An element of a token that is no number or infinite makes its
  * sequence's states and outputs so from there on, in a prompt from the start of its chunk on; never another sequence's.
  * `workspace`: device memory of kvhip_gated_delta_workspace bytes (16-byte aligned; NULL if that is 0), of no content before or after; calls that

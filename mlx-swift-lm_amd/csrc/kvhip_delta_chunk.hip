@@ -849,12 +849,15 @@ template <int DT, int KD> hipError_t launch_chunks(const DeltaArgs &x, ChunkSpac
 
 }  // namespace
 
-// From how many tokens on, by the rows of all states (a token costs the other kernel what they take to pass through the vector
-// units, a chunk costs much the same whatever it holds).  32 heads x 128 x 128, us by chunks / by tokens: one sequence, 6 tokens 14.8 / 14.0, 8: 14.8 /
-// 17.5; 8 sequences, 10: 34.4 / 28.9, 12: 34.5 / 33.7, 16: 34.5 / 42.4; 64 sequences, 12: 200 / 189, 16: 204 / 242.
+// From how many tokens on: a chunk costs much the same whatever it holds, each of few heads a launch's time more; a token costs the other
+// kernel a chain of sums, and what the states take to pass through the vector units.  us by chunks / by tokens, heads of 128 x 128: 32, 10
+// tokens 15.5 / 14.9, 12: 15.5 / 16.9; 128, 14: 23.2 / 21.0, 16: 23.2 / 23.4; 256, 20: 36.5 / 34.5, 24: 36.5 / 40.3; 2048, 16: 211 / 190,
+// 20: 216 / 227.  256 of 64 x 64, 20: 20.3 / 18.5, 24: 20.3 / 21.1.  Of 512 x 256, whose tokens have twice the registers: 8, 8: 19.0 / 20.6;
+// 32, 10: 31.5 / 28.7, 12: 31.6 / 32.4; 128, 16: 89.9 / 102.8.
 bool delta_takes_chunks(const DeltaArgs &x) {
-    const int64_t rows = (int64_t)x.B * x.Hv * x.Dv;
-    return x.dtype != KVHIP_F32 && x.L > (rows <= 8192 ? 7 : rows <= 65536 ? 11 : 15) && rows < ((int64_t)1 << 31);
+    const int64_t heads = (int64_t)x.B * x.Hv;
+    const int tokens = x.Dk <= 128 ? (heads <= 32 ? 10 : heads <= 128 ? 14 : 20) : (heads <= 16 ? 7 : heads <= 32 ? 11 : 14);
+    return x.dtype != KVHIP_F32 && x.L > tokens && heads * x.Dv < ((int64_t)1 << 31);
 }
 
 size_t delta_chunk_workspace(const DeltaArgs &x) {
