@@ -427,7 +427,7 @@ kvhip_status kvhip_beam_select(const void *logits, int64_t stride, int32_t group
  * stay are not touched.  B up to 2048.  KVHIP_ERR_STATE while a round is staged.
  */
 kvhip_status kvhip_cache_reorder(kvhip_cache *cache, const int32_t *order, int64_t shared, void *stream);
-/* The same for up to 8 dense arrays of `rows` rows, row_bytes[i] bytes each (a recurrent layer's window and state). */
+/* The same for up to 8 dense arrays of `rows` rows, row_bytes[i] bytes each (a recurrent layer's window and state), none of which overlap. */
 kvhip_status kvhip_reorder_rows(int32_t count, void *const *arrays, const size_t *row_bytes, int32_t rows, const int32_t *order,
                                 void *stream);
 

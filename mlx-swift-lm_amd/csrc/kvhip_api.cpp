@@ -1913,6 +1913,9 @@ kvhip_status kvhip_reorder_rows(int32_t count, void *const *arrays, const size_t
         if (row_bytes[i] > ((size_t)1 << 32)) return fail(KVHIP_ERR_UNSUPPORTED, "rows of more than 4 GiB");
         x.at[i] = static_cast<char *>(arrays[i]);
         x.bytes[i] = row_bytes[i];
+        for (int m = 0; m < i; ++m)  // (rows that two workgroups move would be what the later one finds)
+            if (x.at[i] < x.at[m] + x.bytes[m] * rows && x.at[m] < x.at[i] + x.bytes[i] * rows)
+                return fail(KVHIP_ERR_INVALID_ARG, "arrays overlap");
     }
     KV_HIP(launch_reorder_arrays(x, rows, order, S(stream)));
     return KVHIP_OK;
