@@ -367,7 +367,7 @@ kvhip_status kvhip_cache_update_attend_blocks(kvhip_cache *cache, const void *qu
  * y_l = f(bias + sum_w weight[:, w] e_{l + w}), by channel, e the window's W - 1 rows and then the sequence's tokens; f is x sigmoid(x)
  * when `silu`.  The new window is the last W - 1 rows of e.  x [B,L,C], sequences and tokens x_stride_b / x_stride_l elements
  * apart; weight [C,W], bias [C] or NULL, window [B,W-1,C], out [B,L,C], all of `dtype`, sums in float32.  window_in NULL: zeros.
- * 1 <= W <= 8.
+ * 1 <= W <= 8, B up to 65535, L up to 2^20.  A token that is no number reaches the outputs of W tokens and no further.
  */
 kvhip_status kvhip_short_convolution(const void *x, int64_t x_stride_b, int64_t x_stride_l, const void *weight, const void *bias,
                                      int32_t B, int32_t L, int32_t C, int32_t W, int32_t dtype, int32_t silu, const int32_t *left_pad,
@@ -387,7 +387,8 @@ kvhip_status kvhip_short_convolution(const void *x, int64_t x_stride_b, int64_t 
  * largest of their channel in it, whether that one is remembered or not, and lose it from there on.  An element of a token that is no number or infinite makes its
  * sequence's states and outputs so from there on, in a prompt from the start of its chunk on; never another sequence's.
  * `workspace`: device memory of kvhip_gated_delta_workspace bytes (16-byte aligned; NULL if that is 0), of no content before or after; calls that
- * can overlap need one each.
+ * can overlap need one each.  It holds up to 384 MiB of chunks, or four chunks of all sequences where those are more: 128 sequences of 32 heads of
+ * 128 x 128 (16 key heads) 920 MiB.  B and Hv up to 65535, L up to 2^24.
  */
 typedef struct kvhip_gated_delta_args {
     const void *q, *k, *v, *a, *b;
@@ -409,7 +410,7 @@ kvhip_status kvhip_gated_delta(const kvhip_gated_delta_args *args, void *workspa
 /*
  * The `count` best continuations of each of `groups` groups of `beams` rows of logits [groups * beams, vocabulary] (rows `stride`
  * elements apart).  Row r continued by token t scores scores[r] + x[r,t] - log sum_j exp x[r,j] (scores NULL: 0), in float64
- * from float32 sums.  Best first; among equals the lower beam, then the higher logit, then the lower token.  A row whose `done` (bytes, or
+ * from float32 sums: candidates of two beams that lie closer than those are rounded, some 1e-7, come in either order.  Best first; among equals the lower beam, then the higher logit, then the lower token.  A row whose `done` (bytes, or
  * NULL) is set offers pad_token alone, at scores[r].  A logit that is no number counts as minus infinity, infinity as the
  * largest float32; a score that is no number as minus infinity.  rows (numbers of logits rows: an order for kvhip_cache_reorder), tokens, best:
  * [groups, count]; where fewer candidates are there, -1, -1 and minus infinity behind them.

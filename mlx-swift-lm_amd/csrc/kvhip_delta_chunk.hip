@@ -20,11 +20,11 @@
 // float64: e^-1000 beside e^-0.001 loses nothing.  The outputs take the same parts: of one part, 11 bits, more than one in ten
 // bfloat16 outputs would be another value than the float32 arithmetic's.
 //
-// 8192 tokens x 32 heads x 128 x 128 in bfloat16, one sequence: 72 us of preparation (its writes and reads, 5 TB/s) and 234 of the
-// scan, whose 128 chunks follow one another, 1.8 us each: about 1.1 are the chain of products and barriers from state to state, the
-// rest comes with the 74 KB of operands and with the outputs of a chunk, wherever they lie (two chunks' operands again and again, in the
-// L2, take as long).  One wavefront to 16 columns in place of one to 16 rows took 151 us for half the tokens.
-// 2000 tokens of 8 sequences in float16: 101 and 310 us, in two stretches of the workspace.
+// 8192 tokens x 32 heads x 128 x 128 in bfloat16, one sequence: 76 us of preparation (its writes and reads, 5 TB/s) and 280 of the
+// scan, whose 128 chunks follow one another, 2.2 us each: the chain of products and barriers from state to state, the 82 KB of operands,
+// wherever they lie (two chunks' again and again, in the L2, take as long), and the outputs, whose second parts are 25 us of the 280.  One
+// wavefront to 16 columns in place of one to 16 rows took 1.3 times as long.
+// 2000 tokens of 8 sequences in float16: 99 and 317 us, in two stretches of the workspace.
 //
 // Operands lie in the workspace as the lanes take them, 1 KB to an instruction: contractions may be summed in any
 // order, so that lane (n, g)'s eight elements of a step are those at 4 g and 16 + 4 g of it -- which is where a product leaves them: S, U
@@ -793,8 +793,9 @@ __global__ void __launch_bounds__(512, 2) chunk_scan_kernel(DeltaArgs x, ChunkSp
 inline int chunk_key_dim(const DeltaArgs &x) { return x.Dk <= 64 ? 64 : x.Dk <= 128 ? 128 : 256; }
 // What a chunk of all sequences and heads takes, and how many chunks are laid out at a time: what they take is to stay near the
 // last-level cache between the two kernels, and a round is to be long enough to pay for its start.  96 / 192 / 384 / 768 MiB, 32 heads of
-// 128 x 128 in bfloat16, us: 8 x 2000 tokens 637 / 574 / 576 / 558; 16 x 4096 2224 / 2061 / 1910 / 1840; 32768 of one 1165 / 1111 /
-// 1154 / 1139.  More than 384 gains little for twice the memory.
+// 128 x 128 in bfloat16, us: 8 x 2000 tokens 622 / 550 / 525 / 499; 16 x 4096 2490 / 2316 / 2106 / 2038; 32768 of one 1306 / 1256 /
+// 1301 / 1276.  More than 384 gains little for twice the memory.  Four chunks at least, whatever they take, because every round reads and
+// writes the states: 256 x 333 with 1 / 2 / 4 at least 5325 / 4091 / 3750.
 constexpr uint64_t CHUNK_SPACE = (uint64_t)384 << 20;
 inline ChunkSpace chunk_space(const DeltaArgs &x, void *workspace, uint64_t *bytes) {
     ChunkSpace w{};
@@ -830,9 +831,9 @@ template <int DT, int KD> hipError_t launch_chunks(const DeltaArgs &x, ChunkSpac
         };
         const int64_t groups = (int64_t)x.B * x.Hv * ((x.Dv + 15) / 16);
         // Every workgroup of a head reads the head's whole operands: few columns to each fill the chip, many read less.  Whole calls in
-        // us with 16 / 32 / 64 columns, 32 heads of 128 x 128 in bfloat16: 8192 tokens (256 groups) 319 / 415 / 652; 2 x 2048 (512)
-        // 152 / 129 / 191; 4 x 2048 (1024) 318 / 264 / 245; 8 x 2000 in float16 (2048) 1073 / 656 / 545 (but 6 x 2048, 1536, 590 / 395 / 410).
-        // 256 channels have no registers for 64; 4 heads of 512 x 256: 4096 tokens (128) 151 / 224; 4 x 2048 (512) 166 / 143.
+        // us with 16 / 32 / 64 columns, 32 heads of 128 x 128 in bfloat16: 8192 tokens (256 groups) 318 / 468 / 778; 2 x 2048 (512)
+        // 154 / 136 / 214; 4 x 2048 (1024) 336 / 275 / 255; 8 x 2000 in float16 (2048) 1071 / 635 / 524 (but 6 x 2048, 1536, 650 / 420 / 461).
+        // 256 channels have no registers for 64; 4 heads of 512 x 256: 4096 tokens (128) 166 / 264; 4 x 2048 (512) 176 / 151.
         if (groups <= 256) {
             scan(chunk_scan_kernel<DT, KD, 1>, 16);
         } else if (KD > 128 || groups <= 512) {
