@@ -87,6 +87,11 @@ __device__ __forceinline__ float column_max(float v) {
 // registers hold.)
 __device__ __forceinline__ int wave_number() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
+// what a wavefront's lanes hand one another through LDS: its requests are answered in their order, the compiler keeps them in it
+__device__ __forceinline__ void lanes_meet() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 // what wavefronts hand one another through LDS; requests past it stay in flight
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -295,6 +300,7 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
             }
         }
     }
+    lanes_meet();
     {  // P in float16 over a unit of each row: rows 16 w + n (that this wavefront wrote), tokens 32 s + 4 g and 16 on
         float v[2][8], top = 0.f;
 #pragma unroll
@@ -320,6 +326,7 @@ __global__ void __launch_bounds__(256, KD > 128 ? 2 : 4) chunk_prep_kernel(Delta
             *reinterpret_cast<kv_u4 *>(p + 8192 + (wave * 2 + s) * 1024 + lane * 16) = low;
         }
     }
+    lanes_meet();
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
